@@ -204,3 +204,34 @@ def pretrain_tmix_lnx_rkvres_xg_backward(grad_output, x, r, k, v, residual_scale
     return ops.pretrain_tmix_lnx_rkvres_xg_backward(grad_output, x, r, k, v, residual_scale,
                                                     weight, bias, g, mean, rstd,
                                                     int(head_size))
+
+
+def layer_norm_forward(x, residual, weight, bias, eps, statistics=False):
+    """[y] or [y, stream], then [mean, rstd] where statistics are asked for."""
+    return ops.layer_norm_forward(x, residual, weight, bias, float(eps), bool(statistics))
+
+
+def layer_norm_backward(grad_y, normed, grad_stream, weight, mean, rstd):
+    """[grad_x, grad_weight, grad_bias]; normed is x, or the stream of a call with a residual."""
+    return ops.layer_norm_backward(grad_y, normed, grad_stream, weight, mean, rstd)
+
+
+def linear_cross_entropy_forward(hidden, weight, targets, ignore_index, reduction):
+    """(loss, saved); reduction 0 none, 1 mean, 2 sum."""
+    return ops.linear_cross_entropy_forward(hidden, weight, targets, int(ignore_index),
+                                            int(reduction))
+
+
+def linear_topk_distillation_forward(hidden, weight, teacher_logits, teacher_indices,
+                                     temperature, reduction):
+    """(loss, saved); reduction 0 none, 1 mean, 2 sum."""
+    return ops.linear_topk_distillation_forward(hidden, weight, teacher_logits, teacher_indices,
+                                                float(temperature), int(reduction))
+
+
+def linear_loss_backward(grad_loss, weight, saved, rows, top, temperature, reduction,
+                         want_hidden, want_weight):
+    """The gradients asked for, of hidden ([rows, C]) and of weight, in that order."""
+    return ops.linear_loss_backward(grad_loss, weight, saved, int(rows), int(top),
+                                    float(temperature), int(reduction), bool(want_hidden),
+                                    bool(want_weight))

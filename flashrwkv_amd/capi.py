@@ -62,6 +62,18 @@ SIGNATURES = {
     "frwkv_lnx_pretrain_backward_workspace_bytes": [_I64, _I32, _I32],
     "frwkv_lnx_pretrain_backward": [_INT, _I64, _I32, _I32] + [_VP] * 20 + [_SZ, _VP],
     "frwkv_recurrent_tmix_fused_forward": [_INT] * 2 + [_I32] * 5 + [_VP] * 18 + [_F32, _VP],
+    "frwkv_layer_norm_forward": [_INT, _I64, _I64] + [_VP] * 4 + [_F32] + [_VP] * 5,
+    "frwkv_layer_norm_backward_workspace_bytes": [_I64] * 2,
+    "frwkv_layer_norm_backward": [_INT, _I64, _I64] + [_VP] * 10 + [_SZ, _VP],
+    "frwkv_linear_loss_saved_bytes": [_I64] * 3,
+    "frwkv_linear_loss_forward_workspace_bytes": [_I64] * 2,
+    "frwkv_linear_loss_backward_workspace_bytes": [_I64] * 3 + [_INT],
+    "frwkv_linear_cross_entropy_forward": [_INT] + [_I64] * 3 + [_VP, _VP, _INT, _VP, _I64, _INT]
+                                          + [_VP, _VP, _SZ, _VP, _SZ, _VP],
+    "frwkv_linear_topk_distillation_forward": [_INT] + [_I64] * 4 + [_VP, _VP, _INT, _VP, _INT]
+                                              + [_VP, _F32, _INT, _VP, _VP, _SZ, _VP, _SZ, _VP],
+    "frwkv_linear_loss_backward": [_INT] + [_I64] * 4 + [_VP, _F32, _INT, _VP, _VP, _SZ]
+                                  + [_VP] * 3 + [_SZ, _VP],
 }
 
 _LIB = None

@@ -1450,6 +1450,8 @@ Tensor recurrent_tmix_fused_forward(Tensor query_start_loc, Tensor state_indices
   return output;
 }
 
+#include "head_ops.h"
+
 TORCH_LIBRARY(flashrwkv2, m) {
   m.class_<MetadataTicket>("MetadataTicket")
       .def("max_seqlen", [](const TicketPtr& t) { return t->max_seqlen(); })
@@ -1509,6 +1511,26 @@ TORCH_LIBRARY(flashrwkv2, m) {
       "Tensor v, Tensor residual_scale, Tensor weight, Tensor bias, Tensor g, Tensor mean, "
       "Tensor rstd, int head_size=64) -> Tensor[]",
       &pretrain_tmix_lnx_rkvres_xg_backward);
+  m.def(
+      "layer_norm_forward(Tensor x, Tensor? residual, Tensor weight, Tensor bias, float eps, "
+      "bool statistics) -> Tensor[]",
+      &layer_norm_forward);
+  m.def(
+      "layer_norm_backward(Tensor grad_y, Tensor normed, Tensor? grad_stream, Tensor weight, "
+      "Tensor mean, Tensor rstd) -> Tensor[]",
+      &layer_norm_backward);
+  m.def(
+      "linear_cross_entropy_forward(Tensor hidden, Tensor weight, Tensor targets, "
+      "int ignore_index, int reduction) -> (Tensor, Tensor)",
+      &linear_cross_entropy_forward);
+  m.def(
+      "linear_topk_distillation_forward(Tensor hidden, Tensor weight, Tensor teacher_logits, "
+      "Tensor teacher_indices, float temperature, int reduction) -> (Tensor, Tensor)",
+      &linear_topk_distillation_forward);
+  m.def(
+      "linear_loss_backward(Tensor grad_loss, Tensor weight, Tensor saved, int rows, int top, "
+      "float temperature, int reduction, bool want_hidden, bool want_weight) -> Tensor[]",
+      &linear_loss_backward);
   m.def("set_recurrent_long_route(int route) -> int", &set_recurrent_long_route);
   m.def("recurrent_long_route() -> int", &recurrent_long_route);
   m.def(

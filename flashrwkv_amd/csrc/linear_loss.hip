@@ -1,0 +1,1057 @@
+// Losses of a language model's head from its hidden rows: softmax cross
+// entropy and distillation from a teacher's top logits, both over the whole
+// vocabulary and both without keeping the logits.
+//
+// With z = h W^T (rows i, vocabulary v), s = 1 / T (1 for cross entropy) and a
+// sparse target b_i (one entry 1 for cross entropy; the K shares p_ik =
+// softmax over the row's present teacher logits / T for distillation):
+//   lse_i = log sum_v exp(s z_iv)
+//   loss_i = T^2 (lse_i + sum_k p_ik (log p_ik - s z_i,k))
+//   dL/dz_iv = w_i T (exp(s z_iv - lse_i) - b_iv),  w_i the upstream weight
+//   dh = dz W,  dW = dz^T h.
+//
+// Rows that take no part (target = ignore_index; no teacher entry) are left
+// out at the start: the hidden rows of the others are copied together (2 N C
+// elements moved against 2 N V C operations a product), so masked rows cost
+// nothing afterwards and what stands in them reaches nothing. How many rows
+// are left stays on the device; grids are sized for all rows and tiles past
+// the count end at once.
+//
+// Forward: one product h W^T whose epilogue keeps the maximum and the sum of
+// exponentials of each 256-column tile, row by row; a second kernel joins the
+// tiles. The K target logits of a row are dot products of their own (fp32).
+// Backward, for one piece of the vocabulary after another: the product again,
+// its epilogue turning logits into dz of the piece (16 bits, [rows][piece]);
+// the target entries are overwritten from the fp32 target logits, so that
+// p - b does not lose digits where the two are close; then dz W into an fp32
+// slab (its sum over slabs, in order, is dh) and dz^T h, which is dW's rows.
+// Everything is summed in fp32 in a fixed order; dz is the only rounding to
+// 16 bits before the outputs, as a matrix operand has to be (relative error
+// 2^-9 an entry for bf16, independent between entries).
+#include <algorithm>
+
+#include "capi_internal.h"
+#include "gemm_tile.h"
+#include "wkv7_device.h"
+
+namespace frwkv {
+namespace {
+
+using gemm::f32x4;
+using gemm::Major;
+using gemm::Operand;
+
+constexpr float kLn2 = 0.69314718055994531f;
+constexpr int kRowPad = 256;       // rows of workspaces, and a product's largest tile
+constexpr int kVocabTile = 256;    // columns whose maximum and sum the forward keeps together
+constexpr int kScanThreads = 1024;
+constexpr float kNaN = __builtin_nanf("");
+
+__host__ __device__ constexpr int64_t round_up(int64_t x, int64_t to) {
+  return (x + to - 1) / to * to;
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack8(uint4 q, float (&out)[8]) {
+  const uint16_t* s = reinterpret_cast<const uint16_t*>(&q);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) out[e] = to_f32<T>(s[e]);
+}
+
+__device__ __forceinline__ float wave_sum(float x) {
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) x += __shfl_xor(x, off, 64);
+  return x;
+}
+
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) x = fmaxf(x, __shfl_xor(x, off, 64));
+  return x;
+}
+
+// What the forward leaves for the backward. Row indices m count the rows that
+// take part, in order; i is the row's place in the caller's tensors.
+struct Saved {
+  int32_t* count;   // [1]     rows that take part
+  int32_t* row;     // [pad]   m -> i
+  int32_t* place;   // [N]     i -> m, or -1
+  int32_t* index;   // [N][K]  target tokens (by i); -1 absent, V or more out of range
+  float* share;     // [N][K]  p (by i)
+  float* target;    // [N][K]  b at that token: the sum of p over equal tokens (by i)
+  float* base;      // [N]     sum p log p (by i)
+  float* lse2;      // [pad]   log2 sum exp (by m)
+  float* logit;     // [pad][K] z at the target tokens (by m)
+  uint16_t* hidden; // [pad][C] the rows that take part, zeros after the last up to a tile
+};
+
+struct Layout {
+  size_t bytes = 0;
+  size_t take(size_t n) {
+    const size_t at = bytes;
+    bytes += (n + 255) / 256 * 256;
+    return at;
+  }
+};
+
+Saved saved_of(char* p, int64_t n, int64_t c, int64_t k, size_t* bytes) {
+  const int64_t pad = round_up(n, kRowPad);
+  Layout l;
+  Saved s;
+  const size_t count = l.take(4), row = l.take(pad * 4), place = l.take(n * 4);
+  const size_t index = l.take(n * k * 4), share = l.take(n * k * 4);
+  const size_t target = l.take(n * k * 4), base = l.take(n * 4), lse2 = l.take(pad * 4);
+  const size_t logit = l.take(pad * k * 4), hidden = l.take(pad * c * 2);
+  s.count = reinterpret_cast<int32_t*>(p + count);
+  s.row = reinterpret_cast<int32_t*>(p + row);
+  s.place = reinterpret_cast<int32_t*>(p + place);
+  s.index = reinterpret_cast<int32_t*>(p + index);
+  s.share = reinterpret_cast<float*>(p + share);
+  s.target = reinterpret_cast<float*>(p + target);
+  s.base = reinterpret_cast<float*>(p + base);
+  s.lse2 = reinterpret_cast<float*>(p + lse2);
+  s.logit = reinterpret_cast<float*>(p + logit);
+  s.hidden = reinterpret_cast<uint16_t*>(p + hidden);
+  *bytes = l.bytes;
+  return s;
+}
+
+// ---------------------------------------------------------------- targets
+__device__ __forceinline__ int32_t as_token(int64_t t, int32_t vocab) {
+  // Negative tokens are absent for distillation and out of range for cross
+  // entropy, whose caller has taken ignore_index out before.
+  return t < 0 ? -1 : t >= vocab ? vocab : static_cast<int32_t>(t);
+}
+
+// Cross entropy: one entry a row, share 1. place[i] = 1 for rows that take part.
+template <typename Index>
+__global__ __launch_bounds__(256) void label_targets_kernel(const Index* __restrict__ targets,
+                                                            int64_t ignore, int32_t n,
+                                                            int32_t vocab, Saved s) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  const int64_t t = targets[i];
+  const bool part = t != ignore;
+  s.place[i] = part;
+  const int32_t token = as_token(t, vocab);
+  s.index[i] = part && token < 0 ? vocab : token;
+  s.share[i] = 1.0f;
+  s.target[i] = 1.0f;
+  s.base[i] = 0.0f;
+}
+
+// Distillation, a wave a row: shares from the teacher's logits. An entry is
+// present where its token is not negative and its logit not -inf; a row
+// without one takes no part. Tokens that occur twice in a row count with the
+// sum of their shares. Dynamic LDS: K tokens and K shares a wave.
+template <typename T, typename Index>
+__global__ __launch_bounds__(256) void teacher_targets_kernel(
+    const typename IoTraits<T>::storage* __restrict__ logits, const Index* __restrict__ indices,
+    int32_t n, int32_t k, int32_t vocab, float inv_temperature, Saved s) {
+  extern __shared__ char smem[];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int i = blockIdx.x * 4 + wave;
+  int32_t* tokens = reinterpret_cast<int32_t*>(smem) + wave * 2 * k;
+  float* shares = reinterpret_cast<float*>(tokens + k);
+  const int64_t at = static_cast<int64_t>(i) * k;
+  float top = -__builtin_inff();
+  bool any = false;
+  if (i < n) {
+    for (int j = lane; j < k; j += 64) {
+      const float x = to_f32<T>(logits[at + j]) * inv_temperature;
+      const int32_t token = x == -__builtin_inff() ? -1 : as_token(indices[at + j], vocab);
+      tokens[j] = token;
+      shares[j] = x;
+      if (token >= 0) {
+        any = true;
+        top = fmaxf(top, x);
+      }
+    }
+  }
+  const bool part = __ballot(any) != 0;
+  top = wave_max(top);
+  float total = 0.0f;
+  if (i < n) {
+    for (int j = lane; j < k; j += 64) {
+      const float e =
+          tokens[j] >= 0 ? __builtin_amdgcn_exp2f((shares[j] - top) * kLog2E) : 0.0f;
+      total += e;
+    }
+  }
+  total = wave_sum(total);
+  const float log_total = __logf(total);
+  float base = 0.0f;
+  if (i < n) {
+    for (int j = lane; j < k; j += 64) {
+      float p = 0.0f;
+      if (part && tokens[j] >= 0) {
+        const float log_p = shares[j] - top - log_total;
+        p = __builtin_amdgcn_exp2f(log_p * kLog2E);
+        base += p == 0.0f ? 0.0f : p * log_p;
+      }
+      shares[j] = p;
+    }
+  }
+  base = wave_sum(base);
+  __syncthreads();
+  if (i >= n) return;
+  for (int j = lane; j < k; j += 64) {
+    const int32_t token = tokens[j];
+    float sum = 0.0f;
+    for (int q = 0; q < k; ++q) sum += tokens[q] == token ? shares[q] : 0.0f;
+    s.index[at + j] = token;
+    s.share[at + j] = shares[j];
+    s.target[at + j] = sum;
+  }
+  if (lane == 0) {
+    s.place[i] = part;
+    s.base[i] = base;
+  }
+}
+
+// Numbers the rows that take part, in order (one workgroup). place[i]: 1 or 0
+// in, m or -1 out.
+__global__ __launch_bounds__(kScanThreads) void number_rows_kernel(int32_t n, Saved s) {
+  __shared__ int32_t waves[kScanThreads / 64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int32_t before = 0;
+  for (int32_t first = 0; first < n; first += kScanThreads) {
+    const int32_t i = first + static_cast<int32_t>(threadIdx.x);
+    const bool part = i < n && s.place[i] != 0;
+    const uint64_t mask = __ballot(part);
+    if (lane == 0) waves[wave] = __popcll(mask);
+    __syncthreads();
+    int32_t m = before + __popcll(mask & ((1ull << lane) - 1));
+    int32_t all = 0;
+#pragma unroll
+    for (int w = 0; w < kScanThreads / 64; ++w) {
+      if (w < wave) m += waves[w];
+      all += waves[w];
+    }
+    if (i < n) s.place[i] = part ? m : -1;
+    if (part) s.row[m] = i;
+    before += all;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) *s.count = before;
+}
+
+// A workgroup a row m: copies its hidden row (zeros for the rows that fill up
+// the last tile) and computes its target logits, a wave a token.
+// base[i] becomes sum p (log p - s z), what lse is added to.
+template <typename T>
+__global__ __launch_bounds__(256) void gather_rows_kernel(
+    const uint16_t* __restrict__ hidden, const uint16_t* __restrict__ weight, int32_t c,
+    int32_t k, int32_t vocab, float inv_temperature, float* __restrict__ target_term, Saved s) {
+  __shared__ float part[4];
+  const int m = blockIdx.x;
+  const int count = *s.count;
+  if (m >= round_up(count, kRowPad)) return;
+  uint16_t* to = s.hidden + static_cast<int64_t>(m) * c;
+  if (m >= count) {
+    for (int x = threadIdx.x * 8; x < c; x += 2048) {
+      *reinterpret_cast<uint4*>(to + x) = make_uint4(0, 0, 0, 0);
+    }
+    return;
+  }
+  const int64_t i = s.row[m];
+  const uint16_t* from = hidden + i * c;
+  for (int x = threadIdx.x * 8; x < c; x += 2048) {
+    *reinterpret_cast<uint4*>(to + x) = *reinterpret_cast<const uint4*>(from + x);
+  }
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  float term = 0.0f;
+  for (int j = wave; j < k; j += 4) {
+    const int32_t token = s.index[i * k + j];
+    float z = 0.0f;
+    if (token >= 0 && token < vocab) {
+      const uint16_t* w = weight + static_cast<int64_t>(token) * c;
+      float sum = 0.0f;
+      for (int x = lane * 8; x < c; x += 512) {
+        float a[8], b[8];
+        unpack8<T>(*reinterpret_cast<const uint4*>(from + x), a);
+        unpack8<T>(*reinterpret_cast<const uint4*>(w + x), b);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum = fmaf(a[e], b[e], sum);
+      }
+      z = wave_sum(sum);
+    } else if (token >= vocab) {
+      z = kNaN;
+    }
+    if (lane == 0) s.logit[static_cast<int64_t>(m) * k + j] = z;
+    const float p = s.share[i * k + j];
+    if (token >= 0) term += p == 0.0f && token < vocab ? 0.0f : p * (z * inv_temperature);
+  }
+  if (lane == 0) part[wave] = term;
+  __syncthreads();
+  if (threadIdx.x == 0) target_term[m] = s.base[i] - (part[0] + part[1] + part[2] + part[3]);
+}
+
+// ------------------------------------------------------------- products
+// Tile shapes. Few rows: 64 of them against 256 vocabulary columns, three
+// stages deep, since such a call only streams the weight. Otherwise 256 x 256.
+template <typename T, Major MA, Major MB>
+using LargeTile = gemm::Tile<T, MA, MB, 256, 256, 2, 4, 2>;
+template <typename T, Major MA, Major MB>
+using FewRowsTile = gemm::Tile<T, MA, MB, 256, 64, 8, 1, 3>;
+constexpr int kFewRows = 64;
+
+// D[v][m] of a vocabulary range: per tile of 256 v and row m the maximum of
+// s z log2 e and the sum of 2^(s z log2 e - maximum), to part[tile][m].
+template <typename G, typename T>
+__global__ __launch_bounds__(gemm::kThreads, 2) void lse_tiles_kernel(
+    Operand w, Operand h, const int32_t* __restrict__ count, int32_t c, int32_t np, int32_t nq,
+    float scale, float2* __restrict__ part, int64_t pad) {
+  __shared__ __attribute__((aligned(1024))) char smem[G::kLdsBytes];
+  int tp, tq;
+  gemm::tile_of(gemm::xcd_run(blockIdx.x, gridDim.x), np, nq, tp, tq);
+  const int p0 = tp * G::kBP, q0 = tq * G::kBQ;
+  if (q0 >= *count) return;
+  G tile;
+  tile.run(w, h, p0, q0, 0, c / gemm::kStep, smem);
+  __syncthreads();
+  const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
+  const int left = w.rows - p0 - G::wave_p0() - 4 * g;  // of this lane's first row on
+  float* maxima = reinterpret_cast<float*>(smem);
+  float* sums = maxima + G::kWP * G::kBQ;
+  const int wp = G::wave() / G::kWQ;
+#pragma unroll
+  for (int j = 0; j < G::TQ; ++j) {
+    float top = -__builtin_inff();
+#pragma unroll
+    for (int i = 0; i < G::TP; ++i) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        tile.acc[i][j][r] = 16 * i + r < left ? tile.acc[i][j][r] * scale : -__builtin_inff();
+        top = fmaxf(top, tile.acc[i][j][r]);
+      }
+    }
+    top = fmaxf(top, __shfl_xor(top, 16, 64));
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    // -inf everywhere (columns beyond the vocabulary): a sum of 0, not NaN.
+    const float from = top == -__builtin_inff() ? 0.0f : top;
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < G::TP; ++i) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) sum += __builtin_amdgcn_exp2f(tile.acc[i][j][r] - from);
+    }
+    sum += __shfl_xor(sum, 16, 64);
+    sum += __shfl_xor(sum, 32, 64);
+    if (g == 0) {
+      const int q = G::wave_q0() + 16 * j + n;
+      maxima[wp * G::kBQ + q] = top;
+      sums[wp * G::kBQ + q] = sum;
+    }
+  }
+  __syncthreads();
+  for (int q = threadIdx.x; q < G::kBQ; q += gemm::kThreads) {
+    float top = maxima[q];
+#pragma unroll
+    for (int x = 1; x < G::kWP; ++x) top = fmaxf(top, maxima[x * G::kBQ + q]);
+    float sum = 0.0f;
+#pragma unroll
+    for (int x = 0; x < G::kWP; ++x) {
+      const float s = sums[x * G::kBQ + q];
+      if (s != 0.0f) sum += s * __builtin_amdgcn_exp2f(maxima[x * G::kBQ + q] - top);
+    }
+    part[static_cast<int64_t>(tp) * pad + q0 + q] = make_float2(top, sum);
+  }
+}
+
+// D[v][m] of a piece of the vocabulary: dz[m][v] = coef_m (2^(s z log2 e -
+// lse2_m)), zero for rows and columns that are not there.
+template <typename G, typename T>
+__global__ __launch_bounds__(gemm::kThreads, 2) void softmax_grad_kernel(
+    Operand w, Operand h, const int32_t* __restrict__ count, int32_t c, int32_t np, int32_t nq,
+    float scale, const float* __restrict__ lse2, const float* __restrict__ coef,
+    uint16_t* __restrict__ dz, int64_t ld) {
+  __shared__ __attribute__((aligned(1024))) char smem[G::kLdsBytes];
+  int tp, tq;
+  gemm::tile_of(gemm::xcd_run(blockIdx.x, gridDim.x), np, nq, tp, tq);
+  const int p0 = tp * G::kBP, q0 = tq * G::kBQ;
+  const int rows = *count;
+  if (q0 >= round_up(rows, kRowPad)) return;
+  G tile;
+  tile.run(w, h, p0, q0, 0, c / gemm::kStep, smem);
+  const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
+  const int left = w.rows - p0 - G::wave_p0() - 4 * g;
+#pragma unroll
+  for (int j = 0; j < G::TQ; ++j) {
+    const int m = q0 + G::wave_q0() + 16 * j + n;
+    const bool row = m < rows;
+    const float from = row ? lse2[m] : 0.0f;
+    const float co = row ? coef[m] : 0.0f;
+    uint16_t* to = dz + static_cast<int64_t>(m) * ld + p0 + G::wave_p0() + 4 * g;
+#pragma unroll
+    for (int i = 0; i < G::TP; ++i) {
+      float x[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float e = co * __builtin_amdgcn_exp2f(fmaf(tile.acc[i][j][r], scale, -from));
+        x[r] = row && 16 * i + r < left ? e : 0.0f;
+      }
+      *reinterpret_cast<uint2*>(to + 16 * i) =
+          make_uint2(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]));
+    }
+  }
+}
+
+// The entries of dz that have a target: coef (p - b) in fp32 from the fp32
+// logit, over what the product's epilogue wrote. A thread an entry; equal
+// tokens of a row write the same value.
+template <typename T>
+__global__ __launch_bounds__(256) void target_grad_kernel(int32_t k, int32_t vocab0,
+                                                          int32_t columns, float scale,
+                                                          const float* __restrict__ coef,
+                                                          uint16_t* __restrict__ dz, int64_t ld,
+                                                          Saved s) {
+  const int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t m = e / k;
+  if (m >= *s.count) return;
+  const int64_t at = static_cast<int64_t>(s.row[m]) * k + (e - m * k);
+  const int32_t v = s.index[at] - vocab0;
+  if (s.index[at] < 0 || v < 0 || v >= columns) return;
+  const float p = __builtin_amdgcn_exp2f(fmaf(s.logit[e], scale, -s.lse2[m]));
+  dz[m * ld + v] = from_f32<T>(coef[m] * (p - s.target[at]));
+}
+
+// D[c][m] = sum over this split's vocabulary of W[v][c] dz[m][v], to slab
+// [m][c] (fp32).
+template <typename G, typename T>
+__global__ __launch_bounds__(gemm::kThreads, 2) void hidden_grad_kernel(
+    Operand w, Operand dz, const int32_t* __restrict__ count, int32_t steps, int32_t split_steps,
+    int32_t np, int32_t nq, float* __restrict__ slabs, int64_t slab) {
+  __shared__ __attribute__((aligned(1024))) char smem[G::kLdsBytes];
+  int tp, tq;
+  gemm::tile_of(gemm::xcd_run(blockIdx.x, gridDim.x), np, nq, tp, tq);
+  const int p0 = tp * G::kBP, q0 = tq * G::kBQ;
+  const int rows = *count;
+  if (q0 >= rows) return;
+  const int first = blockIdx.y * split_steps;
+  const int mine = steps - first < split_steps ? steps - first : split_steps;
+  G tile;
+  tile.run(w, dz, p0, q0, first * gemm::kStep, mine, smem);
+  const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
+  float* out = slabs + blockIdx.y * slab;
+#pragma unroll
+  for (int j = 0; j < G::TQ; ++j) {
+    const int m = q0 + G::wave_q0() + 16 * j + n;
+    if (m >= rows) continue;
+#pragma unroll
+    for (int i = 0; i < G::TP; ++i) {
+      const int c = p0 + G::wave_p0() + 16 * i + 4 * g;
+      if (c < w.cols) {
+        *reinterpret_cast<f32x4*>(out + static_cast<int64_t>(m) * w.cols + c) = tile.acc[i][j];
+      }
+    }
+  }
+}
+
+// dh[i][c] = scale x sum of the slabs of row place[i], in order; zeros for
+// rows that took no part.
+template <typename T>
+__global__ __launch_bounds__(256) void hidden_grad_rows_kernel(
+    const float* __restrict__ slabs, int64_t slab, int32_t count, int32_t c, int64_t n,
+    const float* __restrict__ scale, const int32_t* __restrict__ place,
+    uint16_t* __restrict__ dh) {
+  const int64_t quads = n * (c / 4);
+  const float by = *scale;
+  for (int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; e < quads;
+       e += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t i = e / (c / 4);
+    const int64_t x = (e - i * (c / 4)) * 4;
+    const int32_t m = place[i];
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    if (m >= 0) {
+      for (int s = 0; s < count; ++s) {
+        sum += *reinterpret_cast<const f32x4*>(slabs + s * slab + static_cast<int64_t>(m) * c + x);
+      }
+      sum *= by;
+    }
+    *reinterpret_cast<uint2*>(dh + i * c + x) =
+        make_uint2(pack2<T>(sum[0], sum[1]), pack2<T>(sum[2], sum[3]));
+  }
+}
+
+// D[c][v] = sum_m h[m][c] dz[m][v]: dW of a piece of the vocabulary.
+template <typename G, typename T>
+__global__ __launch_bounds__(gemm::kThreads, 2) void weight_grad_kernel(
+    Operand h, Operand dz, const int32_t* __restrict__ count, int32_t columns, int32_t np,
+    int32_t nq, const float* __restrict__ scale, uint16_t* __restrict__ dw) {
+  __shared__ __attribute__((aligned(1024))) char smem[G::kLdsBytes];
+  int tp, tq;
+  gemm::tile_of(gemm::xcd_run(blockIdx.x, gridDim.x), np, nq, tp, tq);
+  const int p0 = tp * G::kBP, q0 = tq * G::kBQ;
+  const int steps = static_cast<int>(round_up(*count, gemm::kStep) / gemm::kStep);
+  G tile;
+  tile.run(h, dz, p0, q0, 0, steps, smem);
+  const float by = *scale;
+  const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
+#pragma unroll
+  for (int j = 0; j < G::TQ; ++j) {
+    const int v = q0 + G::wave_q0() + 16 * j + n;
+    if (v >= columns) continue;
+#pragma unroll
+    for (int i = 0; i < G::TP; ++i) {
+      const int c = p0 + G::wave_p0() + 16 * i + 4 * g;
+      if (c < h.cols) {
+        const f32x4 x = tile.acc[i][j] * by;
+        *reinterpret_cast<uint2*>(dw + static_cast<int64_t>(v) * h.cols + c) =
+            make_uint2(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]));
+      }
+    }
+  }
+}
+
+// -------------------------------------------------------- row reductions
+// (maximum, sum of 2^(x - maximum)) of two sets; a sum of 0 is an empty set.
+__device__ __forceinline__ float2 joined(float2 a, float2 b) {
+  if (b.y == 0.0f) return a;
+  if (a.y == 0.0f) return b;
+  const float top = fmaxf(a.x, b.x);
+  return make_float2(top, a.y * __builtin_amdgcn_exp2f(a.x - top) +
+                              b.y * __builtin_amdgcn_exp2f(b.x - top));
+}
+
+// A workgroup takes 32 rows, 8 threads a row: joins the tiles' maxima and
+// sums to lse2[m], and the row's loss. row_loss (by i) or partial (by m).
+__global__ __launch_bounds__(256) void join_tiles_kernel(const float2* __restrict__ part,
+                                                         int32_t tiles, int64_t pad,
+                                                         const float* __restrict__ target_term,
+                                                         float temperature2, float* row_loss,
+                                                         float* partial, Saved s) {
+  __shared__ float2 shared[8][32];
+  const int q = threadIdx.x & 31, slice = threadIdx.x >> 5;
+  const int m = blockIdx.x * 32 + q;
+  const int count = *s.count;
+  if (static_cast<int>(blockIdx.x) * 32 >= count) return;
+  float2 all = make_float2(-__builtin_inff(), 0.0f);
+  if (m < count) {
+    for (int t = slice; t < tiles; t += 8) all = joined(all, part[t * pad + m]);
+  }
+  shared[slice][q] = all;
+  __syncthreads();
+  if (slice != 0 || m >= count) return;
+#pragma unroll
+  for (int t = 1; t < 8; ++t) all = joined(all, shared[t][q]);
+  const float lse2 = all.x + __builtin_amdgcn_logf(all.y);
+  const float term = target_term[m];
+  // A target out of range makes its row NaN in the backward too.
+  s.lse2[m] = term == term ? lse2 : term;
+  const float loss = temperature2 * (lse2 * kLn2 + term);
+  if (row_loss) row_loss[s.row[m]] = loss;
+  if (partial) partial[m] = loss;
+}
+
+// Loss 0 for rows that take no part (reduction none).
+__global__ __launch_bounds__(256) void zero_loss_kernel(int32_t n,
+                                                        const int32_t* __restrict__ place,
+                                                        float* __restrict__ row_loss) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i < n && place[i] < 0) row_loss[i] = 0.0f;
+}
+
+// Sum over one workgroup of 1024, in a fixed order.
+__device__ __forceinline__ float block_sum(float x, float* waves) {
+  x = wave_sum(x);
+  if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = x;
+  __syncthreads();
+  float sum = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kScanThreads / 64; ++w) sum += waves[w];
+  return sum;
+}
+
+__global__ __launch_bounds__(kScanThreads) void sum_losses_kernel(
+    const float* __restrict__ partial, const int32_t* __restrict__ count, bool mean,
+    float* __restrict__ loss) {
+  __shared__ float waves[kScanThreads / 64];
+  const int n = *count;
+  float sum = 0.0f;
+  for (int m = threadIdx.x; m < n; m += kScanThreads) sum += partial[m];
+  sum = block_sum(sum, waves);
+  if (threadIdx.x == 0) *loss = n == 0 ? 0.0f : mean ? sum / static_cast<float>(n) : sum;
+}
+
+// coef[m] multiplies (p - b) of row m in dz, *scale the finished gradients;
+// together they are the row's upstream weight x T (/ count for a mean).
+// One weight for all rows: all of it is in the scale, so that dz is p - b
+// itself, whose target entries (near -1 where p is small) round to 16 bits with
+// little error and not all with the same one. Weights of their own: in coef,
+// divided by a power of two near the largest one.
+// 2^up on top of that keeps fp16's small entries normal numbers: |coef (p - b)|
+// is at most 2^14, and 2^-28 of that is the smallest one.
+__global__ __launch_bounds__(kScanThreads) void row_coefficients_kernel(
+    const float* __restrict__ upstream, bool per_row, bool mean, float temperature, int up,
+    float* __restrict__ coef, float* __restrict__ scale, Saved s) {
+  __shared__ float waves[kScanThreads / 64];
+  const int n = *s.count;
+  const float by = mean ? temperature / static_cast<float>(n > 0 ? n : 1) : temperature;
+  const float lift = ldexpf(1.0f, up);
+  if (!per_row) {
+    for (int m = threadIdx.x; m < n; m += kScanThreads) coef[m] = lift;
+    if (threadIdx.x == 0) *scale = *upstream * by / lift;
+    return;
+  }
+  float top = 0.0f;
+  for (int m = threadIdx.x; m < n; m += kScanThreads) {
+    top = fmaxf(top, fabsf(upstream[s.row[m]] * by));
+  }
+  top = wave_max(top);
+  if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kScanThreads / 64; ++w) top = fmaxf(top, waves[w]);
+  const bool usable = top > 1e-30f && top < 1e30f;
+  const int exponent = usable ? static_cast<int>(ceilf(__builtin_amdgcn_logf(top))) : 0;
+  const float divide = ldexpf(1.0f, up - exponent);
+  for (int m = threadIdx.x; m < n; m += kScanThreads) {
+    coef[m] = upstream[s.row[m]] * by * divide;
+  }
+  if (threadIdx.x == 0) *scale = ldexpf(1.0f, exponent - up);
+}
+
+// ---------------------------------------------------------------- launches
+// Bytes of one piece's dz: large enough that a piece's three products fill the
+// GPU for any row count, small beside the logits of a long batch.
+constexpr int64_t kPieceBytes = int64_t{512} << 20;
+constexpr int kCus = 256;
+
+struct Pieces {
+  int32_t columns;  // a multiple of kVocabTile
+  int32_t count;
+  int32_t splits;   // of a piece's columns in dz W
+};
+
+bool few_rows(int64_t n) { return n <= kFewRows; }
+
+int64_t row_tiles(int64_t n) { return few_rows(n) ? 1 : round_up(n, 256) / 256; }
+
+// dz W has (C / 256) x (rows / 256) tiles, often fewer than CUs, over a long k:
+// split k so that the rounds of tiles are full. Work of a choice, in steps of
+// 64 k a CU: rounds x steps a split, plus about 6 steps for each slab written.
+int32_t hidden_grad_splits(int64_t tiles, int64_t steps) {
+  int32_t best = 1;
+  int64_t least = INT64_MAX;
+  for (int32_t s = 1; s <= 16 && (s == 1 || steps / s >= 8); ++s) {
+    const int64_t each = (steps + s - 1) / s;
+    const int64_t cost = (tiles * s + kCus - 1) / kCus * (each + 6);
+    if (cost < least) {
+      least = cost;
+      best = s;
+    }
+  }
+  return best;
+}
+
+Pieces pieces_of(int64_t n, int64_t c, int64_t vocab) {
+  const int64_t pad = round_up(n, kRowPad);
+  const int64_t all = round_up(vocab, kVocabTile);
+  int64_t columns = kPieceBytes / (pad * 2) / kVocabTile * kVocabTile;
+  columns = std::min(std::max<int64_t>(columns, kVocabTile), all);
+  Pieces p;
+  p.count = static_cast<int32_t>((all + columns - 1) / columns);
+  p.columns = static_cast<int32_t>(round_up((all + p.count - 1) / p.count, kVocabTile));
+  p.count = static_cast<int32_t>((all + p.columns - 1) / p.columns);
+  p.splits = hidden_grad_splits(round_up(c, 256) / 256 * row_tiles(n),
+                                p.columns / gemm::kStep);
+  return p;
+}
+
+struct ForwardWork {
+  float2* part;
+  float* target_term;
+  float* partial;
+};
+
+ForwardWork forward_work(char* p, int64_t n, int64_t vocab, size_t* bytes) {
+  const int64_t pad = round_up(n, kRowPad);
+  Layout l;
+  const size_t part = l.take(round_up(vocab, kVocabTile) / kVocabTile * pad * 8);
+  const size_t term = l.take(pad * 4), partial = l.take(pad * 4);
+  *bytes = l.bytes;
+  return {reinterpret_cast<float2*>(p + part), reinterpret_cast<float*>(p + term),
+          reinterpret_cast<float*>(p + partial)};
+}
+
+struct BackwardWork {
+  float* coef;
+  float* scale;
+  uint16_t* dz;
+  float* slabs;
+};
+
+BackwardWork backward_work(char* p, int64_t n, int64_t c, const Pieces& pieces, bool hidden,
+                           size_t* bytes) {
+  const int64_t pad = round_up(n, kRowPad);
+  Layout l;
+  const size_t coef = l.take(pad * 4), scale = l.take(4), dz = l.take(pad * pieces.columns * 2);
+  const size_t slabs =
+      l.take(hidden ? static_cast<size_t>(pieces.count) * pieces.splits * n * c * 4 : 0);
+  *bytes = l.bytes;
+  return {reinterpret_cast<float*>(p + coef), reinterpret_cast<float*>(p + scale),
+          reinterpret_cast<uint16_t*>(p + dz), reinterpret_cast<float*>(p + slabs)};
+}
+
+struct Shape {
+  int64_t n;
+  int32_t c, vocab, k;
+};
+
+template <typename G, typename T>
+void launch_lse_tiles(const Shape& d, const void* weight, const Saved& s, const ForwardWork& w,
+                      float scale, hipStream_t stream) {
+  const int64_t pad = round_up(d.n, kRowPad);
+  const int np = static_cast<int>(round_up(d.vocab, G::kBP) / G::kBP);
+  const int nq = static_cast<int>(row_tiles(d.n));
+  const Operand a{static_cast<const uint16_t*>(weight), d.c, d.vocab, d.c};
+  const Operand b{s.hidden, d.c, static_cast<int32_t>(pad), d.c};
+  hipLaunchKernelGGL((lse_tiles_kernel<G, T>), dim3(np * nq), dim3(gemm::kThreads), 0, stream, a,
+                     b, s.count, d.c, np, nq, scale, w.part, pad);
+}
+
+template <typename T>
+int run_forward(const Shape& d, const void* hidden, const void* weight, float temperature,
+                bool mean, bool per_row, float* loss, const Saved& s, const ForwardWork& w,
+                hipStream_t stream) {
+  const int64_t pad = round_up(d.n, kRowPad);
+  const float scale = kLog2E / temperature;
+  const int n = static_cast<int>(d.n);
+  hipLaunchKernelGGL(number_rows_kernel, dim3(1), dim3(kScanThreads), 0, stream, n, s);
+  hipLaunchKernelGGL((gather_rows_kernel<T>), dim3(static_cast<unsigned>(pad)), dim3(256), 0,
+                     stream, static_cast<const uint16_t*>(hidden),
+                     static_cast<const uint16_t*>(weight), d.c, d.k, d.vocab, 1.0f / temperature,
+                     w.target_term, s);
+  if (few_rows(d.n)) {
+    launch_lse_tiles<FewRowsTile<T, Major::kK, Major::kK>, T>(d, weight, s, w, scale, stream);
+  } else {
+    launch_lse_tiles<LargeTile<T, Major::kK, Major::kK>, T>(d, weight, s, w, scale, stream);
+  }
+  const int tiles = static_cast<int>(round_up(d.vocab, kVocabTile) / kVocabTile);
+  hipLaunchKernelGGL(join_tiles_kernel, dim3((n + 31) / 32), dim3(256), 0, stream, w.part, tiles,
+                     pad, w.target_term, temperature * temperature, per_row ? loss : nullptr,
+                     per_row ? nullptr : w.partial, s);
+  if (per_row) {
+    hipLaunchKernelGGL(zero_loss_kernel, dim3((n + 255) / 256), dim3(256), 0, stream, n, s.place,
+                       loss);
+  } else {
+    hipLaunchKernelGGL(sum_losses_kernel, dim3(1), dim3(kScanThreads), 0, stream, w.partial,
+                       s.count, mean, loss);
+  }
+  return check_launch("linear loss forward");
+}
+
+template <typename T, template <typename, Major, Major> class G>
+void launch_piece(const Shape& d, const Pieces& pieces, int piece, const uint16_t* weight,
+                  float scale, uint16_t* dh, uint16_t* dw, const Saved& s, const BackwardWork& w,
+                  hipStream_t stream) {
+  using Logits = G<T, Major::kK, Major::kK>;
+  using Hidden = G<T, Major::kX, Major::kK>;
+  using Weight = LargeTile<T, Major::kX, Major::kX>;
+  const int64_t pad = round_up(d.n, kRowPad);
+  const int nq = static_cast<int>(row_tiles(d.n));
+  const int first = piece * pieces.columns;
+  const int columns = std::min(pieces.columns, d.vocab - first);
+  const int np = static_cast<int>(round_up(columns, kVocabTile) / kVocabTile);
+  const int nc = static_cast<int>(round_up(d.c, 256) / 256);
+  const int64_t ld = pieces.columns;
+  const uint16_t* from = weight + static_cast<int64_t>(first) * d.c;
+  const Operand wp{from, d.c, columns, d.c};
+  const Operand h{s.hidden, d.c, static_cast<int32_t>(pad), d.c};
+  // Rows of dz that hold something: whole tiles.
+  const Operand dz{w.dz, ld, static_cast<int32_t>(std::min<int64_t>(pad, nq * Logits::kBQ)),
+                   np * kVocabTile};
+  hipLaunchKernelGGL((softmax_grad_kernel<Logits, T>), dim3(np * nq), dim3(gemm::kThreads), 0,
+                     stream, wp, h, s.count, d.c, np, nq, scale, s.lse2, w.coef, w.dz, ld);
+  const int64_t entries = d.n * d.k;
+  hipLaunchKernelGGL((target_grad_kernel<T>), dim3(static_cast<unsigned>((entries + 255) / 256)),
+                     dim3(256), 0, stream, d.k, first, columns, scale, w.coef, w.dz, ld, s);
+  if (dh != nullptr) {
+    const int steps = static_cast<int>(round_up(columns, gemm::kStep) / gemm::kStep);
+    const int each = (pieces.columns / gemm::kStep + pieces.splits - 1) / pieces.splits;
+    const int64_t slab = d.n * d.c;
+    hipLaunchKernelGGL((hidden_grad_kernel<Hidden, T>),
+                       dim3(nc * nq, static_cast<unsigned>(pieces.splits)), dim3(gemm::kThreads),
+                       0, stream, wp, dz, s.count, steps, each, nc, nq,
+                       w.slabs + piece * pieces.splits * slab, slab);
+  }
+  if (dw != nullptr) {
+    hipLaunchKernelGGL((weight_grad_kernel<Weight, T>), dim3(nc * np), dim3(gemm::kThreads), 0,
+                       stream, h, dz, s.count, columns, nc, np, w.scale,
+                       dw + static_cast<int64_t>(first) * d.c);
+  }
+}
+
+template <typename T>
+int run_backward(const Shape& d, const void* weight, const float* upstream, bool per_row,
+                 bool mean, float temperature, void* dh, void* dw, const Saved& s,
+                 const Pieces& pieces, const BackwardWork& w, hipStream_t stream) {
+  const float scale = kLog2E / temperature;
+  hipLaunchKernelGGL(row_coefficients_kernel, dim3(1), dim3(kScanThreads), 0, stream, upstream,
+                     per_row, mean, temperature, __is_same(T, F16) ? 14 : 0, w.coef, w.scale, s);
+  for (int p = 0; p < pieces.count; ++p) {
+    if (few_rows(d.n)) {
+      launch_piece<T, FewRowsTile>(d, pieces, p, static_cast<const uint16_t*>(weight), scale,
+                                   static_cast<uint16_t*>(dh), static_cast<uint16_t*>(dw), s, w,
+                                   stream);
+    } else {
+      launch_piece<T, LargeTile>(d, pieces, p, static_cast<const uint16_t*>(weight), scale,
+                                 static_cast<uint16_t*>(dh), static_cast<uint16_t*>(dw), s, w,
+                                 stream);
+    }
+  }
+  if (dh != nullptr) {
+    const int64_t quads = d.n * (d.c / 4);
+    const int64_t blocks = std::min<int64_t>((quads + 255) / 256, 8192);
+    hipLaunchKernelGGL((hidden_grad_rows_kernel<T>), dim3(static_cast<unsigned>(blocks)),
+                       dim3(256), 0, stream, w.slabs, d.n * d.c, pieces.count * pieces.splits,
+                       d.c, d.n, w.scale, s.place, static_cast<uint16_t*>(dh));
+  }
+  return check_launch("linear loss backward");
+}
+
+int check_shape(const char* what, int io_dtype, int64_t n, int64_t c, int64_t vocab, int64_t k) {
+  if (io_dtype != FRWKV_DTYPE_F16 && io_dtype != FRWKV_DTYPE_BF16) {
+    return set_error(FRWKV_ERR_UNSUPPORTED, "%s: io dtype must be float16 or bfloat16", what);
+  }
+  if (n <= 0 || n > (int64_t{1} << 28)) {
+    return set_error(FRWKV_ERR_INVALID_ARGUMENT, "%s: rows must be in [1, 2^28], got %lld", what,
+                     static_cast<long long>(n));
+  }
+  if (c <= 0 || c % gemm::kStep != 0 || c > 65536) {
+    return set_error(FRWKV_ERR_UNSUPPORTED,
+                     "%s: channels must be a multiple of 64, at most 65536, got %lld", what,
+                     static_cast<long long>(c));
+  }
+  if (vocab <= 0 || vocab > (int64_t{1} << 28)) {
+    return set_error(FRWKV_ERR_INVALID_ARGUMENT, "%s: vocabulary must be in [1, 2^28], got %lld",
+                     what, static_cast<long long>(vocab));
+  }
+  if (k <= 0 || k > 1024) {
+    return set_error(FRWKV_ERR_UNSUPPORTED,
+                     "%s: targets of a row must be in [1, 1024], got %lld", what,
+                     static_cast<long long>(k));
+  }
+  const int64_t tiles = round_up(vocab, kVocabTile) / kVocabTile * row_tiles(n);
+  if (tiles > (int64_t{1} << 22) || n * k > (int64_t{1} << 38)) {
+    return set_error(FRWKV_ERR_UNSUPPORTED, "%s: rows x vocabulary too large for one call", what);
+  }
+  return FRWKV_OK;
+}
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+int check_memory(const char* what, const char* name, const void* p, size_t have, size_t need) {
+  if (p == nullptr || have < need) {
+    return set_error(FRWKV_ERR_INVALID_ARGUMENT, "%s: %s of %zu bytes given, %zu needed", what,
+                     name, p == nullptr ? size_t{0} : have, need);
+  }
+  if (reinterpret_cast<uintptr_t>(p) % 256 != 0) {
+    return set_error(FRWKV_ERR_INVALID_ARGUMENT, "%s: %s must be 256-byte aligned", what, name);
+  }
+  return FRWKV_OK;
+}
+
+int check_reduction(const char* what, int reduction) {
+  if (reduction != FRWKV_REDUCE_NONE && reduction != FRWKV_REDUCE_MEAN &&
+      reduction != FRWKV_REDUCE_SUM) {
+    return set_error(FRWKV_ERR_INVALID_ARGUMENT, "%s: unknown reduction %d", what, reduction);
+  }
+  return FRWKV_OK;
+}
+
+int check_temperature(const char* what, float t) {
+  if (!(t > 0.0f) || t > 1e30f || t < 1e-30f) {
+    return set_error(FRWKV_ERR_INVALID_ARGUMENT, "%s: temperature must be positive and finite",
+                     what);
+  }
+  return FRWKV_OK;
+}
+
+int forward(const char* what, int io_dtype, const Shape& d, const void* hidden,
+            const void* weight, float temperature, int reduction, float* loss, const Saved& s,
+            void* workspace, hipStream_t stream) {
+  size_t need = 0;
+  const ForwardWork w = forward_work(static_cast<char*>(workspace), d.n, d.vocab, &need);
+  const bool mean = reduction == FRWKV_REDUCE_MEAN, per_row = reduction == FRWKV_REDUCE_NONE;
+  (void)what;
+  return io_dtype == FRWKV_DTYPE_F16
+             ? run_forward<F16>(d, hidden, weight, temperature, mean, per_row, loss, s, w, stream)
+             : run_forward<Bf16>(d, hidden, weight, temperature, mean, per_row, loss, s, w,
+                                 stream);
+}
+
+// The checks that both forwards share, and the layout of what they leave.
+int begin_forward(const char* what, int io_dtype, int64_t n, int64_t c, int64_t vocab, int64_t k,
+                  const void* hidden, const void* weight, int reduction, const float* loss,
+                  void* saved, size_t saved_bytes, void* workspace, size_t workspace_bytes,
+                  Saved* s) {
+  if (!hidden || !weight || !loss) {
+    return set_error(FRWKV_ERR_INVALID_ARGUMENT, "%s: null pointer argument", what);
+  }
+  int rc = check_shape(what, io_dtype, n, c, vocab, k);
+  if (rc == FRWKV_OK) rc = check_reduction(what, reduction);
+  if (rc != FRWKV_OK) return rc;
+  if (!aligned16(hidden) || !aligned16(weight)) {
+    return set_error(FRWKV_ERR_INVALID_ARGUMENT,
+                     "%s: hidden and weight must be 16-byte aligned", what);
+  }
+  size_t need = 0;
+  *s = saved_of(static_cast<char*>(saved), n, c, k, &need);
+  rc = check_memory(what, "saved", saved, saved_bytes, need);
+  if (rc != FRWKV_OK) return rc;
+  (void)forward_work(nullptr, n, vocab, &need);
+  return check_memory(what, "workspace", workspace, workspace_bytes, need);
+}
+
+}  // namespace
+}  // namespace frwkv
+
+extern "C" {
+
+size_t frwkv_linear_loss_saved_bytes(int64_t rows, int64_t channels, int64_t top) {
+  if (rows <= 0 || channels <= 0 || top <= 0) return 0;
+  size_t bytes = 0;
+  (void)frwkv::saved_of(nullptr, rows, channels, top, &bytes);
+  return bytes;
+}
+
+size_t frwkv_linear_loss_forward_workspace_bytes(int64_t rows, int64_t vocab) {
+  if (rows <= 0 || vocab <= 0) return 0;
+  size_t bytes = 0;
+  (void)frwkv::forward_work(nullptr, rows, vocab, &bytes);
+  return bytes;
+}
+
+size_t frwkv_linear_loss_backward_workspace_bytes(int64_t rows, int64_t channels, int64_t vocab,
+                                                  int want_grad_hidden) {
+  if (rows <= 0 || channels <= 0 || vocab <= 0) return 0;
+  size_t bytes = 0;
+  (void)frwkv::backward_work(nullptr, rows, channels, frwkv::pieces_of(rows, channels, vocab),
+                             want_grad_hidden != 0, &bytes);
+  return bytes;
+}
+
+int frwkv_linear_cross_entropy_forward(int io_dtype, int64_t rows, int64_t channels,
+                                       int64_t vocab, const void* hidden, const void* weight,
+                                       int target_bytes, const void* targets,
+                                       int64_t ignore_index, int reduction, float* loss,
+                                       void* saved, size_t saved_bytes, void* workspace,
+                                       size_t workspace_bytes, void* stream) {
+  using namespace frwkv;
+  const char* what = "frwkv_linear_cross_entropy_forward";
+  Saved s;
+  const int rc = begin_forward(what, io_dtype, rows, channels, vocab, 1, hidden, weight,
+                               reduction, loss, saved, saved_bytes, workspace, workspace_bytes,
+                               &s);
+  if (rc != FRWKV_OK) return rc;
+  if (!targets || (target_bytes != 4 && target_bytes != 8)) {
+    return set_error(FRWKV_ERR_INVALID_ARGUMENT, "%s: targets must be int32 or int64", what);
+  }
+  const hipStream_t q = static_cast<hipStream_t>(stream);
+  const int32_t n = static_cast<int32_t>(rows), v = static_cast<int32_t>(vocab);
+  const dim3 grid((n + 255) / 256);
+  if (target_bytes == 8) {
+    hipLaunchKernelGGL((label_targets_kernel<int64_t>), grid, dim3(256), 0, q,
+                       static_cast<const int64_t*>(targets), ignore_index, n, v, s);
+  } else {
+    hipLaunchKernelGGL((label_targets_kernel<int32_t>), grid, dim3(256), 0, q,
+                       static_cast<const int32_t*>(targets), ignore_index, n, v, s);
+  }
+  return forward(what, io_dtype, Shape{rows, static_cast<int32_t>(channels), v, 1}, hidden,
+                 weight, 1.0f, reduction, loss, s, workspace, q);
+}
+
+int frwkv_linear_topk_distillation_forward(
+    int io_dtype, int64_t rows, int64_t channels, int64_t vocab, int64_t top, const void* hidden,
+    const void* weight, int teacher_dtype, const void* teacher_logits, int index_bytes,
+    const void* teacher_indices, float temperature, int reduction, float* loss, void* saved,
+    size_t saved_bytes, void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace frwkv;
+  const char* what = "frwkv_linear_topk_distillation_forward";
+  Saved s;
+  int rc = begin_forward(what, io_dtype, rows, channels, vocab, top, hidden, weight, reduction,
+                         loss, saved, saved_bytes, workspace, workspace_bytes, &s);
+  if (rc == FRWKV_OK) rc = check_temperature(what, temperature);
+  if (rc != FRWKV_OK) return rc;
+  if (!teacher_logits || (teacher_dtype != FRWKV_DTYPE_F32 && teacher_dtype != FRWKV_DTYPE_F16 &&
+                          teacher_dtype != FRWKV_DTYPE_BF16)) {
+    return set_error(FRWKV_ERR_INVALID_ARGUMENT,
+                     "%s: teacher_logits must be float32, float16 or bfloat16", what);
+  }
+  if (!teacher_indices || (index_bytes != 4 && index_bytes != 8)) {
+    return set_error(FRWKV_ERR_INVALID_ARGUMENT, "%s: teacher_indices must be int32 or int64",
+                     what);
+  }
+  const hipStream_t q = static_cast<hipStream_t>(stream);
+  const int32_t n = static_cast<int32_t>(rows), k = static_cast<int32_t>(top);
+  const int32_t v = static_cast<int32_t>(vocab);
+  const auto launch = [&](auto io, auto index) {
+    using T = decltype(io);
+    using I = decltype(index);
+    using S = typename IoTraits<T>::storage;
+    hipLaunchKernelGGL((teacher_targets_kernel<T, I>), dim3((n + 3) / 4), dim3(256),
+                       static_cast<size_t>(k) * 32, q, static_cast<const S*>(teacher_logits),
+                       static_cast<const I*>(teacher_indices), n, k, v, 1.0f / temperature, s);
+  };
+  const auto with_index = [&](auto io) {
+    if (index_bytes == 8) {
+      launch(io, int64_t{});
+    } else {
+      launch(io, int32_t{});
+    }
+  };
+  if (teacher_dtype == FRWKV_DTYPE_F32) {
+    with_index(float{});
+  } else if (teacher_dtype == FRWKV_DTYPE_F16) {
+    with_index(F16{});
+  } else {
+    with_index(Bf16{});
+  }
+  return forward(what, io_dtype, Shape{rows, static_cast<int32_t>(channels), v, k}, hidden,
+                 weight, temperature, reduction, loss, s, workspace, q);
+}
+
+int frwkv_linear_loss_backward(int io_dtype, int64_t rows, int64_t channels, int64_t vocab,
+                               int64_t top, const void* weight, float temperature, int reduction,
+                               const float* grad_loss, const void* saved, size_t saved_bytes,
+                               void* grad_hidden, void* grad_weight, void* workspace,
+                               size_t workspace_bytes, void* stream) {
+  using namespace frwkv;
+  const char* what = "frwkv_linear_loss_backward";
+  if (!weight || !grad_loss) {
+    return set_error(FRWKV_ERR_INVALID_ARGUMENT, "%s: null pointer argument", what);
+  }
+  int rc = check_shape(what, io_dtype, rows, channels, vocab, top);
+  if (rc == FRWKV_OK) rc = check_reduction(what, reduction);
+  if (rc == FRWKV_OK) rc = check_temperature(what, temperature);
+  if (rc != FRWKV_OK) return rc;
+  if (!aligned16(weight) || !aligned16(grad_hidden) || !aligned16(grad_weight)) {
+    return set_error(FRWKV_ERR_INVALID_ARGUMENT,
+                     "%s: weight and gradients must be 16-byte aligned", what);
+  }
+  size_t need = 0;
+  // The forward's buffer is only read here.
+  const Saved s = saved_of(const_cast<char*>(static_cast<const char*>(saved)), rows, channels,
+                           top, &need);
+  rc = check_memory(what, "saved", saved, saved_bytes, need);
+  if (rc != FRWKV_OK) return rc;
+  const Pieces pieces = pieces_of(rows, channels, vocab);
+  const BackwardWork w = backward_work(static_cast<char*>(workspace), rows, channels, pieces,
+                                       grad_hidden != nullptr, &need);
+  rc = check_memory(what, "workspace", workspace, workspace_bytes, need);
+  if (rc != FRWKV_OK) return rc;
+  if (!grad_hidden && !grad_weight) return FRWKV_OK;
+  const bool mean = reduction == FRWKV_REDUCE_MEAN, per_row = reduction == FRWKV_REDUCE_NONE;
+  const Shape d{rows, static_cast<int32_t>(channels), static_cast<int32_t>(vocab),
+                static_cast<int32_t>(top)};
+  const hipStream_t q = static_cast<hipStream_t>(stream);
+  return io_dtype == FRWKV_DTYPE_F16
+             ? run_backward<F16>(d, weight, grad_loss, per_row, mean, temperature, grad_hidden,
+                                 grad_weight, s, pieces, w, q)
+             : run_backward<Bf16>(d, weight, grad_loss, per_row, mean, temperature, grad_hidden,
+                                  grad_weight, s, pieces, w, q);
+}
+
+}  // extern "C"

@@ -50,6 +50,12 @@ enum frwkv_dtype {
   FRWKV_DTYPE_BF16 = 2
 };
 
+enum frwkv_reduction {
+  FRWKV_REDUCE_NONE = 0,
+  FRWKV_REDUCE_MEAN = 1,
+  FRWKV_REDUCE_SUM = 2
+};
+
 enum frwkv_decay_mode {
   FRWKV_DECAY_LOGITS = 0,
   FRWKV_DECAY_RAW_W = 1
@@ -614,6 +620,87 @@ int frwkv_recurrent_tmix_fused_forward(
     const void* k, const void* v, const void* a12, const void* g, const void* k_k,
     const void* a0, const void* k_a, const void* r_k, const void* ln_weight,
     const void* ln_bias, void* output, float scale, void* stream);
+
+/*
+ * Layer norm of [rows, channels] (io dtype float32, float16 or bfloat16, channels
+ * 1..16384), with the residual add in front of it: s = x + residual rounded to
+ * the io dtype and written to stream_out (both NULL: s = x),
+ * y = (s - mean) / sqrt(var + eps) weight + bias, biased variance over the
+ * channels, fp32 inside. mean, rstd [rows] fp32 are what the backward reads
+ * (both NULL: not written). Rows of 16-byte aligned buffers with channels a
+ * multiple of 8 take 16-byte loads, others elementwise ones. No counterpart in
+ * the reference.
+ */
+int frwkv_layer_norm_forward(int io_dtype, int64_t rows, int64_t channels, const void* x,
+                             const void* residual, const void* weight, const void* bias,
+                             float eps, void* y, void* stream_out, float* mean, float* rstd,
+                             void* stream);
+
+/* Workspace bytes of frwkv_layer_norm_backward: 2 x channels fp32 for each of
+ * at most 512 workgroups. */
+size_t frwkv_layer_norm_backward_workspace_bytes(int64_t rows, int64_t channels);
+
+/*
+ * Backward of the above from normed (s: x, or stream_out where there was a
+ * residual), mean and rstd: grad_x (the residual's gradient is the same) with
+ * grad_stream added (NULL: none), grad_weight and grad_bias summed over rows in
+ * a fixed order. workspace: 16-byte aligned.
+ */
+int frwkv_layer_norm_backward(int io_dtype, int64_t rows, int64_t channels, const void* grad_y,
+                              const void* normed, const void* grad_stream, const void* weight,
+                              const float* mean, const float* rstd, void* grad_x,
+                              void* grad_weight, void* grad_bias, void* workspace,
+                              size_t workspace_bytes, void* stream);
+
+/*
+ * Losses of a head from its hidden rows, without the logits in memory:
+ * z = hidden [rows, channels] weight [vocab, channels]^T (io dtype float16 or
+ * bfloat16, channels a multiple of 64, fp32 sums).
+ *
+ * frwkv_linear_cross_entropy_forward: loss = logsumexp(z) - z[target] of rows
+ * whose target (int32 or int64, target_bytes 4 or 8) is not ignore_index.
+ * frwkv_linear_topk_distillation_forward: p = softmax(teacher_logits / T) over
+ * a row's present entries (index not negative, logit not -inf), q =
+ * softmax(z / T), loss = T^2 sum p (log p - log q). top at most 1024 entries a
+ * row; a token that occurs twice counts with the sum of its p.
+ *
+ * Rows without a target have loss 0 and count nowhere; what they hold is not
+ * read by the products. A target at or beyond vocab (for cross entropy: any
+ * out of range) makes its row's loss NaN. reduction: per row (loss fp32
+ * [rows]), or the mean over rows with a target (0 without one) or the sum
+ * (loss fp32 [1]).
+ *
+ * saved (256-byte aligned) is what frwkv_linear_loss_backward reads: the
+ * rows that take part, their log sum and target logits. temperature is 1 for
+ * cross entropy, top 1.
+ *
+ * frwkv_linear_loss_backward: grad_loss fp32 [1], or [rows] where reduction is
+ * FRWKV_REDUCE_NONE; grad_hidden [rows, channels] and grad_weight [vocab,
+ * channels] of the io dtype, either NULL where it is not wanted. It goes
+ * through the vocabulary in pieces whose logit gradients (16 bits) fit the
+ * workspace. All sums are in a fixed order. Both directions need at least one
+ * row. No counterpart in the reference.
+ */
+size_t frwkv_linear_loss_saved_bytes(int64_t rows, int64_t channels, int64_t top);
+size_t frwkv_linear_loss_forward_workspace_bytes(int64_t rows, int64_t vocab);
+size_t frwkv_linear_loss_backward_workspace_bytes(int64_t rows, int64_t channels, int64_t vocab,
+                                                  int want_grad_hidden);
+int frwkv_linear_cross_entropy_forward(int io_dtype, int64_t rows, int64_t channels,
+                                       int64_t vocab, const void* hidden, const void* weight,
+                                       int target_bytes, const void* targets,
+                                       int64_t ignore_index, int reduction, float* loss,
+                                       void* saved, size_t saved_bytes, void* workspace,
+                                       size_t workspace_bytes, void* stream);
+int frwkv_linear_topk_distillation_forward(
+    int io_dtype, int64_t rows, int64_t channels, int64_t vocab, int64_t top, const void* hidden,
+    const void* weight, int teacher_dtype, const void* teacher_logits, int index_bytes,
+    const void* teacher_indices, float temperature, int reduction, float* loss, void* saved,
+    size_t saved_bytes, void* workspace, size_t workspace_bytes, void* stream);
+int frwkv_linear_loss_backward(int io_dtype, int64_t rows, int64_t channels, int64_t vocab,
+                               int64_t top, const void* weight, float temperature, int reduction,
+                               const float* grad_loss, const void* saved, size_t saved_bytes,
+                               void* grad_hidden, void* grad_weight, void* workspace,
+                               size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
