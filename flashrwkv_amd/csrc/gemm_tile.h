@@ -29,6 +29,7 @@ namespace frwkv {
 namespace gemm {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef short i16x8 __attribute__((ext_vector_type(8)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -50,29 +51,28 @@ __device__ __forceinline__ f32x4 mfma(i16x8 a, i16x8 b, f32x4 c) {
   }
 }
 
-// One operand in memory. `rows` and `cols` bound what may be read: a k-major
-// operand has `rows` values of p / q, an x-major one `rows` values of k and
-// `cols` of p / q (a multiple of 8). Reads beyond a bound are turned to the
-// last row or to column 0; what they bring has to be multiplied by zeros or
+// One operand in memory: `rows` rows of `ld` elements (rows are p or q of a
+// k-major operand, k of an x-major one). Rows beyond the last read as zeros.
+// Reads of an x-major operand may go past a row's end into the next row: they
 // land in rows and columns of D that the caller drops.
 struct Operand {
   const uint16_t* data;
-  int64_t ld;  // elements between rows
+  int64_t ld;
   int32_t rows;
-  int32_t cols;
 };
 
-// 64 lanes x 16 bytes from per-lane addresses to LDS bytes [lds, lds + 1024).
-// The hardware adds lane * 16 to the address in m0, which is wave-uniform. In
-// asm because the compiler, unable to tell the stages apart, puts a wait for
-// the whole queue before every LDS read that follows the builtin.
-__device__ __forceinline__ void load_to_lds(const void* src, uint32_t lds) {
+// 64 lanes x 16 bytes from a buffer to LDS bytes [lds, lds + 1024): the hardware
+// adds lane * 16 to the address in m0, which is wave-uniform, and writes zeros
+// for lanes whose offset lies beyond the buffer. In asm because the compiler,
+// unable to tell the stages apart, puts a wait for the whole queue before every
+// LDS read that follows the builtin.
+__device__ __forceinline__ void load_to_lds(u32x4 buffer, uint32_t offset, uint32_t lds) {
   asm volatile(
-      "s_mov_b32 m0, %1\n\t"
+      "s_mov_b32 m0, %2\n\t"
       "s_nop 0\n\t"
-      "global_load_lds_dwordx4 %0, off"
+      "buffer_load_dwordx4 %0, %1, 0 offen lds"
       :
-      : "v"(src), "s"(lds));
+      : "v"(offset), "s"(buffer), "s"(lds));
 }
 
 // Waits until at most kLeft of this wave's loads are outstanding and its LDS
@@ -82,69 +82,71 @@ __device__ __forceinline__ void wait_and_barrier() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(kLeft) : "memory");
 }
 
-// The loads of one operand's stages by the whole workgroup.
+// The loads of one operand's stages by the whole workgroup: 16-byte pieces, one
+// a thread and round. A thread's offset from the round's first row never
+// changes; the rounds' and stages' first rows are scalars.
 template <Major M, int BX>
 struct Loader {
   static constexpr int kRounds = BX * 8 / kThreads;
   static constexpr int kBytes = BX * kStep * 2;
+  static constexpr int kRoundRows = M == Major::kK ? kThreads / 8 : kThreads / (BX / 8);
   static_assert(kRounds >= 1, "a stage is at least one piece a thread");
   static_assert(M == Major::kK || BX >= 128, "x-major rows hold at least 8 granules");
 
-  const uint16_t* src[kRounds];  // k-major: this thread's rows; x-major: its column
-  int64_t ld;
-  int32_t row;
-  int32_t last;
+  const char* base;  // the next stage's first row (k-major: at its first k)
+  int32_t row_bytes;
+  int32_t left;      // rows from there on
+  int32_t into;      // x-major: bytes of base into its row
+  uint32_t offset;   // of this thread's piece from a round's first row
+  uint32_t wave_lds;
 
   __device__ __forceinline__ void init(const Operand& op, int x0, int k0) {
     const int tid = threadIdx.x;
+    row_bytes = static_cast<int32_t>(op.ld * 2);
+    const int first = M == Major::kK ? x0 : k0;
+    into = 2 * (M == Major::kK ? k0 : x0);
+    left = op.rows - first;
+    base = reinterpret_cast<const char*>(op.data) + static_cast<int64_t>(first) * row_bytes + into;
+    wave_lds = __builtin_amdgcn_readfirstlane(tid >> 6) * 1024u;
     if constexpr (M == Major::kK) {
-      const int piece = (tid & 7) ^ ((tid >> 4) & 7);
-#pragma unroll
-      for (int j = 0; j < kRounds; ++j) {
-        int r = x0 + j * (kThreads / 8) + (tid >> 3);
-        r = r < op.rows ? r : op.rows - 1;
-        src[j] = op.data + r * op.ld + k0 + piece * 8;
-      }
+      offset = static_cast<uint32_t>(tid >> 3) * row_bytes + (((tid & 7) ^ ((tid >> 4) & 7)) << 4);
     } else {
-      constexpr int kPieces = BX / 8;
-      row = k0 + tid / kPieces;
-      last = op.rows - 1;
-      ld = op.ld;
-      const int at = tid % kPieces;
-      const int k = tid / kPieces;
+      const int at = tid % (BX / 8), k = tid / (BX / 8);
       const int f = (k & 3) | (((k >> 3) & 1) << 2);
-      int x = x0 + (((at >> 1) ^ f) << 4) + ((at & 1) << 3);
-      x = x < op.cols ? x : 0;
-      src[0] = op.data + x;
+      offset = static_cast<uint32_t>(k) * row_bytes + (((at >> 1) ^ f) << 5) + ((at & 1) << 4);
     }
   }
 
-  // Starts the loads of the next stage (stages are taken in order).
-  __device__ __forceinline__ void next(uint32_t lds) {
-    const uint32_t base =
-        lds + __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6)) * 1024u;
-#pragma unroll
-    for (int j = 0; j < kRounds; ++j) {
-      const uint16_t* p;
-      if constexpr (M == Major::kK) {
-        p = src[j];
-        src[j] += kStep;
-      } else {
-        int r = row + j * (kThreads / (BX / 8));
-        r = r < last ? r : last;
-        p = src[0] + r * ld;
-      }
-      load_to_lds(p, base + static_cast<uint32_t>(j) * (kThreads * 16u));
+  // Starts round j of the next stage's loads; there = 0: of zeros, for a stage
+  // beyond the last.
+  __device__ __forceinline__ void load(int j, int there, uint32_t lds) const {
+    const char* from = base + static_cast<int64_t>(j * kRoundRows) * row_bytes;
+    // The buffer ends where the round's last row does, if not before it.
+    int rows = left - j * kRoundRows;
+    rows = rows < kRoundRows + 1 ? rows : kRoundRows + 1;
+    int bytes = M == Major::kK ? (rows - 1) * row_bytes + kStep * 2 : rows * row_bytes - into;
+    bytes = rows > 0 && there ? bytes : 0;
+    const uint64_t address = reinterpret_cast<uint64_t>(from);
+    const u32x4 buffer = {static_cast<uint32_t>(address), static_cast<uint32_t>(address >> 32),
+                          static_cast<uint32_t>(bytes), 0x00020000u};
+    load_to_lds(buffer, offset, lds + j * (kThreads * 16u) + wave_lds);
+  }
+  // Moves on to the stage after it.
+  __device__ __forceinline__ void next() {
+    if constexpr (M == Major::kK) {
+      base += kStep * 2;
+    } else {
+      base += static_cast<int64_t>(kStep) * row_bytes;
+      left -= kStep;
     }
-    if constexpr (M == Major::kX) row += kStep;
   }
 };
 
 // Operand registers of 16 x 32 blocks read from a stage. Lane (g = lane / 16,
 // n = lane % 16) holds x = n, k = 8g .. 8g + 7 of the block.
-template <Major M, int BX>
+template <Major M, int BX, int kBlocks>
 struct Reader {
-  uint32_t at[M == Major::kK ? 2 : 8];
+  uint32_t at[M == Major::kK ? 2 : kBlocks];
 
   // x0: the wave's first x in the tile, a multiple of 16.
   __device__ __forceinline__ void init(int x0) {
@@ -158,7 +160,7 @@ struct Reader {
     } else {
       const int f = (n >> 2) | ((g & 1) << 2);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < kBlocks; ++i) {
         at[i] = (8 * g + (n >> 2)) * (BX * 2) + (((x0 / 16 + i) ^ f) << 5) + ((n & 3) << 3);
       }
     }
@@ -189,8 +191,6 @@ struct Tile {
   static constexpr int kStageBytes = (BP + BQ) * kStep * 2;
   static constexpr int kLdsBytes = NS * kStageBytes;
   static_assert(WP * WQ * 64 == kThreads, "8 waves");
-  static_assert(MA == Major::kK || TP <= 8, "x-major block addresses");
-  static_assert(MB == Major::kK || TQ <= 8, "x-major block addresses");
   static_assert(kLdsBytes <= 160 * 1024, "LDS of a CU");
 
   using LoadA = Loader<MA, BP>;
@@ -204,8 +204,22 @@ struct Tile {
   }
   static __device__ __forceinline__ int wave_p0() { return (wave() / WQ) * (BP / WP); }
   static __device__ __forceinline__ int wave_q0() { return (wave() % WQ) * (BQ / WQ); }
+  // Lane l holds of D the columns column(j), j < TQ, and in them the rows row(i) .. + 3.
+  static __device__ __forceinline__ int row(int i) {
+    return wave_p0() + 16 * i + 4 * static_cast<int>((threadIdx.x & 63) >> 4);
+  }
+  static __device__ __forceinline__ int column(int j) {
+    return wave_q0() + 16 * j + static_cast<int>(threadIdx.x & 15);
+  }
 
-  // steps: number of 64-k stages from k0 on (at least 1). smem: kLdsBytes.
+  // steps: number of 64-k stages from k0 on; 0 leaves zeros. smem: kLdsBytes,
+  // free for other use afterwards.
+  //
+  // A stage is two halves of 32 k. While a half's matrix instructions run, the
+  // other half's operands come from LDS into the registers that the half
+  // before used, and in the second half the loads of stage t + NS start into
+  // the buffer that stage t has left. One barrier a stage, between the halves:
+  // there stage t + 1 has arrived and every wave has read all of stage t.
   __device__ __forceinline__ void run(const Operand& a, const Operand& b, int p0, int q0, int k0,
                                       int steps, char* smem) {
     const uint32_t lds = static_cast<uint32_t>(
@@ -214,8 +228,8 @@ struct Tile {
     LoadB lb;
     la.init(a, p0, k0);
     lb.init(b, q0, k0);
-    Reader<MA, BP> ra;
-    Reader<MB, BQ> rb;
+    Reader<MA, BP, TP> ra;
+    Reader<MB, BQ, TQ> rb;
     ra.init(wave_p0());
     rb.init(wave_q0());
 #pragma unroll
@@ -223,41 +237,77 @@ struct Tile {
 #pragma unroll
       for (int j = 0; j < TQ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
+    if (steps <= 0) return;
 #pragma unroll
-    for (int s = 0; s < NS - 1; ++s) {
-      if (s < steps) {
-        la.next(lds + s * kStageBytes);
-        lb.next(lds + s * kStageBytes + LoadA::kBytes);
-      }
+    for (int s = 0; s < NS; ++s) {
+#pragma unroll
+      for (int l = 0; l < kLoads; ++l) load(la, lb, l, s < steps, lds + s * kStageBytes);
+      la.next();
+      lb.next();
     }
-    int read_at = 0, load_at = NS - 1;
+    wait_and_barrier<(NS - 1) * kLoads>();
+    i16x8 fa[2][TP], fb[2][TQ];
+#pragma unroll
+    for (int r = 0; r < TP + TQ; ++r) fetch(ra, rb, smem, r, 0, fa[0], fb[0]);
+    int at = 0;
     for (int t = 0; t < steps; ++t) {
-      if (NS > 2 && t + NS - 1 <= steps) {
-        wait_and_barrier<(NS - 2) * kLoads>();
-      } else {
-        wait_and_barrier<0>();
-      }
-      if (t + NS - 1 < steps) {
-        la.next(lds + load_at * kStageBytes);
-        lb.next(lds + load_at * kStageBytes + LoadA::kBytes);
-      }
-      const char* sa = smem + read_at * kStageBytes;
-      const char* sb = sa + LoadA::kBytes;
+      const char* stage = smem + at * kStageBytes;
+      const int after = at + 1 == NS ? 0 : at + 1;
 #pragma unroll
-      for (int kk = 0; kk < 2; ++kk) {
-        i16x8 af[TP], bf[TQ];
+      for (int i = 0; i < TP; ++i) {
 #pragma unroll
-        for (int j = 0; j < TQ; ++j) bf[j] = rb.read(sb, j, kk);
+        for (int j = 0; j < TQ; ++j) acc[i][j] = mfma<T>(fa[0][i], fb[0][j], acc[i][j]);
 #pragma unroll
-        for (int i = 0; i < TP; ++i) af[i] = ra.read(sa, i, kk);
-#pragma unroll
-        for (int i = 0; i < TP; ++i) {
-#pragma unroll
-          for (int j = 0; j < TQ; ++j) acc[i][j] = mfma<T>(af[i], bf[j], acc[i][j]);
+        for (int r = i * kReads; r < (i + 1) * kReads && r < TP + TQ; ++r) {
+          fetch(ra, rb, stage, r, 1, fa[1], fb[1]);
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
-      read_at = read_at + 1 == NS ? 0 : read_at + 1;
-      load_at = load_at + 1 == NS ? 0 : load_at + 1;
+      wait_and_barrier<(NS - 2) * kLoads>();
+      const int there = t + NS < steps;
+      const char* next = smem + after * kStageBytes;
+#pragma unroll
+      for (int i = 0; i < TP; ++i) {
+#pragma unroll
+        for (int j = 0; j < TQ; ++j) acc[i][j] = mfma<T>(fa[1][i], fb[1][j], acc[i][j]);
+#pragma unroll
+        for (int l = i * kStarts; l < (i + 1) * kStarts && l < kLoads; ++l) {
+          load(la, lb, l, there, lds + at * kStageBytes);
+        }
+#pragma unroll
+        for (int r = i * kReads; r < (i + 1) * kReads && r < TP + TQ; ++r) {
+          fetch(ra, rb, next, r, 0, fa[0], fb[0]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      la.next();
+      lb.next();
+      at = after;
+    }
+    wait_and_barrier<0>();
+  }
+
+ private:
+  // LDS reads and started loads beside each block row of matrix instructions.
+  static constexpr int kReads = (TP + TQ + TP - 1) / TP;
+  static constexpr int kStarts = (kLoads + TP - 1) / TP;
+
+  static __device__ __forceinline__ void load(const LoadA& la, const LoadB& lb, int l, int there,
+                                              uint32_t lds) {
+    if (l < LoadA::kRounds) {
+      la.load(l, there, lds);
+    } else {
+      lb.load(l - LoadA::kRounds, there, lds + LoadA::kBytes);
+    }
+  }
+  // Operand r of a half: the q blocks first, which all matrix instructions use.
+  template <typename RA, typename RB>
+  static __device__ __forceinline__ void fetch(const RA& ra, const RB& rb, const char* stage,
+                                               int r, int kk, i16x8 (&fa)[TP], i16x8 (&fb)[TQ]) {
+    if (r < TQ) {
+      fb[r] = rb.read(stage + LoadA::kBytes, r, kk);
+    } else {
+      fa[r - TQ] = ra.read(stage, r - TQ, kk);
     }
   }
 };

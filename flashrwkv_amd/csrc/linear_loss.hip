@@ -310,38 +310,35 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void lse_tiles_kernel(
   G tile;
   tile.run(w, h, p0, q0, 0, c / gemm::kStep, smem);
   __syncthreads();
-  const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
-  const int left = w.rows - p0 - G::wave_p0() - 4 * g;  // of this lane's first row on
+  const int left = w.rows - p0;
   float* maxima = reinterpret_cast<float*>(smem);
   float* sums = maxima + G::kWP * G::kBQ;
   const int wp = G::wave() / G::kWQ;
 #pragma unroll
   for (int j = 0; j < G::TQ; ++j) {
+    float x[4 * G::TP];
     float top = -__builtin_inff();
 #pragma unroll
-    for (int i = 0; i < G::TP; ++i) {
+    for (int q = 0; q < G::TP; ++q) {
+      const f32x4 z = tile.acc[q][j];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        tile.acc[i][j][r] = 16 * i + r < left ? tile.acc[i][j][r] * scale : -__builtin_inff();
-        top = fmaxf(top, tile.acc[i][j][r]);
+        x[4 * q + r] = G::row(q) + r < left ? z[r] * scale : -__builtin_inff();
+        top = fmaxf(top, x[4 * q + r]);
       }
     }
-    top = fmaxf(top, __shfl_xor(top, 16, 64));
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
+#pragma unroll
+    for (int off = 16; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
     // -inf everywhere (columns beyond the vocabulary): a sum of 0, not NaN.
     const float from = top == -__builtin_inff() ? 0.0f : top;
     float sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < G::TP; ++i) {
+    for (int e = 0; e < 4 * G::TP; ++e) sum += __builtin_amdgcn_exp2f(x[e] - from);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) sum += __builtin_amdgcn_exp2f(tile.acc[i][j][r] - from);
-    }
-    sum += __shfl_xor(sum, 16, 64);
-    sum += __shfl_xor(sum, 32, 64);
-    if (g == 0) {
-      const int q = G::wave_q0() + 16 * j + n;
-      maxima[wp * G::kBQ + q] = top;
-      sums[wp * G::kBQ + q] = sum;
+    for (int off = 16; off < 64; off <<= 1) sum += __shfl_xor(sum, off, 64);
+    if ((threadIdx.x & 63) < 16) {
+      maxima[wp * G::kBQ + G::column(j)] = top;
+      sums[wp * G::kBQ + G::column(j)] = sum;
     }
   }
   __syncthreads();
@@ -374,24 +371,24 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void softmax_grad_kernel(
   if (q0 >= round_up(rows, kRowPad)) return;
   G tile;
   tile.run(w, h, p0, q0, 0, c / gemm::kStep, smem);
-  const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
-  const int left = w.rows - p0 - G::wave_p0() - 4 * g;
+  const int left = w.rows - p0;
 #pragma unroll
   for (int j = 0; j < G::TQ; ++j) {
-    const int m = q0 + G::wave_q0() + 16 * j + n;
-    const bool row = m < rows;
-    const float from = row ? lse2[m] : 0.0f;
-    const float co = row ? coef[m] : 0.0f;
-    uint16_t* to = dz + static_cast<int64_t>(m) * ld + p0 + G::wave_p0() + 4 * g;
+    const int m = q0 + G::column(j);
+    const bool here = m < rows;
+    const float from = here ? lse2[m] : 0.0f;
+    const float co = here ? coef[m] : 0.0f;
+    uint16_t* to = dz + static_cast<int64_t>(m) * ld + p0;
 #pragma unroll
-    for (int i = 0; i < G::TP; ++i) {
+    for (int q = 0; q < G::TP; ++q) {
+      const f32x4 z = tile.acc[q][j];
       float x[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float e = co * __builtin_amdgcn_exp2f(fmaf(tile.acc[i][j][r], scale, -from));
-        x[r] = row && 16 * i + r < left ? e : 0.0f;
+        const float e = co * __builtin_amdgcn_exp2f(fmaf(z[r], scale, -from));
+        x[r] = here && G::row(q) + r < left ? e : 0.0f;
       }
-      *reinterpret_cast<uint2*>(to + 16 * i) =
+      *reinterpret_cast<uint2*>(to + G::row(q)) =
           make_uint2(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]));
     }
   }
@@ -421,7 +418,8 @@ __global__ __launch_bounds__(256) void target_grad_kernel(int32_t k, int32_t voc
 template <typename G, typename T>
 __global__ __launch_bounds__(gemm::kThreads, 2) void hidden_grad_kernel(
     Operand w, Operand dz, const int32_t* __restrict__ count, int32_t steps, int32_t split_steps,
-    int32_t np, int32_t nq, float* __restrict__ slabs, int64_t slab) {
+    int32_t np, int32_t nq, int32_t c_all,
+    float* __restrict__ slabs, int64_t slab) {
   __shared__ __attribute__((aligned(1024))) char smem[G::kLdsBytes];
   int tp, tq;
   gemm::tile_of(gemm::xcd_run(blockIdx.x, gridDim.x), np, nq, tp, tq);
@@ -432,17 +430,16 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void hidden_grad_kernel(
   const int mine = steps - first < split_steps ? steps - first : split_steps;
   G tile;
   tile.run(w, dz, p0, q0, first * gemm::kStep, mine, smem);
-  const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
   float* out = slabs + blockIdx.y * slab;
 #pragma unroll
   for (int j = 0; j < G::TQ; ++j) {
-    const int m = q0 + G::wave_q0() + 16 * j + n;
+    const int m = q0 + G::column(j);
     if (m >= rows) continue;
 #pragma unroll
-    for (int i = 0; i < G::TP; ++i) {
-      const int c = p0 + G::wave_p0() + 16 * i + 4 * g;
-      if (c < w.cols) {
-        *reinterpret_cast<f32x4*>(out + static_cast<int64_t>(m) * w.cols + c) = tile.acc[i][j];
+    for (int q = 0; q < G::TP; ++q) {
+      const int c = p0 + G::row(q);
+      if (c < c_all) {
+        *reinterpret_cast<f32x4*>(out + static_cast<int64_t>(m) * c_all + c) = tile.acc[q][j];
       }
     }
   }
@@ -478,7 +475,7 @@ __global__ __launch_bounds__(256) void hidden_grad_rows_kernel(
 template <typename G, typename T>
 __global__ __launch_bounds__(gemm::kThreads, 2) void weight_grad_kernel(
     Operand h, Operand dz, const int32_t* __restrict__ count, int32_t columns, int32_t np,
-    int32_t nq, const float* __restrict__ scale, uint16_t* __restrict__ dw) {
+    int32_t nq, int32_t c_all, const float* __restrict__ scale, uint16_t* __restrict__ dw) {
   __shared__ __attribute__((aligned(1024))) char smem[G::kLdsBytes];
   int tp, tq;
   gemm::tile_of(gemm::xcd_run(blockIdx.x, gridDim.x), np, nq, tp, tq);
@@ -487,17 +484,16 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void weight_grad_kernel(
   G tile;
   tile.run(h, dz, p0, q0, 0, steps, smem);
   const float by = *scale;
-  const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
 #pragma unroll
   for (int j = 0; j < G::TQ; ++j) {
-    const int v = q0 + G::wave_q0() + 16 * j + n;
+    const int v = q0 + G::column(j);
     if (v >= columns) continue;
 #pragma unroll
-    for (int i = 0; i < G::TP; ++i) {
-      const int c = p0 + G::wave_p0() + 16 * i + 4 * g;
-      if (c < h.cols) {
-        const f32x4 x = tile.acc[i][j] * by;
-        *reinterpret_cast<uint2*>(dw + static_cast<int64_t>(v) * h.cols + c) =
+    for (int q = 0; q < G::TP; ++q) {
+      const int c = p0 + G::row(q);
+      if (c < c_all) {
+        const f32x4 x = tile.acc[q][j] * by;
+        *reinterpret_cast<uint2*>(dw + static_cast<int64_t>(v) * c_all + c) =
             make_uint2(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]));
       }
     }
@@ -615,7 +611,7 @@ __global__ __launch_bounds__(kScanThreads) void row_coefficients_kernel(
 // ---------------------------------------------------------------- launches
 // Bytes of one piece's dz: large enough that a piece's three products fill the
 // GPU for any row count, small beside the logits of a long batch.
-constexpr int64_t kPieceBytes = int64_t{512} << 20;
+constexpr int64_t kPieceBytes = int64_t{128} << 20;
 constexpr int kCus = 256;
 
 struct Pieces {
@@ -705,8 +701,8 @@ void launch_lse_tiles(const Shape& d, const void* weight, const Saved& s, const 
   const int64_t pad = round_up(d.n, kRowPad);
   const int np = static_cast<int>(round_up(d.vocab, G::kBP) / G::kBP);
   const int nq = static_cast<int>(row_tiles(d.n));
-  const Operand a{static_cast<const uint16_t*>(weight), d.c, d.vocab, d.c};
-  const Operand b{s.hidden, d.c, static_cast<int32_t>(pad), d.c};
+  const Operand a{static_cast<const uint16_t*>(weight), d.c, d.vocab};
+  const Operand b{s.hidden, d.c, static_cast<int32_t>(pad)};
   hipLaunchKernelGGL((lse_tiles_kernel<G, T>), dim3(np * nq), dim3(gemm::kThreads), 0, stream, a,
                      b, s.count, d.c, np, nq, scale, w.part, pad);
 }
@@ -757,11 +753,10 @@ void launch_piece(const Shape& d, const Pieces& pieces, int piece, const uint16_
   const int nc = static_cast<int>(round_up(d.c, 256) / 256);
   const int64_t ld = pieces.columns;
   const uint16_t* from = weight + static_cast<int64_t>(first) * d.c;
-  const Operand wp{from, d.c, columns, d.c};
-  const Operand h{s.hidden, d.c, static_cast<int32_t>(pad), d.c};
+  const Operand wp{from, d.c, columns};
+  const Operand h{s.hidden, d.c, static_cast<int32_t>(pad)};
   // Rows of dz that hold something: whole tiles.
-  const Operand dz{w.dz, ld, static_cast<int32_t>(std::min<int64_t>(pad, nq * Logits::kBQ)),
-                   np * kVocabTile};
+  const Operand dz{w.dz, ld, static_cast<int32_t>(std::min<int64_t>(pad, nq * Logits::kBQ))};
   hipLaunchKernelGGL((softmax_grad_kernel<Logits, T>), dim3(np * nq), dim3(gemm::kThreads), 0,
                      stream, wp, h, s.count, d.c, np, nq, scale, s.lse2, w.coef, w.dz, ld);
   const int64_t entries = d.n * d.k;
@@ -773,12 +768,12 @@ void launch_piece(const Shape& d, const Pieces& pieces, int piece, const uint16_
     const int64_t slab = d.n * d.c;
     hipLaunchKernelGGL((hidden_grad_kernel<Hidden, T>),
                        dim3(nc * nq, static_cast<unsigned>(pieces.splits)), dim3(gemm::kThreads),
-                       0, stream, wp, dz, s.count, steps, each, nc, nq,
+                       0, stream, wp, dz, s.count, steps, each, nc, nq, d.c,
                        w.slabs + piece * pieces.splits * slab, slab);
   }
   if (dw != nullptr) {
     hipLaunchKernelGGL((weight_grad_kernel<Weight, T>), dim3(nc * np), dim3(gemm::kThreads), 0,
-                       stream, h, dz, s.count, columns, nc, np, w.scale,
+                       stream, h, dz, s.count, columns, nc, np, d.c, w.scale,
                        dw + static_cast<int64_t>(first) * d.c);
   }
 }

@@ -314,7 +314,7 @@ def test_upstream_scales(scale):
 
 
 def test_several_pieces_of_the_vocabulary():
-    """4096 rows and 70000 tokens need two pieces of logit gradients; a target
+    """4096 rows and 70000 tokens need several pieces of logit gradients; a target
     list that reaches into both, and the last piece ragged."""
     n, c, v = 4096, 64, 70000
     h, w = _head(n, c, v, torch.bfloat16, seed=20)
