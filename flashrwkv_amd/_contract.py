@@ -146,6 +146,18 @@ METADATA = (
 )
 
 
+def whole_call(name: str):
+    """The native whole call of an entry (checks, outputs and launches at once;
+    it declines what its checks do not pass), or None without the native
+    library or while compiling."""
+    import flashrwkv_amd
+
+    facade = getattr(flashrwkv_amd, "_C", None)
+    if facade is None or torch.compiler.is_compiling():
+        return None
+    return getattr(facade.direct, name)
+
+
 def native():
     """The loaded native facade, or RuntimeError when it is not built."""
     import flashrwkv_amd

@@ -1873,6 +1873,8 @@ bool advance_varlen_call(const pybind11::object& elapsed, const pybind11::object
   return true;
 }
 
+#include "head_calls.h"
+
 PYBIND11_MODULE(_flashrwkv_amd_ops, m) {
   namespace py = pybind11;
   // TORCH_CHECK failures surface as RuntimeError with the check's message,
@@ -1918,6 +1920,9 @@ PYBIND11_MODULE(_flashrwkv_amd_ops, m) {
           recurrent_fp16_advance_i32_varlen(cu, slots, elapsed, total_tokens,
                                             ticket_arg(ticket));
         });
+  m.def("layer_norm_infer_call", &layer_norm_infer_call);
+  m.def("layer_norm_train_call", &layer_norm_train_call);
+  m.def("linear_loss_call", &linear_loss_call);
   m.def("recurrent_add_vec_forward_varlen", &recurrent_add_vec_forward_varlen);
   m.def("tmix_kk_a_gate_forward_varlen", &tmix_kk_a_gate_forward_varlen);
   m.def("tmix_lnx_rkvres_xg_forward_varlen", &tmix_lnx_rkvres_xg_forward_varlen);

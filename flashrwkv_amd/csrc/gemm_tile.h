@@ -4,9 +4,7 @@
 //
 // Either operand may lie in memory with k contiguous ("k-major": rows are p or
 // q) or with p / q contiguous ("x-major": rows are k). Tiles of 64 k go from
-// HBM straight into LDS (16 bytes a lane, no registers), NS stages deep: at
-// step t the workgroup waits for stage t, starts the load of stage t + NS - 1
-// into the buffer that step t - 1 has read, and multiplies stage t.
+// HBM straight into LDS (16 bytes a lane, no registers) up to NS stages ahead.
 //
 // LDS holds a stage unpadded (the load writes 64 consecutive 16-byte pieces a
 // wave), so bank conflicts are avoided by which piece goes where:
@@ -212,22 +210,36 @@ struct Tile {
     return wave_q0() + 16 * j + static_cast<int>(threadIdx.x & 15);
   }
 
-  // steps: number of 64-k stages from k0 on; 0 leaves zeros. smem: kLdsBytes,
-  // free for other use afterwards.
+  // A product is begin (starts the loads of its first stages), arrive (this
+  // wave's have arrived) and multiply. Between begin and arrive a workgroup can
+  // finish the tile before: its accumulators are its own until multiply, and
+  // the LDS beyond kLdsBytes is not touched.
   //
+  // steps: number of 64-k stages from k0 on; 0 leaves zeros.
+  __device__ __forceinline__ void begin(const Operand& a, const Operand& b, int p0, int q0, int k0,
+                                        int steps_, char* smem) {
+    lds = static_cast<uint32_t>(
+        reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)smem));
+    steps = steps_;
+    la.init(a, p0, k0);
+    lb.init(b, q0, k0);
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+#pragma unroll
+      for (int l = 0; l < kLoads; ++l) load(la, lb, l, s < steps, lds + s * kStageBytes);
+      la.next();
+      lb.next();
+    }
+  }
+
+  static __device__ __forceinline__ void arrive() { asm volatile("s_waitcnt vmcnt(0)"); }
+
   // A stage is two halves of 32 k. While a half's matrix instructions run, the
   // other half's operands come from LDS into the registers that the half
   // before used, and in the second half the loads of stage t + NS start into
   // the buffer that stage t has left. One barrier a stage, between the halves:
   // there stage t + 1 has arrived and every wave has read all of stage t.
-  __device__ __forceinline__ void run(const Operand& a, const Operand& b, int p0, int q0, int k0,
-                                      int steps, char* smem) {
-    const uint32_t lds = static_cast<uint32_t>(
-        reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)smem));
-    LoadA la;
-    LoadB lb;
-    la.init(a, p0, k0);
-    lb.init(b, q0, k0);
+  __device__ __forceinline__ void multiply(const char* smem) {
     Reader<MA, BP, TP> ra;
     Reader<MB, BQ, TQ> rb;
     ra.init(wave_p0());
@@ -237,15 +249,7 @@ struct Tile {
 #pragma unroll
       for (int j = 0; j < TQ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    if (steps <= 0) return;
-#pragma unroll
-    for (int s = 0; s < NS; ++s) {
-#pragma unroll
-      for (int l = 0; l < kLoads; ++l) load(la, lb, l, s < steps, lds + s * kStageBytes);
-      la.next();
-      lb.next();
-    }
-    wait_and_barrier<(NS - 1) * kLoads>();
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory");
     i16x8 fa[2][TP], fb[2][TQ];
 #pragma unroll
     for (int r = 0; r < TP + TQ; ++r) fetch(ra, rb, smem, r, 0, fa[0], fb[0]);
@@ -288,6 +292,11 @@ struct Tile {
   }
 
  private:
+  LoadA la;
+  LoadB lb;
+  uint32_t lds;
+  int steps;
+
   // LDS reads and started loads beside each block row of matrix instructions.
   static constexpr int kReads = (TP + TQ + TP - 1) / TP;
   static constexpr int kStarts = (kLoads + TP - 1) / TP;
@@ -311,6 +320,31 @@ struct Tile {
     }
   }
 };
+
+// Stores column j of a tile's lanes as 16 bits: element (p, q) of the tile to
+// to[q * ld + p], for q < columns and p < rows (a multiple of 32). quad[i] holds
+// rows row(i) .. + 3: 8 bytes a lane, 32 bytes apart. Exchanged between odd and
+// even groups of 16 lanes, quads i and i + 1 become 16 consecutive bytes a lane
+// and 64 a column; half the stores and half the requests to L2 (a backward of
+// 1000 x 50277 x 2560: 797 -> 764 us).
+template <typename G>
+__device__ __forceinline__ void store_column(uint16_t* to, int64_t ld, int rows, int columns,
+                                             int j, const uint2 (&quad)[G::TP]) {
+  static_assert(G::TP % 2 == 0, "quads go in pairs");
+  const int g = static_cast<int>((threadIdx.x & 63) >> 4);
+  const int first = G::wave_p0() + 16 * (g & 1) + 8 * (g >> 1);
+  const int q = G::column(j);
+  uint16_t* column = to + q * ld;
+#pragma unroll
+  for (int i = 0; i < G::TP; i += 2) {
+    const auto x = __builtin_amdgcn_permlane16_swap(quad[i].x, quad[i + 1].x, false, false);
+    const auto y = __builtin_amdgcn_permlane16_swap(quad[i].y, quad[i + 1].y, false, false);
+    const int p = first + 16 * i;
+    if (q < columns && p < rows) {
+      *reinterpret_cast<uint4*>(column + p) = make_uint4(x[0], y[0], x[1], y[1]);
+    }
+  }
+}
 
 // Workgroups go round the 8 XCDs in turn; this gives each XCD one contiguous
 // run of tile numbers, so that tiles sharing operands share its L2.

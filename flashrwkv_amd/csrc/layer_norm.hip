@@ -17,6 +17,7 @@
 // of 2 C partial sums a workgroup goes to memory and a second kernel adds
 // those in order, so the result does not depend on timing.
 #include <algorithm>
+#include <type_traits>
 
 #include "capi_internal.h"
 #include "wkv7_device.h"
@@ -24,27 +25,55 @@
 namespace frwkv {
 namespace {
 
-constexpr int kEpt = 16;  // elements of a row a thread
+constexpr int kEpt = 16;         // elements of a row a thread
+constexpr int kMaxBlocks = 512;  // of the backward: two a CU
 
 template <typename T>
 using Store = typename IoTraits<T>::storage;
 
-// kVec consecutive elements; kVec 8 reads and writes 16-byte pieces.
+// kVec consecutive elements as they lie in memory; kVec 8 reads 16-byte pieces.
+template <typename T, int kVec>
+struct Piece {
+  static constexpr int kWords = kVec == 1 ? 1 : kVec * IoTraits<T>::kBytes / 16;
+  typedef typename std::conditional<kVec == 1, Store<T>, uint4>::type Word;
+  Word word[kWords];
+  __device__ __forceinline__ void load(const Store<T>* p) {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) word[i] = reinterpret_cast<const Word*>(p)[i];
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) word[i] = Word{};
+  }
+  // Conversions before and after this one are not one value kept in registers.
+  __device__ __forceinline__ void again() {
+    if constexpr (kVec != 1) {
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) {
+        asm volatile("" : "+v"(word[i].x), "+v"(word[i].y), "+v"(word[i].z), "+v"(word[i].w));
+      }
+    }
+  }
+  __device__ __forceinline__ float get(int e) const {
+    if constexpr (kVec == 1) {
+      return to_f32<T>(word[0]);
+    } else if constexpr (__is_same(T, float)) {
+      const uint4 q = word[e / 4];
+      return __uint_as_float(e % 4 == 0 ? q.x : e % 4 == 1 ? q.y : e % 4 == 2 ? q.z : q.w);
+    } else {
+      const uint32_t d = e / 2 == 0 ? word[0].x : e / 2 == 1 ? word[0].y
+                         : e / 2 == 2 ? word[0].z : word[0].w;
+      return to_f32<T>(static_cast<uint16_t>(e % 2 ? d >> 16 : d & 0xffffu));
+    }
+  }
+};
+
 template <typename T, int kVec>
 __device__ __forceinline__ void load(const Store<T>* p, float* out) {
-  if constexpr (kVec == 1) {
-    out[0] = to_f32<T>(*p);
-  } else if constexpr (__is_same(T, float)) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0];
-    const float4 b = reinterpret_cast<const float4*>(p)[1];
-    out[0] = a.x; out[1] = a.y; out[2] = a.z; out[3] = a.w;
-    out[4] = b.x; out[5] = b.y; out[6] = b.z; out[7] = b.w;
-  } else {
-    const uint4 q = *reinterpret_cast<const uint4*>(p);
-    const uint16_t* s = reinterpret_cast<const uint16_t*>(&q);
+  Piece<T, kVec> x;
+  x.load(p);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) out[e] = to_f32<T>(s[e]);
-  }
+  for (int e = 0; e < kVec; ++e) out[e] = x.get(e);
 }
 
 template <typename T, int kVec>
@@ -154,7 +183,7 @@ __global__ __launch_bounds__(forward_threads<kWaves>()) void layer_norm_forward_
 
 // partial[block][0][c] = sum over the block's rows of dy xhat, [1][c] of dy.
 template <typename T, int kVec, int kWaves>
-__global__ __launch_bounds__(backward_threads<kWaves>()) void layer_norm_backward_kernel(
+__global__ __launch_bounds__(backward_threads<kWaves>(), kVec == 1 ? 1 : 4) void layer_norm_backward_kernel(
     const Store<T>* __restrict__ dy, const Store<T>* __restrict__ s,
     const Store<T>* __restrict__ ds, const Store<T>* __restrict__ weight,
     const float* __restrict__ mean, const float* __restrict__ rstd, Store<T>* __restrict__ dx,
@@ -166,13 +195,17 @@ __global__ __launch_bounds__(backward_threads<kWaves>()) void layer_norm_backwar
   __shared__ float columns[kGroups > 1 ? kThreads * kEpt : 1];
   const int group = threadIdx.x / kRow, t = threadIdx.x % kRow, wave = t >> 6;
   const float inv_c = 1.0f / static_cast<float>(c);
-  float w[kEpt], pw[kEpt], pb[kEpt];
+  // What is only read again is kept as it lies in memory.
+  constexpr int kPieces = kEpt / kVec;
+  Piece<T, kVec> w[kPieces], up[kPieces], add[kPieces];
+  float pw[kEpt], pb[kEpt];
 #pragma unroll
-  for (int j = 0; j < kEpt; j += kVec) {
-    const int col = (j / kVec * kRow + t) * kVec;
+  for (int j = 0; j < kPieces; ++j) {
+    const int col = (j * kRow + t) * kVec;
+    w[j].zero();
+    if (col < c) w[j].load(weight + col);
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) w[j + e] = pw[j + e] = pb[j + e] = 0.0f;
-    if (col < c) load<T, kVec>(weight + col, w + j);
+    for (int e = 0; e < kVec; ++e) pw[j * kVec + e] = pb[j * kVec + e] = 0.0f;
   }
   int side = 0;
   for (int64_t first = static_cast<int64_t>(blockIdx.x) * kGroups; first < rows;
@@ -181,26 +214,30 @@ __global__ __launch_bounds__(backward_threads<kWaves>()) void layer_norm_backwar
     const bool here = row < rows;
     const int64_t at = (here ? row : 0) * c;
     const float mu = here ? mean[row] : 0.0f, rs = here ? rstd[row] : 0.0f;
-    float xh[kEpt], up[kEpt], add[kEpt];
+    float xh[kEpt];
     float sg = 0.0f, sgx = 0.0f;
 #pragma unroll
-    for (int j = 0; j < kEpt; j += kVec) {
-      const int col = (j / kVec * kRow + t) * kVec;
-#pragma unroll
-      for (int e = 0; e < kVec; ++e) xh[j + e] = up[j + e] = add[j + e] = 0.0f;
+    for (int j = 0; j < kPieces; ++j) {
+      const int col = (j * kRow + t) * kVec;
+      Piece<T, kVec> x;
+      x.zero();
+      up[j].zero();
+      add[j].zero();
+      w[j].again();
       if (here && col < c) {
-        load<T, kVec>(s + at + col, xh + j);
-        load<T, kVec>(dy + at + col, up + j);
-        if (ds != nullptr) load<T, kVec>(ds + at + col, add + j);
+        x.load(s + at + col);
+        up[j].load(dy + at + col);
+        if (ds != nullptr) add[j].load(ds + at + col);
+      }
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) {
-          xh[j + e] = (xh[j + e] - mu) * rs;
-          pw[j + e] = fmaf(up[j + e], xh[j + e], pw[j + e]);
-          pb[j + e] += up[j + e];
-          const float g = up[j + e] * w[j + e];
-          sg += g;
-          sgx = fmaf(g, xh[j + e], sgx);
-        }
+      for (int e = 0; e < kVec; ++e) {
+        const int k = j * kVec + e;
+        const float u = up[j].get(e), g = u * w[j].get(e);
+        xh[k] = col < c ? (x.get(e) - mu) * rs : 0.0f;
+        pw[k] = fmaf(u, xh[k], pw[k]);
+        pb[k] += u;
+        sg += g;
+        sgx = fmaf(g, xh[k], sgx);
       }
     }
 #pragma unroll
@@ -226,13 +263,16 @@ __global__ __launch_bounds__(backward_threads<kWaves>()) void layer_norm_backwar
     const float mg = sg * inv_c, mgx = sgx * inv_c;
     if (!here) continue;
 #pragma unroll
-    for (int j = 0; j < kEpt; j += kVec) {
-      const int col = (j / kVec * kRow + t) * kVec;
+    for (int j = 0; j < kPieces; ++j) {
+      const int col = (j * kRow + t) * kVec;
+      up[j].again();
+      w[j].again();
       if (col < c) {
         float o[kVec];
 #pragma unroll
         for (int e = 0; e < kVec; ++e) {
-          o[e] = fmaf(rs, up[j + e] * w[j + e] - mg - xh[j + e] * mgx, add[j + e]);
+          const float g = up[j].get(e) * w[j].get(e);
+          o[e] = fmaf(rs, g - mg - xh[j * kVec + e] * mgx, add[j].get(e));
         }
         store<T, kVec>(dx + at + col, o);
       }
@@ -266,29 +306,36 @@ __global__ __launch_bounds__(backward_threads<kWaves>()) void layer_norm_backwar
   }
 }
 
-// Sum of the blocks' partial sums, in order: 32 columns a workgroup, 8 runs of
-// blocks each.
+// Sum of the blocks' partial sums, in a fixed order: 32 columns a workgroup,
+// 32 runs of up to 16 blocks, all of a run's loads under way together.
+constexpr int kRuns = 32;
+constexpr int kRunBlocks = kMaxBlocks / kRuns;
+
 template <typename T>
-__global__ __launch_bounds__(256) void layer_norm_columns_kernel(
+__global__ __launch_bounds__(1024) void layer_norm_columns_kernel(
     const float* __restrict__ partial, int32_t blocks, int32_t c, Store<T>* __restrict__ dweight,
     Store<T>* __restrict__ dbias) {
-  __shared__ float runs[8][32];
+  __shared__ float runs[kRuns][33];
   const int lane = threadIdx.x & 31, run = threadIdx.x >> 5;
   const int col = blockIdx.x * 32 + lane;
-  const int each = (blocks + 7) / 8;
-  const int last = min(blocks, (run + 1) * each);
-  float sum = 0.0f;
-  if (col < c) {
-    for (int b = run * each; b < last; ++b) {
-      sum += partial[(static_cast<int64_t>(b) * 2 + blockIdx.y) * c + col];
-    }
+  float x[kRunBlocks];
+#pragma unroll
+  for (int u = 0; u < kRunBlocks; ++u) {
+    const int b = run + kRuns * u;
+    x[u] = col < c && b < blocks
+               ? partial[(static_cast<int64_t>(b) * 2 + blockIdx.y) * c + col] : 0.0f;
   }
+  float sum = 0.0f;
+#pragma unroll
+  for (int u = 0; u < kRunBlocks; ++u) sum += x[u];
   runs[run][lane] = sum;
   __syncthreads();
-  if (run != 0 || col >= c) return;
+  // Turned: the 32 lanes of a half wave add a column's runs.
+  sum = runs[lane][run];
 #pragma unroll
-  for (int q = 1; q < 8; ++q) sum += runs[q][lane];
-  (blockIdx.y == 0 ? dweight : dbias)[col] = from_f32<T>(sum);
+  for (int off = 1; off < 32; off <<= 1) sum += __shfl_xor(sum, off, 64);
+  const int mine = blockIdx.x * 32 + run;
+  if (lane == 0 && mine < c) (blockIdx.y == 0 ? dweight : dbias)[mine] = from_f32<T>(sum);
 }
 
 int waves_of(int64_t c) { return c <= 64 * kEpt ? 1 : c <= 256 * kEpt ? 4 : 16; }
@@ -296,7 +343,7 @@ int waves_of(int64_t c) { return c <= 64 * kEpt ? 1 : c <= 256 * kEpt ? 4 : 16; 
 int64_t backward_blocks(int64_t rows, int64_t c) {
   const int waves = waves_of(c);
   const int64_t groups = waves == 16 ? 1 : 8 / waves;
-  return std::min<int64_t>((rows + groups - 1) / groups, waves == 16 ? 256 : 512);
+  return std::min<int64_t>((rows + groups - 1) / groups, waves == 16 ? kMaxBlocks / 2 : kMaxBlocks);
 }
 
 struct Call {
@@ -439,7 +486,7 @@ int frwkv_layer_norm_backward(int io_dtype, int64_t rows, int64_t channels, cons
                          static_cast<const S*>(grad_stream), static_cast<const S*>(weight), mean,
                          rstd, static_cast<S*>(grad_x), partial, rows, c);
     });
-    hipLaunchKernelGGL((layer_norm_columns_kernel<T>), dim3((c + 31) / 32, 2), dim3(256), 0, q,
+    hipLaunchKernelGGL((layer_norm_columns_kernel<T>), dim3((c + 31) / 32, 2), dim3(1024), 0, q,
                        partial, static_cast<int32_t>(blocks), c, static_cast<S*>(grad_weight),
                        static_cast<S*>(grad_bias));
   });

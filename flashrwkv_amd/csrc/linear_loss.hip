@@ -296,63 +296,93 @@ template <typename T, Major MA, Major MB>
 using FewRowsTile = gemm::Tile<T, MA, MB, 256, 64, 8, 1, 3>;
 constexpr int kFewRows = 64;
 
+// The tiles of a product over rows m, whose count stands on the device: the
+// workgroups of a launch of at most one a CU take them in turn. While a
+// workgroup finishes a tile, the first stages of its next one are on their way.
+__device__ __forceinline__ int row_tiles_of(int rows, int tile) { return (rows + tile - 1) / tile; }
+
 // D[v][m] of a vocabulary range: per tile of 256 v and row m the maximum of
 // s z log2 e and the sum of 2^(s z log2 e - maximum), to part[tile][m].
 template <typename G, typename T>
 __global__ __launch_bounds__(gemm::kThreads, 2) void lse_tiles_kernel(
-    Operand w, Operand h, const int32_t* __restrict__ count, int32_t c, int32_t np, int32_t nq,
-    float scale, float2* __restrict__ part, int64_t pad) {
+    Operand w, Operand h, const int32_t* __restrict__ count, int32_t c, int32_t np, float scale,
+    float2* __restrict__ part, int64_t pad) {
   __shared__ __attribute__((aligned(1024))) char smem[G::kLdsBytes];
-  int tp, tq;
-  gemm::tile_of(gemm::xcd_run(blockIdx.x, gridDim.x), np, nq, tp, tq);
-  const int p0 = tp * G::kBP, q0 = tq * G::kBQ;
-  if (q0 >= *count) return;
+  __shared__ float maxima[G::kWP][G::kBQ], sums[G::kWP][G::kBQ];
+  const int nq = row_tiles_of(*count, G::kBQ), total = np * nq;
+  int id = blockIdx.x;
+  if (id >= total) return;
   G tile;
-  tile.run(w, h, p0, q0, 0, c / gemm::kStep, smem);
-  __syncthreads();
-  const int left = w.rows - p0;
-  float* maxima = reinterpret_cast<float*>(smem);
-  float* sums = maxima + G::kWP * G::kBQ;
-  const int wp = G::wave() / G::kWQ;
+  int tp, tq;
+  gemm::tile_of(gemm::xcd_run(id, total), np, nq, tp, tq);
+  tile.begin(w, h, tp * G::kBP, tq * G::kBQ, 0, c / gemm::kStep, smem);
+  G::arrive();
+  while (true) {
+    tile.multiply(smem);
+    const int p0 = tp * G::kBP, q0 = tq * G::kBQ;
+    const int64_t to = static_cast<int64_t>(tp) * pad + q0;
+    id += gridDim.x;
+    if (id < total) {
+      gemm::tile_of(gemm::xcd_run(id, total), np, nq, tp, tq);
+      tile.begin(w, h, tp * G::kBP, tq * G::kBQ, 0, c / gemm::kStep, smem);
+    }
+    const int left = w.rows - p0;
+    if (left < G::kBP) {  // the last columns do not exist
 #pragma unroll
-  for (int j = 0; j < G::TQ; ++j) {
-    float x[4 * G::TP];
-    float top = -__builtin_inff();
+      for (int i = 0; i < G::TP; ++i) {
 #pragma unroll
-    for (int q = 0; q < G::TP; ++q) {
-      const f32x4 z = tile.acc[q][j];
+        for (int r = 0; r < 4; ++r) {
+          const bool here = G::row(i) + r < left;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        x[4 * q + r] = G::row(q) + r < left ? z[r] * scale : -__builtin_inff();
-        top = fmaxf(top, x[4 * q + r]);
+          for (int j = 0; j < G::TQ; ++j) {
+            tile.acc[i][j][r] = here ? tile.acc[i][j][r] : -__builtin_inff();
+          }
+        }
       }
     }
+    const int wp = G::wave() / G::kWQ;
 #pragma unroll
-    for (int off = 16; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
-    // -inf everywhere (columns beyond the vocabulary): a sum of 0, not NaN.
-    const float from = top == -__builtin_inff() ? 0.0f : top;
-    float sum = 0.0f;
+    for (int j = 0; j < G::TQ; ++j) {
+      float top = -__builtin_inff();
 #pragma unroll
-    for (int e = 0; e < 4 * G::TP; ++e) sum += __builtin_amdgcn_exp2f(x[e] - from);
+      for (int i = 0; i < G::TP; ++i) {
 #pragma unroll
-    for (int off = 16; off < 64; off <<= 1) sum += __shfl_xor(sum, off, 64);
-    if ((threadIdx.x & 63) < 16) {
-      maxima[wp * G::kBQ + G::column(j)] = top;
-      sums[wp * G::kBQ + G::column(j)] = sum;
+        for (int r = 0; r < 4; ++r) top = fmaxf(top, tile.acc[i][j][r]);
+      }
+      top = fmaxf(top, __shfl_xor(top, 16, 64));
+      top = fmaxf(top, __shfl_xor(top, 32, 64)) * scale;
+      // -inf everywhere (columns beyond the vocabulary): a sum of 0, not NaN.
+      const float from = top == -__builtin_inff() ? 0.0f : top;
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < G::TP; ++i) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          sum += __builtin_amdgcn_exp2f(fmaf(tile.acc[i][j][r], scale, -from));
+        }
+      }
+      sum += __shfl_xor(sum, 16, 64);
+      sum += __shfl_xor(sum, 32, 64);
+      if ((threadIdx.x & 63) < 16) {
+        maxima[wp][G::column(j)] = top;
+        sums[wp][G::column(j)] = sum;
+      }
     }
-  }
-  __syncthreads();
-  for (int q = threadIdx.x; q < G::kBQ; q += gemm::kThreads) {
-    float top = maxima[q];
+    G::arrive();
+    __syncthreads();
+    for (int q = threadIdx.x; q < G::kBQ; q += gemm::kThreads) {
+      float top = maxima[0][q];
 #pragma unroll
-    for (int x = 1; x < G::kWP; ++x) top = fmaxf(top, maxima[x * G::kBQ + q]);
-    float sum = 0.0f;
+      for (int x = 1; x < G::kWP; ++x) top = fmaxf(top, maxima[x][q]);
+      float sum = 0.0f;
 #pragma unroll
-    for (int x = 0; x < G::kWP; ++x) {
-      const float s = sums[x * G::kBQ + q];
-      if (s != 0.0f) sum += s * __builtin_amdgcn_exp2f(maxima[x * G::kBQ + q] - top);
+      for (int x = 0; x < G::kWP; ++x) {
+        const float s = sums[x][q];
+        if (s != 0.0f) sum += s * __builtin_amdgcn_exp2f(maxima[x][q] - top);
+      }
+      part[to + q] = make_float2(top, sum);
     }
-    part[static_cast<int64_t>(tp) * pad + q0 + q] = make_float2(top, sum);
+    if (id >= total) return;
   }
 }
 
@@ -360,37 +390,60 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void lse_tiles_kernel(
 // lse2_m)), zero for rows and columns that are not there.
 template <typename G, typename T>
 __global__ __launch_bounds__(gemm::kThreads, 2) void softmax_grad_kernel(
-    Operand w, Operand h, const int32_t* __restrict__ count, int32_t c, int32_t np, int32_t nq,
-    float scale, const float* __restrict__ lse2, const float* __restrict__ coef,
-    uint16_t* __restrict__ dz, int64_t ld) {
+    Operand w, Operand h, const int32_t* __restrict__ count, int32_t c, int32_t np, float scale,
+    const float* __restrict__ lse2, const float* __restrict__ coef, uint16_t* __restrict__ dz,
+    int64_t ld) {
   __shared__ __attribute__((aligned(1024))) char smem[G::kLdsBytes];
-  int tp, tq;
-  gemm::tile_of(gemm::xcd_run(blockIdx.x, gridDim.x), np, nq, tp, tq);
-  const int p0 = tp * G::kBP, q0 = tq * G::kBQ;
   const int rows = *count;
-  if (q0 >= round_up(rows, kRowPad)) return;
+  const int nq = row_tiles_of(rows, G::kBQ), total = np * nq;
+  int id = blockIdx.x;
+  if (id >= total) return;
   G tile;
-  tile.run(w, h, p0, q0, 0, c / gemm::kStep, smem);
-  const int left = w.rows - p0;
+  int tp, tq;
+  gemm::tile_of(gemm::xcd_run(id, total), np, nq, tp, tq);
+  tile.begin(w, h, tp * G::kBP, tq * G::kBQ, 0, c / gemm::kStep, smem);
+  G::arrive();
+  while (true) {
+    const int p0 = tp * G::kBP, q0 = tq * G::kBQ;
+    float from[G::TQ], co[G::TQ];
 #pragma unroll
-  for (int j = 0; j < G::TQ; ++j) {
-    const int m = q0 + G::column(j);
-    const bool here = m < rows;
-    const float from = here ? lse2[m] : 0.0f;
-    const float co = here ? coef[m] : 0.0f;
-    uint16_t* to = dz + static_cast<int64_t>(m) * ld + p0;
-#pragma unroll
-    for (int q = 0; q < G::TP; ++q) {
-      const f32x4 z = tile.acc[q][j];
-      float x[4];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float e = co * __builtin_amdgcn_exp2f(fmaf(z[r], scale, -from));
-        x[r] = here && G::row(q) + r < left ? e : 0.0f;
-      }
-      *reinterpret_cast<uint2*>(to + G::row(q)) =
-          make_uint2(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]));
+    for (int j = 0; j < G::TQ; ++j) {
+      const int m = q0 + G::column(j);
+      from[j] = m < rows ? lse2[m] : 0.0f;
+      co[j] = m < rows ? coef[m] : 0.0f;
     }
+    tile.multiply(smem);
+    // The compiler's wait for these comes here, not behind the loads that
+    // begin starts, which it does not count.
+#pragma unroll
+    for (int j = 0; j < G::TQ; ++j) asm volatile("" : "+v"(from[j]), "+v"(co[j]));
+    id += gridDim.x;
+    if (id < total) {
+      gemm::tile_of(gemm::xcd_run(id, total), np, nq, tp, tq);
+      tile.begin(w, h, tp * G::kBP, tq * G::kBQ, 0, c / gemm::kStep, smem);
+    }
+    const int left = w.rows - p0;
+    const bool all = left >= G::kBP && rows - q0 >= G::kBQ;
+#pragma unroll
+    for (int j = 0; j < G::TQ; ++j) {
+      const bool here = q0 + G::column(j) < rows;
+      uint2 out[G::TP];
+#pragma unroll
+      for (int i = 0; i < G::TP; ++i) {
+        float x[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          x[r] = co[j] * __builtin_amdgcn_exp2f(fmaf(tile.acc[i][j][r], scale, -from[j]));
+          if (!all) x[r] = here && G::row(i) + r < left ? x[r] : 0.0f;
+        }
+        out[i] = make_uint2(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]));
+      }
+      // The next tile's loads are waited for before the first store, which
+      // would have to be waited for with them.
+      if (j == 0) G::arrive();
+      gemm::store_column<G>(dz + q0 * ld + p0, ld, G::kBP, G::kBQ, j, out);
+    }
+    if (id >= total) return;
   }
 }
 
@@ -413,35 +466,52 @@ __global__ __launch_bounds__(256) void target_grad_kernel(int32_t k, int32_t voc
   dz[m * ld + v] = from_f32<T>(coef[m] * (p - s.target[at]));
 }
 
-// D[c][m] = sum over this split's vocabulary of W[v][c] dz[m][v], to slab
-// [m][c] (fp32).
+// D[c][m] = sum over a split's vocabulary of W[v][c] dz[m][v], to slab [m][c]
+// of the split (fp32).
 template <typename G, typename T>
 __global__ __launch_bounds__(gemm::kThreads, 2) void hidden_grad_kernel(
     Operand w, Operand dz, const int32_t* __restrict__ count, int32_t steps, int32_t split_steps,
-    int32_t np, int32_t nq, int32_t c_all,
-    float* __restrict__ slabs, int64_t slab) {
+    int32_t splits, int32_t np, int32_t c, float* __restrict__ slabs, int64_t slab) {
   __shared__ __attribute__((aligned(1024))) char smem[G::kLdsBytes];
-  int tp, tq;
-  gemm::tile_of(gemm::xcd_run(blockIdx.x, gridDim.x), np, nq, tp, tq);
-  const int p0 = tp * G::kBP, q0 = tq * G::kBQ;
   const int rows = *count;
-  if (q0 >= rows) return;
-  const int first = blockIdx.y * split_steps;
-  const int mine = steps - first < split_steps ? steps - first : split_steps;
+  const int nq = row_tiles_of(rows, G::kBQ), each = np * nq, total = each * splits;
+  int id = blockIdx.x;
+  if (id >= total) return;
   G tile;
-  tile.run(w, dz, p0, q0, first * gemm::kStep, mine, smem);
-  float* out = slabs + blockIdx.y * slab;
+  int tp, tq, split;
+  const auto begin = [&] {
+    const int at = gemm::xcd_run(id, total);
+    split = at / each;
+    gemm::tile_of(at - split * each, np, nq, tp, tq);
+    const int first = split * split_steps;
+    const int left = steps - first;
+    tile.begin(w, dz, tp * G::kBP, tq * G::kBQ, first * gemm::kStep,
+               left < split_steps ? left : split_steps, smem);
+  };
+  begin();
+  G::arrive();
+  while (true) {
+    tile.multiply(smem);
+    const int p0 = tp * G::kBP, q0 = tq * G::kBQ;
+    float* out = slabs + split * slab;
+    id += gridDim.x;
+    if (id < total) {
+      begin();
+      G::arrive();
+    }
 #pragma unroll
-  for (int j = 0; j < G::TQ; ++j) {
-    const int m = q0 + G::column(j);
-    if (m >= rows) continue;
+    for (int j = 0; j < G::TQ; ++j) {
+      const int m = q0 + G::column(j);
+      if (m >= rows) continue;
 #pragma unroll
-    for (int q = 0; q < G::TP; ++q) {
-      const int c = p0 + G::row(q);
-      if (c < c_all) {
-        *reinterpret_cast<f32x4*>(out + static_cast<int64_t>(m) * c_all + c) = tile.acc[q][j];
+      for (int i = 0; i < G::TP; ++i) {
+        const int x = p0 + G::row(i);
+        if (x < c) {
+          *reinterpret_cast<f32x4*>(out + static_cast<int64_t>(m) * c + x) = tile.acc[i][j];
+        }
       }
     }
+    if (id >= total) return;
   }
 }
 
@@ -475,28 +545,38 @@ __global__ __launch_bounds__(256) void hidden_grad_rows_kernel(
 template <typename G, typename T>
 __global__ __launch_bounds__(gemm::kThreads, 2) void weight_grad_kernel(
     Operand h, Operand dz, const int32_t* __restrict__ count, int32_t columns, int32_t np,
-    int32_t nq, int32_t c_all, const float* __restrict__ scale, uint16_t* __restrict__ dw) {
+    int32_t nq, int32_t c, const float* __restrict__ scale, uint16_t* __restrict__ dw) {
   __shared__ __attribute__((aligned(1024))) char smem[G::kLdsBytes];
-  int tp, tq;
-  gemm::tile_of(gemm::xcd_run(blockIdx.x, gridDim.x), np, nq, tp, tq);
-  const int p0 = tp * G::kBP, q0 = tq * G::kBQ;
   const int steps = static_cast<int>(round_up(*count, gemm::kStep) / gemm::kStep);
+  const int total = np * nq;
+  int id = blockIdx.x;
   G tile;
-  tile.run(h, dz, p0, q0, 0, steps, smem);
+  int tp, tq;
+  gemm::tile_of(gemm::xcd_run(id, total), np, nq, tp, tq);
+  tile.begin(h, dz, tp * G::kBP, tq * G::kBQ, 0, steps, smem);
+  G::arrive();
   const float by = *scale;
-#pragma unroll
-  for (int j = 0; j < G::TQ; ++j) {
-    const int v = q0 + G::column(j);
-    if (v >= columns) continue;
-#pragma unroll
-    for (int q = 0; q < G::TP; ++q) {
-      const int c = p0 + G::row(q);
-      if (c < c_all) {
-        const f32x4 x = tile.acc[q][j] * by;
-        *reinterpret_cast<uint2*>(dw + static_cast<int64_t>(v) * c_all + c) =
-            make_uint2(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]));
-      }
+  while (true) {
+    tile.multiply(smem);
+    const int p0 = tp * G::kBP, q0 = tq * G::kBQ;
+    id += gridDim.x;
+    if (id < total) {
+      gemm::tile_of(gemm::xcd_run(id, total), np, nq, tp, tq);
+      tile.begin(h, dz, tp * G::kBP, tq * G::kBQ, 0, steps, smem);
+      G::arrive();
     }
+#pragma unroll
+    for (int j = 0; j < G::TQ; ++j) {
+      uint2 out[G::TP];
+#pragma unroll
+      for (int i = 0; i < G::TP; ++i) {
+        const f32x4 y = tile.acc[i][j] * by;
+        out[i] = make_uint2(pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]));
+      }
+      gemm::store_column<G>(dw + static_cast<int64_t>(q0) * c + p0, c, c - p0, columns - q0, j,
+                            out);
+    }
+    if (id >= total) return;
   }
 }
 
@@ -510,34 +590,50 @@ __device__ __forceinline__ float2 joined(float2 a, float2 b) {
                               b.y * __builtin_amdgcn_exp2f(b.x - top));
 }
 
-// A workgroup takes 32 rows, 8 threads a row: joins the tiles' maxima and
-// sums to lse2[m], and the row's loss. row_loss (by i) or partial (by m).
-__global__ __launch_bounds__(256) void join_tiles_kernel(const float2* __restrict__ part,
-                                                         int32_t tiles, int64_t pad,
-                                                         const float* __restrict__ target_term,
-                                                         float temperature2, float* row_loss,
-                                                         float* partial, Saved s) {
-  __shared__ float2 shared[8][32];
+// A workgroup takes 32 rows, 32 threads a row: joins the tiles' maxima and
+// sums to lse2[m], and the row's loss. row_loss (by i) or partial (by m). A
+// thread has 8 tiles under way at a time, all of those of 65536 columns.
+__global__ __launch_bounds__(1024) void join_tiles_kernel(const float2* __restrict__ part,
+                                                          int32_t tiles, int64_t pad,
+                                                          const float* __restrict__ target_term,
+                                                          float temperature2, float* row_loss,
+                                                          float* partial, Saved s) {
+  __shared__ float2 shared[32][33];
   const int q = threadIdx.x & 31, slice = threadIdx.x >> 5;
   const int m = blockIdx.x * 32 + q;
   const int count = *s.count;
   if (static_cast<int>(blockIdx.x) * 32 >= count) return;
   float2 all = make_float2(-__builtin_inff(), 0.0f);
   if (m < count) {
-    for (int t = slice; t < tiles; t += 8) all = joined(all, part[t * pad + m]);
-  }
-  shared[slice][q] = all;
-  __syncthreads();
-  if (slice != 0 || m >= count) return;
+    for (int t = slice; t < tiles; t += 256) {
+      float2 x[8];
 #pragma unroll
-  for (int t = 1; t < 8; ++t) all = joined(all, shared[t][q]);
+      for (int u = 0; u < 8; ++u) {
+        x[u] = t + 32 * u < tiles ? part[(t + 32 * u) * pad + m]
+                                  : make_float2(-__builtin_inff(), 0.0f);
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) all = joined(all, x[u]);
+    }
+  }
+  shared[q][slice] = all;
+  __syncthreads();
+  // 32 rows by 32 slices, turned: 32 lanes join a row's slices.
+  const int row = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  all = shared[row][lane];
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    all = joined(all, make_float2(__shfl_xor(all.x, off, 64), __shfl_xor(all.y, off, 64)));
+  }
+  const int mine = blockIdx.x * 32 + row;
+  if (lane != 0 || mine >= count) return;
   const float lse2 = all.x + __builtin_amdgcn_logf(all.y);
-  const float term = target_term[m];
+  const float term = target_term[mine];
   // A target out of range makes its row NaN in the backward too.
-  s.lse2[m] = term == term ? lse2 : term;
+  s.lse2[mine] = term == term ? lse2 : term;
   const float loss = temperature2 * (lse2 * kLn2 + term);
-  if (row_loss) row_loss[s.row[m]] = loss;
-  if (partial) partial[m] = loss;
+  if (row_loss) row_loss[s.row[mine]] = loss;
+  if (partial) partial[mine] = loss;
 }
 
 // Loss 0 for rows that take no part (reduction none).
@@ -703,8 +799,8 @@ void launch_lse_tiles(const Shape& d, const void* weight, const Saved& s, const 
   const int nq = static_cast<int>(row_tiles(d.n));
   const Operand a{static_cast<const uint16_t*>(weight), d.c, d.vocab};
   const Operand b{s.hidden, d.c, static_cast<int32_t>(pad)};
-  hipLaunchKernelGGL((lse_tiles_kernel<G, T>), dim3(np * nq), dim3(gemm::kThreads), 0, stream, a,
-                     b, s.count, d.c, np, nq, scale, w.part, pad);
+  hipLaunchKernelGGL((lse_tiles_kernel<G, T>), dim3(std::min(np * nq, kCus)),
+                     dim3(gemm::kThreads), 0, stream, a, b, s.count, d.c, np, scale, w.part, pad);
 }
 
 template <typename T>
@@ -725,7 +821,7 @@ int run_forward(const Shape& d, const void* hidden, const void* weight, float te
     launch_lse_tiles<LargeTile<T, Major::kK, Major::kK>, T>(d, weight, s, w, scale, stream);
   }
   const int tiles = static_cast<int>(round_up(d.vocab, kVocabTile) / kVocabTile);
-  hipLaunchKernelGGL(join_tiles_kernel, dim3((n + 31) / 32), dim3(256), 0, stream, w.part, tiles,
+  hipLaunchKernelGGL(join_tiles_kernel, dim3((n + 31) / 32), dim3(1024), 0, stream, w.part, tiles,
                      pad, w.target_term, temperature * temperature, per_row ? loss : nullptr,
                      per_row ? nullptr : w.partial, s);
   if (per_row) {
@@ -757,8 +853,9 @@ void launch_piece(const Shape& d, const Pieces& pieces, int piece, const uint16_
   const Operand h{s.hidden, d.c, static_cast<int32_t>(pad)};
   // Rows of dz that hold something: whole tiles.
   const Operand dz{w.dz, ld, static_cast<int32_t>(std::min<int64_t>(pad, nq * Logits::kBQ))};
-  hipLaunchKernelGGL((softmax_grad_kernel<Logits, T>), dim3(np * nq), dim3(gemm::kThreads), 0,
-                     stream, wp, h, s.count, d.c, np, nq, scale, s.lse2, w.coef, w.dz, ld);
+  hipLaunchKernelGGL((softmax_grad_kernel<Logits, T>), dim3(std::min(np * nq, kCus)),
+                     dim3(gemm::kThreads), 0, stream, wp, h, s.count, d.c, np, scale, s.lse2,
+                     w.coef, w.dz, ld);
   const int64_t entries = d.n * d.k;
   hipLaunchKernelGGL((target_grad_kernel<T>), dim3(static_cast<unsigned>((entries + 255) / 256)),
                      dim3(256), 0, stream, d.k, first, columns, scale, w.coef, w.dz, ld, s);
@@ -767,13 +864,13 @@ void launch_piece(const Shape& d, const Pieces& pieces, int piece, const uint16_
     const int each = (pieces.columns / gemm::kStep + pieces.splits - 1) / pieces.splits;
     const int64_t slab = d.n * d.c;
     hipLaunchKernelGGL((hidden_grad_kernel<Hidden, T>),
-                       dim3(nc * nq, static_cast<unsigned>(pieces.splits)), dim3(gemm::kThreads),
-                       0, stream, wp, dz, s.count, steps, each, nc, nq, d.c,
+                       dim3(std::min(nc * nq * pieces.splits, kCus)), dim3(gemm::kThreads), 0,
+                       stream, wp, dz, s.count, steps, each, pieces.splits, nc, d.c,
                        w.slabs + piece * pieces.splits * slab, slab);
   }
   if (dw != nullptr) {
-    hipLaunchKernelGGL((weight_grad_kernel<Weight, T>), dim3(nc * np), dim3(gemm::kThreads), 0,
-                       stream, h, dz, s.count, columns, nc, np, d.c, w.scale,
+    hipLaunchKernelGGL((weight_grad_kernel<Weight, T>), dim3(std::min(nc * np, kCus)),
+                       dim3(gemm::kThreads), 0, stream, h, dz, s.count, columns, nc, np, d.c, w.scale,
                        dw + static_cast<int64_t>(first) * d.c);
   }
 }

@@ -95,8 +95,10 @@ DISTILLATION = (
 
 
 class _LinearLoss(torch.autograd.Function):
-    """Forward keeps the rows that take part, their log sums and target logits
-    (one buffer) and the weight; backward makes the logits again, piece by piece."""
+    """Calls that the native whole call declines (tensor subclasses, modes, no
+    rows). Forward keeps the rows that take part, their log sums and target
+    logits (one buffer) and the weight; backward makes the logits again, piece
+    by piece."""
 
     @staticmethod
     def forward(ctx, hidden, weight, launch, top, temperature, reduction):
@@ -155,8 +157,13 @@ def pretrain_linear_cross_entropy(
     per row (0 for rows that take no part), their mean over the rows that take
     part (0 if none does) or their sum. Gradients for hidden and weight.
     """
-    ns = dict(locals())
-    C.enforce(CROSS_ENTROPY, ns)
+    call = C.whole_call("linear_loss_call")
+    if call and isinstance(reduction, str) and reduction in REDUCTIONS:
+        loss = call(hidden, weight, targets, None, ignore_index, 1.0, REDUCTIONS[reduction])
+        if loss is not None:
+            return loss
+    C.enforce(CROSS_ENTROPY, {"hidden": hidden, "weight": weight, "targets": targets,
+                              "ignore_index": ignore_index, "reduction": reduction})
 
     def launch(h, w):
         return C.native().linear_cross_entropy_forward(h, w, targets, ignore_index,
@@ -185,8 +192,16 @@ def pretrain_linear_topk_distillation(
     :func:`pretrain_linear_cross_entropy`. A token listed twice counts with the
     sum of its p. Gradients for hidden and weight; none for the teacher.
     """
-    ns = dict(locals())
-    C.enforce(DISTILLATION, ns)
+    call = C.whole_call("linear_loss_call") if teacher_logits is not None else None
+    if call and isinstance(reduction, str) and reduction in REDUCTIONS:
+        loss = call(hidden, weight, teacher_indices, teacher_logits, 0, temperature,
+                    REDUCTIONS[reduction])
+        if loss is not None:
+            return loss
+    C.enforce(DISTILLATION, {"hidden": hidden, "weight": weight,
+                             "teacher_logits": teacher_logits,
+                             "teacher_indices": teacher_indices, "temperature": temperature,
+                             "reduction": reduction})
 
     def launch(h, w):
         return C.native().linear_topk_distillation_forward(

@@ -80,16 +80,21 @@ def infer_layer_norm_forward_varlen(
 ) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
     """Layer norm of packed rows ``[total_tokens, C]``; with ``residual`` the
     norm of ``x + residual``. Returns ``y``, or ``(y, stream)`` with a residual."""
-    ns = dict(locals())
+    if call := C.whole_call("layer_norm_infer_call"):
+        out = call(x, residual, weight, bias, eps)
+        if out is not None:
+            return out
+    ns = {"x": x, "weight": weight, "bias": bias, "residual": residual, "eps": eps}
     _enforce(INFER, ns)
     out = C.native().layer_norm_forward(x, residual, weight, bias, eps)
     return out[0] if residual is None else (out[0], out[1])
 
 
 class _LayerNorm(torch.autograd.Function):
-    """Forward keeps the rows that were normed (x itself without a residual)
-    and their mean and rstd; backward is one pass over them and the ordered
-    sum of the weight's and bias' gradients."""
+    """Calls that the native whole call declines (tensor subclasses, modes, empty
+    rows). Forward keeps the rows that were normed (x itself without a residual)
+    and their mean and rstd; backward is one pass over them and the ordered sum
+    of the weight's and bias' gradients."""
 
     @staticmethod
     def forward(ctx, x, residual, weight, bias, eps):
@@ -134,7 +139,11 @@ def pretrain_layer_norm(
     ``residual`` it is the norm of ``stream = x + residual``, returned as
     ``(y, stream)``: the stream goes on to the next block, and its gradient
     joins the norm's in one pass. ``x`` and ``residual`` have the same gradient."""
-    ns = dict(locals())
+    if call := C.whole_call("layer_norm_train_call"):
+        out = call(x, residual, weight, bias, eps)
+        if out is not None:
+            return out
+    ns = {"x": x, "weight": weight, "bias": bias, "residual": residual, "eps": eps}
     _enforce(PRETRAIN, ns)
     C.native()
     if torch.cuda.is_current_stream_capturing():

@@ -245,3 +245,30 @@ def test_inference_form_under_graph_capture():
         want = step()
         torch.cuda.synchronize()
         assert torch.equal(y, want[0]) and torch.equal(stream, want[1])
+
+
+class _Sub(torch.Tensor):
+    """A tensor subclass: no whole call, the wrapper's own tables and autograd function."""
+
+
+def test_calls_that_are_not_plain_give_the_same_bits():
+    case = _inputs(40, 384, torch.float16, seed=30, residual=True)
+    names = ("x", "weight", "bias", "residual")
+    plain = [case[n].clone().requires_grad_() for n in names]
+    y, stream = pretrain_layer_norm(*plain[:3], residual=plain[3])
+    grads = torch.autograd.grad((y, stream), plain, (case["dy"], case["ds"]))
+    sub = [case[n].clone().as_subclass(_Sub).requires_grad_() for n in names]
+    y2, stream2 = pretrain_layer_norm(*sub[:3], residual=sub[3])
+    grads2 = torch.autograd.grad((y2, stream2), sub, (case["dy"], case["ds"]))
+    for a, b in zip((y, stream, *grads), (y2, stream2, *grads2)):
+        assert torch.equal(a, b.as_subclass(torch.Tensor))
+
+
+@pytest.mark.parametrize("kind", [torch.Tensor, _Sub])
+def test_differentiating_twice_raises(kind):
+    case = _inputs(4, 64, torch.float32, seed=31)
+    x = case["x"].clone().as_subclass(kind).requires_grad_()
+    y = pretrain_layer_norm(x, case["weight"], case["bias"])
+    dx, = torch.autograd.grad(y, x, torch.ones_like(y).requires_grad_(), create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiate twice"):
+        dx.sum().backward()

@@ -375,3 +375,32 @@ def test_shapes_repeats_and_other_streams():
                        h.clone(), w.clone(), one.clone())
     side.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(flat, again))
+
+
+class _Sub(torch.Tensor):
+    """A tensor subclass: no whole call, the wrapper's own tables and autograd function."""
+
+
+@pytest.mark.parametrize("reduction", ["none", "mean"])
+def test_calls_that_are_not_plain_give_the_same_bits(reduction):
+    h, w = _head(50, 128, 300, torch.float16, seed=26)
+    targets = torch.randint(300, (50,), generator=_gen(27)).to(DEV)
+    logits, tokens = _teacher(50, 8, 300, seed=28)
+    upstream = _upstream(reduction, 50, seed=29)
+    for call in (lambda a, b: pretrain_linear_cross_entropy(a, b, targets, reduction=reduction),
+                 lambda a, b: pretrain_linear_topk_distillation(
+                     a, b, logits, tokens, temperature=2, reduction=reduction)):
+        plain = _grads(call, h, w, upstream)
+        other = _grads(call, h.as_subclass(_Sub), w.as_subclass(_Sub), upstream)
+        assert all(torch.equal(a, b.as_subclass(torch.Tensor)) for a, b in zip(plain, other))
+
+
+@pytest.mark.parametrize("kind", [torch.Tensor, _Sub])
+def test_differentiating_twice_raises(kind):
+    h, w = _head(5, 64, 30, torch.bfloat16, seed=30)
+    h = h.as_subclass(kind).requires_grad_()
+    loss = pretrain_linear_cross_entropy(h, w, torch.zeros(5, dtype=torch.int64, device=DEV))
+    dh, = torch.autograd.grad(loss, h, torch.ones((), device=DEV, requires_grad=True),
+                              create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiate twice"):
+        dh.sum().backward()
