@@ -29,6 +29,7 @@
 // 16 bits before the outputs, as a matrix operand has to be (relative error
 // 2^-9 an entry for bf16, independent between entries).
 #include <algorithm>
+#include <type_traits>
 
 #include "capi_internal.h"
 #include "gemm_tile.h"
@@ -43,7 +44,8 @@ using gemm::Operand;
 
 constexpr float kLn2 = 0.69314718055994531f;
 constexpr int kRowPad = 256;       // rows of workspaces, and a product's largest tile
-constexpr int kVocabTile = 256;    // columns whose maximum and sum the forward keeps together
+constexpr int kVocabTile = 256;    // pieces of the vocabulary are whole multiples of it
+constexpr int kMinTile = 128;      // fewest columns whose maximum and sum the forward keeps
 constexpr int kScanThreads = 1024;
 constexpr float kNaN = __builtin_nanf("");
 
@@ -123,23 +125,6 @@ __device__ __forceinline__ int32_t as_token(int64_t t, int32_t vocab) {
   return t < 0 ? -1 : t >= vocab ? vocab : static_cast<int32_t>(t);
 }
 
-// Cross entropy: one entry a row, share 1. place[i] = 1 for rows that take part.
-template <typename Index>
-__global__ __launch_bounds__(256) void label_targets_kernel(const Index* __restrict__ targets,
-                                                            int64_t ignore, int32_t n,
-                                                            int32_t vocab, Saved s) {
-  const int i = blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
-  const int64_t t = targets[i];
-  const bool part = t != ignore;
-  s.place[i] = part;
-  const int32_t token = as_token(t, vocab);
-  s.index[i] = part && token < 0 ? vocab : token;
-  s.share[i] = 1.0f;
-  s.target[i] = 1.0f;
-  s.base[i] = 0.0f;
-}
-
 // Distillation, a wave a row: shares from the teacher's logits. An entry is
 // present where its token is not negative and its logit not -inf; a row
 // without one takes no part. Tokens that occur twice in a row count with the
@@ -209,15 +194,17 @@ __global__ __launch_bounds__(256) void teacher_targets_kernel(
   }
 }
 
-// Numbers the rows that take part, in order (one workgroup). place[i]: 1 or 0
-// in, m or -1 out.
-__global__ __launch_bounds__(kScanThreads) void number_rows_kernel(int32_t n, Saved s) {
+// Numbers the rows that take part, in order: part(i) says whether row i does.
+// One workgroup; row_loss (not null): 0 for the rows that do not.
+template <typename Part>
+__device__ __forceinline__ void number_rows(int32_t n, float* row_loss, const Saved& s,
+                                            Part&& part_of) {
   __shared__ int32_t waves[kScanThreads / 64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int32_t before = 0;
   for (int32_t first = 0; first < n; first += kScanThreads) {
     const int32_t i = first + static_cast<int32_t>(threadIdx.x);
-    const bool part = i < n && s.place[i] != 0;
+    const bool part = i < n && part_of(i);
     const uint64_t mask = __ballot(part);
     if (lane == 0) waves[wave] = __popcll(mask);
     __syncthreads();
@@ -230,10 +217,34 @@ __global__ __launch_bounds__(kScanThreads) void number_rows_kernel(int32_t n, Sa
     }
     if (i < n) s.place[i] = part ? m : -1;
     if (part) s.row[m] = i;
+    if (i < n && !part && row_loss != nullptr) row_loss[i] = 0.0f;
     before += all;
     __syncthreads();
   }
   if (threadIdx.x == 0) *s.count = before;
+}
+
+// Cross entropy: one entry a row, share 1.
+template <typename Index>
+__global__ __launch_bounds__(kScanThreads) void label_rows_kernel(
+    const Index* __restrict__ targets, int64_t ignore, int32_t n, int32_t vocab, float* row_loss,
+    Saved s) {
+  number_rows(n, row_loss, s, [&](int32_t i) {
+    const int64_t t = targets[i];
+    const bool part = t != ignore;
+    const int32_t token = as_token(t, vocab);
+    s.index[i] = part && token < 0 ? vocab : token;
+    s.share[i] = 1.0f;
+    s.target[i] = 1.0f;
+    s.base[i] = 0.0f;
+    return part;
+  });
+}
+
+// Distillation, behind teacher_targets_kernel, which leaves 1 or 0 in place[i].
+__global__ __launch_bounds__(kScanThreads) void teacher_rows_kernel(int32_t n, float* row_loss,
+                                                                    Saved s) {
+  number_rows(n, row_loss, s, [&](int32_t i) { return s.place[i] != 0; });
 }
 
 // A workgroup a row m: copies its hidden row (zeros for the rows that fill up
@@ -288,13 +299,13 @@ __global__ __launch_bounds__(256) void gather_rows_kernel(
 }
 
 // ------------------------------------------------------------- products
-// Tile shapes. Few rows: 64 of them against 256 vocabulary columns, three
-// stages deep, since such a call only streams the weight. Otherwise 256 x 256.
+// Tile shapes, chosen on the host by the time they would take (see plan_of).
 template <typename T, Major MA, Major MB>
 using LargeTile = gemm::Tile<T, MA, MB, 256, 256, 2, 4, 2>;
 template <typename T, Major MA, Major MB>
+using SmallTile = gemm::Tile<T, MA, MB, 128, 128, 2, 4, 4>;
+template <typename T, Major MA, Major MB>
 using FewRowsTile = gemm::Tile<T, MA, MB, 256, 64, 8, 1, 3>;
-constexpr int kFewRows = 64;
 
 // The tiles of a product over rows m, whose count stands on the device: the
 // workgroups of a launch of at most one a CU take them in turn. While a
@@ -636,14 +647,6 @@ __global__ __launch_bounds__(1024) void join_tiles_kernel(const float2* __restri
   if (partial) partial[mine] = loss;
 }
 
-// Loss 0 for rows that take no part (reduction none).
-__global__ __launch_bounds__(256) void zero_loss_kernel(int32_t n,
-                                                        const int32_t* __restrict__ place,
-                                                        float* __restrict__ row_loss) {
-  const int i = blockIdx.x * 256 + threadIdx.x;
-  if (i < n && place[i] < 0) row_loss[i] = 0.0f;
-}
-
 // Sum over one workgroup of 1024, in a fixed order.
 __device__ __forceinline__ float block_sum(float x, float* waves) {
   x = wave_sum(x);
@@ -705,50 +708,92 @@ __global__ __launch_bounds__(kScanThreads) void row_coefficients_kernel(
 }
 
 // ---------------------------------------------------------------- launches
-// Bytes of one piece's dz: large enough that a piece's three products fill the
-// GPU for any row count, small beside the logits of a long batch.
-constexpr int64_t kPieceBytes = int64_t{128} << 20;
 constexpr int kCus = 256;
 
-struct Pieces {
-  int32_t columns;  // a multiple of kVocabTile
-  int32_t count;
-  int32_t splits;   // of a piece's columns in dz W
+enum class Size { kFewRows, kSmall, kLarge };
+
+struct TileTime {
+  int32_t p, q;
+  double step_us, fixed_us;  // of 64 k, and of a tile's start and end beside them
 };
 
-bool few_rows(int64_t n) { return n <= kFewRows; }
+// Measured on products that fill the GPU for many rounds.
+constexpr TileTime kTileTimes[] = {{256, 64, 1.0, 3.0}, {128, 128, 0.6, 3.0}, {256, 256, 1.65, 5.0}};
 
-int64_t row_tiles(int64_t n) { return few_rows(n) ? 1 : round_up(n, 256) / 256; }
+const TileTime& time_of(Size s) { return kTileTimes[static_cast<int>(s)]; }
 
-// dz W has (C / 256) x (rows / 256) tiles, often fewer than CUs, over a long k:
-// split k so that the rounds of tiles are full. Work of a choice, in steps of
-// 64 k a CU: rounds x steps a split, plus about 6 steps for each slab written.
-int32_t hidden_grad_splits(int64_t tiles, int64_t steps) {
-  int32_t best = 1;
-  int64_t least = INT64_MAX;
-  for (int32_t s = 1; s <= 16 && (s == 1 || steps / s >= 8); ++s) {
-    const int64_t each = (steps + s - 1) / s;
-    const int64_t cost = (tiles * s + kCus - 1) / kCus * (each + 6);
-    if (cost < least) {
-      least = cost;
-      best = s;
-    }
-  }
-  return best;
+int64_t tiles_of(Size s, int64_t p, int64_t q) {
+  const TileTime& t = time_of(s);
+  return (p + t.p - 1) / t.p * ((q + t.q - 1) / t.q);
 }
 
-Pieces pieces_of(int64_t n, int64_t c, int64_t vocab) {
-  const int64_t pad = round_up(n, kRowPad);
-  const int64_t all = round_up(vocab, kVocabTile);
-  int64_t columns = kPieceBytes / (pad * 2) / kVocabTile * kVocabTile;
-  columns = std::min(std::max<int64_t>(columns, kVocabTile), all);
-  Pieces p;
-  p.count = static_cast<int32_t>((all + columns - 1) / columns);
-  p.columns = static_cast<int32_t>(round_up((all + p.count - 1) / p.count, kVocabTile));
-  p.count = static_cast<int32_t>((all + p.columns - 1) / p.columns);
-  p.splits = hidden_grad_splits(round_up(c, 256) / 256 * row_tiles(n),
-                                p.columns / gemm::kStep);
-  return p;
+double product_us(Size s, int64_t p, int64_t q, int64_t steps, int64_t splits = 1) {
+  const int64_t rounds = (tiles_of(s, p, q) * splits + kCus - 1) / kCus;
+  return rounds * ((steps + splits - 1) / splits * time_of(s).step_us + time_of(s).fixed_us);
+}
+
+Size size_of(int64_t p, int64_t q, int64_t steps, bool rows_are_q) {
+  if (rows_are_q && q <= time_of(Size::kFewRows).q) return Size::kFewRows;
+  return product_us(Size::kSmall, p, q, steps) < product_us(Size::kLarge, p, q, steps)
+             ? Size::kSmall : Size::kLarge;
+}
+
+// How the backward goes through the vocabulary.
+struct Plan {
+  int32_t columns;  // of a piece, a multiple of kVocabTile
+  int32_t pieces;
+  int32_t splits;   // of a piece's columns in dz W, whose tiles are few and whose k is long
+  Size logits, hidden, weight;
+};
+
+// dz of a piece up to kCachedBytes is written and read in the last-level cache;
+// beyond, its traffic is partly hidden by the products (4096 x 65536 x 2048 in
+// pieces of 128, 256 and 512 MB: 2612, 2700, 2675 us; 8192 x 65536 x 4096, whose
+// slabs weigh more: 9784, 9749, 9715 us). A slab is written once and read once.
+constexpr int64_t kCachedBytes = int64_t{192} << 20;
+constexpr int64_t kMostBytes = int64_t{512} << 20;
+constexpr double kGradBytesPerUs = 20.0e6;
+constexpr double kSlabBytesPerUs = 4.0e6;
+
+Plan plan_of(int64_t n, int64_t c, int64_t vocab) {
+  const int64_t all = round_up(vocab, kVocabTile), pad = round_up(n, kRowPad);
+  const int64_t steps_c = c / gemm::kStep, steps_n = (n + gemm::kStep - 1) / gemm::kStep;
+  Plan best{};
+  double least = 1e300;
+  int32_t last = 0;
+  for (int64_t pieces = 1; pieces <= all / kVocabTile; ++pieces) {
+    Plan p;
+    p.columns = static_cast<int32_t>(round_up((all + pieces - 1) / pieces, kVocabTile));
+    p.pieces = static_cast<int32_t>((all + p.columns - 1) / p.columns);
+    if (p.columns == last) continue;
+    last = p.columns;
+    const int64_t bytes = pad * p.columns * 2;
+    if (bytes > kMostBytes && p.columns > kVocabTile) continue;
+    p.logits = size_of(p.columns, n, steps_c, true);
+    p.weight = size_of(c, p.columns, steps_n, false);
+    double us = 12.0 + product_us(p.logits, p.columns, n, steps_c) +
+                product_us(p.weight, c, p.columns, steps_n) +
+                (bytes > kCachedBytes ? 3 * bytes / kGradBytesPerUs : 0.0);
+    const int64_t steps = p.columns / gemm::kStep;
+    double hidden = 1e300;
+    for (Size size : {Size::kFewRows, Size::kSmall, Size::kLarge}) {
+      if ((size == Size::kFewRows) != (n <= time_of(Size::kFewRows).q)) continue;
+      for (int32_t s = 1; s <= 16 && (s == 1 || steps / s >= 8); ++s) {
+        const double t = product_us(size, c, n, steps, s) + s * (4.0 * n * c / kSlabBytesPerUs);
+        if (t >= hidden) continue;
+        hidden = t;
+        p.splits = s;
+        p.hidden = size;
+      }
+    }
+    us = (us + hidden) * p.pieces;
+    if (us < least) {
+      least = us;
+      best = p;
+    }
+    if (bytes < kCachedBytes / 8) break;  // smaller pieces only add launches
+  }
+  return best;
 }
 
 struct ForwardWork {
@@ -760,7 +805,7 @@ struct ForwardWork {
 ForwardWork forward_work(char* p, int64_t n, int64_t vocab, size_t* bytes) {
   const int64_t pad = round_up(n, kRowPad);
   Layout l;
-  const size_t part = l.take(round_up(vocab, kVocabTile) / kVocabTile * pad * 8);
+  const size_t part = l.take(round_up(vocab, kMinTile) / kMinTile * pad * 8);
   const size_t term = l.take(pad * 4), partial = l.take(pad * 4);
   *bytes = l.bytes;
   return {reinterpret_cast<float2*>(p + part), reinterpret_cast<float*>(p + term),
@@ -774,13 +819,13 @@ struct BackwardWork {
   float* slabs;
 };
 
-BackwardWork backward_work(char* p, int64_t n, int64_t c, const Pieces& pieces, bool hidden,
+BackwardWork backward_work(char* p, int64_t n, int64_t c, const Plan& plan, bool hidden,
                            size_t* bytes) {
   const int64_t pad = round_up(n, kRowPad);
   Layout l;
-  const size_t coef = l.take(pad * 4), scale = l.take(4), dz = l.take(pad * pieces.columns * 2);
+  const size_t coef = l.take(pad * 4), scale = l.take(4), dz = l.take(pad * plan.columns * 2);
   const size_t slabs =
-      l.take(hidden ? static_cast<size_t>(pieces.count) * pieces.splits * n * c * 4 : 0);
+      l.take(hidden ? static_cast<size_t>(plan.pieces) * plan.splits * n * c * 4 : 0);
   *bytes = l.bytes;
   return {reinterpret_cast<float*>(p + coef), reinterpret_cast<float*>(p + scale),
           reinterpret_cast<uint16_t*>(p + dz), reinterpret_cast<float*>(p + slabs)};
@@ -791,17 +836,21 @@ struct Shape {
   int32_t c, vocab, k;
 };
 
-template <typename G, typename T>
-void launch_lse_tiles(const Shape& d, const void* weight, const Saved& s, const ForwardWork& w,
-                      float scale, hipStream_t stream) {
-  const int64_t pad = round_up(d.n, kRowPad);
-  const int np = static_cast<int>(round_up(d.vocab, G::kBP) / G::kBP);
-  const int nq = static_cast<int>(row_tiles(d.n));
-  const Operand a{static_cast<const uint16_t*>(weight), d.c, d.vocab};
-  const Operand b{s.hidden, d.c, static_cast<int32_t>(pad)};
-  hipLaunchKernelGGL((lse_tiles_kernel<G, T>), dim3(std::min(np * nq, kCus)),
-                     dim3(gemm::kThreads), 0, stream, a, b, s.count, d.c, np, scale, w.part, pad);
+// f(tile type) for a size.
+template <typename T, Major MA, Major MB, typename F>
+void with_tile(Size size, F&& f) {
+  switch (size) {
+    case Size::kFewRows:
+      if constexpr (MB == Major::kK) f(static_cast<FewRowsTile<T, MA, MB>*>(nullptr));
+      return;
+    case Size::kSmall:
+      return f(static_cast<SmallTile<T, MA, MB>*>(nullptr));
+    case Size::kLarge:
+      return f(static_cast<LargeTile<T, MA, MB>*>(nullptr));
+  }
 }
+
+int grid_of(int64_t tiles) { return static_cast<int>(std::min<int64_t>(tiles, kCus)); }
 
 template <typename T>
 int run_forward(const Shape& d, const void* hidden, const void* weight, float temperature,
@@ -810,94 +859,93 @@ int run_forward(const Shape& d, const void* hidden, const void* weight, float te
   const int64_t pad = round_up(d.n, kRowPad);
   const float scale = kLog2E / temperature;
   const int n = static_cast<int>(d.n);
-  hipLaunchKernelGGL(number_rows_kernel, dim3(1), dim3(kScanThreads), 0, stream, n, s);
   hipLaunchKernelGGL((gather_rows_kernel<T>), dim3(static_cast<unsigned>(pad)), dim3(256), 0,
                      stream, static_cast<const uint16_t*>(hidden),
                      static_cast<const uint16_t*>(weight), d.c, d.k, d.vocab, 1.0f / temperature,
                      w.target_term, s);
-  if (few_rows(d.n)) {
-    launch_lse_tiles<FewRowsTile<T, Major::kK, Major::kK>, T>(d, weight, s, w, scale, stream);
-  } else {
-    launch_lse_tiles<LargeTile<T, Major::kK, Major::kK>, T>(d, weight, s, w, scale, stream);
-  }
-  const int tiles = static_cast<int>(round_up(d.vocab, kVocabTile) / kVocabTile);
+  const Size size = size_of(d.vocab, d.n, d.c / gemm::kStep, true);
+  const int tiles = (d.vocab + time_of(size).p - 1) / time_of(size).p;
+  const Operand a{static_cast<const uint16_t*>(weight), d.c, d.vocab};
+  const Operand b{s.hidden, d.c, static_cast<int32_t>(pad)};
+  with_tile<T, Major::kK, Major::kK>(size, [&](auto* tile) {
+    using G = std::remove_pointer_t<decltype(tile)>;
+    hipLaunchKernelGGL((lse_tiles_kernel<G, T>), dim3(grid_of(tiles_of(size, d.vocab, d.n))),
+                       dim3(gemm::kThreads), 0, stream, a, b, s.count, d.c, tiles, scale, w.part,
+                       pad);
+  });
   hipLaunchKernelGGL(join_tiles_kernel, dim3((n + 31) / 32), dim3(1024), 0, stream, w.part, tiles,
                      pad, w.target_term, temperature * temperature, per_row ? loss : nullptr,
                      per_row ? nullptr : w.partial, s);
-  if (per_row) {
-    hipLaunchKernelGGL(zero_loss_kernel, dim3((n + 255) / 256), dim3(256), 0, stream, n, s.place,
-                       loss);
-  } else {
+  if (!per_row) {
     hipLaunchKernelGGL(sum_losses_kernel, dim3(1), dim3(kScanThreads), 0, stream, w.partial,
                        s.count, mean, loss);
   }
   return check_launch("linear loss forward");
 }
 
-template <typename T, template <typename, Major, Major> class G>
-void launch_piece(const Shape& d, const Pieces& pieces, int piece, const uint16_t* weight,
+template <typename T>
+void launch_piece(const Shape& d, const Plan& plan, int piece, const uint16_t* weight,
                   float scale, uint16_t* dh, uint16_t* dw, const Saved& s, const BackwardWork& w,
                   hipStream_t stream) {
-  using Logits = G<T, Major::kK, Major::kK>;
-  using Hidden = G<T, Major::kX, Major::kK>;
-  using Weight = LargeTile<T, Major::kX, Major::kX>;
   const int64_t pad = round_up(d.n, kRowPad);
-  const int nq = static_cast<int>(row_tiles(d.n));
-  const int first = piece * pieces.columns;
-  const int columns = std::min(pieces.columns, d.vocab - first);
-  const int np = static_cast<int>(round_up(columns, kVocabTile) / kVocabTile);
-  const int nc = static_cast<int>(round_up(d.c, 256) / 256);
-  const int64_t ld = pieces.columns;
+  const int first = piece * plan.columns;
+  const int columns = std::min(plan.columns, d.vocab - first);
+  const int64_t ld = plan.columns;
   const uint16_t* from = weight + static_cast<int64_t>(first) * d.c;
   const Operand wp{from, d.c, columns};
   const Operand h{s.hidden, d.c, static_cast<int32_t>(pad)};
-  // Rows of dz that hold something: whole tiles.
-  const Operand dz{w.dz, ld, static_cast<int32_t>(std::min<int64_t>(pad, nq * Logits::kBQ))};
-  hipLaunchKernelGGL((softmax_grad_kernel<Logits, T>), dim3(std::min(np * nq, kCus)),
-                     dim3(gemm::kThreads), 0, stream, wp, h, s.count, d.c, np, scale, s.lse2,
-                     w.coef, w.dz, ld);
+  const Operand dz{w.dz, ld, static_cast<int32_t>(pad)};
+  with_tile<T, Major::kK, Major::kK>(plan.logits, [&](auto* tile) {
+    using G = std::remove_pointer_t<decltype(tile)>;
+    hipLaunchKernelGGL((softmax_grad_kernel<G, T>),
+                       dim3(grid_of(tiles_of(plan.logits, columns, d.n))), dim3(gemm::kThreads), 0,
+                       stream, wp, h, s.count, d.c, (columns + G::kBP - 1) / G::kBP, scale, s.lse2,
+                       w.coef, w.dz, ld);
+  });
   const int64_t entries = d.n * d.k;
   hipLaunchKernelGGL((target_grad_kernel<T>), dim3(static_cast<unsigned>((entries + 255) / 256)),
                      dim3(256), 0, stream, d.k, first, columns, scale, w.coef, w.dz, ld, s);
   if (dh != nullptr) {
     const int steps = static_cast<int>(round_up(columns, gemm::kStep) / gemm::kStep);
-    const int each = (pieces.columns / gemm::kStep + pieces.splits - 1) / pieces.splits;
+    const int each = (plan.columns / gemm::kStep + plan.splits - 1) / plan.splits;
     const int64_t slab = d.n * d.c;
-    hipLaunchKernelGGL((hidden_grad_kernel<Hidden, T>),
-                       dim3(std::min(nc * nq * pieces.splits, kCus)), dim3(gemm::kThreads), 0,
-                       stream, wp, dz, s.count, steps, each, pieces.splits, nc, d.c,
-                       w.slabs + piece * pieces.splits * slab, slab);
+    with_tile<T, Major::kX, Major::kK>(plan.hidden, [&](auto* tile) {
+      using G = std::remove_pointer_t<decltype(tile)>;
+      hipLaunchKernelGGL((hidden_grad_kernel<G, T>),
+                         dim3(grid_of(tiles_of(plan.hidden, d.c, d.n) * plan.splits)),
+                         dim3(gemm::kThreads), 0, stream, wp, dz, s.count, steps, each,
+                         plan.splits, (d.c + G::kBP - 1) / G::kBP, d.c,
+                         w.slabs + piece * plan.splits * slab, slab);
+    });
   }
   if (dw != nullptr) {
-    hipLaunchKernelGGL((weight_grad_kernel<Weight, T>), dim3(std::min(nc * np, kCus)),
-                       dim3(gemm::kThreads), 0, stream, h, dz, s.count, columns, nc, np, d.c, w.scale,
-                       dw + static_cast<int64_t>(first) * d.c);
+    with_tile<T, Major::kX, Major::kX>(plan.weight, [&](auto* tile) {
+      using G = std::remove_pointer_t<decltype(tile)>;
+      hipLaunchKernelGGL((weight_grad_kernel<G, T>),
+                         dim3(grid_of(tiles_of(plan.weight, d.c, columns))), dim3(gemm::kThreads),
+                         0, stream, h, dz, s.count, columns, (d.c + G::kBP - 1) / G::kBP,
+                         (columns + G::kBQ - 1) / G::kBQ, d.c, w.scale,
+                         dw + static_cast<int64_t>(first) * d.c);
+    });
   }
 }
 
 template <typename T>
 int run_backward(const Shape& d, const void* weight, const float* upstream, bool per_row,
                  bool mean, float temperature, void* dh, void* dw, const Saved& s,
-                 const Pieces& pieces, const BackwardWork& w, hipStream_t stream) {
+                 const Plan& plan, const BackwardWork& w, hipStream_t stream) {
   const float scale = kLog2E / temperature;
   hipLaunchKernelGGL(row_coefficients_kernel, dim3(1), dim3(kScanThreads), 0, stream, upstream,
                      per_row, mean, temperature, __is_same(T, F16) ? 14 : 0, w.coef, w.scale, s);
-  for (int p = 0; p < pieces.count; ++p) {
-    if (few_rows(d.n)) {
-      launch_piece<T, FewRowsTile>(d, pieces, p, static_cast<const uint16_t*>(weight), scale,
-                                   static_cast<uint16_t*>(dh), static_cast<uint16_t*>(dw), s, w,
-                                   stream);
-    } else {
-      launch_piece<T, LargeTile>(d, pieces, p, static_cast<const uint16_t*>(weight), scale,
-                                 static_cast<uint16_t*>(dh), static_cast<uint16_t*>(dw), s, w,
-                                 stream);
-    }
+  for (int p = 0; p < plan.pieces; ++p) {
+    launch_piece<T>(d, plan, p, static_cast<const uint16_t*>(weight), scale,
+                    static_cast<uint16_t*>(dh), static_cast<uint16_t*>(dw), s, w, stream);
   }
   if (dh != nullptr) {
     const int64_t quads = d.n * (d.c / 4);
     const int64_t blocks = std::min<int64_t>((quads + 255) / 256, 8192);
     hipLaunchKernelGGL((hidden_grad_rows_kernel<T>), dim3(static_cast<unsigned>(blocks)),
-                       dim3(256), 0, stream, w.slabs, d.n * d.c, pieces.count * pieces.splits,
+                       dim3(256), 0, stream, w.slabs, d.n * d.c, plan.pieces * plan.splits,
                        d.c, d.n, w.scale, s.place, static_cast<uint16_t*>(dh));
   }
   return check_launch("linear loss backward");
@@ -925,7 +973,7 @@ int check_shape(const char* what, int io_dtype, int64_t n, int64_t c, int64_t vo
                      "%s: targets of a row must be in [1, 1024], got %lld", what,
                      static_cast<long long>(k));
   }
-  const int64_t tiles = round_up(vocab, kVocabTile) / kVocabTile * row_tiles(n);
+  const int64_t tiles = round_up(vocab, kMinTile) / kMinTile * (round_up(n, kMinTile) / kMinTile);
   if (tiles > (int64_t{1} << 22) || n * k > (int64_t{1} << 38)) {
     return set_error(FRWKV_ERR_UNSUPPORTED, "%s: rows x vocabulary too large for one call", what);
   }
@@ -961,13 +1009,12 @@ int check_temperature(const char* what, float t) {
   return FRWKV_OK;
 }
 
-int forward(const char* what, int io_dtype, const Shape& d, const void* hidden,
+int forward(int io_dtype, const Shape& d, const void* hidden,
             const void* weight, float temperature, int reduction, float* loss, const Saved& s,
             void* workspace, hipStream_t stream) {
   size_t need = 0;
   const ForwardWork w = forward_work(static_cast<char*>(workspace), d.n, d.vocab, &need);
   const bool mean = reduction == FRWKV_REDUCE_MEAN, per_row = reduction == FRWKV_REDUCE_NONE;
-  (void)what;
   return io_dtype == FRWKV_DTYPE_F16
              ? run_forward<F16>(d, hidden, weight, temperature, mean, per_row, loss, s, w, stream)
              : run_forward<Bf16>(d, hidden, weight, temperature, mean, per_row, loss, s, w,
@@ -1020,7 +1067,7 @@ size_t frwkv_linear_loss_backward_workspace_bytes(int64_t rows, int64_t channels
                                                   int want_grad_hidden) {
   if (rows <= 0 || channels <= 0 || vocab <= 0) return 0;
   size_t bytes = 0;
-  (void)frwkv::backward_work(nullptr, rows, channels, frwkv::pieces_of(rows, channels, vocab),
+  (void)frwkv::backward_work(nullptr, rows, channels, frwkv::plan_of(rows, channels, vocab),
                              want_grad_hidden != 0, &bytes);
   return bytes;
 }
@@ -1043,15 +1090,15 @@ int frwkv_linear_cross_entropy_forward(int io_dtype, int64_t rows, int64_t chann
   }
   const hipStream_t q = static_cast<hipStream_t>(stream);
   const int32_t n = static_cast<int32_t>(rows), v = static_cast<int32_t>(vocab);
-  const dim3 grid((n + 255) / 256);
+  float* row_loss = reduction == FRWKV_REDUCE_NONE ? loss : nullptr;
   if (target_bytes == 8) {
-    hipLaunchKernelGGL((label_targets_kernel<int64_t>), grid, dim3(256), 0, q,
-                       static_cast<const int64_t*>(targets), ignore_index, n, v, s);
+    hipLaunchKernelGGL((label_rows_kernel<int64_t>), dim3(1), dim3(kScanThreads), 0, q,
+                       static_cast<const int64_t*>(targets), ignore_index, n, v, row_loss, s);
   } else {
-    hipLaunchKernelGGL((label_targets_kernel<int32_t>), grid, dim3(256), 0, q,
-                       static_cast<const int32_t*>(targets), ignore_index, n, v, s);
+    hipLaunchKernelGGL((label_rows_kernel<int32_t>), dim3(1), dim3(kScanThreads), 0, q,
+                       static_cast<const int32_t*>(targets), ignore_index, n, v, row_loss, s);
   }
-  return forward(what, io_dtype, Shape{rows, static_cast<int32_t>(channels), v, 1}, hidden,
+  return forward(io_dtype, Shape{rows, static_cast<int32_t>(channels), v, 1}, hidden,
                  weight, 1.0f, reduction, loss, s, workspace, q);
 }
 
@@ -1101,7 +1148,9 @@ int frwkv_linear_topk_distillation_forward(
   } else {
     with_index(Bf16{});
   }
-  return forward(what, io_dtype, Shape{rows, static_cast<int32_t>(channels), v, k}, hidden,
+  hipLaunchKernelGGL(teacher_rows_kernel, dim3(1), dim3(kScanThreads), 0, q, n,
+                     reduction == FRWKV_REDUCE_NONE ? loss : nullptr, s);
+  return forward(io_dtype, Shape{rows, static_cast<int32_t>(channels), v, k}, hidden,
                  weight, temperature, reduction, loss, s, workspace, q);
 }
 
@@ -1129,8 +1178,8 @@ int frwkv_linear_loss_backward(int io_dtype, int64_t rows, int64_t channels, int
                            top, &need);
   rc = check_memory(what, "saved", saved, saved_bytes, need);
   if (rc != FRWKV_OK) return rc;
-  const Pieces pieces = pieces_of(rows, channels, vocab);
-  const BackwardWork w = backward_work(static_cast<char*>(workspace), rows, channels, pieces,
+  const Plan plan = plan_of(rows, channels, vocab);
+  const BackwardWork w = backward_work(static_cast<char*>(workspace), rows, channels, plan,
                                        grad_hidden != nullptr, &need);
   rc = check_memory(what, "workspace", workspace, workspace_bytes, need);
   if (rc != FRWKV_OK) return rc;
@@ -1141,9 +1190,9 @@ int frwkv_linear_loss_backward(int io_dtype, int64_t rows, int64_t channels, int
   const hipStream_t q = static_cast<hipStream_t>(stream);
   return io_dtype == FRWKV_DTYPE_F16
              ? run_backward<F16>(d, weight, grad_loss, per_row, mean, temperature, grad_hidden,
-                                 grad_weight, s, pieces, w, q)
+                                 grad_weight, s, plan, w, q)
              : run_backward<Bf16>(d, weight, grad_loss, per_row, mean, temperature, grad_hidden,
-                                  grad_weight, s, pieces, w, q);
+                                  grad_weight, s, plan, w, q);
 }
 
 }  // extern "C"
