@@ -10,9 +10,9 @@
 //   dweight = sum_rows dy xhat,  dbias = sum_rows dy.
 //
 // HBM-bound: x [, residual] -> y [, s] forward, dy, s [, ds] -> dx backward.
-// A row is held in registers by 1, 4 or 16 waves, 16 elements a thread (C up
-// to 1024, 4096, 16384), so each tensor passes once and the variance is taken
-// about the mean. The backward's workgroups walk over rows and keep the
+// A row is held in registers by 1, 4 or 16 waves, 8 or 16 elements a thread (C
+// up to 16384), so each tensor passes once and the variance is taken about the
+// mean. The backward's workgroups walk over rows and keep the
 // weight's and bias' sums of their 16 columns a thread in registers; one row
 // of 2 C partial sums a workgroup goes to memory and a second kernel adds
 // those in order, so the result does not depend on timing.
@@ -25,39 +25,62 @@
 namespace frwkv {
 namespace {
 
-constexpr int kEpt = 16;         // elements of a row a thread
+constexpr int kVec = 8;          // consecutive elements a thread
 constexpr int kMaxBlocks = 512;  // of the backward: two a CU
+constexpr int kMaxChannels = 16384;
 
 template <typename T>
 using Store = typename IoTraits<T>::storage;
 
-// kVec consecutive elements as they lie in memory; kVec 8 reads 16-byte pieces.
-template <typename T, int kVec>
+// Eight consecutive elements as they lie in memory. Aligned rows (16 bytes, C a
+// multiple of 8) are read and written in 16-byte pieces; others in what the
+// hardware takes at any address, with a last piece of fewer than eight.
+template <typename T, bool kAligned>
 struct Piece {
-  static constexpr int kWords = kVec == 1 ? 1 : kVec * IoTraits<T>::kBytes / 16;
-  typedef typename std::conditional<kVec == 1, Store<T>, uint4>::type Word;
-  Word word[kWords];
-  __device__ __forceinline__ void load(const Store<T>* p) {
+  static constexpr int kWords = kVec * IoTraits<T>::kBytes / 16;
+  uint4 word[kWords];
+  // left: elements of the row from p on (1 or more).
+  __device__ __forceinline__ void load(const Store<T>* p, int left) {
+    if (kAligned) {
 #pragma unroll
-    for (int i = 0; i < kWords; ++i) word[i] = reinterpret_cast<const Word*>(p)[i];
+      for (int i = 0; i < kWords; ++i) word[i] = reinterpret_cast<const uint4*>(p)[i];
+    } else if (left >= kVec) {
+      __builtin_memcpy(word, p, sizeof(word));
+    } else {
+      Store<T> x[kVec];
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) x[e] = e < left ? p[e] : Store<T>(0);
+      __builtin_memcpy(word, x, sizeof(word));
+    }
   }
-  __device__ __forceinline__ void zero() {
+  __device__ __forceinline__ void store(Store<T>* p, int left) const {
+    if (kAligned) {
 #pragma unroll
-    for (int i = 0; i < kWords; ++i) word[i] = Word{};
-  }
-  // Conversions before and after this one are not one value kept in registers.
-  __device__ __forceinline__ void again() {
-    if constexpr (kVec != 1) {
+      for (int i = 0; i < kWords; ++i) reinterpret_cast<uint4*>(p)[i] = word[i];
+    } else if (left >= kVec) {
+      __builtin_memcpy(p, word, sizeof(word));
+    } else {
+      Store<T> x[kVec];
+      __builtin_memcpy(x, word, sizeof(word));
 #pragma unroll
-      for (int i = 0; i < kWords; ++i) {
-        asm volatile("" : "+v"(word[i].x), "+v"(word[i].y), "+v"(word[i].z), "+v"(word[i].w));
+      for (int e = 0; e < kVec; ++e) {
+        if (e < left) p[e] = x[e];
       }
     }
   }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) word[i] = make_uint4(0, 0, 0, 0);
+  }
+  // Conversions before and after this one are not one value kept in registers.
+  __device__ __forceinline__ void again() {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      asm volatile("" : "+v"(word[i].x), "+v"(word[i].y), "+v"(word[i].z), "+v"(word[i].w));
+    }
+  }
   __device__ __forceinline__ float get(int e) const {
-    if constexpr (kVec == 1) {
-      return to_f32<T>(word[0]);
-    } else if constexpr (__is_same(T, float)) {
+    if constexpr (__is_same(T, float)) {
       const uint4 q = word[e / 4];
       return __uint_as_float(e % 4 == 0 ? q.x : e % 4 == 1 ? q.y : e % 4 == 2 ? q.z : q.w);
     } else {
@@ -66,27 +89,24 @@ struct Piece {
       return to_f32<T>(static_cast<uint16_t>(e % 2 ? d >> 16 : d & 0xffffu));
     }
   }
+  __device__ __forceinline__ void set(const float* x) {
+    if constexpr (__is_same(T, float)) {
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) {
+        word[i] = make_uint4(__float_as_uint(x[4 * i]), __float_as_uint(x[4 * i + 1]),
+                             __float_as_uint(x[4 * i + 2]), __float_as_uint(x[4 * i + 3]));
+      }
+    } else {
+      word[0] = make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]),
+                           pack2<T>(x[6], x[7]));
+    }
+  }
 };
 
-template <typename T, int kVec>
-__device__ __forceinline__ void load(const Store<T>* p, float* out) {
-  Piece<T, kVec> x;
-  x.load(p);
-#pragma unroll
-  for (int e = 0; e < kVec; ++e) out[e] = x.get(e);
-}
-
-template <typename T, int kVec>
-__device__ __forceinline__ void store(Store<T>* p, const float* x) {
-  if constexpr (kVec == 1) {
-    *p = from_f32<T>(x[0]);
-  } else if constexpr (__is_same(T, float)) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
-  } else {
-    *reinterpret_cast<uint4*>(p) = make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]),
-                                              pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
-  }
+// Whether element e of the piece at col < c belongs to the row.
+template <bool kAligned>
+__device__ __forceinline__ bool inside(int col, int e, int c) {
+  return kAligned || col + e < c;
 }
 
 // Sum over the kWaves waves of a row; red holds kWaves floats of the row's
@@ -110,7 +130,7 @@ constexpr int forward_threads() { return kWaves == 16 ? 1024 : 256; }
 template <int kWaves>
 constexpr int backward_threads() { return kWaves == 16 ? 1024 : 512; }
 
-template <typename T, int kVec, int kWaves>
+template <typename T, bool kAligned, int kWaves, int kE>
 __global__ __launch_bounds__(forward_threads<kWaves>()) void layer_norm_forward_kernel(
     const Store<T>* __restrict__ x, const Store<T>* __restrict__ residual,
     const Store<T>* __restrict__ weight, const Store<T>* __restrict__ bias,
@@ -118,6 +138,7 @@ __global__ __launch_bounds__(forward_threads<kWaves>()) void layer_norm_forward_
     float* __restrict__ rstd_out, int64_t rows, int32_t c, float eps) {
   constexpr int kGroups = forward_threads<kWaves>() / (64 * kWaves);
   constexpr int kRow = 64 * kWaves;
+  constexpr int kPieces = kE / kVec;
   __shared__ float red[2][kGroups][kWaves];
   const int group = threadIdx.x / kRow, t = threadIdx.x % kRow, wave = t >> 6;
   const float inv_c = 1.0f / static_cast<float>(c);
@@ -126,36 +147,43 @@ __global__ __launch_bounds__(forward_threads<kWaves>()) void layer_norm_forward_
     const int64_t row = first + group;
     const bool here = row < rows;
     const int64_t at = (here ? row : 0) * c;
-    float s[kEpt];
+    float s[kE];
     float sum = 0.0f;
 #pragma unroll
-    for (int j = 0; j < kEpt; j += kVec) {
-      const int col = (j / kVec * kRow + t) * kVec;
-#pragma unroll
-      for (int e = 0; e < kVec; ++e) s[j + e] = 0.0f;
+    for (int j = 0; j < kPieces; ++j) {
+      const int col = (j * kRow + t) * kVec;
+      Piece<T, kAligned> a, r;
+      a.zero();
+      r.zero();
       if (here && col < c) {
-        load<T, kVec>(x + at + col, s + j);
-        if (residual != nullptr) {
-          float r[kVec];
-          load<T, kVec>(residual + at + col, r);
-#pragma unroll
-          for (int e = 0; e < kVec; ++e) s[j + e] = to_f32<T>(from_f32<T>(s[j + e] + r[e]));
-          store<T, kVec>(stream + at + col, s + j);
-        }
-#pragma unroll
-        for (int e = 0; e < kVec; ++e) sum += s[j + e];
+        a.load(x + at + col, c - col);
+        if (residual != nullptr) r.load(residual + at + col, c - col);
       }
+      float* own = s + j * kVec;
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) own[e] = a.get(e);
+      if (residual != nullptr) {
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) own[e] += r.get(e);
+        a.set(own);
+        if (here && col < c) a.store(stream + at + col, c - col);
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) own[e] = a.get(e);
+      }
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) sum += own[e];
     }
     const float mean = row_sum<kWaves>(sum, red[0][group], wave) * inv_c;
     float sq = 0.0f;
 #pragma unroll
-    for (int j = 0; j < kEpt; j += kVec) {
-      const int col = (j / kVec * kRow + t) * kVec;
+    for (int j = 0; j < kPieces; ++j) {
+      const int col = (j * kRow + t) * kVec;
       if (col < c) {
 #pragma unroll
         for (int e = 0; e < kVec; ++e) {
-          s[j + e] -= mean;
-          sq = fmaf(s[j + e], s[j + e], sq);
+          const float d = s[j * kVec + e] - mean;
+          s[j * kVec + e] = d;
+          if (inside<kAligned>(col, e, c)) sq = fmaf(d, d, sq);
         }
       }
     }
@@ -167,23 +195,58 @@ __global__ __launch_bounds__(forward_threads<kWaves>()) void layer_norm_forward_
       rstd_out[row] = rstd;
     }
 #pragma unroll
-    for (int j = 0; j < kEpt; j += kVec) {
-      const int col = (j / kVec * kRow + t) * kVec;
+    for (int j = 0; j < kPieces; ++j) {
+      const int col = (j * kRow + t) * kVec;
       if (col < c) {
-        float w[kVec], b[kVec], o[kVec];
-        load<T, kVec>(weight + col, w);
-        load<T, kVec>(bias + col, b);
+        Piece<T, kAligned> w, b, o;
+        w.load(weight + col, c - col);
+        b.load(bias + col, c - col);
+        float out[kVec];
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) o[e] = fmaf(s[j + e] * rstd, w[e], b[e]);
-        store<T, kVec>(y + at + col, o);
+        for (int e = 0; e < kVec; ++e) {
+          out[e] = fmaf(s[j * kVec + e] * rstd, w.get(e), b.get(e));
+        }
+        o.set(out);
+        o.store(y + at + col, c - col);
       }
     }
   }
 }
 
+// What the backward reads of a row, as it lies in memory (zeros where there is
+// nothing).
+template <typename T, bool kAligned, int kPieces, int kRow>
+struct Row {
+  Piece<T, kAligned> x[kPieces], up[kPieces], add[kPieces];
+  float mu, rs;
+  __device__ __forceinline__ void load(const Store<T>* s, const Store<T>* dy, const Store<T>* ds,
+                                       const float* mean, const float* rstd, int64_t row,
+                                       int64_t rows, int32_t c, int t) {
+    const bool here = row < rows;
+    const int64_t at = row * c;
+    mu = here ? mean[row] : 0.0f;
+    rs = here ? rstd[row] : 0.0f;
+#pragma unroll
+    for (int j = 0; j < kPieces; ++j) {
+      const int col = (j * kRow + t) * kVec;
+      x[j].zero();
+      up[j].zero();
+      add[j].zero();
+      if (here && col < c) {
+        x[j].load(s + at + col, c - col);
+        up[j].load(dy + at + col, c - col);
+        if (ds != nullptr) add[j].load(ds + at + col, c - col);
+      }
+    }
+  }
+};
+
 // partial[block][0][c] = sum over the block's rows of dy xhat, [1][c] of dy.
-template <typename T, int kVec, int kWaves>
-__global__ __launch_bounds__(backward_threads<kWaves>(), kVec == 1 ? 1 : 4) void layer_norm_backward_kernel(
+// With 8 elements a thread the next row's loads are under way while a row is
+// summed up and written; with 16 there are no registers for that, and the two
+// workgroups of a CU cover for each other.
+template <typename T, bool kAligned, int kWaves, int kE>
+__global__ __launch_bounds__(backward_threads<kWaves>(), 4) void layer_norm_backward_kernel(
     const Store<T>* __restrict__ dy, const Store<T>* __restrict__ s,
     const Store<T>* __restrict__ ds, const Store<T>* __restrict__ weight,
     const float* __restrict__ mean, const float* __restrict__ rstd, Store<T>* __restrict__ dx,
@@ -191,49 +254,48 @@ __global__ __launch_bounds__(backward_threads<kWaves>(), kVec == 1 ? 1 : 4) void
   constexpr int kThreads = backward_threads<kWaves>();
   constexpr int kGroups = kThreads / (64 * kWaves);
   constexpr int kRow = 64 * kWaves;
+  constexpr int kPieces = kE / kVec;
   __shared__ float red[2][2][kGroups][kWaves];
-  __shared__ float columns[kGroups > 1 ? kThreads * kEpt : 1];
+  __shared__ float columns[kGroups > 1 ? kThreads * kE : 1];
   const int group = threadIdx.x / kRow, t = threadIdx.x % kRow, wave = t >> 6;
   const float inv_c = 1.0f / static_cast<float>(c);
-  // What is only read again is kept as it lies in memory.
-  constexpr int kPieces = kEpt / kVec;
-  Piece<T, kVec> w[kPieces], up[kPieces], add[kPieces];
-  float pw[kEpt], pb[kEpt];
+  Piece<T, kAligned> w[kPieces];
+  float pw[kE], pb[kE];
 #pragma unroll
   for (int j = 0; j < kPieces; ++j) {
     const int col = (j * kRow + t) * kVec;
     w[j].zero();
-    if (col < c) w[j].load(weight + col);
+    if (col < c) w[j].load(weight + col, c - col);
 #pragma unroll
     for (int e = 0; e < kVec; ++e) pw[j * kVec + e] = pb[j * kVec + e] = 0.0f;
   }
   int side = 0;
-  for (int64_t first = static_cast<int64_t>(blockIdx.x) * kGroups; first < rows;
-       first += static_cast<int64_t>(gridDim.x) * kGroups) {
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups;
+  constexpr bool kAhead = kE == 8;
+  Row<T, kAligned, kPieces, kRow> now, next;
+  if constexpr (kAhead) {
+    next.load(s, dy, ds, mean, rstd, static_cast<int64_t>(blockIdx.x) * kGroups + group, rows, c,
+              t);
+  }
+  for (int64_t first = static_cast<int64_t>(blockIdx.x) * kGroups; first < rows; first += step) {
     const int64_t row = first + group;
-    const bool here = row < rows;
-    const int64_t at = (here ? row : 0) * c;
-    const float mu = here ? mean[row] : 0.0f, rs = here ? rstd[row] : 0.0f;
-    float xh[kEpt];
+    if constexpr (kAhead) {
+      now = next;
+      next.load(s, dy, ds, mean, rstd, row + step, rows, c, t);
+    } else {
+      now.load(s, dy, ds, mean, rstd, row, rows, c, t);
+    }
+    float xh[kE];
     float sg = 0.0f, sgx = 0.0f;
 #pragma unroll
     for (int j = 0; j < kPieces; ++j) {
       const int col = (j * kRow + t) * kVec;
-      Piece<T, kVec> x;
-      x.zero();
-      up[j].zero();
-      add[j].zero();
       w[j].again();
-      if (here && col < c) {
-        x.load(s + at + col);
-        up[j].load(dy + at + col);
-        if (ds != nullptr) add[j].load(ds + at + col);
-      }
 #pragma unroll
       for (int e = 0; e < kVec; ++e) {
         const int k = j * kVec + e;
-        const float u = up[j].get(e), g = u * w[j].get(e);
-        xh[k] = col < c ? (x.get(e) - mu) * rs : 0.0f;
+        const float u = now.up[j].get(e), g = u * w[j].get(e);
+        xh[k] = col < c && inside<kAligned>(col, e, c) ? (now.x[j].get(e) - now.mu) * now.rs : 0.0f;
         pw[k] = fmaf(u, xh[k], pw[k]);
         pb[k] += u;
         sg += g;
@@ -261,20 +323,22 @@ __global__ __launch_bounds__(backward_threads<kWaves>(), kVec == 1 ? 1 : 4) void
       side ^= 1;
     }
     const float mg = sg * inv_c, mgx = sgx * inv_c;
-    if (!here) continue;
+    if (row >= rows) continue;
 #pragma unroll
     for (int j = 0; j < kPieces; ++j) {
       const int col = (j * kRow + t) * kVec;
-      up[j].again();
+      now.up[j].again();
       w[j].again();
       if (col < c) {
         float o[kVec];
 #pragma unroll
         for (int e = 0; e < kVec; ++e) {
-          const float g = up[j].get(e) * w[j].get(e);
-          o[e] = fmaf(rs, g - mg - xh[j * kVec + e] * mgx, add[j].get(e));
+          const float g = now.up[j].get(e) * w[j].get(e);
+          o[e] = fmaf(now.rs, g - mg - xh[j * kVec + e] * mgx, now.add[j].get(e));
         }
-        store<T, kVec>(dx + at + col, o);
+        Piece<T, kAligned> out;
+        out.set(o);
+        out.store(dx + row * c + col, c - col);
       }
     }
   }
@@ -285,22 +349,24 @@ __global__ __launch_bounds__(backward_threads<kWaves>(), kVec == 1 ? 1 : 4) void
     if constexpr (kGroups > 1) {
       __syncthreads();
 #pragma unroll
-      for (int e = 0; e < kEpt; ++e) columns[(group * kEpt + e) * kRow + t] = mine[e];
+      for (int e = 0; e < kE; ++e) columns[(group * kE + e) * kRow + t] = mine[e];
       __syncthreads();
       if (group == 0) {
 #pragma unroll
         for (int q = 1; q < kGroups; ++q) {
 #pragma unroll
-          for (int e = 0; e < kEpt; ++e) mine[e] += columns[(q * kEpt + e) * kRow + t];
+          for (int e = 0; e < kE; ++e) mine[e] += columns[(q * kE + e) * kRow + t];
         }
       }
     }
     if (group == 0) {
       float* to = partial + (static_cast<int64_t>(blockIdx.x) * 2 + which) * c;
 #pragma unroll
-      for (int j = 0; j < kEpt; j += kVec) {
-        const int col = (j / kVec * kRow + t) * kVec;
-        if (col < c) store<float, kVec>(to + col, mine + j);
+      for (int j = 0; j < kPieces; ++j) {
+        const int col = (j * kRow + t) * kVec;
+        Piece<float, kAligned> out;
+        out.set(mine + j * kVec);
+        if (col < c) out.store(to + col, c - col);
       }
     }
   }
@@ -338,7 +404,12 @@ __global__ __launch_bounds__(1024) void layer_norm_columns_kernel(
   if (lane == 0 && mine < c) (blockIdx.y == 0 ? dweight : dbias)[mine] = from_f32<T>(sum);
 }
 
-int waves_of(int64_t c) { return c <= 64 * kEpt ? 1 : c <= 256 * kEpt ? 4 : 16; }
+// Waves and elements a thread that hold a row: the fewest that do, since lanes
+// without elements cost time (16384 x 2560 in bf16, backward: 4 waves with 16
+// elements 69 us, 8 with 8 elements 75; 65536 x 768: one wave with 16 elements
+// 84, 4 with 8 elements 121; 16384 x 2048: 4 waves with 8 elements 48, with 16 51).
+int waves_of(int64_t c) { return c <= 1024 ? 1 : c <= 4096 ? 4 : 16; }
+int elements_of(int64_t c) { return c <= waves_of(c) * 64 * kVec ? kVec : 2 * kVec; }
 
 int64_t backward_blocks(int64_t rows, int64_t c) {
   const int waves = waves_of(c);
@@ -346,24 +417,25 @@ int64_t backward_blocks(int64_t rows, int64_t c) {
   return std::min<int64_t>((rows + groups - 1) / groups, waves == 16 ? kMaxBlocks / 2 : kMaxBlocks);
 }
 
-struct Call {
-  int64_t rows;
-  int32_t c;
-  hipStream_t stream;
-};
+template <int kValue>
+using Int = std::integral_constant<int, kValue>;
 
+// f(aligned, waves a row, elements a thread)
 template <typename F>
-void with_shape(int64_t c, bool vector, F&& f) {
-  const int waves = waves_of(c);
-  const auto with_waves = [&](auto vec) {
-    if (waves == 1) f(vec, std::integral_constant<int, 1>{});
-    if (waves == 4) f(vec, std::integral_constant<int, 4>{});
-    if (waves == 16) f(vec, std::integral_constant<int, 16>{});
+void with_shape(int64_t c, bool aligned, F&& f) {
+  const int waves = waves_of(c), elements = elements_of(c);
+  const auto with_waves = [&](auto is_aligned) {
+    if (waves == 1 && elements == 8) f(is_aligned, Int<1>{}, Int<8>{});
+    if (waves == 1 && elements == 16) f(is_aligned, Int<1>{}, Int<16>{});
+    if (waves == 4 && elements == 8) f(is_aligned, Int<4>{}, Int<8>{});
+    if (waves == 4 && elements == 16) f(is_aligned, Int<4>{}, Int<16>{});
+    if (waves == 16 && elements == 8) f(is_aligned, Int<16>{}, Int<8>{});
+    if (waves == 16 && elements == 16) f(is_aligned, Int<16>{}, Int<16>{});
   };
-  if (vector) {
-    with_waves(std::integral_constant<int, 8>{});
+  if (aligned) {
+    with_waves(Int<1>{});
   } else {
-    with_waves(std::integral_constant<int, 1>{});
+    with_waves(Int<0>{});
   }
 }
 
@@ -377,11 +449,11 @@ void with_type(int io_dtype, F&& f) {
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 template <size_t N>
-bool vector_call(int64_t c, const void* const (&pointers)[N]) {
+bool aligned_call(int64_t c, const void* const (&pointers)[N]) {
   for (const void* p : pointers) {
     if (!aligned16(p)) return false;
   }
-  return c % 8 == 0;
+  return c % kVec == 0;
 }
 
 int check_shape(const char* what, int io_dtype, int64_t rows, int64_t c) {
@@ -394,7 +466,7 @@ int check_shape(const char* what, int io_dtype, int64_t rows, int64_t c) {
     return set_error(FRWKV_ERR_INVALID_ARGUMENT, "%s: rows must be positive, got %lld", what,
                      static_cast<long long>(rows));
   }
-  if (c <= 0 || c > 1024 * kEpt) {
+  if (c <= 0 || c > kMaxChannels) {
     return set_error(FRWKV_ERR_UNSUPPORTED, "%s: channels must be in [1, 16384], got %lld", what,
                      static_cast<long long>(c));
   }
@@ -429,12 +501,13 @@ int frwkv_layer_norm_forward(int io_dtype, int64_t rows, int64_t channels, const
   with_type(io_dtype, [&](auto io) {
     using T = decltype(io);
     using S = Store<T>;
-    with_shape(c, vector_call(c, all), [&](auto vec, auto waves) {
-      constexpr int kVec = decltype(vec)::value, kWaves = decltype(waves)::value;
+    with_shape(c, aligned_call(c, all), [&](auto aligned, auto waves, auto elements) {
+      constexpr bool kAligned = decltype(aligned)::value != 0;
+      constexpr int kWaves = decltype(waves)::value, kE = decltype(elements)::value;
       constexpr int kThreads = forward_threads<kWaves>();
       constexpr int kGroups = kThreads / (64 * kWaves);
       const int64_t blocks = std::min<int64_t>((rows + kGroups - 1) / kGroups, 1 << 20);
-      hipLaunchKernelGGL((layer_norm_forward_kernel<T, kVec, kWaves>),
+      hipLaunchKernelGGL((layer_norm_forward_kernel<T, kAligned, kWaves, kE>),
                          dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0,
                          static_cast<hipStream_t>(stream), static_cast<const S*>(x),
                          static_cast<const S*>(residual), static_cast<const S*>(weight),
@@ -478,9 +551,10 @@ int frwkv_layer_norm_backward(int io_dtype, int64_t rows, int64_t channels, cons
   with_type(io_dtype, [&](auto io) {
     using T = decltype(io);
     using S = Store<T>;
-    with_shape(c, vector_call(c, all), [&](auto vec, auto waves) {
-      constexpr int kVec = decltype(vec)::value, kWaves = decltype(waves)::value;
-      hipLaunchKernelGGL((layer_norm_backward_kernel<T, kVec, kWaves>),
+    with_shape(c, aligned_call(c, all), [&](auto aligned, auto waves, auto elements) {
+      constexpr bool kAligned = decltype(aligned)::value != 0;
+      constexpr int kWaves = decltype(waves)::value, kE = decltype(elements)::value;
+      hipLaunchKernelGGL((layer_norm_backward_kernel<T, kAligned, kWaves, kE>),
                          dim3(static_cast<unsigned>(blocks)), dim3(backward_threads<kWaves>()), 0,
                          q, static_cast<const S*>(grad_y), static_cast<const S*>(normed),
                          static_cast<const S*>(grad_stream), static_cast<const S*>(weight), mean,
