@@ -83,13 +83,14 @@ __device__ __forceinline__ void wait_and_barrier() {
 // The loads of one operand's stages by the whole workgroup: 16-byte pieces, one
 // a thread and round. A thread's offset from the round's first row never
 // changes; the rounds' and stages' first rows are scalars.
-template <Major M, int BX>
+template <Major M, int BX, bool kTurn>
 struct Loader {
   static constexpr int kRounds = BX * 8 / kThreads;
   static constexpr int kBytes = BX * kStep * 2;
   static constexpr int kRoundRows = M == Major::kK ? kThreads / 8 : kThreads / (BX / 8);
   static_assert(kRounds >= 1, "a stage is at least one piece a thread");
   static_assert(M == Major::kK || BX >= 128, "x-major rows hold at least 8 granules");
+  static_assert(M == Major::kK || !kTurn, "k-major operands turn");
 
   const char* base;  // the next stage's first row (k-major: at its first k)
   int32_t row_bytes;
@@ -98,13 +99,22 @@ struct Loader {
   uint32_t offset;   // of this thread's piece from a round's first row
   uint32_t wave_lds;
 
-  __device__ __forceinline__ void init(const Operand& op, int x0, int k0) {
+  int32_t ahead;     // kTurn: stages until the product's k begins again
+  int32_t span;
+
+  // turn < steps: the stage that is taken first (kTurn).
+  __device__ __forceinline__ void init(const Operand& op, int x0, int k0, int steps, int turn) {
     const int tid = threadIdx.x;
+    if (kTurn) {
+      ahead = steps - turn;
+      span = steps * (kStep * 2);
+    }
     row_bytes = static_cast<int32_t>(op.ld * 2);
     const int first = M == Major::kK ? x0 : k0;
     into = 2 * (M == Major::kK ? k0 : x0);
     left = op.rows - first;
     base = reinterpret_cast<const char*>(op.data) + static_cast<int64_t>(first) * row_bytes + into;
+    if (kTurn) base += turn * (kStep * 2);
     wave_lds = __builtin_amdgcn_readfirstlane(tid >> 6) * 1024u;
     if constexpr (M == Major::kK) {
       offset = static_cast<uint32_t>(tid >> 3) * row_bytes + (((tid & 7) ^ ((tid >> 4) & 7)) << 4);
@@ -133,6 +143,10 @@ struct Loader {
   __device__ __forceinline__ void next() {
     if constexpr (M == Major::kK) {
       base += kStep * 2;
+      if (kTurn) {
+        ahead -= 1;
+        base -= ahead == 0 ? span : 0;
+      }
     } else {
       base += static_cast<int64_t>(kStep) * row_bytes;
       left -= kStep;
@@ -181,8 +195,10 @@ struct Reader {
 // A workgroup's product. WP x WQ waves, each with TP x TQ blocks of 16 x 16;
 // acc[i][j] of lane (g, n) is D[p0 + 16 i + 4 g + r][q0 + 16 j + n], r = 0..3,
 // p0 = BP / WP * (wave / WQ), q0 = BQ / WQ * (wave % WQ).
-template <typename T, Major MA, Major MB, int BP, int BQ, int WP, int WQ, int NS>
+template <typename T, Major MA, Major MB, int BP, int BQ, int WP, int WQ, int NS,
+          bool kTurn = false>
 struct Tile {
+  static constexpr bool kTurns = kTurn;
   static constexpr int kBP = BP, kBQ = BQ, kWP = WP, kWQ = WQ;
   static constexpr int TP = BP / WP / 16;
   static constexpr int TQ = BQ / WQ / 16;
@@ -191,8 +207,8 @@ struct Tile {
   static_assert(WP * WQ * 64 == kThreads, "8 waves");
   static_assert(kLdsBytes <= 160 * 1024, "LDS of a CU");
 
-  using LoadA = Loader<MA, BP>;
-  using LoadB = Loader<MB, BQ>;
+  using LoadA = Loader<MA, BP, kTurn>;
+  using LoadB = Loader<MB, BQ, kTurn>;
   static constexpr int kLoads = LoadA::kRounds + LoadB::kRounds;
 
   f32x4 acc[TP][TQ];
@@ -215,14 +231,15 @@ struct Tile {
   // finish the tile before: its accumulators are its own until multiply, and
   // the LDS beyond kLdsBytes is not touched.
   //
-  // steps: number of 64-k stages from k0 on; 0 leaves zeros.
+  // steps: number of 64-k stages from k0 on; 0 leaves zeros. turn: which of them
+  // comes first, the others follow round (kTurn).
   __device__ __forceinline__ void begin(const Operand& a, const Operand& b, int p0, int q0, int k0,
-                                        int steps_, char* smem) {
+                                        int steps_, char* smem, int turn = 0) {
     lds = static_cast<uint32_t>(
         reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)smem));
     steps = steps_;
-    la.init(a, p0, k0);
-    lb.init(b, q0, k0);
+    la.init(a, p0, k0, steps, turn);
+    lb.init(b, q0, k0, steps, turn);
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
 #pragma unroll

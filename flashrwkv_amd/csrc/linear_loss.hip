@@ -72,6 +72,15 @@ __device__ __forceinline__ float wave_max(float x) {
   return x;
 }
 
+// (maximum, sum of 2^(x - maximum)) of two sets; a sum of 0 is an empty set.
+__device__ __forceinline__ float2 joined(float2 a, float2 b) {
+  if (b.y == 0.0f) return a;
+  if (a.y == 0.0f) return b;
+  const float top = fmaxf(a.x, b.x);
+  return make_float2(top, a.y * __builtin_amdgcn_exp2f(a.x - top) +
+                              b.y * __builtin_amdgcn_exp2f(b.x - top));
+}
+
 // What the forward leaves for the backward. Row indices m count the rows that
 // take part, in order; i is the row's place in the caller's tensors.
 struct Saved {
@@ -304,8 +313,12 @@ template <typename T, Major MA, Major MB>
 using LargeTile = gemm::Tile<T, MA, MB, 256, 256, 2, 4, 2>;
 template <typename T, Major MA, Major MB>
 using SmallTile = gemm::Tile<T, MA, MB, 128, 128, 2, 4, 4>;
+// Few rows only stream the weight, and every workgroup starting at the first k
+// hits the same memory channels where rows are a power of two apart: they
+// start at different ones (scoring 1 row, 65536 x 2048, from memory: 79 -> 63 us;
+// for the large tile, bound by the products, it costs 1%).
 template <typename T, Major MA, Major MB>
-using FewRowsTile = gemm::Tile<T, MA, MB, 256, 64, 8, 1, 3>;
+using FewRowsTile = gemm::Tile<T, MA, MB, 256, 64, 8, 1, 3, MA == Major::kK && MB == Major::kK>;
 
 // The tiles of a product over rows m, whose count stands on the device: the
 // workgroups of a launch of at most one a CU take them in turn. While a
@@ -320,13 +333,13 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void lse_tiles_kernel(
     float2* __restrict__ part, int64_t pad) {
   __shared__ __attribute__((aligned(1024))) char smem[G::kLdsBytes];
   __shared__ float maxima[G::kWP][G::kBQ], sums[G::kWP][G::kBQ];
-  const int nq = row_tiles_of(*count, G::kBQ), total = np * nq;
+  const int nq = row_tiles_of(*count, G::kBQ), total = np * nq, steps = c / gemm::kStep;
   int id = blockIdx.x;
   if (id >= total) return;
   G tile;
   int tp, tq;
   gemm::tile_of(gemm::xcd_run(id, total), np, nq, tp, tq);
-  tile.begin(w, h, tp * G::kBP, tq * G::kBQ, 0, c / gemm::kStep, smem);
+  tile.begin(w, h, tp * G::kBP, tq * G::kBQ, 0, steps, smem, G::kTurns ? tp % steps : 0);
   G::arrive();
   while (true) {
     tile.multiply(smem);
@@ -335,7 +348,7 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void lse_tiles_kernel(
     id += gridDim.x;
     if (id < total) {
       gemm::tile_of(gemm::xcd_run(id, total), np, nq, tp, tq);
-      tile.begin(w, h, tp * G::kBP, tq * G::kBQ, 0, c / gemm::kStep, smem);
+      tile.begin(w, h, tp * G::kBP, tq * G::kBQ, 0, steps, smem, G::kTurns ? tp % steps : 0);
     }
     const int left = w.rows - p0;
     if (left < G::kBP) {  // the last columns do not exist
@@ -406,13 +419,13 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void softmax_grad_kernel(
     int64_t ld) {
   __shared__ __attribute__((aligned(1024))) char smem[G::kLdsBytes];
   const int rows = *count;
-  const int nq = row_tiles_of(rows, G::kBQ), total = np * nq;
+  const int nq = row_tiles_of(rows, G::kBQ), total = np * nq, steps = c / gemm::kStep;
   int id = blockIdx.x;
   if (id >= total) return;
   G tile;
   int tp, tq;
   gemm::tile_of(gemm::xcd_run(id, total), np, nq, tp, tq);
-  tile.begin(w, h, tp * G::kBP, tq * G::kBQ, 0, c / gemm::kStep, smem);
+  tile.begin(w, h, tp * G::kBP, tq * G::kBQ, 0, steps, smem, G::kTurns ? tp % steps : 0);
   G::arrive();
   while (true) {
     const int p0 = tp * G::kBP, q0 = tq * G::kBQ;
@@ -431,7 +444,7 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void softmax_grad_kernel(
     id += gridDim.x;
     if (id < total) {
       gemm::tile_of(gemm::xcd_run(id, total), np, nq, tp, tq);
-      tile.begin(w, h, tp * G::kBP, tq * G::kBQ, 0, c / gemm::kStep, smem);
+      tile.begin(w, h, tp * G::kBP, tq * G::kBQ, 0, steps, smem, G::kTurns ? tp % steps : 0);
     }
     const int left = w.rows - p0;
     const bool all = left >= G::kBP && rows - q0 >= G::kBQ;
@@ -592,15 +605,6 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void weight_grad_kernel(
 }
 
 // -------------------------------------------------------- row reductions
-// (maximum, sum of 2^(x - maximum)) of two sets; a sum of 0 is an empty set.
-__device__ __forceinline__ float2 joined(float2 a, float2 b) {
-  if (b.y == 0.0f) return a;
-  if (a.y == 0.0f) return b;
-  const float top = fmaxf(a.x, b.x);
-  return make_float2(top, a.y * __builtin_amdgcn_exp2f(a.x - top) +
-                              b.y * __builtin_amdgcn_exp2f(b.x - top));
-}
-
 // A workgroup takes 32 rows, 32 threads a row: joins the tiles' maxima and
 // sums to lse2[m], and the row's loss. row_loss (by i) or partial (by m). A
 // thread has 8 tiles under way at a time, all of those of 65536 columns.
@@ -895,8 +899,8 @@ int run_forward(const Shape& d, const void* hidden, const void* weight, float te
                      stream, static_cast<const uint16_t*>(hidden),
                      static_cast<const uint16_t*>(weight), d.c, d.k, d.vocab, 1.0f / temperature,
                      w.target_term, s);
-  const Operand b{s.hidden, d.c, static_cast<int32_t>(pad)};
   int tiles = 0;
+  const Operand b{s.hidden, d.c, static_cast<int32_t>(pad)};
   for_cut(cut_of(d.vocab, d.n, d.c / gemm::kStep, true), d.vocab,
           [&](int64_t first, int32_t columns, Size size) {
     const Operand a{static_cast<const uint16_t*>(weight) + first * d.c, d.c, columns};
