@@ -323,3 +323,72 @@ def lnx_pretrain_backward(grad_output, x, r, k, v, residual_scale, weight, bias,
         DTYPE[x.dtype], n, c // head_size, head_size, _p(grad_output), _p(x), _p(r), _p(k),
         _p(v), _p(residual_scale), _p(weight), _p(bias), _p(g), _p(mean), _p(rstd),
         *(_p(t) for t in grads), _p(work), 0 if work is None else work.numel(), _stream()))
+
+
+REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+
+
+def layer_norm_forward(x, weight, bias, *, y, eps=1e-5, residual=None, stream_out=None, mean=None,
+                       rstd=None):
+    """Rows of the last axis; ``mean`` / ``rstd`` fp32 with one element a row."""
+    c = x.shape[-1]
+    _check(library().frwkv_layer_norm_forward(
+        DTYPE[x.dtype], x.numel() // c, c, _p(x), _p(residual), _p(weight), _p(bias), float(eps),
+        _p(y), _p(stream_out), _p(mean), _p(rstd), _stream()))
+
+
+def layer_norm_backward(grad_y, normed, weight, mean, rstd, *, grads, grad_stream=None):
+    """``grads`` = (grad_x, grad_weight, grad_bias)."""
+    c = normed.shape[-1]
+    rows = normed.numel() // c
+    need = int(library().frwkv_layer_norm_backward_workspace_bytes(rows, c))
+    work = workspace(need, normed.device)
+    _check(library().frwkv_layer_norm_backward(
+        DTYPE[normed.dtype], rows, c, _p(grad_y), _p(normed), _p(grad_stream), _p(weight),
+        _p(mean), _p(rstd), *(_p(t) for t in grads), _p(work), need, _stream()))
+
+
+def _loss_buffers(hidden, vocab, top):
+    c = hidden.shape[-1]
+    rows = hidden.numel() // c
+    saved = workspace(int(library().frwkv_linear_loss_saved_bytes(rows, c, top)), hidden.device)
+    work = workspace(int(library().frwkv_linear_loss_forward_workspace_bytes(rows, vocab)),
+                     hidden.device)
+    return rows, c, saved, work
+
+
+def linear_cross_entropy_forward(hidden, weight, targets, *, loss, ignore_index=-100,
+                                 reduction="mean"):
+    """Writes ``loss`` (fp32) and returns the buffer that the backward reads."""
+    rows, c, saved, work = _loss_buffers(hidden, weight.shape[0], 1)
+    _check(library().frwkv_linear_cross_entropy_forward(
+        DTYPE[hidden.dtype], rows, c, weight.shape[0], _p(hidden), _p(weight),
+        targets.element_size(), _p(targets), int(ignore_index), REDUCTIONS[reduction], _p(loss),
+        _p(saved), saved.numel(), _p(work), work.numel(), _stream()))
+    return saved
+
+
+def linear_topk_distillation_forward(hidden, weight, teacher_logits, teacher_indices, *, loss,
+                                     temperature=1.0, reduction="mean"):
+    """Writes ``loss`` (fp32) and returns the buffer that the backward reads."""
+    top = teacher_logits.shape[-1]
+    rows, c, saved, work = _loss_buffers(hidden, weight.shape[0], top)
+    _check(library().frwkv_linear_topk_distillation_forward(
+        DTYPE[hidden.dtype], rows, c, weight.shape[0], top, _p(hidden), _p(weight),
+        DTYPE[teacher_logits.dtype], _p(teacher_logits), teacher_indices.element_size(),
+        _p(teacher_indices), float(temperature), REDUCTIONS[reduction], _p(loss), _p(saved),
+        saved.numel(), _p(work), work.numel(), _stream()))
+    return saved
+
+
+def linear_loss_backward(grad_loss, weight, saved, *, rows, top, temperature=1.0,
+                         reduction="mean", grad_hidden=None, grad_weight=None):
+    """Either gradient may be None: it is then not computed."""
+    vocab, c = weight.shape
+    need = int(library().frwkv_linear_loss_backward_workspace_bytes(rows, c, vocab,
+                                                                    grad_hidden is not None))
+    work = workspace(need, weight.device)
+    _check(library().frwkv_linear_loss_backward(
+        DTYPE[weight.dtype], rows, c, vocab, top, _p(weight), float(temperature),
+        REDUCTIONS[reduction], _p(grad_loss), _p(saved), saved.numel(), _p(grad_hidden),
+        _p(grad_weight), _p(work), need, _stream()))
