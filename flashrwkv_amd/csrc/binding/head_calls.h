@@ -3,9 +3,9 @@
 // training, the autograd node in native code. A call that these checks do not
 // pass, or whose arguments are not plain, returns None; the wrapper then runs
 // its tables (which raise their errors) and its own autograd function. Part of
-// torch_ops.cpp. Host time of a call: norm of one row 9.7 -> 4.6 us; norm of one
-// row with its gradients 109 -> 44 us, cross entropy with its gradients 133 ->
-// 75 us (a Python node costs the engine about 60 us).
+// torch_ops.cpp. Host time of a call: norm of one row 9.7 -> 5.4 us; norm of one
+// row with its gradients 109 -> 45 us, a small cross entropy with its gradients
+// 133 -> 68 us (a Python node costs the engine about 60 us).
 #pragma once
 
 #include <torch/csrc/autograd/custom_function.h>

@@ -47,6 +47,8 @@ constexpr int kRowPad = 256;       // rows of workspaces, and a product's larges
 constexpr int kVocabTile = 256;    // pieces of the vocabulary are whole multiples of it
 constexpr int kMinTile = 128;      // fewest columns whose maximum and sum the forward keeps
 constexpr int kScanThreads = 1024;
+constexpr int kCus = 256;
+constexpr int kMostSplits = 16;
 constexpr float kNaN = __builtin_nanf("");
 
 __host__ __device__ constexpr int64_t round_up(int64_t x, int64_t to) {
@@ -490,15 +492,69 @@ __global__ __launch_bounds__(256) void target_grad_kernel(int32_t k, int32_t voc
   dz[m * ld + v] = from_f32<T>(coef[m] * (p - s.target[at]));
 }
 
+// dz W has (C / tile) x (rows / tile) tiles, often fewer than CUs, over a long k:
+// k is split so that the rounds of tiles are full, by the estimate
+//   rounds x (steps of a split x step_us + fixed_us) + splits x slab_us,
+// a slab being written and read once. The host allocates room for the splits
+// of all rows; how many the rows that take part want, fewer rows more of them,
+// is found where their count is known.
+struct Splitting {
+  int32_t steps;  // of a whole piece
+  int32_t across; // tiles over C
+  int32_t tile;   // rows of a tile
+  float step_us, fixed_us, row_slab_us;
+  int64_t room;   // rows of all slabs of a piece
+};
+
+__host__ __device__ inline float split_us(const Splitting& x, int64_t rows, int32_t s) {
+  const int64_t tiles = (rows + x.tile - 1) / x.tile * x.across;
+  return static_cast<float>((tiles * s + kCus - 1) / kCus) *
+             (static_cast<float>((x.steps + s - 1) / s) * x.step_us + x.fixed_us) +
+         static_cast<float>(s) * static_cast<float>(rows) * x.row_slab_us;
+}
+
+__host__ __device__ inline bool may_split(const Splitting& x, int64_t rows, int32_t s) {
+  return s == 1 || (x.steps / s >= 8 && s * rows <= x.room);
+}
+
+int32_t splits_of(const Splitting& x, int64_t rows) {
+  int32_t best = 1;
+  for (int32_t s = 2; s <= kMostSplits; ++s) {
+    if (may_split(x, rows, s) && split_us(x, rows, s) < split_us(x, rows, best)) best = s;
+  }
+  return best;
+}
+
+// The same by one wave, a lane a choice.
+__device__ __forceinline__ int32_t wave_splits_of(const Splitting& x, int64_t rows) {
+  const int lane = threadIdx.x & 63;
+  int32_t best = lane + 1;
+  float least = lane < kMostSplits && may_split(x, rows, best) ? split_us(x, rows, best) : 3e38f;
+#pragma unroll
+  for (int off = 1; off < kMostSplits; off <<= 1) {
+    const float us = __shfl_xor(least, off, 64);
+    const int32_t s = __shfl_xor(best, off, 64);
+    if (us < least || (us == least && s < best)) {
+      least = us;
+      best = s;
+    }
+  }
+  return __shfl(best, 0, 64);
+}
+
 // D[c][m] = sum over a split's vocabulary of W[v][c] dz[m][v], to slab [m][c]
 // of the split (fp32).
 template <typename G, typename T>
 __global__ __launch_bounds__(gemm::kThreads, 2) void hidden_grad_kernel(
-    Operand w, Operand dz, const int32_t* __restrict__ count, int32_t steps, int32_t split_steps,
-    int32_t splits, int32_t np, int32_t c, float* __restrict__ slabs, int64_t slab) {
+    Operand w, Operand dz, const int32_t* __restrict__ count,
+    const int32_t* __restrict__ split_count, int32_t steps, int32_t whole_steps, int32_t np,
+    int32_t piece, int32_t c, float* __restrict__ slabs) {
   __shared__ __attribute__((aligned(1024))) char smem[G::kLdsBytes];
   const int rows = *count;
+  const int splits = *split_count;
+  const int split_steps = (whole_steps + splits - 1) / splits;
   const int nq = row_tiles_of(rows, G::kBQ), each = np * nq, total = each * splits;
+  const int64_t slab = static_cast<int64_t>(rows) * c;
   int id = blockIdx.x;
   if (id >= total) return;
   G tile;
@@ -517,7 +573,7 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void hidden_grad_kernel(
   while (true) {
     tile.multiply(smem);
     const int p0 = tp * G::kBP, q0 = tq * G::kBQ;
-    float* out = slabs + split * slab;
+    float* out = slabs + (static_cast<int64_t>(piece) * splits + split) * slab;
     id += gridDim.x;
     if (id < total) {
       begin();
@@ -543,10 +599,11 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void hidden_grad_kernel(
 // rows that took no part.
 template <typename T>
 __global__ __launch_bounds__(256) void hidden_grad_rows_kernel(
-    const float* __restrict__ slabs, int64_t slab, int32_t count, int32_t c, int64_t n,
-    const float* __restrict__ scale, const int32_t* __restrict__ place,
-    uint16_t* __restrict__ dh) {
-  const int64_t quads = n * (c / 4);
+    const float* __restrict__ slabs, const int32_t* __restrict__ rows,
+    const int32_t* __restrict__ split_count, int32_t pieces, int32_t c, int64_t n, const float* __restrict__ scale,
+    const int32_t* __restrict__ place, uint16_t* __restrict__ dh) {
+  const int64_t quads = n * (c / 4), slab = static_cast<int64_t>(*rows) * c;
+  const int count = pieces * *split_count;
   const float by = *scale;
   for (int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; e < quads;
        e += static_cast<int64_t>(gridDim.x) * 256) {
@@ -683,9 +740,14 @@ __global__ __launch_bounds__(kScanThreads) void sum_losses_kernel(
 // is at most 2^14, and 2^-28 of that is the smallest one.
 __global__ __launch_bounds__(kScanThreads) void row_coefficients_kernel(
     const float* __restrict__ upstream, bool per_row, bool mean, float temperature, int up,
-    float* __restrict__ coef, float* __restrict__ scale, Saved s) {
+    Splitting splitting, float* __restrict__ coef, float* __restrict__ scale,
+    int32_t* __restrict__ splits, Saved s) {
   __shared__ float waves[kScanThreads / 64];
   const int n = *s.count;
+  if (threadIdx.x < 64) {
+    const int32_t most = wave_splits_of(splitting, n);
+    if (threadIdx.x == 0) *splits = most;
+  }
   const float by = mean ? temperature / static_cast<float>(n > 0 ? n : 1) : temperature;
   const float lift = ldexpf(1.0f, up);
   if (!per_row) {
@@ -712,8 +774,6 @@ __global__ __launch_bounds__(kScanThreads) void row_coefficients_kernel(
 }
 
 // ---------------------------------------------------------------- launches
-constexpr int kCus = 256;
-
 enum class Size { kFewRows, kSmall, kLarge };
 
 struct TileTime {
@@ -731,9 +791,9 @@ int64_t tiles_of(Size s, int64_t p, int64_t q) {
   return (p + t.p - 1) / t.p * ((q + t.q - 1) / t.q);
 }
 
-double product_us(Size s, int64_t p, int64_t q, int64_t steps, int64_t splits = 1) {
-  const int64_t rounds = (tiles_of(s, p, q) * splits + kCus - 1) / kCus;
-  return rounds * ((steps + splits - 1) / splits * time_of(s).step_us + time_of(s).fixed_us);
+double product_us(Size s, int64_t p, int64_t q, int64_t steps) {
+  const int64_t rounds = (tiles_of(s, p, q) + kCus - 1) / kCus;
+  return rounds * (steps * time_of(s).step_us + time_of(s).fixed_us);
 }
 
 // How a product over a range of the vocabulary is tiled: `first` columns with
@@ -772,7 +832,7 @@ Cut cut_of(int64_t vocab, int64_t across, int64_t steps, bool rows) {
 struct Plan {
   int32_t columns;  // of a piece, a multiple of kVocabTile
   int32_t pieces;
-  int32_t splits;   // of a piece's columns in dz W, whose tiles are few and whose k is long
+  int32_t splits;   // of a piece's columns in dz W, for all rows
   Size hidden;
 };
 
@@ -784,6 +844,13 @@ constexpr int64_t kCachedBytes = int64_t{192} << 20;
 constexpr int64_t kMostBytes = int64_t{512} << 20;
 constexpr double kGradBytesPerUs = 20.0e6;
 constexpr double kSlabBytesPerUs = 4.0e6;
+
+Splitting splitting_of(Size size, int64_t columns, int64_t c, int64_t room) {
+  const TileTime& t = time_of(size);
+  return {static_cast<int32_t>(columns / gemm::kStep), static_cast<int32_t>((c + t.p - 1) / t.p),
+          t.q, static_cast<float>(t.step_us), static_cast<float>(t.fixed_us),
+          static_cast<float>(4.0 * c / kSlabBytesPerUs), room};
+}
 
 Plan plan_of(int64_t n, int64_t c, int64_t vocab) {
   const int64_t all = round_up(vocab, kVocabTile), pad = round_up(n, kRowPad);
@@ -802,17 +869,16 @@ Plan plan_of(int64_t n, int64_t c, int64_t vocab) {
     double us = 12.0 + cut_of(p.columns, n, steps_c, true).us +
                 cut_of(p.columns, c, steps_n, false).us +
                 (bytes > kCachedBytes ? 3 * bytes / kGradBytesPerUs : 0.0);
-    const int64_t steps = p.columns / gemm::kStep;
     double hidden = 1e300;
     for (Size size : {Size::kFewRows, Size::kSmall, Size::kLarge}) {
       if ((size == Size::kFewRows) != (n <= time_of(Size::kFewRows).q)) continue;
-      for (int32_t s = 1; s <= 16 && (s == 1 || steps / s >= 8); ++s) {
-        const double t = product_us(size, c, n, steps, s) + s * (4.0 * n * c / kSlabBytesPerUs);
-        if (t >= hidden) continue;
-        hidden = t;
-        p.splits = s;
-        p.hidden = size;
-      }
+      const Splitting x = splitting_of(size, p.columns, c, kMostSplits * n);
+      const int32_t splits = splits_of(x, n);
+      const double t = split_us(x, n, splits);
+      if (t >= hidden) continue;
+      hidden = t;
+      p.splits = splits;
+      p.hidden = size;
     }
     us = (us + hidden) * p.pieces;
     if (us < least) {
@@ -822,6 +888,12 @@ Plan plan_of(int64_t n, int64_t c, int64_t vocab) {
     if (bytes < kCachedBytes / 8) break;  // smaller pieces only add launches
   }
   return best;
+}
+
+// Rows of a piece's slabs: a slab more than all rows want, so that a part of the
+// rows, which want more splits, can have them.
+int64_t slab_rows(const Plan& plan, int64_t n) {
+  return plan.splits == 1 ? n : (plan.splits + 1) * n;
 }
 
 struct ForwardWork {
@@ -843,6 +915,7 @@ ForwardWork forward_work(char* p, int64_t n, int64_t vocab, size_t* bytes) {
 struct BackwardWork {
   float* coef;
   float* scale;
+  int32_t* splits;
   uint16_t* dz;
   float* slabs;
 };
@@ -851,12 +924,13 @@ BackwardWork backward_work(char* p, int64_t n, int64_t c, const Plan& plan, bool
                            size_t* bytes) {
   const int64_t pad = round_up(n, kRowPad);
   Layout l;
-  const size_t coef = l.take(pad * 4), scale = l.take(4), dz = l.take(pad * plan.columns * 2);
+  const size_t coef = l.take(pad * 4), scale = l.take(4), splits = l.take(4);
+  const size_t dz = l.take(pad * plan.columns * 2);
   const size_t slabs =
-      l.take(hidden ? static_cast<size_t>(plan.pieces) * plan.splits * n * c * 4 : 0);
+      l.take(hidden ? static_cast<size_t>(plan.pieces) * slab_rows(plan, n) * c * 4 : 0);
   *bytes = l.bytes;
   return {reinterpret_cast<float*>(p + coef), reinterpret_cast<float*>(p + scale),
-          reinterpret_cast<uint16_t*>(p + dz), reinterpret_cast<float*>(p + slabs)};
+          reinterpret_cast<int32_t*>(p + splits), reinterpret_cast<uint16_t*>(p + dz), reinterpret_cast<float*>(p + slabs)};
 }
 
 struct Shape {
@@ -950,15 +1024,11 @@ void launch_piece(const Shape& d, const Plan& plan, int piece, const uint16_t* w
                      dim3(256), 0, stream, d.k, first, columns, scale, w.coef, w.dz, ld, s);
   if (dh != nullptr) {
     const int steps = static_cast<int>(round_up(columns, gemm::kStep) / gemm::kStep);
-    const int each = (plan.columns / gemm::kStep + plan.splits - 1) / plan.splits;
-    const int64_t slab = d.n * d.c;
     with_tile<T, Major::kX, Major::kK>(plan.hidden, [&](auto* tile) {
       using G = std::remove_pointer_t<decltype(tile)>;
-      hipLaunchKernelGGL((hidden_grad_kernel<G, T>),
-                         dim3(grid_of(tiles_of(plan.hidden, d.c, d.n) * plan.splits)),
-                         dim3(gemm::kThreads), 0, stream, wp, dz, s.count, steps, each,
-                         plan.splits, (d.c + G::kBP - 1) / G::kBP, d.c,
-                         w.slabs + piece * plan.splits * slab, slab);
+      hipLaunchKernelGGL((hidden_grad_kernel<G, T>), dim3(kCus), dim3(gemm::kThreads), 0, stream,
+                         wp, dz, s.count, w.splits, steps, plan.columns / gemm::kStep,
+                         (d.c + G::kBP - 1) / G::kBP, piece, d.c, w.slabs);
     });
   }
   if (dw != nullptr) {
@@ -982,7 +1052,9 @@ int run_backward(const Shape& d, const void* weight, const float* upstream, bool
                  const Plan& plan, const BackwardWork& w, hipStream_t stream) {
   const float scale = kLog2E / temperature;
   hipLaunchKernelGGL(row_coefficients_kernel, dim3(1), dim3(kScanThreads), 0, stream, upstream,
-                     per_row, mean, temperature, __is_same(T, F16) ? 14 : 0, w.coef, w.scale, s);
+                     per_row, mean, temperature, __is_same(T, F16) ? 14 : 0,
+                     splitting_of(plan.hidden, plan.columns, d.c, slab_rows(plan, d.n)), w.coef,
+                     w.scale, w.splits, s);
   for (int p = 0; p < plan.pieces; ++p) {
     launch_piece<T>(d, plan, p, static_cast<const uint16_t*>(weight), scale,
                     static_cast<uint16_t*>(dh), static_cast<uint16_t*>(dw), s, w, stream);
@@ -991,7 +1063,7 @@ int run_backward(const Shape& d, const void* weight, const float* upstream, bool
     const int64_t quads = d.n * (d.c / 4);
     const int64_t blocks = std::min<int64_t>((quads + 255) / 256, 8192);
     hipLaunchKernelGGL((hidden_grad_rows_kernel<T>), dim3(static_cast<unsigned>(blocks)),
-                       dim3(256), 0, stream, w.slabs, d.n * d.c, plan.pieces * plan.splits,
+                       dim3(256), 0, stream, w.slabs, s.count, w.splits, plan.pieces,
                        d.c, d.n, w.scale, s.place, static_cast<uint16_t*>(dh));
   }
   return check_launch("linear loss backward");
@@ -1001,8 +1073,9 @@ int check_shape(const char* what, int io_dtype, int64_t n, int64_t c, int64_t vo
   if (io_dtype != FRWKV_DTYPE_F16 && io_dtype != FRWKV_DTYPE_BF16) {
     return set_error(FRWKV_ERR_UNSUPPORTED, "%s: io dtype must be float16 or bfloat16", what);
   }
-  if (n <= 0 || n > (int64_t{1} << 28)) {
-    return set_error(FRWKV_ERR_INVALID_ARGUMENT, "%s: rows must be in [1, 2^28], got %lld", what,
+  // A launch holds less than 2^32 threads, 256 a row.
+  if (n <= 0 || n > (int64_t{1} << 23)) {
+    return set_error(FRWKV_ERR_INVALID_ARGUMENT, "%s: rows must be in [1, 2^23], got %lld", what,
                      static_cast<long long>(n));
   }
   if (c <= 0 || c % gemm::kStep != 0 || c > 65536) {
@@ -1020,8 +1093,9 @@ int check_shape(const char* what, int io_dtype, int64_t n, int64_t c, int64_t vo
                      static_cast<long long>(k));
   }
   const int64_t tiles = round_up(vocab, kMinTile) / kMinTile * (round_up(n, kMinTile) / kMinTile);
-  if (tiles > (int64_t{1} << 22) || n * k > (int64_t{1} << 38)) {
-    return set_error(FRWKV_ERR_UNSUPPORTED, "%s: rows x vocabulary too large for one call", what);
+  if (tiles >= (int64_t{1} << 30) || n * k >= (int64_t{1} << 31)) {
+    return set_error(FRWKV_ERR_UNSUPPORTED,
+                     "%s: rows x vocabulary or rows x targets too large for one call", what);
   }
   return FRWKV_OK;
 }

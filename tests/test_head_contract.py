@@ -176,6 +176,7 @@ def test_c_abi_rejects_bad_loss_calls_without_a_gpu():
     for kw, rc, message in (
             ({"hidden": null}, 1, b"null pointer"), ({"dtype": 0}, 2, b"io dtype"),
             ({"c": 100}, 2, b"multiple of 64"), ({"n": 0}, 1, b"rows must be"),
+            ({"n": 1 << 24}, 1, b"rows must be"), ({"n": 1 << 22, "v": 1 << 24}, 2, b"too large"),
             ({"v": 0}, 1, b"vocabulary"), ({"reduction": 3}, 1, b"unknown reduction"),
             ({"hidden": ctypes.c_void_p(0x1008)}, 1, b"16-byte aligned"),
             ({"saved_": saved - 1}, 1, b"saved of"), ({"work_": work - 1}, 1, b"workspace of"),
