@@ -18,16 +18,17 @@
 // the count end at once.
 //
 // Forward: one product h W^T whose epilogue keeps the maximum and the sum of
-// exponentials of each 256-column tile, row by row; a second kernel joins the
-// tiles. The K target logits of a row are dot products of their own (fp32).
+// exponentials of each tile's columns, row by row; a second kernel joins the
+// tiles. A row's one target logit is taken from the accumulators that hold it;
+// K > 1 of them are dot products of their own (fp32).
 // Backward, for one piece of the vocabulary after another: the product again,
 // its epilogue turning logits into dz of the piece (16 bits, [rows][piece]);
 // the target entries are overwritten from the fp32 target logits, so that
 // p - b does not lose digits where the two are close; then dz W into an fp32
 // slab (its sum over slabs, in order, is dh) and dz^T h, which is dW's rows.
 // Everything is summed in fp32 in a fixed order; dz is the only rounding to
-// 16 bits before the outputs, as a matrix operand has to be (relative error
-// 2^-9 an entry for bf16, independent between entries).
+// 16 bits before the outputs, as a matrix operand has to be (relative error at
+// most 2^-8 an entry for bf16, independent between entries).
 #include <algorithm>
 #include <type_traits>
 
@@ -46,6 +47,7 @@ constexpr float kLn2 = 0.69314718055994531f;
 constexpr int kRowPad = 256;       // rows of workspaces, and a product's largest tile
 constexpr int kVocabTile = 256;    // pieces of the vocabulary are whole multiples of it
 constexpr int kMinTile = 128;      // fewest columns whose maximum and sum the forward keeps
+constexpr int kFewest = 32;        // rows up to here: see Twice below
 constexpr int kScanThreads = 1024;
 constexpr int kCus = 256;
 constexpr int kMostSplits = 16;
@@ -60,6 +62,16 @@ __device__ __forceinline__ void unpack8(uint4 q, float (&out)[8]) {
   const uint16_t* s = reinterpret_cast<const uint16_t*>(&q);
 #pragma unroll
   for (int e = 0; e < 8; ++e) out[e] = to_f32<T>(s[e]);
+}
+
+template <typename T>
+__device__ __forceinline__ float low(uint32_t pair) {
+  return to_f32<T>(static_cast<uint16_t>(pair & 0xffffu));
+}
+
+template <typename T>
+__device__ __forceinline__ float high(uint32_t pair) {
+  return to_f32<T>(static_cast<uint16_t>(pair >> 16));
 }
 
 __device__ __forceinline__ float wave_sum(float x) {
@@ -259,17 +271,18 @@ __global__ __launch_bounds__(kScanThreads) void teacher_rows_kernel(int32_t n, f
 }
 
 // A workgroup a row m: copies its hidden row (zeros for the rows that fill up
-// the last tile) and computes its target logits, a wave a token.
-// base[i] becomes sum p (log p - s z), what lse is added to.
+// the last tile; few rows a second time kFewest rows on) and computes its K > 1
+// target logits, a wave a token (NaN for one out of range). Bound by the K weight
+// rows a row (64 of 2048 channels for 4096 rows: 152 us, 7.1 TB/s).
 template <typename T>
 __global__ __launch_bounds__(256) void gather_rows_kernel(
     const uint16_t* __restrict__ hidden, const uint16_t* __restrict__ weight, int32_t c,
-    int32_t k, int32_t vocab, float inv_temperature, float* __restrict__ target_term, Saved s) {
-  __shared__ float part[4];
-  const int m = blockIdx.x;
+    int32_t k, int32_t vocab, bool twice, Saved s) {
   const int count = *s.count;
+  const int second = twice && blockIdx.x >= kFewest ? kFewest : 0;
+  const int m = static_cast<int>(blockIdx.x) - second;
   if (m >= round_up(count, kRowPad)) return;
-  uint16_t* to = s.hidden + static_cast<int64_t>(m) * c;
+  uint16_t* to = s.hidden + static_cast<int64_t>(blockIdx.x) * c;
   if (m >= count) {
     for (int x = threadIdx.x * 8; x < c; x += 2048) {
       *reinterpret_cast<uint4*>(to + x) = make_uint4(0, 0, 0, 0);
@@ -281,8 +294,12 @@ __global__ __launch_bounds__(256) void gather_rows_kernel(
   for (int x = threadIdx.x * 8; x < c; x += 2048) {
     *reinterpret_cast<uint4*>(to + x) = *reinterpret_cast<const uint4*>(from + x);
   }
+  if (second > 0) return;
+  if (k == 1) {  // one out of range; lse_tiles_kernel writes the others
+    if (threadIdx.x == 0) s.logit[m] = kNaN;
+    return;
+  }
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  float term = 0.0f;
   for (int j = wave; j < k; j += 4) {
     const int32_t token = s.index[i * k + j];
     float z = 0.0f;
@@ -301,12 +318,7 @@ __global__ __launch_bounds__(256) void gather_rows_kernel(
       z = kNaN;
     }
     if (lane == 0) s.logit[static_cast<int64_t>(m) * k + j] = z;
-    const float p = s.share[i * k + j];
-    if (token >= 0) term += p == 0.0f && token < vocab ? 0.0f : p * (z * inv_temperature);
   }
-  if (lane == 0) part[wave] = term;
-  __syncthreads();
-  if (threadIdx.x == 0) target_term[m] = s.base[i] - (part[0] + part[1] + part[2] + part[3]);
 }
 
 // ------------------------------------------------------------- products
@@ -327,15 +339,18 @@ using FewRowsTile = gemm::Tile<T, MA, MB, 256, 64, 8, 1, 3, MA == Major::kK && M
 // workgroup finishes a tile, the first stages of its next one are on their way.
 __device__ __forceinline__ int row_tiles_of(int rows, int tile) { return (rows + tile - 1) / tile; }
 
-// D[v][m] of a vocabulary range: per tile of 256 v and row m the maximum of
-// s z log2 e and the sum of 2^(s z log2 e - maximum), to part[tile][m].
+// D[v][m] of a vocabulary range: per tile of v and row m the maximum of
+// s z log2 e and the sum of 2^(s z log2 e - maximum), to part[tile][m]. one: rows
+// have one target each, whose logit goes to s.logit as it stands here, so that
+// it cancels against a maximum that it is.
 template <typename G, typename T>
 __global__ __launch_bounds__(gemm::kThreads, 2) void lse_tiles_kernel(
-    Operand w, Operand h, const int32_t* __restrict__ count, int32_t c, int32_t np, float scale,
-    float2* __restrict__ part, int64_t pad) {
+    Operand w, Operand h, int32_t c, int32_t np, float scale, int32_t vocab0, bool one,
+    float2* __restrict__ part, int64_t pad, Saved s) {
   __shared__ __attribute__((aligned(1024))) char smem[G::kLdsBytes];
   __shared__ float maxima[G::kWP][G::kBQ], sums[G::kWP][G::kBQ];
-  const int nq = row_tiles_of(*count, G::kBQ), total = np * nq, steps = c / gemm::kStep;
+  const int rows = *s.count;
+  const int nq = row_tiles_of(rows, G::kBQ), total = np * nq, steps = c / gemm::kStep;
   int id = blockIdx.x;
   if (id >= total) return;
   G tile;
@@ -344,8 +359,18 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void lse_tiles_kernel(
   tile.begin(w, h, tp * G::kBP, tq * G::kBQ, 0, steps, smem, G::kTurns ? tp % steps : 0);
   G::arrive();
   while (true) {
-    tile.multiply(smem);
     const int p0 = tp * G::kBP, q0 = tq * G::kBQ;
+    int token[G::TQ];
+#pragma unroll
+    for (int j = 0; j < G::TQ; ++j) {
+      const int m = q0 + G::column(j);
+      token[j] = one && m < rows ? s.index[s.row[m]] : -1;
+    }
+    tile.multiply(smem);
+    // The compiler's wait for these comes here, not behind the loads that
+    // begin starts, which it does not count.
+#pragma unroll
+    for (int j = 0; j < G::TQ; ++j) asm volatile("" : "+v"(token[j]));
     const int64_t to = static_cast<int64_t>(tp) * pad + q0;
     id += gridDim.x;
     if (id < total) {
@@ -395,6 +420,21 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void lse_tiles_kernel(
       }
     }
     G::arrive();
+#pragma unroll
+    for (int j = 0; j < G::TQ; ++j) {
+      // Rows 16 i + r from here on are this lane's.
+      const int at = token[j] - vocab0 - p0, row = at - G::row(0);
+      const bool here =
+          token[j] >= 0 && at < left && row >= 0 && row < 16 * G::TP && (row & 15) < 4;
+      if (__ballot(here) == 0) continue;
+      float z = 0.0f;
+#pragma unroll
+      for (int i = 0; i < G::TP; ++i) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) z = row == 16 * i + r ? tile.acc[i][j][r] : z;
+      }
+      if (here) s.logit[q0 + G::column(j)] = z;
+    }
     __syncthreads();
     for (int q = threadIdx.x; q < G::kBQ; q += gemm::kThreads) {
       float top = maxima[0][q];
@@ -414,11 +454,20 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void lse_tiles_kernel(
 
 // D[v][m] of a piece of the vocabulary: dz[m][v] = coef_m (2^(s z log2 e -
 // lse2_m)), zero for rows and columns that are not there.
+//
+// Twice: rounding dz to 16 bits is one error for all elements that a target
+// entry dominates, up to 2^-9 of the entry 1 for bf16. Over many rows such
+// errors average out below the outputs' own rounding; in a few rows one can be
+// twice that. Up to kFewest rows leave half of a tile's columns unused, so there
+// dz has two terms, row m the rounded value and row kFewest + m what is left of
+// it, and the products add both at no cost (bf16 gradients of 3 weighted rows,
+// 3001 x 512: up to 3.8e-3 off with one term, 1.7e-3 with two, the outputs' own
+// rounding).
 template <typename G, typename T>
 __global__ __launch_bounds__(gemm::kThreads, 2) void softmax_grad_kernel(
     Operand w, Operand h, const int32_t* __restrict__ count, int32_t c, int32_t np, float scale,
-    const float* __restrict__ lse2, const float* __restrict__ coef, uint16_t* __restrict__ dz,
-    int64_t ld) {
+    const float* __restrict__ lse2, const float* __restrict__ coef, bool twice,
+    uint16_t* __restrict__ dz, int64_t ld) {
   __shared__ __attribute__((aligned(1024))) char smem[G::kLdsBytes];
   const int rows = *count;
   const int nq = row_tiles_of(rows, G::kBQ), total = np * nq, steps = c / gemm::kStep;
@@ -450,10 +499,13 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void softmax_grad_kernel(
     }
     const int left = w.rows - p0;
     const bool all = left >= G::kBP && rows - q0 >= G::kBQ;
+    constexpr int kHalf = kFewest / 16;  // columns j of the first term
+    const bool second = G::kBQ == 2 * kFewest && twice;
 #pragma unroll
     for (int j = 0; j < G::TQ; ++j) {
+      if (second && j >= kHalf) break;
       const bool here = q0 + G::column(j) < rows;
-      uint2 out[G::TP];
+      uint2 out[G::TP], rest[G::TP];
 #pragma unroll
       for (int i = 0; i < G::TP; ++i) {
         float x[4];
@@ -463,11 +515,21 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void softmax_grad_kernel(
           if (!all) x[r] = here && G::row(i) + r < left ? x[r] : 0.0f;
         }
         out[i] = make_uint2(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]));
+        if (second) {
+          rest[i] = make_uint2(
+              pack2<T>(x[0] - low<T>(out[i].x), x[1] - high<T>(out[i].x)),
+              pack2<T>(x[2] - low<T>(out[i].y), x[3] - high<T>(out[i].y)));
+        }
       }
       // The next tile's loads are waited for before the first store, which
       // would have to be waited for with them.
       if (j == 0) G::arrive();
       gemm::store_column<G>(dz + q0 * ld + p0, ld, G::kBP, G::kBQ, j, out);
+      if constexpr (G::kBQ == 2 * kFewest) {
+        if (second) {
+          gemm::store_column<G>(dz + q0 * ld + p0, ld, G::kBP, G::kBQ, (j + kHalf) % G::TQ, rest);
+        }
+      }
     }
     if (id >= total) return;
   }
@@ -480,8 +542,8 @@ template <typename T>
 __global__ __launch_bounds__(256) void target_grad_kernel(int32_t k, int32_t vocab0,
                                                           int32_t columns, float scale,
                                                           const float* __restrict__ coef,
-                                                          uint16_t* __restrict__ dz, int64_t ld,
-                                                          Saved s) {
+                                                          bool twice, uint16_t* __restrict__ dz,
+                                                          int64_t ld, Saved s) {
   const int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   const int64_t m = e / k;
   if (m >= *s.count) return;
@@ -489,7 +551,10 @@ __global__ __launch_bounds__(256) void target_grad_kernel(int32_t k, int32_t voc
   const int32_t v = s.index[at] - vocab0;
   if (s.index[at] < 0 || v < 0 || v >= columns) return;
   const float p = __builtin_amdgcn_exp2f(fmaf(s.logit[e], scale, -s.lse2[m]));
-  dz[m * ld + v] = from_f32<T>(coef[m] * (p - s.target[at]));
+  const float x = coef[m] * (p - s.target[at]);
+  const uint16_t rounded = from_f32<T>(x);
+  dz[m * ld + v] = rounded;
+  if (twice) dz[(m + kFewest) * ld + v] = from_f32<T>(x - to_f32<T>(rounded));
 }
 
 // dz W has (C / tile) x (rows / tile) tiles, often fewer than CUs, over a long k:
@@ -548,7 +613,7 @@ template <typename G, typename T>
 __global__ __launch_bounds__(gemm::kThreads, 2) void hidden_grad_kernel(
     Operand w, Operand dz, const int32_t* __restrict__ count,
     const int32_t* __restrict__ split_count, int32_t steps, int32_t whole_steps, int32_t np,
-    int32_t piece, int32_t c, float* __restrict__ slabs) {
+    int32_t piece, int32_t c, bool twice, float* __restrict__ slabs) {
   __shared__ __attribute__((aligned(1024))) char smem[G::kLdsBytes];
   const int rows = *count;
   const int splits = *split_count;
@@ -579,6 +644,16 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void hidden_grad_kernel(
       begin();
       G::arrive();
     }
+    if constexpr (G::kBQ == 2 * kFewest) {
+      if (twice) {  // both terms of dz; they lie in one lane
+        constexpr int kHalf = kFewest / 16;
+#pragma unroll
+        for (int j = 0; j < kHalf; ++j) {
+#pragma unroll
+          for (int i = 0; i < G::TP; ++i) tile.acc[i][j] += tile.acc[i][j + kHalf];
+        }
+      }
+    }
 #pragma unroll
     for (int j = 0; j < G::TQ; ++j) {
       const int m = q0 + G::column(j);
@@ -600,8 +675,8 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void hidden_grad_kernel(
 template <typename T>
 __global__ __launch_bounds__(256) void hidden_grad_rows_kernel(
     const float* __restrict__ slabs, const int32_t* __restrict__ rows,
-    const int32_t* __restrict__ split_count, int32_t pieces, int32_t c, int64_t n, const float* __restrict__ scale,
-    const int32_t* __restrict__ place, uint16_t* __restrict__ dh) {
+    const int32_t* __restrict__ split_count, int32_t pieces, int32_t c, int64_t n,
+    const float* __restrict__ scale, const int32_t* __restrict__ place, uint16_t* __restrict__ dh) {
   const int64_t quads = n * (c / 4), slab = static_cast<int64_t>(*rows) * c;
   const int count = pieces * *split_count;
   const float by = *scale;
@@ -665,11 +740,14 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void weight_grad_kernel(
 // A workgroup takes 32 rows, 32 threads a row: joins the tiles' maxima and
 // sums to lse2[m], and the row's loss. row_loss (by i) or partial (by m). A
 // thread has 8 tiles under way at a time, all of those of 65536 columns.
+// In the loss the target logits are taken from the row's maximum, a difference
+// that is exact where they are close, and not from lse, whose rounding alone
+// (half a unit of 16 in base 2) is 1e-6 of a loss near 1.
 __global__ __launch_bounds__(1024) void join_tiles_kernel(const float2* __restrict__ part,
-                                                          int32_t tiles, int64_t pad,
-                                                          const float* __restrict__ target_term,
-                                                          float temperature2, float* row_loss,
-                                                          float* partial, Saved s) {
+                                                          int32_t tiles, int64_t pad, int32_t k,
+                                                          float scale, float temperature2,
+                                                          float* row_loss, float* partial,
+                                                          Saved s) {
   __shared__ float2 shared[32][33];
   const int q = threadIdx.x & 31, slice = threadIdx.x >> 5;
   const int m = blockIdx.x * 32 + q;
@@ -697,14 +775,27 @@ __global__ __launch_bounds__(1024) void join_tiles_kernel(const float2* __restri
   for (int off = 1; off < 32; off <<= 1) {
     all = joined(all, make_float2(__shfl_xor(all.x, off, 64), __shfl_xor(all.y, off, 64)));
   }
+  // The lanes' orders differ: the first one's result.
+  const float top = __shfl(all.x, threadIdx.x & 32, 64);
   const int mine = blockIdx.x * 32 + row;
+  float term = 0.0f;
+  int64_t i = 0;
+  if (mine < count) {
+    i = s.row[mine];
+    for (int j = lane; j < k; j += 32) {
+      const float p = s.share[i * k + j], z = s.logit[static_cast<int64_t>(mine) * k + j];
+      // Absent entries have p = 0; one out of range has z = NaN.
+      if (p != 0.0f || z != z) term = fmaf(p, fmaf(-z, scale, top), term);
+    }
+  }
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) term += __shfl_xor(term, off, 64);
   if (lane != 0 || mine >= count) return;
-  const float lse2 = all.x + __builtin_amdgcn_logf(all.y);
-  const float term = target_term[mine];
+  const float log_sum = __builtin_amdgcn_logf(all.y);
   // A target out of range makes its row NaN in the backward too.
-  s.lse2[mine] = term == term ? lse2 : term;
-  const float loss = temperature2 * (lse2 * kLn2 + term);
-  if (row_loss) row_loss[s.row[mine]] = loss;
+  s.lse2[mine] = term == term ? top + log_sum : term;
+  const float loss = temperature2 * ((term + log_sum) * kLn2 + s.base[i]);
+  if (row_loss) row_loss[i] = loss;
   if (partial) partial[mine] = loss;
 }
 
@@ -782,7 +873,8 @@ struct TileTime {
 };
 
 // Measured on products that fill the GPU for many rounds.
-constexpr TileTime kTileTimes[] = {{256, 64, 1.0, 3.0}, {128, 128, 0.6, 3.0}, {256, 256, 1.65, 5.0}};
+constexpr TileTime kTileTimes[] = {
+    {256, 64, 1.0, 3.0}, {128, 128, 0.6, 3.0}, {256, 256, 1.65, 5.0}};
 
 const TileTime& time_of(Size s) { return kTileTimes[static_cast<int>(s)]; }
 
@@ -898,7 +990,6 @@ int64_t slab_rows(const Plan& plan, int64_t n) {
 
 struct ForwardWork {
   float2* part;
-  float* target_term;
   float* partial;
 };
 
@@ -906,10 +997,9 @@ ForwardWork forward_work(char* p, int64_t n, int64_t vocab, size_t* bytes) {
   const int64_t pad = round_up(n, kRowPad);
   Layout l;
   const size_t part = l.take(round_up(vocab, kMinTile) / kMinTile * pad * 8);
-  const size_t term = l.take(pad * 4), partial = l.take(pad * 4);
+  const size_t partial = l.take(pad * 4);
   *bytes = l.bytes;
-  return {reinterpret_cast<float2*>(p + part), reinterpret_cast<float*>(p + term),
-          reinterpret_cast<float*>(p + partial)};
+  return {reinterpret_cast<float2*>(p + part), reinterpret_cast<float*>(p + partial)};
 }
 
 struct BackwardWork {
@@ -930,7 +1020,8 @@ BackwardWork backward_work(char* p, int64_t n, int64_t c, const Plan& plan, bool
       l.take(hidden ? static_cast<size_t>(plan.pieces) * slab_rows(plan, n) * c * 4 : 0);
   *bytes = l.bytes;
   return {reinterpret_cast<float*>(p + coef), reinterpret_cast<float*>(p + scale),
-          reinterpret_cast<int32_t*>(p + splits), reinterpret_cast<uint16_t*>(p + dz), reinterpret_cast<float*>(p + slabs)};
+          reinterpret_cast<int32_t*>(p + splits), reinterpret_cast<uint16_t*>(p + dz),
+          reinterpret_cast<float*>(p + slabs)};
 }
 
 struct Shape {
@@ -971,8 +1062,7 @@ int run_forward(const Shape& d, const void* hidden, const void* weight, float te
   const int n = static_cast<int>(d.n);
   hipLaunchKernelGGL((gather_rows_kernel<T>), dim3(static_cast<unsigned>(pad)), dim3(256), 0,
                      stream, static_cast<const uint16_t*>(hidden),
-                     static_cast<const uint16_t*>(weight), d.c, d.k, d.vocab, 1.0f / temperature,
-                     w.target_term, s);
+                     static_cast<const uint16_t*>(weight), d.c, d.k, d.vocab, d.n <= kFewest, s);
   int tiles = 0;
   const Operand b{s.hidden, d.c, static_cast<int32_t>(pad)};
   for_cut(cut_of(d.vocab, d.n, d.c / gemm::kStep, true), d.vocab,
@@ -982,13 +1072,13 @@ int run_forward(const Shape& d, const void* hidden, const void* weight, float te
     with_tile<T, Major::kK, Major::kK>(size, [&](auto* tile) {
       using G = std::remove_pointer_t<decltype(tile)>;
       hipLaunchKernelGGL((lse_tiles_kernel<G, T>), dim3(grid_of(tiles_of(size, columns, d.n))),
-                         dim3(gemm::kThreads), 0, stream, a, b, s.count, d.c, np, scale,
-                         w.part + tiles * pad, pad);
+                         dim3(gemm::kThreads), 0, stream, a, b, d.c, np, scale,
+                         static_cast<int32_t>(first), d.k == 1, w.part + tiles * pad, pad, s);
     });
     tiles += np;
   });
   hipLaunchKernelGGL(join_tiles_kernel, dim3((n + 31) / 32), dim3(1024), 0, stream, w.part, tiles,
-                     pad, w.target_term, temperature * temperature, per_row ? loss : nullptr,
+                     pad, d.k, scale, temperature * temperature, per_row ? loss : nullptr,
                      per_row ? nullptr : w.partial, s);
   if (!per_row) {
     hipLaunchKernelGGL(sum_losses_kernel, dim3(1), dim3(kScanThreads), 0, stream, w.partial,
@@ -1005,6 +1095,7 @@ void launch_piece(const Shape& d, const Plan& plan, int piece, const uint16_t* w
   const int first = piece * plan.columns;
   const int columns = std::min(plan.columns, d.vocab - first);
   const int64_t ld = plan.columns;
+  const bool twice = d.n <= kFewest;
   const uint16_t* from = weight + static_cast<int64_t>(first) * d.c;
   const Operand wp{from, d.c, columns};
   const Operand h{s.hidden, d.c, static_cast<int32_t>(pad)};
@@ -1016,19 +1107,19 @@ void launch_piece(const Shape& d, const Plan& plan, int piece, const uint16_t* w
       using G = std::remove_pointer_t<decltype(tile)>;
       hipLaunchKernelGGL((softmax_grad_kernel<G, T>), dim3(grid_of(tiles_of(size, part, d.n))),
                          dim3(gemm::kThreads), 0, stream, a, h, s.count, d.c,
-                         (part + G::kBP - 1) / G::kBP, scale, s.lse2, w.coef, w.dz + at, ld);
+                         (part + G::kBP - 1) / G::kBP, scale, s.lse2, w.coef, twice, w.dz + at, ld);
     });
   });
   const int64_t entries = d.n * d.k;
   hipLaunchKernelGGL((target_grad_kernel<T>), dim3(static_cast<unsigned>((entries + 255) / 256)),
-                     dim3(256), 0, stream, d.k, first, columns, scale, w.coef, w.dz, ld, s);
+                     dim3(256), 0, stream, d.k, first, columns, scale, w.coef, twice, w.dz, ld, s);
   if (dh != nullptr) {
     const int steps = static_cast<int>(round_up(columns, gemm::kStep) / gemm::kStep);
     with_tile<T, Major::kX, Major::kK>(plan.hidden, [&](auto* tile) {
       using G = std::remove_pointer_t<decltype(tile)>;
       hipLaunchKernelGGL((hidden_grad_kernel<G, T>), dim3(kCus), dim3(gemm::kThreads), 0, stream,
                          wp, dz, s.count, w.splits, steps, plan.columns / gemm::kStep,
-                         (d.c + G::kBP - 1) / G::kBP, piece, d.c, w.slabs);
+                         (d.c + G::kBP - 1) / G::kBP, piece, d.c, twice, w.slabs);
     });
   }
   if (dw != nullptr) {

@@ -9,8 +9,8 @@ bias`` with the biased variance over the channels, all inside in fp32.
   no gradient, runs under HIP graph capture (decode).
 * :func:`pretrain_layer_norm`: any leading shape, with autograd.
 
-float32, float16 and bfloat16; any ``C`` up to 16384. ``C`` a multiple of 8 (and
-16-byte aligned tensors) takes 16-byte loads. The weight's and bias'
+float32, float16 and bfloat16; any ``C`` up to 16384. ``C`` a multiple of 8 with
+16-byte aligned tensors is the fastest; any other works. The weight's and bias'
 gradients are summed over rows in a fixed order. The kernels are in
 ``csrc/layer_norm.hip``; the reference's normalization operators are not part
 of this package, and these do not take their names.

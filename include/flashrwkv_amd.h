@@ -627,8 +627,8 @@ int frwkv_recurrent_tmix_fused_forward(
  * the io dtype and written to stream_out (both NULL: s = x),
  * y = (s - mean) / sqrt(var + eps) weight + bias, biased variance over the
  * channels, fp32 inside. mean, rstd [rows] fp32 are what the backward reads
- * (both NULL: not written). Rows of 16-byte aligned buffers with channels a
- * multiple of 8 take 16-byte loads, others elementwise ones. No counterpart in
+ * (both NULL: not written). Buffers need no alignment beyond their type's; 16-byte
+ * aligned ones with channels a multiple of 8 are the fastest. No counterpart in
  * the reference.
  */
 int frwkv_layer_norm_forward(int io_dtype, int64_t rows, int64_t channels, const void* x,

@@ -123,7 +123,7 @@ def test_forward_and_gradients(rows, c, dtype, residual):
 @pytest.mark.parametrize("dtype", ROUND)
 def test_tensors_off_16_byte_boundaries(dtype):
     """Contiguous views that start one element into their storage take the
-    elementwise path and give the aligned call's result."""
+    path of unaligned rows and give the aligned call's result."""
     case = _inputs(37, 192, dtype, seed=3)
     case["s"] = case["x"]
 

@@ -72,8 +72,9 @@ def _bounds(h, w, ref, temperature):
     return loss, delta
 
 
-def _check(h, w, entry, got, *, temperature=1.0, row_weight, reduction):
-    """got: loss, dhidden, dweight (the gradients may be None)."""
+def _check(h, w, entry, got, *, temperature=1.0, row_weight, reduction, terms_of_dz=1):
+    """got: loss, dhidden, dweight (the gradients may be None). terms_of_dz: the 16-bit
+    terms that a logit gradient is kept in; each leaves u of what the one before left."""
     dtype = h.dtype
     u, step = ROUND[dtype], STEP[dtype]
     ref = head.head_loss(h, w, *entry, temperature=temperature, row_weight=row_weight,
@@ -108,7 +109,7 @@ def _check(h, w, entry, got, *, temperature=1.0, row_weight, reduction):
         if value is None:
             continue
         gamma = (math.sqrt(terms) + 16) * E
-        allowed = ((u + delta + gamma) * ref[f"abs_{name}"] + delta * extra
+        allowed = ((u ** terms_of_dz + delta + gamma) * ref[f"abs_{name}"] + delta * extra
                    + u * ref[name].abs() * (1 + u) + step
                    + grid * terms * float(factor.double().abs().max()))
         off = (value.double().view(ref[name].shape) - ref[name]).abs()
@@ -311,6 +312,52 @@ def test_upstream_scales(scale):
                  w, upstream)
     _check(h, w, head.labels(targets, 200, -100), got, row_weight=upstream, reduction="none")
     assert not got[1][::7].any()
+
+
+@pytest.mark.parametrize("dtype", ROUND)
+@pytest.mark.parametrize("n,c,v,masked", [
+    (520, 768, 25000, 0.0), (520, 768, 25000, 0.3), (300, 64, 20000, 0.5), (60, 128, 20000, 0.5),
+    (700, 64, 20000, 0.97)])
+def test_wide_vocabularies(n, c, v, masked, dtype):
+    """More tiles than CUs, the last ones smaller; dz W split over the vocabulary,
+    into more parts the fewer rows take part."""
+    h, w = _head(n, c, v, dtype, seed=n + c)
+    targets = torch.randint(v, (n,), generator=_gen(n))
+    targets[torch.rand(n, generator=_gen(n + 1)) < masked] = -100
+    targets[-1] = v - 1
+    targets = targets.to(DEV)
+    upstream = _upstream("none", n, seed=n + 2)
+    got = _grads(lambda a, b: pretrain_linear_cross_entropy(a, b, targets, reduction="none"), h,
+                 w, upstream)
+    _check(h, w, head.labels(targets, v, -100), got, row_weight=upstream, reduction="none")
+    again = _grads(lambda a, b: pretrain_linear_cross_entropy(a, b, targets, reduction="none"), h,
+                   w, upstream)
+    assert all(torch.equal(a, b) for a, b in zip(got, again))
+
+
+@pytest.mark.parametrize("dtype", ROUND)
+@pytest.mark.parametrize("n,c,v,k", [(1, 512, 300, 1), (3, 64, 1000, 1), (31, 320, 257, 1),
+                                     (32, 1024, 700, 1), (20, 128, 400, 9)])
+def test_few_rows_lose_nothing_to_their_logit_gradients(n, c, v, k, dtype):
+    """Up to 32 rows keep them in two terms, with per-row weights as well."""
+    h, w = _head(n, c, v, dtype, seed=31 + n)
+    upstream = _upstream("none", n, seed=n + 2)
+    if k == 1:
+        targets = torch.randint(v, (n,), generator=_gen(n)).to(DEV)
+        targets[n // 2] = -100 if n > 1 else 7
+        entry = head.labels(targets, v, -100)
+
+        def call(a, b):
+            return pretrain_linear_cross_entropy(a, b, targets, reduction="none")
+    else:
+        logits, tokens = _teacher(n, k, v, seed=32)
+        entry = head.teacher(logits, tokens, 1.0)
+
+        def call(a, b):
+            return pretrain_linear_topk_distillation(a, b, logits, tokens, reduction="none")
+
+    _check(h, w, entry, _grads(call, h, w, upstream), row_weight=upstream, reduction="none",
+           terms_of_dz=2)
 
 
 def test_several_pieces_of_the_vocabulary():
