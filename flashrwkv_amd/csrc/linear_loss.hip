@@ -99,6 +99,7 @@ __device__ __forceinline__ float2 joined(float2 a, float2 b) {
 // take part, in order; i is the row's place in the caller's tensors.
 struct Saved {
   int32_t* count;   // [1]     rows that take part
+  int32_t* cut;     // [1]     columns of the forward that large tiles take
   int32_t* row;     // [pad]   m -> i
   int32_t* place;   // [N]     i -> m, or -1
   int32_t* index;   // [N][K]  target tokens (by i); -1 absent, V or more out of range
@@ -123,11 +124,13 @@ Saved saved_of(char* p, int64_t n, int64_t c, int64_t k, size_t* bytes) {
   const int64_t pad = round_up(n, kRowPad);
   Layout l;
   Saved s;
-  const size_t count = l.take(4), row = l.take(pad * 4), place = l.take(n * 4);
+  const size_t count = l.take(4), cut = l.take(4);
+  const size_t row = l.take(pad * 4), place = l.take(n * 4);
   const size_t index = l.take(n * k * 4), share = l.take(n * k * 4);
   const size_t target = l.take(n * k * 4), base = l.take(n * 4), lse2 = l.take(pad * 4);
   const size_t logit = l.take(pad * k * 4), hidden = l.take(pad * c * 2);
   s.count = reinterpret_cast<int32_t*>(p + count);
+  s.cut = reinterpret_cast<int32_t*>(p + cut);
   s.row = reinterpret_cast<int32_t*>(p + row);
   s.place = reinterpret_cast<int32_t*>(p + place);
   s.index = reinterpret_cast<int32_t*>(p + index);
@@ -139,6 +142,96 @@ Saved saved_of(char* p, int64_t n, int64_t c, int64_t k, size_t* bytes) {
   s.hidden = reinterpret_cast<uint16_t*>(p + hidden);
   *bytes = l.bytes;
   return s;
+}
+
+// -------------------------------------------------- tile sizes and their times
+enum class Size { kFewRows, kSmall, kLarge };
+
+struct TileTime {
+  int32_t p, q;
+  float step_us, fixed_us;  // of 64 k, and of a tile's start and end beside them
+};
+
+// Measured on products that fill the GPU for many rounds.
+__host__ __device__ constexpr TileTime time_of(Size s) {
+  return s == Size::kFewRows ? TileTime{256, 64, 1.0f, 3.0f}
+         : s == Size::kSmall ? TileTime{128, 128, 0.6f, 3.0f}
+                             : TileTime{256, 256, 1.65f, 5.0f};
+}
+
+// Fewer than 2^30 tiles, checked at the entry points.
+__host__ __device__ inline int32_t tiles_of(Size s, int32_t p, int32_t q) {
+  const TileTime t = time_of(s);
+  return (p + t.p - 1) / t.p * ((q + t.q - 1) / t.q);
+}
+
+__host__ __device__ inline float product_us(Size s, int32_t p, int32_t q, int32_t steps) {
+  const int32_t rounds = (tiles_of(s, p, q) + kCus - 1) / kCus;
+  return static_cast<float>(rounds) *
+         (static_cast<float>(steps) * time_of(s).step_us + time_of(s).fixed_us);
+}
+
+// How a product over a range of the vocabulary is tiled: `first` columns with
+// large tiles, the rest with small ones. Large tiles leave a last round with few
+// of them; small ones, less efficient by half but four times as many, take its
+// place where that is faster (forward of 1000 x 50277 x 2560, 3.1 rounds: 248 ->
+// 233 us).
+struct Cut {
+  int32_t first;
+  float us;
+};
+
+// Tile sizes that may be used.
+struct Sizes {
+  bool small, large;
+};
+
+// vocab: columns of the range; across: the other extent (rows or channels).
+__host__ __device__ inline Cut cut_of(int32_t vocab, int32_t across, int32_t steps, Sizes sizes) {
+  if (!sizes.large || (sizes.small && across <= time_of(Size::kSmall).q)) {
+    return {0, product_us(Size::kSmall, vocab, across, steps)};
+  }
+  const float large = product_us(Size::kLarge, vocab, across, steps);
+  if (!sizes.small) return {vocab, large};
+  const float small = product_us(Size::kSmall, vocab, across, steps);
+  Cut best = small < large ? Cut{0, small} : Cut{vocab, large};
+  const int32_t full = tiles_of(Size::kLarge, vocab, across) / kCus * kCus;
+  const int32_t first = full / ((across + 255) / 256) * 256;
+  if (first > 0 && first < vocab) {
+    const float both = product_us(Size::kLarge, first, across, steps) +
+                       product_us(Size::kSmall, vocab - first, across, steps) + 3.0f;
+    if (both < best.us) best = {first, both};
+  }
+  return best;
+}
+
+constexpr Sizes kBothSizes = {true, true};
+
+// For products over the rows that take part the device decides, where their
+// count is (777 rows, of which 520 take part, 20011 x 768: forward and backward
+// 138 -> 127 us). A launch that finds no columns of its own ends at once, which takes 1 to
+// 2 us; sizes that no count from half of the rows on asks for are not launched.
+inline Sizes sizes_of(int32_t vocab, int32_t rows, int32_t steps) {
+  Sizes sizes = {false, false};
+  for (int eighths = 4; eighths <= 8; ++eighths) {
+    const Cut cut = cut_of(vocab, (rows * eighths + 7) / 8, steps, kBothSizes);
+    sizes.large |= cut.first > 0;
+    sizes.small |= cut.first < vocab;
+  }
+  return sizes;
+}
+
+// The columns that a kernel of tiles G takes of `columns`, cut at *cut.
+template <typename G>
+__device__ __forceinline__ void own_columns(const int32_t* cut, int32_t& from, int32_t& columns) {
+  from = 0;
+  if (G::kBQ == 64) return;  // few rows: all of them
+  if (G::kBQ == 256) {
+    columns = *cut;
+  } else {
+    from = *cut;
+    columns -= from;
+  }
 }
 
 // ---------------------------------------------------------------- targets
@@ -218,10 +311,11 @@ __global__ __launch_bounds__(256) void teacher_targets_kernel(
 }
 
 // Numbers the rows that take part, in order: part(i) says whether row i does.
-// One workgroup; row_loss (not null): 0 for the rows that do not.
+// One workgroup; row_loss (not null): 0 for the rows that do not. steps: of the
+// product, sizes: launched for it.
 template <typename Part>
-__device__ __forceinline__ void number_rows(int32_t n, float* row_loss, const Saved& s,
-                                            Part&& part_of) {
+__device__ __forceinline__ void number_rows(int32_t n, int32_t vocab, int32_t steps, Sizes sizes,
+                                            float* row_loss, const Saved& s, Part&& part_of) {
   __shared__ int32_t waves[kScanThreads / 64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int32_t before = 0;
@@ -244,15 +338,18 @@ __device__ __forceinline__ void number_rows(int32_t n, float* row_loss, const Sa
     before += all;
     __syncthreads();
   }
-  if (threadIdx.x == 0) *s.count = before;
+  if (threadIdx.x == 0) {
+    *s.count = before;
+    *s.cut = cut_of(vocab, before, steps, sizes).first;
+  }
 }
 
 // Cross entropy: one entry a row, share 1.
 template <typename Index>
 __global__ __launch_bounds__(kScanThreads) void label_rows_kernel(
-    const Index* __restrict__ targets, int64_t ignore, int32_t n, int32_t vocab, float* row_loss,
-    Saved s) {
-  number_rows(n, row_loss, s, [&](int32_t i) {
+    const Index* __restrict__ targets, int64_t ignore, int32_t n, int32_t vocab, int32_t steps,
+    Sizes sizes, float* row_loss, Saved s) {
+  number_rows(n, vocab, steps, sizes, row_loss, s, [&](int32_t i) {
     const int64_t t = targets[i];
     const bool part = t != ignore;
     const int32_t token = as_token(t, vocab);
@@ -265,9 +362,10 @@ __global__ __launch_bounds__(kScanThreads) void label_rows_kernel(
 }
 
 // Distillation, behind teacher_targets_kernel, which leaves 1 or 0 in place[i].
-__global__ __launch_bounds__(kScanThreads) void teacher_rows_kernel(int32_t n, float* row_loss,
-                                                                    Saved s) {
-  number_rows(n, row_loss, s, [&](int32_t i) { return s.place[i] != 0; });
+__global__ __launch_bounds__(kScanThreads) void teacher_rows_kernel(int32_t n, int32_t vocab,
+                                                                    int32_t steps, Sizes sizes,
+                                                                    float* row_loss, Saved s) {
+  number_rows(n, vocab, steps, sizes, row_loss, s, [&](int32_t i) { return s.place[i] != 0; });
 }
 
 // A workgroup a row m: copies its hidden row (zeros for the rows that fill up
@@ -337,7 +435,15 @@ using FewRowsTile = gemm::Tile<T, MA, MB, 256, 64, 8, 1, 3, MA == Major::kK && M
 // The tiles of a product over rows m, whose count stands on the device: the
 // workgroups of a launch of at most one a CU take them in turn. While a
 // workgroup finishes a tile, the first stages of its next one are on their way.
-__device__ __forceinline__ int row_tiles_of(int rows, int tile) { return (rows + tile - 1) / tile; }
+__host__ __device__ __forceinline__ int tiles_along(int size, int tile) { return (size + tile - 1) / tile; }
+
+// Where this lane's accumulators hold a token: 16 i + r, or -1. p0: the tile's
+// first token, left: tokens from there on.
+template <typename G>
+__device__ __forceinline__ int own_row(int token, int p0, int left) {
+  const int at = token - p0, row = at - G::row(0);
+  return token >= 0 && at < left && row >= 0 && row < 16 * G::TP && (row & 15) < 4 ? row : -1;
+}
 
 // D[v][m] of a vocabulary range: per tile of v and row m the maximum of
 // s z log2 e and the sum of 2^(s z log2 e - maximum), to part[tile][m]. one: rows
@@ -345,12 +451,17 @@ __device__ __forceinline__ int row_tiles_of(int rows, int tile) { return (rows +
 // it cancels against a maximum that it is.
 template <typename G, typename T>
 __global__ __launch_bounds__(gemm::kThreads, 2) void lse_tiles_kernel(
-    Operand w, Operand h, int32_t c, int32_t np, float scale, int32_t vocab0, bool one,
-    float2* __restrict__ part, int64_t pad, Saved s) {
+    Operand w, Operand h, int32_t c, float scale, bool one, float2* __restrict__ part,
+    int64_t pad, Saved s) {
   __shared__ __attribute__((aligned(1024))) char smem[G::kLdsBytes];
   __shared__ float maxima[G::kWP][G::kBQ], sums[G::kWP][G::kBQ];
+  int vocab0;
+  own_columns<G>(s.cut, vocab0, w.rows);
+  w.data += static_cast<int64_t>(vocab0) * w.ld;
+  part += vocab0 / 256 * pad;  // behind the large tiles'
   const int rows = *s.count;
-  const int nq = row_tiles_of(rows, G::kBQ), total = np * nq, steps = c / gemm::kStep;
+  const int np = tiles_along(w.rows, G::kBP);
+  const int nq = tiles_along(rows, G::kBQ), total = np * nq, steps = c / gemm::kStep;
   int id = blockIdx.x;
   if (id >= total) return;
   G tile;
@@ -422,18 +533,15 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void lse_tiles_kernel(
     G::arrive();
 #pragma unroll
     for (int j = 0; j < G::TQ; ++j) {
-      // Rows 16 i + r from here on are this lane's.
-      const int at = token[j] - vocab0 - p0, row = at - G::row(0);
-      const bool here =
-          token[j] >= 0 && at < left && row >= 0 && row < 16 * G::TP && (row & 15) < 4;
-      if (__ballot(here) == 0) continue;
+      const int own = own_row<G>(token[j], vocab0 + p0, left);
+      if (__ballot(own >= 0) == 0) continue;
       float z = 0.0f;
 #pragma unroll
       for (int i = 0; i < G::TP; ++i) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) z = row == 16 * i + r ? tile.acc[i][j][r] : z;
+        for (int r = 0; r < 4; ++r) z = own == 16 * i + r ? tile.acc[i][j][r] : z;
       }
-      if (here) s.logit[q0 + G::column(j)] = z;
+      if (own >= 0) s.logit[q0 + G::column(j)] = z;
     }
     __syncthreads();
     for (int q = threadIdx.x; q < G::kBQ; q += gemm::kThreads) {
@@ -465,12 +573,16 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void lse_tiles_kernel(
 // rounding).
 template <typename G, typename T>
 __global__ __launch_bounds__(gemm::kThreads, 2) void softmax_grad_kernel(
-    Operand w, Operand h, const int32_t* __restrict__ count, int32_t c, int32_t np, float scale,
-    const float* __restrict__ lse2, const float* __restrict__ coef, bool twice,
-    uint16_t* __restrict__ dz, int64_t ld) {
+    Operand w, Operand h, const int32_t* __restrict__ cut, int32_t c, float scale,
+    const float* __restrict__ coef, bool twice, uint16_t* __restrict__ dz, int64_t ld, Saved s) {
   __shared__ __attribute__((aligned(1024))) char smem[G::kLdsBytes];
-  const int rows = *count;
-  const int nq = row_tiles_of(rows, G::kBQ), total = np * nq, steps = c / gemm::kStep;
+  int at;
+  own_columns<G>(cut, at, w.rows);
+  w.data += static_cast<int64_t>(at) * w.ld;
+  dz += at;
+  const int rows = *s.count;
+  const int np = tiles_along(w.rows, G::kBP);
+  const int nq = tiles_along(rows, G::kBQ), total = np * nq, steps = c / gemm::kStep;
   int id = blockIdx.x;
   if (id >= total) return;
   G tile;
@@ -484,7 +596,7 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void softmax_grad_kernel(
 #pragma unroll
     for (int j = 0; j < G::TQ; ++j) {
       const int m = q0 + G::column(j);
-      from[j] = m < rows ? lse2[m] : 0.0f;
+      from[j] = m < rows ? s.lse2[m] : 0.0f;
       co[j] = m < rows ? coef[m] : 0.0f;
     }
     tile.multiply(smem);
@@ -536,7 +648,8 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void softmax_grad_kernel(
 }
 
 // The entries of dz that have a target: coef (p - b) in fp32 from the fp32
-// logit, over what the product's epilogue wrote. A thread an entry; equal
+// logit, over what the product's epilogue wrote (which as a part of that epilogue
+// costs more, 2 to 4% of a backward, than this launch's 5 us). A thread an entry; equal
 // tokens of a row write the same value.
 template <typename T>
 __global__ __launch_bounds__(256) void target_grad_kernel(int32_t k, int32_t vocab0,
@@ -607,6 +720,14 @@ __device__ __forceinline__ int32_t wave_splits_of(const Splitting& x, int64_t ro
   return __shfl(best, 0, 64);
 }
 
+// The columns of a piece of the backward, and the tile sizes launched over them:
+// [0] of the pieces before the last, [1] of the last one.
+struct Pieces {
+  int32_t columns[2];
+  Sizes sizes[2];
+  int32_t steps;
+};
+
 // D[c][m] = sum over a split's vocabulary of W[v][c] dz[m][v], to slab [m][c]
 // of the split (fp32).
 template <typename G, typename T>
@@ -618,7 +739,7 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void hidden_grad_kernel(
   const int rows = *count;
   const int splits = *split_count;
   const int split_steps = (whole_steps + splits - 1) / splits;
-  const int nq = row_tiles_of(rows, G::kBQ), each = np * nq, total = each * splits;
+  const int nq = tiles_along(rows, G::kBQ), each = np * nq, total = each * splits;
   const int64_t slab = static_cast<int64_t>(rows) * c;
   int id = blockIdx.x;
   if (id >= total) return;
@@ -700,11 +821,11 @@ __global__ __launch_bounds__(256) void hidden_grad_rows_kernel(
 // D[c][v] = sum_m h[m][c] dz[m][v]: dW of a piece of the vocabulary.
 template <typename G, typename T>
 __global__ __launch_bounds__(gemm::kThreads, 2) void weight_grad_kernel(
-    Operand h, Operand dz, const int32_t* __restrict__ count, int32_t columns, int32_t np,
-    int32_t nq, int32_t c, const float* __restrict__ scale, uint16_t* __restrict__ dw) {
+    Operand h, Operand dz, const int32_t* __restrict__ count, int32_t columns, int32_t c,
+    const float* __restrict__ scale, uint16_t* __restrict__ dw) {
   __shared__ __attribute__((aligned(1024))) char smem[G::kLdsBytes];
   const int steps = static_cast<int>(round_up(*count, gemm::kStep) / gemm::kStep);
-  const int total = np * nq;
+  const int np = tiles_along(c, G::kBP), nq = tiles_along(columns, G::kBQ), total = np * nq;
   int id = blockIdx.x;
   G tile;
   int tp, tq;
@@ -744,15 +865,17 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void weight_grad_kernel(
 // that is exact where they are close, and not from lse, whose rounding alone
 // (half a unit of 16 in base 2) is 1e-6 of a loss near 1.
 __global__ __launch_bounds__(1024) void join_tiles_kernel(const float2* __restrict__ part,
-                                                          int32_t tiles, int64_t pad, int32_t k,
-                                                          float scale, float temperature2,
-                                                          float* row_loss, float* partial,
-                                                          Saved s) {
+                                                          int32_t vocab, int32_t rest_tile,
+                                                          int64_t pad, int32_t k, float scale,
+                                                          float temperature2, float* row_loss,
+                                                          float* partial, Saved s) {
   __shared__ float2 shared[32][33];
   const int q = threadIdx.x & 31, slice = threadIdx.x >> 5;
   const int m = blockIdx.x * 32 + q;
   const int count = *s.count;
   if (static_cast<int>(blockIdx.x) * 32 >= count) return;
+  const int cut = *s.cut;
+  const int tiles = tiles_along(cut, 256) + tiles_along(vocab - cut, rest_tile);
   float2 all = make_float2(-__builtin_inff(), 0.0f);
   if (m < count) {
     for (int t = slice; t < tiles; t += 256) {
@@ -831,13 +954,16 @@ __global__ __launch_bounds__(kScanThreads) void sum_losses_kernel(
 // is at most 2^14, and 2^-28 of that is the smallest one.
 __global__ __launch_bounds__(kScanThreads) void row_coefficients_kernel(
     const float* __restrict__ upstream, bool per_row, bool mean, float temperature, int up,
-    Splitting splitting, float* __restrict__ coef, float* __restrict__ scale,
-    int32_t* __restrict__ splits, Saved s) {
+    Splitting splitting, Pieces pieces, float* __restrict__ coef, float* __restrict__ scale,
+    int32_t* __restrict__ splits, int32_t* __restrict__ cuts, Saved s) {
   __shared__ float waves[kScanThreads / 64];
   const int n = *s.count;
   if (threadIdx.x < 64) {
     const int32_t most = wave_splits_of(splitting, n);
     if (threadIdx.x == 0) *splits = most;
+  } else if (threadIdx.x < 66) {
+    const int which = threadIdx.x - 64;
+    cuts[which] = cut_of(pieces.columns[which], n, pieces.steps, pieces.sizes[which]).first;
   }
   const float by = mean ? temperature / static_cast<float>(n > 0 ? n : 1) : temperature;
   const float lift = ldexpf(1.0f, up);
@@ -865,61 +991,6 @@ __global__ __launch_bounds__(kScanThreads) void row_coefficients_kernel(
 }
 
 // ---------------------------------------------------------------- launches
-enum class Size { kFewRows, kSmall, kLarge };
-
-struct TileTime {
-  int32_t p, q;
-  double step_us, fixed_us;  // of 64 k, and of a tile's start and end beside them
-};
-
-// Measured on products that fill the GPU for many rounds.
-constexpr TileTime kTileTimes[] = {
-    {256, 64, 1.0, 3.0}, {128, 128, 0.6, 3.0}, {256, 256, 1.65, 5.0}};
-
-const TileTime& time_of(Size s) { return kTileTimes[static_cast<int>(s)]; }
-
-int64_t tiles_of(Size s, int64_t p, int64_t q) {
-  const TileTime& t = time_of(s);
-  return (p + t.p - 1) / t.p * ((q + t.q - 1) / t.q);
-}
-
-double product_us(Size s, int64_t p, int64_t q, int64_t steps) {
-  const int64_t rounds = (tiles_of(s, p, q) + kCus - 1) / kCus;
-  return rounds * (steps * time_of(s).step_us + time_of(s).fixed_us);
-}
-
-// How a product over a range of the vocabulary is tiled: `first` columns with
-// one size, the rest with another (or with none). Tiles of 256 leave a last
-// round with few of them; 128 x 128 tiles, less efficient by half but four times
-// as many, take its place where that is faster (forward of 1000 x 50277 x 2560,
-// 3.1 rounds: 248 -> 233 us).
-struct Cut {
-  int64_t first;
-  Size size, rest;
-  double us;
-};
-
-// vocab: columns of the range; across: the other extent (rows or channels);
-// rows: whether that is the rows, of which few have a tile of their own.
-Cut cut_of(int64_t vocab, int64_t across, int64_t steps, bool rows) {
-  if (rows && across <= time_of(Size::kFewRows).q) {
-    return {vocab, Size::kFewRows, Size::kFewRows,
-            product_us(Size::kFewRows, vocab, across, steps)};
-  }
-  const double large = product_us(Size::kLarge, vocab, across, steps);
-  const double small = product_us(Size::kSmall, vocab, across, steps);
-  Cut best = small < large ? Cut{vocab, Size::kSmall, Size::kSmall, small}
-                           : Cut{vocab, Size::kLarge, Size::kLarge, large};
-  const int64_t full = tiles_of(Size::kLarge, vocab, across) / kCus * kCus;
-  const int64_t first = full / ((across + 255) / 256) * 256;
-  if (first > 0 && first < vocab) {
-    const double both = product_us(Size::kLarge, first, across, steps) +
-                        product_us(Size::kSmall, vocab - first, across, steps) + 3.0;
-    if (both < best.us) best = {first, Size::kLarge, Size::kSmall, both};
-  }
-  return best;
-}
-
 // How the backward goes through the vocabulary.
 struct Plan {
   int32_t columns;  // of a piece, a multiple of kVocabTile
@@ -938,11 +1009,12 @@ constexpr double kGradBytesPerUs = 20.0e6;
 constexpr double kSlabBytesPerUs = 4.0e6;
 
 Splitting splitting_of(Size size, int64_t columns, int64_t c, int64_t room) {
-  const TileTime& t = time_of(size);
+  const TileTime t = time_of(size);
   return {static_cast<int32_t>(columns / gemm::kStep), static_cast<int32_t>((c + t.p - 1) / t.p),
-          t.q, static_cast<float>(t.step_us), static_cast<float>(t.fixed_us),
-          static_cast<float>(4.0 * c / kSlabBytesPerUs), room};
+          t.q, t.step_us, t.fixed_us, static_cast<float>(4.0 * c / kSlabBytesPerUs), room};
 }
+
+bool few(int64_t n) { return n <= time_of(Size::kFewRows).q; }
 
 Plan plan_of(int64_t n, int64_t c, int64_t vocab) {
   const int64_t all = round_up(vocab, kVocabTile), pad = round_up(n, kRowPad);
@@ -958,12 +1030,14 @@ Plan plan_of(int64_t n, int64_t c, int64_t vocab) {
     last = p.columns;
     const int64_t bytes = pad * p.columns * 2;
     if (bytes > kMostBytes && p.columns > kVocabTile) continue;
-    double us = 12.0 + cut_of(p.columns, n, steps_c, true).us +
-                cut_of(p.columns, c, steps_n, false).us +
+    double us = 12.0 +
+                (few(n) ? product_us(Size::kFewRows, p.columns, n, steps_c)
+                        : cut_of(p.columns, n, steps_c, kBothSizes).us) +
+                cut_of(p.columns, c, steps_n, kBothSizes).us +
                 (bytes > kCachedBytes ? 3 * bytes / kGradBytesPerUs : 0.0);
     double hidden = 1e300;
     for (Size size : {Size::kFewRows, Size::kSmall, Size::kLarge}) {
-      if ((size == Size::kFewRows) != (n <= time_of(Size::kFewRows).q)) continue;
+      if ((size == Size::kFewRows) != few(n)) continue;
       const Splitting x = splitting_of(size, p.columns, c, kMostSplits * n);
       const int32_t splits = splits_of(x, n);
       const double t = split_us(x, n, splits);
@@ -1006,6 +1080,7 @@ struct BackwardWork {
   float* coef;
   float* scale;
   int32_t* splits;
+  int32_t* cuts;
   uint16_t* dz;
   float* slabs;
 };
@@ -1015,19 +1090,21 @@ BackwardWork backward_work(char* p, int64_t n, int64_t c, const Plan& plan, bool
   const int64_t pad = round_up(n, kRowPad);
   Layout l;
   const size_t coef = l.take(pad * 4), scale = l.take(4), splits = l.take(4);
+  const size_t cuts = l.take(8);
   const size_t dz = l.take(pad * plan.columns * 2);
   const size_t slabs =
       l.take(hidden ? static_cast<size_t>(plan.pieces) * slab_rows(plan, n) * c * 4 : 0);
   *bytes = l.bytes;
   return {reinterpret_cast<float*>(p + coef), reinterpret_cast<float*>(p + scale),
-          reinterpret_cast<int32_t*>(p + splits), reinterpret_cast<uint16_t*>(p + dz),
-          reinterpret_cast<float*>(p + slabs)};
+          reinterpret_cast<int32_t*>(p + splits), reinterpret_cast<int32_t*>(p + cuts),
+          reinterpret_cast<uint16_t*>(p + dz), reinterpret_cast<float*>(p + slabs)};
 }
 
 struct Shape {
-  int64_t n;
-  int32_t c, vocab, k;
+  int32_t n, c, vocab, k;
 };
+
+int grid_of(int32_t tiles) { return std::min(tiles, kCus); }
 
 // f(tile type) for a size.
 template <typename T, Major MA, Major MB, typename F>
@@ -1043,15 +1120,19 @@ void with_tile(Size size, F&& f) {
   }
 }
 
-// f(first column, columns, size) for the parts of a cut.
-template <typename F>
-void for_cut(const Cut& cut, int32_t columns, F&& f) {
-  const int32_t first = static_cast<int32_t>(std::min<int64_t>(cut.first, columns));
-  f(int64_t{0}, first, cut.size);
-  if (first < columns) f(int64_t{first}, columns - first, cut.rest);
+// f(tile type, grid) for the sizes that a product over `vocab` columns and
+// `rows` rows may be cut into on the device. Few rows have a tile of their own.
+template <typename T, typename F>
+void for_sizes(int32_t vocab, int32_t rows, int32_t steps, F&& f) {
+  const auto launch = [&](Size size) {
+    const int grid = grid_of(tiles_of(size, vocab, rows));
+    with_tile<T, Major::kK, Major::kK>(size, [&](auto* tile) { f(tile, grid); });
+  };
+  if (few(rows)) return launch(Size::kFewRows);
+  const Sizes sizes = sizes_of(vocab, rows, steps);
+  if (sizes.large) launch(Size::kLarge);
+  if (sizes.small) launch(Size::kSmall);
 }
-
-int grid_of(int64_t tiles) { return static_cast<int>(std::min<int64_t>(tiles, kCus)); }
 
 template <typename T>
 int run_forward(const Shape& d, const void* hidden, const void* weight, float temperature,
@@ -1059,26 +1140,20 @@ int run_forward(const Shape& d, const void* hidden, const void* weight, float te
                 hipStream_t stream) {
   const int64_t pad = round_up(d.n, kRowPad);
   const float scale = kLog2E / temperature;
-  const int n = static_cast<int>(d.n);
+  const int n = d.n;
   hipLaunchKernelGGL((gather_rows_kernel<T>), dim3(static_cast<unsigned>(pad)), dim3(256), 0,
                      stream, static_cast<const uint16_t*>(hidden),
                      static_cast<const uint16_t*>(weight), d.c, d.k, d.vocab, d.n <= kFewest, s);
-  int tiles = 0;
+  const Operand a{static_cast<const uint16_t*>(weight), d.c, d.vocab};
   const Operand b{s.hidden, d.c, static_cast<int32_t>(pad)};
-  for_cut(cut_of(d.vocab, d.n, d.c / gemm::kStep, true), d.vocab,
-          [&](int64_t first, int32_t columns, Size size) {
-    const Operand a{static_cast<const uint16_t*>(weight) + first * d.c, d.c, columns};
-    const int np = (columns + time_of(size).p - 1) / time_of(size).p;
-    with_tile<T, Major::kK, Major::kK>(size, [&](auto* tile) {
-      using G = std::remove_pointer_t<decltype(tile)>;
-      hipLaunchKernelGGL((lse_tiles_kernel<G, T>), dim3(grid_of(tiles_of(size, columns, d.n))),
-                         dim3(gemm::kThreads), 0, stream, a, b, d.c, np, scale,
-                         static_cast<int32_t>(first), d.k == 1, w.part + tiles * pad, pad, s);
-    });
-    tiles += np;
+  for_sizes<T>(d.vocab, d.n, d.c / gemm::kStep, [&](auto* tile, int grid) {
+    using G = std::remove_pointer_t<decltype(tile)>;
+    hipLaunchKernelGGL((lse_tiles_kernel<G, T>), dim3(grid), dim3(gemm::kThreads), 0, stream, a, b,
+                       d.c, scale, d.k == 1, w.part, pad, s);
   });
-  hipLaunchKernelGGL(join_tiles_kernel, dim3((n + 31) / 32), dim3(1024), 0, stream, w.part, tiles,
-                     pad, d.k, scale, temperature * temperature, per_row ? loss : nullptr,
+  hipLaunchKernelGGL(join_tiles_kernel, dim3((n + 31) / 32), dim3(1024), 0, stream, w.part,
+                     d.vocab, time_of(few(d.n) ? Size::kFewRows : Size::kSmall).p, pad, d.k, scale,
+                     temperature * temperature, per_row ? loss : nullptr,
                      per_row ? nullptr : w.partial, s);
   if (!per_row) {
     hipLaunchKernelGGL(sum_losses_kernel, dim3(1), dim3(kScanThreads), 0, stream, w.partial,
@@ -1100,17 +1175,13 @@ void launch_piece(const Shape& d, const Plan& plan, int piece, const uint16_t* w
   const Operand wp{from, d.c, columns};
   const Operand h{s.hidden, d.c, static_cast<int32_t>(pad)};
   const Operand dz{w.dz, ld, static_cast<int32_t>(pad)};
-  for_cut(cut_of(columns, d.n, d.c / gemm::kStep, true), columns,
-          [&](int64_t at, int32_t part, Size size) {
-    const Operand a{from + at * d.c, d.c, part};
-    with_tile<T, Major::kK, Major::kK>(size, [&](auto* tile) {
-      using G = std::remove_pointer_t<decltype(tile)>;
-      hipLaunchKernelGGL((softmax_grad_kernel<G, T>), dim3(grid_of(tiles_of(size, part, d.n))),
-                         dim3(gemm::kThreads), 0, stream, a, h, s.count, d.c,
-                         (part + G::kBP - 1) / G::kBP, scale, s.lse2, w.coef, twice, w.dz + at, ld);
-    });
+  const int32_t* cut = w.cuts + (piece + 1 == plan.pieces);
+  for_sizes<T>(columns, d.n, d.c / gemm::kStep, [&](auto* tile, int grid) {
+    using G = std::remove_pointer_t<decltype(tile)>;
+    hipLaunchKernelGGL((softmax_grad_kernel<G, T>), dim3(grid), dim3(gemm::kThreads), 0, stream,
+                       wp, h, cut, d.c, scale, w.coef, twice, w.dz, ld, s);
   });
-  const int64_t entries = d.n * d.k;
+  const int64_t entries = static_cast<int64_t>(d.n) * d.k;
   hipLaunchKernelGGL((target_grad_kernel<T>), dim3(static_cast<unsigned>((entries + 255) / 256)),
                      dim3(256), 0, stream, d.k, first, columns, scale, w.coef, twice, w.dz, ld, s);
   if (dh != nullptr) {
@@ -1123,17 +1194,20 @@ void launch_piece(const Shape& d, const Plan& plan, int piece, const uint16_t* w
     });
   }
   if (dw != nullptr) {
-    for_cut(cut_of(columns, d.c, (d.n + gemm::kStep - 1) / gemm::kStep, false), columns,
-            [&](int64_t at, int32_t part, Size size) {
+    // Masks shorten its tiles and leave their number.
+    const Cut cut = cut_of(columns, d.c, tiles_along(d.n, gemm::kStep), kBothSizes);
+    const auto launch = [&](Size size, int32_t at, int32_t part) {
+      if (part == 0) return;
       const Operand b{w.dz + at, ld, static_cast<int32_t>(pad)};
       with_tile<T, Major::kX, Major::kX>(size, [&](auto* tile) {
         using G = std::remove_pointer_t<decltype(tile)>;
         hipLaunchKernelGGL((weight_grad_kernel<G, T>), dim3(grid_of(tiles_of(size, d.c, part))),
-                           dim3(gemm::kThreads), 0, stream, h, b, s.count, part,
-                           (d.c + G::kBP - 1) / G::kBP, (part + G::kBQ - 1) / G::kBQ, d.c, w.scale,
-                           dw + (first + at) * d.c);
+                           dim3(gemm::kThreads), 0, stream, h, b, s.count,
+                           part, d.c, w.scale, dw + static_cast<int64_t>(first + at) * d.c);
       });
-    });
+    };
+    launch(Size::kLarge, 0, cut.first);
+    launch(Size::kSmall, cut.first, columns - cut.first);
   }
 }
 
@@ -1142,16 +1216,21 @@ int run_backward(const Shape& d, const void* weight, const float* upstream, bool
                  bool mean, float temperature, void* dh, void* dw, const Saved& s,
                  const Plan& plan, const BackwardWork& w, hipStream_t stream) {
   const float scale = kLog2E / temperature;
+  const int steps = d.c / gemm::kStep, last = d.vocab - (plan.pieces - 1) * plan.columns;
+  const Pieces pieces{{plan.columns, last},
+                      {sizes_of(plan.columns, d.n, steps), sizes_of(last, d.n, steps)},
+                      steps};
   hipLaunchKernelGGL(row_coefficients_kernel, dim3(1), dim3(kScanThreads), 0, stream, upstream,
                      per_row, mean, temperature, __is_same(T, F16) ? 14 : 0,
-                     splitting_of(plan.hidden, plan.columns, d.c, slab_rows(plan, d.n)), w.coef,
-                     w.scale, w.splits, s);
+                     splitting_of(plan.hidden, plan.columns, d.c, slab_rows(plan, d.n)),
+                     pieces,
+                     w.coef, w.scale, w.splits, w.cuts, s);
   for (int p = 0; p < plan.pieces; ++p) {
     launch_piece<T>(d, plan, p, static_cast<const uint16_t*>(weight), scale,
                     static_cast<uint16_t*>(dh), static_cast<uint16_t*>(dw), s, w, stream);
   }
   if (dh != nullptr) {
-    const int64_t quads = d.n * (d.c / 4);
+    const int64_t quads = static_cast<int64_t>(d.n) * (d.c / 4);
     const int64_t blocks = std::min<int64_t>((quads + 255) / 256, 8192);
     hipLaunchKernelGGL((hidden_grad_rows_kernel<T>), dim3(static_cast<unsigned>(blocks)),
                        dim3(256), 0, stream, w.slabs, s.count, w.splits, plan.pieces,
@@ -1160,25 +1239,31 @@ int run_backward(const Shape& d, const void* weight, const float* upstream, bool
   return check_launch("linear loss backward");
 }
 
+constexpr int64_t kMostRows = int64_t{1} << 23;  // a launch: less than 2^32 threads, 256 a row
+constexpr int64_t kMostChannels = 65536;
+constexpr int64_t kMostVocab = int64_t{1} << 28;
+constexpr int64_t kMostTargets = 1024;
+
+bool within(int64_t x, int64_t most) { return x > 0 && x <= most; }
+
 int check_shape(const char* what, int io_dtype, int64_t n, int64_t c, int64_t vocab, int64_t k) {
   if (io_dtype != FRWKV_DTYPE_F16 && io_dtype != FRWKV_DTYPE_BF16) {
     return set_error(FRWKV_ERR_UNSUPPORTED, "%s: io dtype must be float16 or bfloat16", what);
   }
-  // A launch holds less than 2^32 threads, 256 a row.
-  if (n <= 0 || n > (int64_t{1} << 23)) {
+  if (!within(n, kMostRows)) {
     return set_error(FRWKV_ERR_INVALID_ARGUMENT, "%s: rows must be in [1, 2^23], got %lld", what,
                      static_cast<long long>(n));
   }
-  if (c <= 0 || c % gemm::kStep != 0 || c > 65536) {
+  if (!within(c, kMostChannels) || c % gemm::kStep != 0) {
     return set_error(FRWKV_ERR_UNSUPPORTED,
                      "%s: channels must be a multiple of 64, at most 65536, got %lld", what,
                      static_cast<long long>(c));
   }
-  if (vocab <= 0 || vocab > (int64_t{1} << 28)) {
+  if (!within(vocab, kMostVocab)) {
     return set_error(FRWKV_ERR_INVALID_ARGUMENT, "%s: vocabulary must be in [1, 2^28], got %lld",
                      what, static_cast<long long>(vocab));
   }
-  if (k <= 0 || k > 1024) {
+  if (!within(k, kMostTargets)) {
     return set_error(FRWKV_ERR_UNSUPPORTED,
                      "%s: targets of a row must be in [1, 1024], got %lld", what,
                      static_cast<long long>(k));
@@ -1261,14 +1346,18 @@ int begin_forward(const char* what, int io_dtype, int64_t n, int64_t c, int64_t 
 extern "C" {
 
 size_t frwkv_linear_loss_saved_bytes(int64_t rows, int64_t channels, int64_t top) {
-  if (rows <= 0 || channels <= 0 || top <= 0) return 0;
+  using namespace frwkv;
+  if (!within(rows, kMostRows) || !within(channels, kMostChannels) || !within(top, kMostTargets)) {
+    return 0;
+  }
   size_t bytes = 0;
   (void)frwkv::saved_of(nullptr, rows, channels, top, &bytes);
   return bytes;
 }
 
 size_t frwkv_linear_loss_forward_workspace_bytes(int64_t rows, int64_t vocab) {
-  if (rows <= 0 || vocab <= 0) return 0;
+  using namespace frwkv;
+  if (!within(rows, kMostRows) || !within(vocab, kMostVocab)) return 0;
   size_t bytes = 0;
   (void)frwkv::forward_work(nullptr, rows, vocab, &bytes);
   return bytes;
@@ -1276,7 +1365,11 @@ size_t frwkv_linear_loss_forward_workspace_bytes(int64_t rows, int64_t vocab) {
 
 size_t frwkv_linear_loss_backward_workspace_bytes(int64_t rows, int64_t channels, int64_t vocab,
                                                   int want_grad_hidden) {
-  if (rows <= 0 || channels <= 0 || vocab <= 0) return 0;
+  using namespace frwkv;
+  if (!within(rows, kMostRows) || !within(channels, kMostChannels) ||
+      !within(vocab, kMostVocab)) {
+    return 0;
+  }
   size_t bytes = 0;
   (void)frwkv::backward_work(nullptr, rows, channels, frwkv::plan_of(rows, channels, vocab),
                              want_grad_hidden != 0, &bytes);
@@ -1301,15 +1394,19 @@ int frwkv_linear_cross_entropy_forward(int io_dtype, int64_t rows, int64_t chann
   }
   const hipStream_t q = static_cast<hipStream_t>(stream);
   const int32_t n = static_cast<int32_t>(rows), v = static_cast<int32_t>(vocab);
+  const int32_t steps = static_cast<int32_t>(channels / gemm::kStep);
+  const Sizes sizes = sizes_of(vocab, rows, steps);
   float* row_loss = reduction == FRWKV_REDUCE_NONE ? loss : nullptr;
   if (target_bytes == 8) {
     hipLaunchKernelGGL((label_rows_kernel<int64_t>), dim3(1), dim3(kScanThreads), 0, q,
-                       static_cast<const int64_t*>(targets), ignore_index, n, v, row_loss, s);
+                       static_cast<const int64_t*>(targets), ignore_index, n, v,
+                       steps, sizes, row_loss, s);
   } else {
     hipLaunchKernelGGL((label_rows_kernel<int32_t>), dim3(1), dim3(kScanThreads), 0, q,
-                       static_cast<const int32_t*>(targets), ignore_index, n, v, row_loss, s);
+                       static_cast<const int32_t*>(targets), ignore_index, n, v,
+                       steps, sizes, row_loss, s);
   }
-  return forward(io_dtype, Shape{rows, static_cast<int32_t>(channels), v, 1}, hidden,
+  return forward(io_dtype, Shape{n, static_cast<int32_t>(channels), v, 1}, hidden,
                  weight, 1.0f, reduction, loss, s, workspace, q);
 }
 
@@ -1359,9 +1456,11 @@ int frwkv_linear_topk_distillation_forward(
   } else {
     with_index(Bf16{});
   }
-  hipLaunchKernelGGL(teacher_rows_kernel, dim3(1), dim3(kScanThreads), 0, q, n,
+  const int32_t steps = static_cast<int32_t>(channels / gemm::kStep);
+  const Sizes sizes = sizes_of(vocab, rows, steps);
+  hipLaunchKernelGGL(teacher_rows_kernel, dim3(1), dim3(kScanThreads), 0, q, n, v, steps, sizes,
                      reduction == FRWKV_REDUCE_NONE ? loss : nullptr, s);
-  return forward(io_dtype, Shape{rows, static_cast<int32_t>(channels), v, k}, hidden,
+  return forward(io_dtype, Shape{n, static_cast<int32_t>(channels), v, k}, hidden,
                  weight, temperature, reduction, loss, s, workspace, q);
 }
 
@@ -1396,8 +1495,8 @@ int frwkv_linear_loss_backward(int io_dtype, int64_t rows, int64_t channels, int
   if (rc != FRWKV_OK) return rc;
   if (!grad_hidden && !grad_weight) return FRWKV_OK;
   const bool mean = reduction == FRWKV_REDUCE_MEAN, per_row = reduction == FRWKV_REDUCE_NONE;
-  const Shape d{rows, static_cast<int32_t>(channels), static_cast<int32_t>(vocab),
-                static_cast<int32_t>(top)};
+  const Shape d{static_cast<int32_t>(rows), static_cast<int32_t>(channels),
+                static_cast<int32_t>(vocab), static_cast<int32_t>(top)};
   const hipStream_t q = static_cast<hipStream_t>(stream);
   return io_dtype == FRWKV_DTYPE_F16
              ? run_backward<F16>(d, weight, grad_loss, per_row, mean, temperature, grad_hidden,

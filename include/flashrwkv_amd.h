@@ -679,7 +679,9 @@ int frwkv_layer_norm_backward(int io_dtype, int64_t rows, int64_t channels, cons
  * channels] of the io dtype, either NULL where it is not wanted. It goes
  * through the vocabulary in pieces whose logit gradients (16 bits) fit the
  * workspace. All sums are in a fixed order. Both directions need at least one
- * row. No counterpart in the reference.
+ * row. The byte queries give 0 for sizes that the calls refuse: more than 2^23
+ * rows, 65536 channels, 2^28 tokens or 1024 targets a row. No counterpart in the
+ * reference.
  */
 size_t frwkv_linear_loss_saved_bytes(int64_t rows, int64_t channels, int64_t top);
 size_t frwkv_linear_loss_forward_workspace_bytes(int64_t rows, int64_t vocab);

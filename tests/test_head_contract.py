@@ -167,6 +167,10 @@ def test_c_abi_rejects_bad_loss_calls_without_a_gpu():
     assert saved >= 512 * c * 2 and work >= 4 * 512 * 8 and back >= 512 * 1024 * 2 + n * c * 4
     assert lib.frwkv_linear_loss_backward_workspace_bytes(n, c, v, 0) < back
     assert lib.frwkv_linear_loss_saved_bytes(0, c, 1) == 0
+    assert lib.frwkv_linear_loss_saved_bytes(n, c, 1025) == 0
+    assert lib.frwkv_linear_loss_forward_workspace_bytes(n, 2 ** 40) == 0
+    assert lib.frwkv_linear_loss_backward_workspace_bytes(n, c, 2 ** 62, 1) == 0
+    assert lib.frwkv_linear_loss_backward_workspace_bytes(2 ** 40, c, v, 1) == 0
 
     def forward(dtype=2, n=n, c=c, v=v, hidden=p, bytes_=8, reduction=1, saved_=saved,
                 work_=work):
