@@ -368,10 +368,15 @@ __global__ __launch_bounds__(kScanThreads) void teacher_rows_kernel(int32_t n, i
   number_rows(n, vocab, steps, sizes, row_loss, s, [&](int32_t i) { return s.place[i] != 0; });
 }
 
-// A workgroup a row m: copies its hidden row (zeros for the rows that fill up
-// the last tile; few rows a second time kFewest rows on) and computes its K > 1
-// target logits, a wave a token (NaN for one out of range). Bound by the K weight
-// rows a row (64 of 2048 channels for 4096 rows: 152 us, 7.1 TB/s).
+// blockIdx.x: a row m, whose hidden row the first workgroup copies (zeros for the
+// rows that fill up the last tile; few rows a second time kFewest rows on).
+// blockIdx.y: kGather of its K > 1 target logits, a wave each (NaN for a token out
+// of range). Bound by the K weight rows a row where rows are many (4096 of 64
+// tokens of 2048 channels: 151 us, 7.1 TB/s), by one read of a weight row where
+// they are few (6 rows of 94 tokens of 3712 channels, forward and backward with
+// all of a row's tokens in one workgroup: 191 us, so: 120 us).
+constexpr int kGather = 4;
+
 template <typename T>
 __global__ __launch_bounds__(256) void gather_rows_kernel(
     const uint16_t* __restrict__ hidden, const uint16_t* __restrict__ weight, int32_t c,
@@ -379,17 +384,18 @@ __global__ __launch_bounds__(256) void gather_rows_kernel(
   const int count = *s.count;
   const int second = twice && blockIdx.x >= kFewest ? kFewest : 0;
   const int m = static_cast<int>(blockIdx.x) - second;
+  const bool first = blockIdx.y == 0;
   if (m >= round_up(count, kRowPad)) return;
   uint16_t* to = s.hidden + static_cast<int64_t>(blockIdx.x) * c;
   if (m >= count) {
-    for (int x = threadIdx.x * 8; x < c; x += 2048) {
+    for (int x = threadIdx.x * 8; first && x < c; x += 2048) {
       *reinterpret_cast<uint4*>(to + x) = make_uint4(0, 0, 0, 0);
     }
     return;
   }
   const int64_t i = s.row[m];
   const uint16_t* from = hidden + i * c;
-  for (int x = threadIdx.x * 8; x < c; x += 2048) {
+  for (int x = threadIdx.x * 8; first && x < c; x += 2048) {
     *reinterpret_cast<uint4*>(to + x) = *reinterpret_cast<const uint4*>(from + x);
   }
   if (second > 0) return;
@@ -397,26 +403,37 @@ __global__ __launch_bounds__(256) void gather_rows_kernel(
     if (threadIdx.x == 0) s.logit[m] = kNaN;
     return;
   }
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  for (int j = wave; j < k; j += 4) {
-    const int32_t token = s.index[i * k + j];
-    float z = 0.0f;
-    if (token >= 0 && token < vocab) {
-      const uint16_t* w = weight + static_cast<int64_t>(token) * c;
-      float sum = 0.0f;
-      for (int x = lane * 8; x < c; x += 512) {
+  const int j = static_cast<int>(blockIdx.y) * kGather + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  if (j >= k) return;
+  const int32_t token = s.index[i * k + j];
+  float z = token >= vocab ? kNaN : 0.0f;
+  if (token >= 0 && token < vocab) {
+    const uint16_t* w = weight + static_cast<int64_t>(token) * c;
+    float sum = 0.0f;
+    for (int x0 = lane * 8; x0 < c; x0 += 2048) {
+      uint4 h4[4], w4[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int x = x0 + 512 * u;
+        h4[u] = w4[u] = make_uint4(0, 0, 0, 0);
+        if (x < c) {
+          h4[u] = *reinterpret_cast<const uint4*>(from + x);
+          w4[u] = *reinterpret_cast<const uint4*>(w + x);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
         float a[8], b[8];
-        unpack8<T>(*reinterpret_cast<const uint4*>(from + x), a);
-        unpack8<T>(*reinterpret_cast<const uint4*>(w + x), b);
+        unpack8<T>(h4[u], a);
+        unpack8<T>(w4[u], b);
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum = fmaf(a[e], b[e], sum);
       }
-      z = wave_sum(sum);
-    } else if (token >= vocab) {
-      z = kNaN;
     }
-    if (lane == 0) s.logit[static_cast<int64_t>(m) * k + j] = z;
+    z = wave_sum(sum);
   }
+  if (lane == 0) s.logit[static_cast<int64_t>(m) * k + j] = z;
 }
 
 // ------------------------------------------------------------- products
@@ -435,7 +452,9 @@ using FewRowsTile = gemm::Tile<T, MA, MB, 256, 64, 8, 1, 3, MA == Major::kK && M
 // The tiles of a product over rows m, whose count stands on the device: the
 // workgroups of a launch of at most one a CU take them in turn. While a
 // workgroup finishes a tile, the first stages of its next one are on their way.
-__host__ __device__ __forceinline__ int tiles_along(int size, int tile) { return (size + tile - 1) / tile; }
+__host__ __device__ __forceinline__ int tiles_along(int size, int tile) {
+  return (size + tile - 1) / tile;
+}
 
 // Where this lane's accumulators hold a token: 16 i + r, or -1. p0: the tile's
 // first token, left: tokens from there on.
@@ -1141,8 +1160,9 @@ int run_forward(const Shape& d, const void* hidden, const void* weight, float te
   const int64_t pad = round_up(d.n, kRowPad);
   const float scale = kLog2E / temperature;
   const int n = d.n;
-  hipLaunchKernelGGL((gather_rows_kernel<T>), dim3(static_cast<unsigned>(pad)), dim3(256), 0,
-                     stream, static_cast<const uint16_t*>(hidden),
+  const int groups = d.k == 1 ? 1 : (d.k + kGather - 1) / kGather;
+  hipLaunchKernelGGL((gather_rows_kernel<T>), dim3(static_cast<unsigned>(pad), groups), dim3(256),
+                     0, stream, static_cast<const uint16_t*>(hidden),
                      static_cast<const uint16_t*>(weight), d.c, d.k, d.vocab, d.n <= kFewest, s);
   const Operand a{static_cast<const uint16_t*>(weight), d.c, d.vocab};
   const Operand b{s.hidden, d.c, static_cast<int32_t>(pad)};
