@@ -100,8 +100,10 @@ __device__ __forceinline__ float2 joined(float2 a, float2 b) {
 struct Saved {
   int32_t* count;   // [1]     rows that take part
   int32_t* cut;     // [1]     columns of the forward that large tiles take
+  int32_t* done;    // [1]     workgroups of join_tiles_kernel that have ended
   int32_t* row;     // [pad]   m -> i
   int32_t* place;   // [N]     i -> m, or -1
+  int32_t* part;    // [N]     distillation: whether row i takes part
   int32_t* index;   // [N][K]  target tokens (by i); -1 absent, V or more out of range
   float* share;     // [N][K]  p (by i)
   float* target;    // [N][K]  b at that token: the sum of p over equal tokens (by i)
@@ -124,15 +126,17 @@ Saved saved_of(char* p, int64_t n, int64_t c, int64_t k, size_t* bytes) {
   const int64_t pad = round_up(n, kRowPad);
   Layout l;
   Saved s;
-  const size_t count = l.take(4), cut = l.take(4);
-  const size_t row = l.take(pad * 4), place = l.take(n * 4);
+  const size_t count = l.take(4), cut = l.take(4), done = l.take(4);
+  const size_t row = l.take(pad * 4), place = l.take(n * 4), part = l.take(n * 4);
   const size_t index = l.take(n * k * 4), share = l.take(n * k * 4);
   const size_t target = l.take(n * k * 4), base = l.take(n * 4), lse2 = l.take(pad * 4);
   const size_t logit = l.take(pad * k * 4), hidden = l.take(pad * c * 2);
   s.count = reinterpret_cast<int32_t*>(p + count);
   s.cut = reinterpret_cast<int32_t*>(p + cut);
+  s.done = reinterpret_cast<int32_t*>(p + done);
   s.row = reinterpret_cast<int32_t*>(p + row);
   s.place = reinterpret_cast<int32_t*>(p + place);
+  s.part = reinterpret_cast<int32_t*>(p + part);
   s.index = reinterpret_cast<int32_t*>(p + index);
   s.share = reinterpret_cast<float*>(p + share);
   s.target = reinterpret_cast<float*>(p + target);
@@ -305,23 +309,57 @@ __global__ __launch_bounds__(256) void teacher_targets_kernel(
     s.target[at + j] = sum;
   }
   if (lane == 0) {
-    s.place[i] = part;
+    s.part[i] = part;
     s.base[i] = base;
   }
 }
 
-// Numbers the rows that take part, in order: part(i) says whether row i does.
-// One workgroup; row_loss (not null): 0 for the rows that do not. steps: of the
-// product, sizes: launched for it.
-template <typename Part>
-__device__ __forceinline__ void number_rows(int32_t n, int32_t vocab, int32_t steps, Sizes sizes,
-                                            float* row_loss, const Saved& s, Part&& part_of) {
+// Which rows take part, and what is noted of one that stands in no tensor yet.
+// Cross entropy: one entry a row, share 1.
+template <typename Index>
+struct Labels {
+  const Index* targets;
+  int64_t ignore;
+  __device__ __forceinline__ bool part(int32_t i) const { return targets[i] != ignore; }
+  __device__ __forceinline__ void note(int32_t i, int32_t vocab, const Saved& s) const {
+    const int64_t t = targets[i];
+    const int32_t token = as_token(t, vocab);
+    s.index[i] = t != ignore && token < 0 ? vocab : token;
+    s.share[i] = 1.0f;
+    s.target[i] = 1.0f;
+    s.base[i] = 0.0f;
+  }
+};
+
+// Distillation, behind teacher_targets_kernel.
+struct Teacher {
+  const int32_t* parts;
+  __device__ __forceinline__ bool part(int32_t i) const { return parts[i] != 0; }
+  __device__ __forceinline__ void note(int32_t, int32_t, const Saved&) const {}
+};
+
+// What the numbering of the rows needs to know of the product.
+struct Rows {
+  int32_t n, vocab, steps;
+  Sizes sizes;      // launched for it
+  float* row_loss;  // not null: 0 for the rows that take no part
+};
+
+__device__ __forceinline__ void note_count(const Rows& d, int32_t count, const Saved& s) {
+  *s.count = count;
+  *s.cut = cut_of(d.vocab, count, d.steps, d.sizes).first;
+  *s.done = 0;
+}
+
+// Numbers the rows that take part, in order. One workgroup.
+template <typename Source>
+__global__ __launch_bounds__(kScanThreads) void number_rows_kernel(Source source, Rows d, Saved s) {
   __shared__ int32_t waves[kScanThreads / 64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int32_t before = 0;
-  for (int32_t first = 0; first < n; first += kScanThreads) {
+  for (int32_t first = 0; first < d.n; first += kScanThreads) {
     const int32_t i = first + static_cast<int32_t>(threadIdx.x);
-    const bool part = i < n && part_of(i);
+    const bool part = i < d.n && source.part(i);
     const uint64_t mask = __ballot(part);
     if (lane == 0) waves[wave] = __popcll(mask);
     __syncthreads();
@@ -332,73 +370,105 @@ __device__ __forceinline__ void number_rows(int32_t n, int32_t vocab, int32_t st
       if (w < wave) m += waves[w];
       all += waves[w];
     }
-    if (i < n) s.place[i] = part ? m : -1;
+    if (i < d.n) {
+      source.note(i, d.vocab, s);
+      s.place[i] = part ? m : -1;
+      if (!part && d.row_loss != nullptr) d.row_loss[i] = 0.0f;
+    }
     if (part) s.row[m] = i;
-    if (i < n && !part && row_loss != nullptr) row_loss[i] = 0.0f;
     before += all;
     __syncthreads();
   }
-  if (threadIdx.x == 0) {
-    *s.count = before;
-    *s.cut = cut_of(vocab, before, steps, sizes).first;
+  if (threadIdx.x == 0) note_count(d, before, s);
+}
+
+// The same by every workgroup for itself, for up to kOwnNumbers rows: a launch less
+// (with the sum over rows in join_tiles_kernel, forward of 300 x 2000 x 768: 20.7 ->
+// 19.3 us). m: how many take part before row `mine`; count: of all. Returns whether
+// `mine` does.
+constexpr int kOwnNumbers = 1024;
+constexpr int kGatherThreads = 256;
+
+template <typename Source>
+__device__ __forceinline__ bool own_number(const Source& source, int32_t n, int32_t mine,
+                                           int32_t& m, int32_t& count) {
+  constexpr int kWaves = kGatherThreads / 64, kTurns = kOwnNumbers / kGatherThreads;
+  __shared__ uint64_t masks[kTurns * kWaves];
+  const int wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int u = 0; u < kTurns; ++u) {
+    const int32_t i = u * kGatherThreads + static_cast<int32_t>(threadIdx.x);
+    const uint64_t mask = __ballot(i < n && source.part(i));
+    if ((threadIdx.x & 63) == 0) masks[u * kWaves + wave] = mask;
   }
+  __syncthreads();
+  m = count = 0;
+  bool part = false;
+#pragma unroll
+  for (int g = 0; g < kTurns * kWaves; ++g) {
+    const uint64_t mask = masks[g];
+    count += __popcll(mask);
+    const int32_t at = mine - 64 * g;
+    if (at >= 64) m += __popcll(mask);
+    if (at >= 0 && at < 64) {
+      m += __popcll(mask & ((1ull << at) - 1));
+      part = (mask >> at & 1) != 0;
+    }
+  }
+  return part;
 }
 
-// Cross entropy: one entry a row, share 1.
-template <typename Index>
-__global__ __launch_bounds__(kScanThreads) void label_rows_kernel(
-    const Index* __restrict__ targets, int64_t ignore, int32_t n, int32_t vocab, int32_t steps,
-    Sizes sizes, float* row_loss, Saved s) {
-  number_rows(n, vocab, steps, sizes, row_loss, s, [&](int32_t i) {
-    const int64_t t = targets[i];
-    const bool part = t != ignore;
-    const int32_t token = as_token(t, vocab);
-    s.index[i] = part && token < 0 ? vocab : token;
-    s.share[i] = 1.0f;
-    s.target[i] = 1.0f;
-    s.base[i] = 0.0f;
-    return part;
-  });
-}
-
-// Distillation, behind teacher_targets_kernel, which leaves 1 or 0 in place[i].
-__global__ __launch_bounds__(kScanThreads) void teacher_rows_kernel(int32_t n, int32_t vocab,
-                                                                    int32_t steps, Sizes sizes,
-                                                                    float* row_loss, Saved s) {
-  number_rows(n, vocab, steps, sizes, row_loss, s, [&](int32_t i) { return s.place[i] != 0; });
-}
-
-// blockIdx.x: a row m, whose hidden row the first workgroup copies (zeros for the
-// rows that fill up the last tile; few rows a second time kFewest rows on).
-// blockIdx.y: kGather of its K > 1 target logits, a wave each (NaN for a token out
-// of range). Bound by the K weight rows a row where rows are many (4096 of 64
-// tokens of 2048 channels: 151 us, 7.1 TB/s), by one read of a weight row where
-// they are few (6 rows of 94 tokens of 3712 channels, forward and backward with
-// all of a row's tokens in one workgroup: 191 us, so: 120 us).
+// Copies the hidden rows that take part together (zeros for the rows that fill up
+// the last tile; few rows a second time kFewest rows on) and computes their K > 1
+// target logits, kGather a workgroup, a wave each (NaN for a token out of range).
+// blockIdx.x: a row i of the caller's, which the workgroup numbers itself (kOwn),
+// or a row m; blockIdx.y: the tokens.
+// Bound by the K weight rows a row where rows are many (4096 of 64 tokens of 2048
+// channels: 151 us, 7.1 TB/s), by one read of a weight row where they are few (6
+// rows of 94 tokens of 3712 channels, forward and backward with all of a row's
+// tokens in one workgroup: 191 us, so: 120 us).
 constexpr int kGather = 4;
 
-template <typename T>
-__global__ __launch_bounds__(256) void gather_rows_kernel(
+template <typename T, bool kOwn, typename Source>
+__global__ __launch_bounds__(kGatherThreads) void gather_rows_kernel(
     const uint16_t* __restrict__ hidden, const uint16_t* __restrict__ weight, int32_t c,
-    int32_t k, int32_t vocab, bool twice, Saved s) {
-  const int count = *s.count;
-  const int second = twice && blockIdx.x >= kFewest ? kFewest : 0;
-  const int m = static_cast<int>(blockIdx.x) - second;
+    int32_t k, bool twice, Source source, Rows d, Saved s) {
+  const int block = blockIdx.x;
   const bool first = blockIdx.y == 0;
-  if (m >= round_up(count, kRowPad)) return;
-  uint16_t* to = s.hidden + static_cast<int64_t>(blockIdx.x) * c;
-  if (m >= count) {
-    for (int x = threadIdx.x * 8; first && x < c; x += 2048) {
-      *reinterpret_cast<uint4*>(to + x) = make_uint4(0, 0, 0, 0);
+  int32_t m = block, i = 0, count;
+  bool part;
+  if constexpr (kOwn) {
+    i = block;
+    part = own_number(source, d.n, i, m, count);
+    if (first && threadIdx.x == 0) {
+      if (block == 0) note_count(d, count, s);
+      if (i < d.n) {
+        source.note(i, d.vocab, s);
+        s.place[i] = part ? m : -1;
+        if (!part && d.row_loss != nullptr) d.row_loss[i] = 0.0f;
+      }
+      if (part) s.row[m] = i;
     }
-    return;
+  } else {
+    count = *s.count;
+    part = m < count;
+    if (part) i = s.row[m];
   }
-  const int64_t i = s.row[m];
-  const uint16_t* from = hidden + i * c;
-  for (int x = threadIdx.x * 8; first && x < c; x += 2048) {
-    *reinterpret_cast<uint4*>(to + x) = *reinterpret_cast<const uint4*>(from + x);
+  const auto fill = [&](int row, const uint16_t* from) {
+    uint16_t* to = s.hidden + static_cast<int64_t>(row) * c;
+    for (int x = threadIdx.x * 8; x < c; x += kGatherThreads * 8) {
+      *reinterpret_cast<uint4*>(to + x) =
+          from == nullptr ? make_uint4(0, 0, 0, 0) : *reinterpret_cast<const uint4*>(from + x);
+    }
+  };
+  const uint16_t* from = hidden + static_cast<int64_t>(i) * c;
+  if (first) {
+    const bool copied = twice && block >= kFewest && block < kFewest + count;
+    if (block >= count && block < round_up(count, kRowPad) && !copied) fill(block, nullptr);
+    if (part) fill(m, from);
+    if (part && twice) fill(kFewest + m, from);
   }
-  if (second > 0) return;
+  if (!part) return;
   if (k == 1) {  // one out of range; lse_tiles_kernel writes the others
     if (threadIdx.x == 0) s.logit[m] = kNaN;
     return;
@@ -406,9 +476,9 @@ __global__ __launch_bounds__(256) void gather_rows_kernel(
   const int j = static_cast<int>(blockIdx.y) * kGather + (threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   if (j >= k) return;
-  const int32_t token = s.index[i * k + j];
-  float z = token >= vocab ? kNaN : 0.0f;
-  if (token >= 0 && token < vocab) {
+  const int32_t token = s.index[static_cast<int64_t>(i) * k + j];
+  float z = token >= d.vocab ? kNaN : 0.0f;
+  if (token >= 0 && token < d.vocab) {
     const uint16_t* w = weight + static_cast<int64_t>(token) * c;
     float sum = 0.0f;
     for (int x0 = lane * 8; x0 < c; x0 += 2048) {
@@ -878,21 +948,29 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void weight_grad_kernel(
 
 // -------------------------------------------------------- row reductions
 // A workgroup takes 32 rows, 32 threads a row: joins the tiles' maxima and
-// sums to lse2[m], and the row's loss. row_loss (by i) or partial (by m). A
-// thread has 8 tiles under way at a time, all of those of 65536 columns.
+// sums to lse2[m], and the row's loss, to row_loss (by i) or into the sum of all
+// rows. A thread has 8 tiles under way at a time, all of those of 65536 columns.
 // In the loss the target logits are taken from the row's maximum, a difference
 // that is exact where they are close, and not from lse, whose rounding alone
 // (half a unit of 16 in base 2) is 1e-6 of a loss near 1.
+// The last workgroup to end adds the workgroups' sums, in their order: a launch
+// less than a kernel of its own.
 __global__ __launch_bounds__(1024) void join_tiles_kernel(const float2* __restrict__ part,
                                                           int32_t vocab, int32_t rest_tile,
                                                           int64_t pad, int32_t k, float scale,
-                                                          float temperature2, float* row_loss,
+                                                          float temperature2, bool mean,
+                                                          float* row_loss, float* loss,
                                                           float* partial, Saved s) {
   __shared__ float2 shared[32][33];
+  __shared__ float losses[32];
+  __shared__ bool last;
   const int q = threadIdx.x & 31, slice = threadIdx.x >> 5;
   const int m = blockIdx.x * 32 + q;
   const int count = *s.count;
-  if (static_cast<int>(blockIdx.x) * 32 >= count) return;
+  if (static_cast<int>(blockIdx.x) * 32 >= count) {
+    if (count == 0 && blockIdx.x == 0 && threadIdx.x == 0 && loss != nullptr) *loss = 0.0f;
+    return;
+  }
   const int cut = *s.cut;
   const int tiles = tiles_along(cut, 256) + tiles_along(vocab - cut, rest_tile);
   float2 all = make_float2(-__builtin_inff(), 0.0f);
@@ -932,35 +1010,36 @@ __global__ __launch_bounds__(1024) void join_tiles_kernel(const float2* __restri
   }
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) term += __shfl_xor(term, off, 64);
-  if (lane != 0 || mine >= count) return;
-  const float log_sum = __builtin_amdgcn_logf(all.y);
-  // A target out of range makes its row NaN in the backward too.
-  s.lse2[mine] = term == term ? top + log_sum : term;
-  const float loss = temperature2 * ((term + log_sum) * kLn2 + s.base[i]);
-  if (row_loss) row_loss[i] = loss;
-  if (partial) partial[mine] = loss;
-}
-
-// Sum over one workgroup of 1024, in a fixed order.
-__device__ __forceinline__ float block_sum(float x, float* waves) {
-  x = wave_sum(x);
-  if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = x;
+  if (lane == 0) {
+    float value = 0.0f;
+    if (mine < count) {
+      const float log_sum = __builtin_amdgcn_logf(all.y);
+      // A target out of range makes its row NaN in the backward too.
+      s.lse2[mine] = term == term ? top + log_sum : term;
+      value = temperature2 * ((term + log_sum) * kLn2 + s.base[i]);
+      if (row_loss != nullptr) row_loss[i] = value;
+    }
+    losses[row] = value;
+  }
+  if (loss == nullptr) return;
   __syncthreads();
+  const int blocks = (count + 31) / 32;
+  if (threadIdx.x < 64) {
+    const float sum = wave_sum(threadIdx.x < 32 ? losses[threadIdx.x] : 0.0f);
+    if (threadIdx.x == 0) {
+      __hip_atomic_store(partial + blockIdx.x, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      last = __hip_atomic_fetch_add(s.done, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) ==
+             blocks - 1;
+    }
+  }
+  __syncthreads();
+  if (!last || threadIdx.x >= 64) return;
   float sum = 0.0f;
-#pragma unroll
-  for (int w = 0; w < kScanThreads / 64; ++w) sum += waves[w];
-  return sum;
-}
-
-__global__ __launch_bounds__(kScanThreads) void sum_losses_kernel(
-    const float* __restrict__ partial, const int32_t* __restrict__ count, bool mean,
-    float* __restrict__ loss) {
-  __shared__ float waves[kScanThreads / 64];
-  const int n = *count;
-  float sum = 0.0f;
-  for (int m = threadIdx.x; m < n; m += kScanThreads) sum += partial[m];
-  sum = block_sum(sum, waves);
-  if (threadIdx.x == 0) *loss = n == 0 ? 0.0f : mean ? sum / static_cast<float>(n) : sum;
+  for (int b = threadIdx.x; b < blocks; b += 64) {
+    sum += __hip_atomic_load(partial + b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  sum = wave_sum(sum);
+  if (threadIdx.x == 0) *loss = mean ? sum / static_cast<float>(count) : sum;
 }
 
 // coef[m] multiplies (p - b) of row m in dz, *scale the finished gradients;
@@ -1090,7 +1169,7 @@ ForwardWork forward_work(char* p, int64_t n, int64_t vocab, size_t* bytes) {
   const int64_t pad = round_up(n, kRowPad);
   Layout l;
   const size_t part = l.take(round_up(vocab, kMinTile) / kMinTile * pad * 8);
-  const size_t partial = l.take(pad * 4);
+  const size_t partial = l.take(pad / 32 * 4);
   *bytes = l.bytes;
   return {reinterpret_cast<float2*>(p + part), reinterpret_cast<float*>(p + partial)};
 }
@@ -1153,32 +1232,40 @@ void for_sizes(int32_t vocab, int32_t rows, int32_t steps, F&& f) {
   if (sizes.small) launch(Size::kSmall);
 }
 
-template <typename T>
-int run_forward(const Shape& d, const void* hidden, const void* weight, float temperature,
-                bool mean, bool per_row, float* loss, const Saved& s, const ForwardWork& w,
-                hipStream_t stream) {
+template <typename T, typename Source>
+int run_forward(const Shape& d, const Source& source, const void* hidden, const void* weight,
+                float temperature, int reduction, float* loss, const Saved& s,
+                const ForwardWork& w, hipStream_t stream) {
   const int64_t pad = round_up(d.n, kRowPad);
+  const int steps = d.c / gemm::kStep;
   const float scale = kLog2E / temperature;
-  const int n = d.n;
-  const int groups = d.k == 1 ? 1 : (d.k + kGather - 1) / kGather;
-  hipLaunchKernelGGL((gather_rows_kernel<T>), dim3(static_cast<unsigned>(pad), groups), dim3(256),
-                     0, stream, static_cast<const uint16_t*>(hidden),
-                     static_cast<const uint16_t*>(weight), d.c, d.k, d.vocab, d.n <= kFewest, s);
+  float* row_loss = reduction == FRWKV_REDUCE_NONE ? loss : nullptr;
+  const Rows rows{d.n, d.vocab, steps, sizes_of(d.vocab, d.n, steps), row_loss};
+  const auto gather = [&](auto* kernel) {
+    const int groups = d.k == 1 ? 1 : (d.k + kGather - 1) / kGather;
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(pad), groups), dim3(kGatherThreads), 0,
+                       stream, static_cast<const uint16_t*>(hidden),
+                       static_cast<const uint16_t*>(weight), d.c, d.k, d.n <= kFewest, source,
+                       rows, s);
+  };
+  if (d.n <= kOwnNumbers) {
+    gather(gather_rows_kernel<T, true, Source>);
+  } else {
+    hipLaunchKernelGGL((number_rows_kernel<Source>), dim3(1), dim3(kScanThreads), 0, stream,
+                       source, rows, s);
+    gather(gather_rows_kernel<T, false, Source>);
+  }
   const Operand a{static_cast<const uint16_t*>(weight), d.c, d.vocab};
   const Operand b{s.hidden, d.c, static_cast<int32_t>(pad)};
-  for_sizes<T>(d.vocab, d.n, d.c / gemm::kStep, [&](auto* tile, int grid) {
+  for_sizes<T>(d.vocab, d.n, steps, [&](auto* tile, int grid) {
     using G = std::remove_pointer_t<decltype(tile)>;
     hipLaunchKernelGGL((lse_tiles_kernel<G, T>), dim3(grid), dim3(gemm::kThreads), 0, stream, a, b,
                        d.c, scale, d.k == 1, w.part, pad, s);
   });
-  hipLaunchKernelGGL(join_tiles_kernel, dim3((n + 31) / 32), dim3(1024), 0, stream, w.part,
+  hipLaunchKernelGGL(join_tiles_kernel, dim3((d.n + 31) / 32), dim3(1024), 0, stream, w.part,
                      d.vocab, time_of(few(d.n) ? Size::kFewRows : Size::kSmall).p, pad, d.k, scale,
-                     temperature * temperature, per_row ? loss : nullptr,
-                     per_row ? nullptr : w.partial, s);
-  if (!per_row) {
-    hipLaunchKernelGGL(sum_losses_kernel, dim3(1), dim3(kScanThreads), 0, stream, w.partial,
-                       s.count, mean, loss);
-  }
+                     temperature * temperature, reduction == FRWKV_REDUCE_MEAN, row_loss,
+                     row_loss == nullptr ? loss : nullptr, w.partial, s);
   return check_launch("linear loss forward");
 }
 
@@ -1325,15 +1412,16 @@ int check_temperature(const char* what, float t) {
   return FRWKV_OK;
 }
 
-int forward(int io_dtype, const Shape& d, const void* hidden,
+template <typename Source>
+int forward(int io_dtype, const Shape& d, const Source& source, const void* hidden,
             const void* weight, float temperature, int reduction, float* loss, const Saved& s,
             void* workspace, hipStream_t stream) {
   size_t need = 0;
   const ForwardWork w = forward_work(static_cast<char*>(workspace), d.n, d.vocab, &need);
-  const bool mean = reduction == FRWKV_REDUCE_MEAN, per_row = reduction == FRWKV_REDUCE_NONE;
   return io_dtype == FRWKV_DTYPE_F16
-             ? run_forward<F16>(d, hidden, weight, temperature, mean, per_row, loss, s, w, stream)
-             : run_forward<Bf16>(d, hidden, weight, temperature, mean, per_row, loss, s, w,
+             ? run_forward<F16>(d, source, hidden, weight, temperature, reduction, loss, s, w,
+                                stream)
+             : run_forward<Bf16>(d, source, hidden, weight, temperature, reduction, loss, s, w,
                                  stream);
 }
 
@@ -1414,20 +1502,13 @@ int frwkv_linear_cross_entropy_forward(int io_dtype, int64_t rows, int64_t chann
   }
   const hipStream_t q = static_cast<hipStream_t>(stream);
   const int32_t n = static_cast<int32_t>(rows), v = static_cast<int32_t>(vocab);
-  const int32_t steps = static_cast<int32_t>(channels / gemm::kStep);
-  const Sizes sizes = sizes_of(vocab, rows, steps);
-  float* row_loss = reduction == FRWKV_REDUCE_NONE ? loss : nullptr;
+  const Shape d{n, static_cast<int32_t>(channels), v, 1};
   if (target_bytes == 8) {
-    hipLaunchKernelGGL((label_rows_kernel<int64_t>), dim3(1), dim3(kScanThreads), 0, q,
-                       static_cast<const int64_t*>(targets), ignore_index, n, v,
-                       steps, sizes, row_loss, s);
-  } else {
-    hipLaunchKernelGGL((label_rows_kernel<int32_t>), dim3(1), dim3(kScanThreads), 0, q,
-                       static_cast<const int32_t*>(targets), ignore_index, n, v,
-                       steps, sizes, row_loss, s);
+    const Labels<int64_t> labels{static_cast<const int64_t*>(targets), ignore_index};
+    return forward(io_dtype, d, labels, hidden, weight, 1.0f, reduction, loss, s, workspace, q);
   }
-  return forward(io_dtype, Shape{n, static_cast<int32_t>(channels), v, 1}, hidden,
-                 weight, 1.0f, reduction, loss, s, workspace, q);
+  const Labels<int32_t> labels{static_cast<const int32_t*>(targets), ignore_index};
+  return forward(io_dtype, d, labels, hidden, weight, 1.0f, reduction, loss, s, workspace, q);
 }
 
 int frwkv_linear_topk_distillation_forward(
@@ -1476,12 +1557,8 @@ int frwkv_linear_topk_distillation_forward(
   } else {
     with_index(Bf16{});
   }
-  const int32_t steps = static_cast<int32_t>(channels / gemm::kStep);
-  const Sizes sizes = sizes_of(vocab, rows, steps);
-  hipLaunchKernelGGL(teacher_rows_kernel, dim3(1), dim3(kScanThreads), 0, q, n, v, steps, sizes,
-                     reduction == FRWKV_REDUCE_NONE ? loss : nullptr, s);
-  return forward(io_dtype, Shape{n, static_cast<int32_t>(channels), v, k}, hidden,
-                 weight, temperature, reduction, loss, s, workspace, q);
+  return forward(io_dtype, Shape{n, static_cast<int32_t>(channels), v, k}, Teacher{s.part},
+                 hidden, weight, temperature, reduction, loss, s, workspace, q);
 }
 
 int frwkv_linear_loss_backward(int io_dtype, int64_t rows, int64_t channels, int64_t vocab,
