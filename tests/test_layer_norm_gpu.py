@@ -120,6 +120,35 @@ def test_forward_and_gradients(rows, c, dtype, residual):
     assert all(torch.equal(a, b) for a, b in zip(grads, again))
 
 
+def test_offsets_beyond_32_bits():
+    """More than 2^31 elements: the first and last rows, and the sums over all."""
+    rows, c, dtype = 530003, 4096, torch.bfloat16
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    x, dy = (torch.empty(rows, c, dtype=dtype, device=DEV).normal_(generator=gen)
+             for _ in range(2))
+    small = _inputs(1, c, dtype, seed=6)
+    weight = small["weight"].clone().requires_grad_()
+    bias = small["bias"].clone().requires_grad_()
+    leaf = x.requires_grad_()
+    y = pretrain_layer_norm(leaf, weight, bias)
+    grads = torch.autograd.grad(y, [leaf, weight, bias], dy)
+    y = y.detach()
+    for part in (slice(0, 3), slice(rows // 2, rows // 2 + 3), slice(rows - 3, rows)):
+        case = {"x": x.detach()[part], "weight": small["weight"], "bias": small["bias"],
+                "dy": dy[part]}
+        alone = {k: case[k].clone().requires_grad_() for k in ("x", "weight", "bias")}
+        want = pretrain_layer_norm(alone["x"], alone["weight"], alone["bias"])
+        dx, = torch.autograd.grad(want, [alone["x"]], case["dy"])
+        case["s"] = case["x"]
+        _check(case, 1e-5, want.detach())
+        assert torch.equal(y[part], want) and torch.equal(grads[0][part], dx)
+    dbias, abs_dbias = 0.0, 0.0
+    for at in range(0, rows, 53000):
+        part = dy[at:at + 53000].double()
+        dbias, abs_dbias = dbias + part.sum(0), abs_dbias + part.abs().sum(0)
+    _within("dbias", grads[2], dbias, ROUND[dtype] * dbias.abs() + 2 * INNER * abs_dbias)
+
+
 @pytest.mark.parametrize("dtype", ROUND)
 def test_tensors_off_16_byte_boundaries(dtype):
     """Contiguous views that start one element into their storage take the

@@ -376,6 +376,78 @@ def test_several_pieces_of_the_vocabulary():
            reduction="mean")
 
 
+@pytest.mark.parametrize("n", [1023, 1024, 1025, 2113])
+@pytest.mark.parametrize("last", [True, False])
+def test_rows_are_numbered_in_order(n, last):
+    """Up to 1024 rows each workgroup numbers them for itself; the last row alone,
+    or with others that are left after two of three were masked."""
+    h, w = _head(n, 64, 130, torch.bfloat16, seed=n)
+    targets = torch.randint(130, (n,), generator=_gen(n))
+    targets[torch.arange(n) % 3 != 1] = -100
+    if last:
+        targets[:-1] = -100
+    targets[-1] = 7
+    targets = targets.to(DEV)
+    upstream = _upstream("none", n, seed=n + 2)
+    entry = head.labels(targets, 130, -100)
+    got = _grads(lambda a, b: pretrain_linear_cross_entropy(a, b, targets, reduction="none"), h,
+                 w, upstream)
+    _check(h, w, entry, got, row_weight=upstream, reduction="none")
+    tokens = torch.where(targets < 0, -1, targets)[:, None].expand(n, 2).contiguous()
+    tokens[:, 1] = -1
+    one = torch.ones((), device=DEV)
+    got = _grads(lambda a, b: pretrain_linear_topk_distillation(
+        a, b, torch.zeros(n, 2, device=DEV), tokens), h, w, one)
+    _check(h, w, entry, got, row_weight=one.expand(n), reduction="mean")
+
+
+def test_offsets_beyond_32_bits():
+    """A weight of more than 2^31 elements, and its gradient; references by blocks."""
+    n, c, v, block = 3, 4096, 530001, 53000
+    gen = torch.Generator(device=DEV).manual_seed(33)
+    h = torch.randn(n, c, generator=gen, device=DEV).bfloat16()
+    w = torch.empty(v, c, dtype=torch.bfloat16, device=DEV)
+    for at in range(0, v, block):
+        part = w[at:at + block]
+        part.copy_(torch.randn(part.shape, generator=gen, device=DEV) * (2 / math.sqrt(c)))
+    targets = torch.tensor([v - 1, 5, v - block - 1], device=DEV)
+    upstream = torch.tensor([1.0, -2.0, 0.5], device=DEV)
+    loss, dh, dw = _grads(lambda a, b: pretrain_linear_cross_entropy(a, b, targets,
+                                                                     reduction="none"),
+                          h, w, upstream)
+    hd = h.double()
+    z = torch.cat([hd @ w[at:at + block].double().t() for at in range(0, v, block)], 1)
+    lse = torch.logsumexp(z, 1, keepdim=True)
+    rows = torch.arange(n, device=DEV)
+    a = (hd.abs().amax() * w.abs().sum(1).max().double()).item()
+    gamma = (math.sqrt(c) + 16) * E
+    size = 1 + lse.abs().max().item() + z.abs().max().item()
+    want = lse[:, 0] - z[rows, targets]
+    assert ((loss.double() - want).abs() <= 3 * gamma * a + 8 * E * size).all()
+    dz = torch.exp(z - lse)
+    dz[rows, targets] -= 1
+    dz *= upstream.double()[:, None]
+    u = ROUND[torch.bfloat16]
+    delta = 2 * gamma * a + 8 * E * size
+    by = upstream.double().abs()
+    ref, scale = torch.zeros_like(hd), torch.zeros_like(hd)
+    for at in range(0, v, block):
+        part = w[at:at + block].double()
+        ref += dz[:, at:at + block] @ part
+        scale += dz[:, at:at + block].abs() @ part.abs()
+    sums = (math.sqrt(v) + 16) * E
+    allowed = ((u * u + delta + sums) * scale + delta * by[:, None] * w[targets].double().abs()
+               + u * ref.abs() * (1 + u))
+    assert ((dh.double() - ref).abs() <= allowed).all()
+    some = torch.cat([torch.arange(0, v, 4999, device=DEV), targets])
+    ref = dz[:, some].t() @ hd
+    target = torch.zeros(n, v, dtype=torch.float64, device=DEV)
+    target[rows, targets] = by
+    allowed = ((u * u + delta + 32 * E) * (dz[:, some].abs().t() @ hd.abs())
+               + delta * (target[:, some].t() @ hd.abs()) + u * ref.abs() * (1 + u))
+    assert ((dw[some].double() - ref).abs() <= allowed).all()
+
+
 def test_gradient_matches_differences_of_the_operator():
     """Central differences of the operator's own loss along directions in which
     the fp16 inputs move exactly (multiples of 1/16): truncation h^2 of a
