@@ -46,7 +46,6 @@ using gemm::Operand;
 constexpr float kLn2 = 0.69314718055994531f;
 constexpr int kRowPad = 256;       // rows of workspaces, and a product's largest tile
 constexpr int kVocabTile = 256;    // pieces of the vocabulary are whole multiples of it
-constexpr int kMinTile = 128;      // fewest columns whose maximum and sum the forward keeps
 constexpr int kFewest = 32;        // rows up to here: see Twice below
 constexpr int kScanThreads = 1024;
 constexpr int kCus = 256;
@@ -149,7 +148,7 @@ Saved saved_of(char* p, int64_t n, int64_t c, int64_t k, size_t* bytes) {
 }
 
 // -------------------------------------------------- tile sizes and their times
-enum class Size { kFewRows, kSmall, kLarge };
+enum class Size { kNarrow64, kNarrow128, kFewRows, kSmall, kLarge };
 
 struct TileTime {
   int32_t p, q;
@@ -158,9 +157,11 @@ struct TileTime {
 
 // Measured on products that fill the GPU for many rounds.
 __host__ __device__ constexpr TileTime time_of(Size s) {
-  return s == Size::kFewRows ? TileTime{256, 64, 1.0f, 3.0f}
-         : s == Size::kSmall ? TileTime{128, 128, 0.6f, 3.0f}
-                             : TileTime{256, 256, 1.65f, 5.0f};
+  return s == Size::kNarrow64    ? TileTime{64, 64, 0.4f, 3.0f}
+         : s == Size::kNarrow128 ? TileTime{128, 64, 0.7f, 3.0f}
+         : s == Size::kFewRows   ? TileTime{256, 64, 1.0f, 3.0f}
+         : s == Size::kSmall     ? TileTime{128, 128, 0.6f, 3.0f}
+                                 : TileTime{256, 256, 1.65f, 5.0f};
 }
 
 // Fewer than 2^30 tiles, checked at the entry points.
@@ -211,12 +212,25 @@ __host__ __device__ inline Cut cut_of(int32_t vocab, int32_t across, int32_t ste
 
 constexpr Sizes kBothSizes = {true, true};
 
-// For products over the rows that take part the device decides, where their
+// Of the products over rows, those whose tiles, narrow as they are, fill the GPU at
+// most once have the narrowest such ones: what bounds them is how many loads are
+// under way (scoring 8 rows of 4096 channels, 64 x 64, 128 x 64 and 256 x 64 tiles:
+// 8192 tokens 27, 30 and 43 us, 32768 tokens 77, 59 and 72, 65536 tokens 127, 112
+// and 106). Otherwise few rows have tiles of 64 of them, and kSmall stands for a cut.
+inline Size size_of(int32_t vocab, int32_t rows) {
+  for (Size size : {Size::kNarrow64, Size::kNarrow128}) {
+    if (tiles_of(size, vocab, rows) <= kCus) return size;
+  }
+  return rows <= time_of(Size::kFewRows).q ? Size::kFewRows : Size::kSmall;
+}
+
+// For products over the rows that take part the device decides the cut, where their
 // count is (777 rows, of which 520 take part, 20011 x 768: forward and backward
-// 138 -> 127 us). A launch that finds no columns of its own ends at once, which takes 1 to
-// 2 us; sizes that no count from half of the rows on asks for are not launched.
+// 138 -> 127 us). A launch that finds no columns of its own ends at once, which takes
+// 1 to 2 us; sizes that no count from half of the rows on asks for are not launched.
 inline Sizes sizes_of(int32_t vocab, int32_t rows, int32_t steps) {
   Sizes sizes = {false, false};
+  if (size_of(vocab, rows) != Size::kSmall) return {true, false};
   for (int eighths = 4; eighths <= 8; ++eighths) {
     const Cut cut = cut_of(vocab, (rows * eighths + 7) / 8, steps, kBothSizes);
     sizes.large |= cut.first > 0;
@@ -229,7 +243,7 @@ inline Sizes sizes_of(int32_t vocab, int32_t rows, int32_t steps) {
 template <typename G>
 __device__ __forceinline__ void own_columns(const int32_t* cut, int32_t& from, int32_t& columns) {
   from = 0;
-  if (G::kBQ == 64) return;  // few rows: all of them
+  if (G::kBQ == 64) return;  // all of them
   if (G::kBQ == 256) {
     columns = *cut;
   } else {
@@ -515,7 +529,12 @@ using SmallTile = gemm::Tile<T, MA, MB, 128, 128, 2, 4, 4>;
 // Few rows only stream the weight, and every workgroup starting at the first k
 // hits the same memory channels where rows are a power of two apart: they
 // start at different ones (scoring 1 row, 65536 x 2048, from memory: 79 -> 63 us;
-// for the large tile, bound by the products, it costs 1%).
+// for the large tile, bound by the products, it costs 1%). So do the narrow tiles,
+// with more stages under way.
+template <typename T, Major MA, Major MB>
+using Narrow64Tile = gemm::Tile<T, MA, MB, 64, 64, 2, 4, 8, true>;
+template <typename T, Major MA, Major MB>
+using Narrow128Tile = gemm::Tile<T, MA, MB, 128, 64, 4, 2, 6, true>;
 template <typename T, Major MA, Major MB>
 using FewRowsTile = gemm::Tile<T, MA, MB, 256, 64, 8, 1, 3, MA == Major::kK && MB == Major::kK>;
 
@@ -700,11 +719,13 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void softmax_grad_kernel(
     }
     const int left = w.rows - p0;
     const bool all = left >= G::kBP && rows - q0 >= G::kBQ;
-    constexpr int kHalf = kFewest / 16;  // columns j of the first term
     const bool second = G::kBQ == 2 * kFewest && twice;
 #pragma unroll
     for (int j = 0; j < G::TQ; ++j) {
-      if (second && j >= kHalf) break;
+      if (second && G::wave_q0() + 16 * j >= kFewest) {  // the second term's
+        if (j == 0) G::arrive();
+        continue;
+      }
       const bool here = q0 + G::column(j) < rows;
       uint2 out[G::TP], rest[G::TP];
 #pragma unroll
@@ -728,7 +749,7 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void softmax_grad_kernel(
       gemm::store_column<G>(dz + q0 * ld + p0, ld, G::kBP, G::kBQ, j, out);
       if constexpr (G::kBQ == 2 * kFewest) {
         if (second) {
-          gemm::store_column<G>(dz + q0 * ld + p0, ld, G::kBP, G::kBQ, (j + kHalf) % G::TQ, rest);
+          gemm::store_column<G>(dz + (q0 + kFewest) * ld + p0, ld, G::kBP, kFewest, j, rest);
         }
       }
     }
@@ -855,7 +876,8 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void hidden_grad_kernel(
       G::arrive();
     }
     if constexpr (G::kBQ == 2 * kFewest) {
-      if (twice) {  // both terms of dz; they lie in one lane
+      static_assert(G::kWQ == 1, "a lane holds both terms");
+      if (twice) {  // both terms of dz
         constexpr int kHalf = kFewest / 16;
 #pragma unroll
         for (int j = 0; j < kHalf; ++j) {
@@ -1114,6 +1136,12 @@ Splitting splitting_of(Size size, int64_t columns, int64_t c, int64_t room) {
 
 bool few(int64_t n) { return n <= time_of(Size::kFewRows).q; }
 
+double rows_us(int32_t columns, int32_t rows, int32_t steps) {
+  const Size size = size_of(columns, rows);
+  return size == Size::kSmall ? cut_of(columns, rows, steps, kBothSizes).us
+                              : product_us(size, columns, rows, steps);
+}
+
 Plan plan_of(int64_t n, int64_t c, int64_t vocab) {
   const int64_t all = round_up(vocab, kVocabTile), pad = round_up(n, kRowPad);
   const int64_t steps_c = c / gemm::kStep, steps_n = (n + gemm::kStep - 1) / gemm::kStep;
@@ -1128,9 +1156,7 @@ Plan plan_of(int64_t n, int64_t c, int64_t vocab) {
     last = p.columns;
     const int64_t bytes = pad * p.columns * 2;
     if (bytes > kMostBytes && p.columns > kVocabTile) continue;
-    double us = 12.0 +
-                (few(n) ? product_us(Size::kFewRows, p.columns, n, steps_c)
-                        : cut_of(p.columns, n, steps_c, kBothSizes).us) +
+    double us = 12.0 + rows_us(p.columns, n, steps_c) +
                 cut_of(p.columns, c, steps_n, kBothSizes).us +
                 (bytes > kCachedBytes ? 3 * bytes / kGradBytesPerUs : 0.0);
     double hidden = 1e300;
@@ -1168,7 +1194,8 @@ struct ForwardWork {
 ForwardWork forward_work(char* p, int64_t n, int64_t vocab, size_t* bytes) {
   const int64_t pad = round_up(n, kRowPad);
   Layout l;
-  const size_t part = l.take(round_up(vocab, kMinTile) / kMinTile * pad * 8);
+  const int64_t tile = time_of(size_of(vocab, n)).p;
+  const size_t part = l.take((vocab + tile - 1) / tile * pad * 8);
   const size_t partial = l.take(pad / 32 * 4);
   *bytes = l.bytes;
   return {reinterpret_cast<float2*>(p + part), reinterpret_cast<float*>(p + partial)};
@@ -1211,6 +1238,16 @@ void with_tile(Size size, F&& f) {
     case Size::kFewRows:
       if constexpr (MB == Major::kK) f(static_cast<FewRowsTile<T, MA, MB>*>(nullptr));
       return;
+    case Size::kNarrow64:
+      if constexpr (MA == Major::kK && MB == Major::kK) {
+        f(static_cast<Narrow64Tile<T, MA, MB>*>(nullptr));
+      }
+      return;
+    case Size::kNarrow128:
+      if constexpr (MA == Major::kK && MB == Major::kK) {
+        f(static_cast<Narrow128Tile<T, MA, MB>*>(nullptr));
+      }
+      return;
     case Size::kSmall:
       return f(static_cast<SmallTile<T, MA, MB>*>(nullptr));
     case Size::kLarge:
@@ -1219,14 +1256,15 @@ void with_tile(Size size, F&& f) {
 }
 
 // f(tile type, grid) for the sizes that a product over `vocab` columns and
-// `rows` rows may be cut into on the device. Few rows have a tile of their own.
+// `rows` rows may be cut into on the device.
 template <typename T, typename F>
 void for_sizes(int32_t vocab, int32_t rows, int32_t steps, F&& f) {
   const auto launch = [&](Size size) {
     const int grid = grid_of(tiles_of(size, vocab, rows));
     with_tile<T, Major::kK, Major::kK>(size, [&](auto* tile) { f(tile, grid); });
   };
-  if (few(rows)) return launch(Size::kFewRows);
+  const Size size = size_of(vocab, rows);
+  if (size != Size::kSmall) return launch(size);
   const Sizes sizes = sizes_of(vocab, rows, steps);
   if (sizes.large) launch(Size::kLarge);
   if (sizes.small) launch(Size::kSmall);
@@ -1263,7 +1301,7 @@ int run_forward(const Shape& d, const Source& source, const void* hidden, const 
                        d.c, scale, d.k == 1, w.part, pad, s);
   });
   hipLaunchKernelGGL(join_tiles_kernel, dim3((d.n + 31) / 32), dim3(1024), 0, stream, w.part,
-                     d.vocab, time_of(few(d.n) ? Size::kFewRows : Size::kSmall).p, pad, d.k, scale,
+                     d.vocab, time_of(size_of(d.vocab, d.n)).p, pad, d.k, scale,
                      temperature * temperature, reduction == FRWKV_REDUCE_MEAN, row_loss,
                      row_loss == nullptr ? loss : nullptr, w.partial, s);
   return check_launch("linear loss forward");
@@ -1375,7 +1413,8 @@ int check_shape(const char* what, int io_dtype, int64_t n, int64_t c, int64_t vo
                      "%s: targets of a row must be in [1, 1024], got %lld", what,
                      static_cast<long long>(k));
   }
-  const int64_t tiles = round_up(vocab, kMinTile) / kMinTile * (round_up(n, kMinTile) / kMinTile);
+  const int64_t tile = time_of(Size::kSmall).p;  // of the most tiles there can be
+  const int64_t tiles = round_up(vocab, tile) / tile * (round_up(n, tile) / tile);
   if (tiles >= (int64_t{1} << 30) || n * k >= (int64_t{1} << 31)) {
     return set_error(FRWKV_ERR_UNSUPPORTED,
                      "%s: rows x vocabulary or rows x targets too large for one call", what);
