@@ -227,7 +227,7 @@ inline Size size_of(int32_t vocab, int32_t rows) {
 // For products over the rows that take part the device decides the cut, where their
 // count is (777 rows, of which 520 take part, 20011 x 768: forward and backward
 // 138 -> 127 us). A launch that finds no columns of its own ends at once, which takes
-// 1 to 2 us; sizes that no count from half of the rows on asks for are not launched.
+// 4 us; sizes that no count from half of the rows on asks for are not launched.
 inline Sizes sizes_of(int32_t vocab, int32_t rows, int32_t steps) {
   Sizes sizes = {false, false};
   if (size_of(vocab, rows) != Size::kSmall) return {true, false};
