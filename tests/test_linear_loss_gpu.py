@@ -317,7 +317,7 @@ def test_upstream_scales(scale):
 @pytest.mark.parametrize("dtype", ROUND)
 @pytest.mark.parametrize("n,c,v,masked", [
     (520, 768, 25000, 0.0), (520, 768, 25000, 0.3), (300, 64, 20000, 0.5), (60, 128, 20000, 0.5),
-    (700, 64, 20000, 0.97)])
+    (50, 128, 40000, 0.1), (700, 64, 20000, 0.97), (130, 640, 5000, 0.2), (250, 320, 7000, 0.0)])
 def test_wide_vocabularies(n, c, v, masked, dtype):
     """More tiles than CUs, the last ones smaller; dz W split over the vocabulary,
     into more parts the fewer rows take part."""
@@ -337,7 +337,8 @@ def test_wide_vocabularies(n, c, v, masked, dtype):
 
 @pytest.mark.parametrize("dtype", ROUND)
 @pytest.mark.parametrize("n,c,v,k", [(1, 512, 300, 1), (3, 64, 1000, 1), (31, 320, 257, 1),
-                                     (32, 1024, 700, 1), (20, 128, 400, 9)])
+                                     (32, 1024, 700, 1), (20, 128, 400, 9), (32, 128, 20000, 1),
+                                     (5, 64, 40000, 1), (17, 192, 70001, 3)])
 def test_few_rows_lose_nothing_to_their_logit_gradients(n, c, v, k, dtype):
     """Up to 32 rows keep them in two terms, with per-row weights as well."""
     h, w = _head(n, c, v, dtype, seed=31 + n)
