@@ -280,7 +280,7 @@ __global__ __launch_bounds__(256) void teacher_targets_kernel(
   bool any = false;
   if (i < n) {
     for (int j = lane; j < k; j += 64) {
-      const float x = to_f32<T>(logits[at + j]) * inv_temperature;
+      const float x = to_f32<T>(logits[at + j]);
       const int32_t token = x == -__builtin_inff() ? -1 : as_token(indices[at + j], vocab);
       tokens[j] = token;
       shares[j] = x;
@@ -291,13 +291,13 @@ __global__ __launch_bounds__(256) void teacher_targets_kernel(
     }
   }
   const bool part = __ballot(any) != 0;
+  // From the maximum before 1 / T, which can take the lowest finite logit to -inf.
   top = wave_max(top);
   float total = 0.0f;
   if (i < n) {
     for (int j = lane; j < k; j += 64) {
-      const float e =
-          tokens[j] >= 0 ? __builtin_amdgcn_exp2f((shares[j] - top) * kLog2E) : 0.0f;
-      total += e;
+      shares[j] = (shares[j] - top) * inv_temperature;
+      total += tokens[j] >= 0 ? __builtin_amdgcn_exp2f(shares[j] * kLog2E) : 0.0f;
     }
   }
   total = wave_sum(total);
@@ -307,7 +307,7 @@ __global__ __launch_bounds__(256) void teacher_targets_kernel(
     for (int j = lane; j < k; j += 64) {
       float p = 0.0f;
       if (part && tokens[j] >= 0) {
-        const float log_p = shares[j] - top - log_total;
+        const float log_p = shares[j] - log_total;
         p = __builtin_amdgcn_exp2f(log_p * kLog2E);
         base += p == 0.0f ? 0.0f : p * log_p;
       }

@@ -524,3 +524,34 @@ def test_differentiating_twice_raises(kind):
                               create_graph=True)
     with pytest.raises(RuntimeError, match="differentiate twice"):
         dh.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("t", [0.1, 0.5, 3.0])
+def test_only_minus_infinity_is_absent_whatever_the_temperature(t, dtype):
+    """Rows whose logits are all the type's lowest finite value are a uniform
+    teacher at any temperature and count in a mean; beside an ordinary logit such
+    an entry has no share; -inf is absent."""
+    n, v, low = 9, 70, torch.finfo(dtype).min
+    h, w = _head(n, 64, v, torch.bfloat16, seed=40)
+    logits = torch.randn(n, 4, generator=_gen(41)).to(dtype)
+    logits[0] = low
+    logits[1, 1:] = low
+    logits[2, 0], logits[2, 1:] = low, -math.inf
+    logits[3] = -math.inf
+    logits = logits.to(DEV)
+    tokens = torch.stack([torch.randperm(v, generator=_gen(42 + i))[:4] for i in range(n)]).to(DEV)
+    one = torch.ones((), device=DEV)
+    entry = head.teacher(logits, tokens, t)
+    assert entry[2].any(1).sum() == n - 1
+    for reduction in ("mean", "none"):
+        upstream = one if reduction == "mean" else _upstream("none", n, seed=43)
+        got = _grads(lambda a, b: pretrain_linear_topk_distillation(
+            a, b, logits, tokens, temperature=t, reduction=reduction), h, w, upstream)
+        _check(h, w, entry, got, temperature=t, row_weight=_row_weight(upstream, n),
+               reduction=reduction)
+    even = logits.clone()
+    even[0] = 0
+    rows = [pretrain_linear_topk_distillation(h, w, x, tokens, temperature=t, reduction="none")
+            for x in (logits, even)]
+    assert torch.equal(*rows)
