@@ -1116,17 +1116,19 @@ __global__ __launch_bounds__(kScanThreads) void row_coefficients_kernel(
     if (threadIdx.x == 0) *scale = *upstream * by / lift;
     return;
   }
+  // A weight of 1e30 or more, infinite ones among them, has gradients beyond fp16 by
+  // itself; the others' power of two is chosen without it, or they would be as well.
   float top = 0.0f;
   for (int m = threadIdx.x; m < n; m += kScanThreads) {
-    top = fmaxf(top, fabsf(upstream[s.row[m]] * by));
+    const float x = fabsf(upstream[s.row[m]] * by);
+    top = x < 1e30f ? fmaxf(top, x) : top;
   }
   top = wave_max(top);
   if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = top;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kScanThreads / 64; ++w) top = fmaxf(top, waves[w]);
-  const bool usable = top > 1e-30f && top < 1e30f;
-  const int exponent = usable ? static_cast<int>(ceilf(__builtin_amdgcn_logf(top))) : 0;
+  const int exponent = top > 1e-30f ? static_cast<int>(ceilf(__builtin_amdgcn_logf(top))) : 0;
   const float divide = ldexpf(1.0f, up - exponent);
   for (int m = threadIdx.x; m < n; m += kScanThreads) {
     coef[m] = upstream[s.row[m]] * by * divide;

@@ -555,3 +555,20 @@ def test_only_minus_infinity_is_absent_whatever_the_temperature(t, dtype):
     rows = [pretrain_linear_topk_distillation(h, w, x, tokens, temperature=t, reduction="none")
             for x in (logits, even)]
     assert torch.equal(*rows)
+
+
+@pytest.mark.parametrize("dtype", ROUND)
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan, 3e38])
+def test_a_row_weight_beyond_the_others_range_stays_with_its_row(bad, dtype):
+    """The other rows' losses and hidden gradients are within their bounds."""
+    h, w = _head(90, 128, 300, dtype, seed=44)
+    targets = torch.randint(300, (90,), generator=_gen(45)).to(DEV)
+    upstream = (torch.randn(90, generator=_gen(46)) * 20).to(DEV)
+    upstream[11] = bad
+    loss, dh, _ = _grads(lambda a, b: pretrain_linear_cross_entropy(a, b, targets,
+                                                                    reduction="none"),
+                         h, w, upstream)
+    keep = [i for i in range(90) if i != 11]
+    entry = head.labels(targets[keep], 300, -100)
+    _check(h[keep], w, entry, (loss[keep], dh[keep], None), row_weight=upstream[keep],
+           reduction="none")
