@@ -85,13 +85,16 @@ __device__ __forceinline__ float wave_max(float x) {
   return x;
 }
 
-// (maximum, sum of 2^(x - maximum)) of two sets; a sum of 0 is an empty set.
-__device__ __forceinline__ float2 joined(float2 a, float2 b) {
+// (maximum, sum of 2^(scale (x - maximum))) of two sets; a sum of 0 is an empty set.
+// Here as wherever an exponential is taken the difference comes before the scale: it
+// is exact near the maximum, while a rounded scale x maximum is off by a part of
+// itself, which is all of the exponent where logits over T are beyond 2^24.
+__device__ __forceinline__ float2 joined(float2 a, float2 b, float scale) {
   if (b.y == 0.0f) return a;
   if (a.y == 0.0f) return b;
   const float top = fmaxf(a.x, b.x);
-  return make_float2(top, a.y * __builtin_amdgcn_exp2f(a.x - top) +
-                              b.y * __builtin_amdgcn_exp2f(b.x - top));
+  return make_float2(top, a.y * __builtin_amdgcn_exp2f((a.x - top) * scale) +
+                              b.y * __builtin_amdgcn_exp2f((b.x - top) * scale));
 }
 
 // What the forward leaves for the backward. Row indices m count the rows that
@@ -107,7 +110,7 @@ struct Saved {
   float* share;     // [N][K]  p (by i)
   float* target;    // [N][K]  b at that token: the sum of p over equal tokens (by i)
   float* base;      // [N]     sum p log p (by i)
-  float* lse2;      // [pad]   log2 sum exp (by m)
+  float* lse;       // [pad]   T log sum exp(z / T), never below the maximum of z (by m)
   float* logit;     // [pad][K] z at the target tokens (by m)
   uint16_t* hidden; // [pad][C] the rows that take part, zeros after the last up to a tile
 };
@@ -128,7 +131,7 @@ Saved saved_of(char* p, int64_t n, int64_t c, int64_t k, size_t* bytes) {
   const size_t count = l.take(4), cut = l.take(4), done = l.take(4);
   const size_t row = l.take(pad * 4), place = l.take(n * 4), part = l.take(n * 4);
   const size_t index = l.take(n * k * 4), share = l.take(n * k * 4);
-  const size_t target = l.take(n * k * 4), base = l.take(n * 4), lse2 = l.take(pad * 4);
+  const size_t target = l.take(n * k * 4), base = l.take(n * 4), lse = l.take(pad * 4);
   const size_t logit = l.take(pad * k * 4), hidden = l.take(pad * c * 2);
   s.count = reinterpret_cast<int32_t*>(p + count);
   s.cut = reinterpret_cast<int32_t*>(p + cut);
@@ -140,7 +143,7 @@ Saved saved_of(char* p, int64_t n, int64_t c, int64_t k, size_t* bytes) {
   s.share = reinterpret_cast<float*>(p + share);
   s.target = reinterpret_cast<float*>(p + target);
   s.base = reinterpret_cast<float*>(p + base);
-  s.lse2 = reinterpret_cast<float*>(p + lse2);
+  s.lse = reinterpret_cast<float*>(p + lse);
   s.logit = reinterpret_cast<float*>(p + logit);
   s.hidden = reinterpret_cast<uint16_t*>(p + hidden);
   *bytes = l.bytes;
@@ -567,8 +570,8 @@ __device__ __forceinline__ int own_row(int token, int p0, int left) {
   return token >= 0 && at < left && row >= 0 && row < 16 * G::TP && (row & 15) < 4 ? row : -1;
 }
 
-// D[v][m] of a vocabulary range: per tile of v and row m the maximum of
-// s z log2 e and the sum of 2^(s z log2 e - maximum), to part[tile][m]. one: rows
+// D[v][m] of a vocabulary range: per tile of v and row m the maximum of z and
+// the sum of 2^(scale (z - maximum)), scale = s log2 e, to part[tile][m]. one: rows
 // have one target each, whose logit goes to s.logit as it stands here, so that
 // it cancels against a maximum that it is.
 // Bound by the matrix units for many rows (8192 x 65536 x 4096 bf16: 3.30 ms, 1331
@@ -638,7 +641,7 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void lse_tiles_kernel(
         for (int r = 0; r < 4; ++r) top = fmaxf(top, tile.acc[i][j][r]);
       }
       top = fmaxf(top, __shfl_xor(top, 16, 64));
-      top = fmaxf(top, __shfl_xor(top, 32, 64)) * scale;
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
       // -inf everywhere (columns beyond the vocabulary): a sum of 0, not NaN.
       const float from = top == -__builtin_inff() ? 0.0f : top;
       float sum = 0.0f;
@@ -646,7 +649,7 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void lse_tiles_kernel(
       for (int i = 0; i < G::TP; ++i) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          sum += __builtin_amdgcn_exp2f(fmaf(tile.acc[i][j][r], scale, -from));
+          sum += __builtin_amdgcn_exp2f((tile.acc[i][j][r] - from) * scale);
         }
       }
       sum += __shfl_xor(sum, 16, 64);
@@ -678,7 +681,7 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void lse_tiles_kernel(
 #pragma unroll
       for (int x = 0; x < G::kWP; ++x) {
         const float s = sums[x][q];
-        if (s != 0.0f) sum += s * __builtin_amdgcn_exp2f(maxima[x][q] - top);
+        if (s != 0.0f) sum += s * __builtin_amdgcn_exp2f((maxima[x][q] - top) * scale);
       }
       part[to + q] = make_float2(top, sum);
     }
@@ -686,8 +689,8 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void lse_tiles_kernel(
   }
 }
 
-// D[v][m] of a piece of the vocabulary: dz[m][v] = coef_m (2^(s z log2 e -
-// lse2_m)), zero for rows and columns that are not there. Bound as the forward is:
+// D[v][m] of a piece of the vocabulary: dz[m][v] = coef_m 2^(scale (z - lse_m)),
+// zero for rows and columns that are not there. Bound as the forward is:
 // 8192 x 32768 x 4096 in 1.69 ms, 1304 TFLOP/s.
 //
 // Twice: rounding dz to 16 bits is one error for all elements that a target
@@ -723,7 +726,7 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void softmax_grad_kernel(
 #pragma unroll
     for (int j = 0; j < G::TQ; ++j) {
       const int m = q0 + G::column(j);
-      from[j] = m < rows ? s.lse2[m] : 0.0f;
+      from[j] = m < rows ? s.lse[m] : 0.0f;
       co[j] = m < rows ? coef[m] : 0.0f;
     }
     tile.multiply(smem);
@@ -752,7 +755,7 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void softmax_grad_kernel(
         float x[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          x[r] = co[j] * __builtin_amdgcn_exp2f(fmaf(tile.acc[i][j][r], scale, -from[j]));
+          x[r] = co[j] * __builtin_amdgcn_exp2f((tile.acc[i][j][r] - from[j]) * scale);
           if (!all) x[r] = here && G::row(i) + r < left ? x[r] : 0.0f;
         }
         out[i] = make_uint2(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]));
@@ -792,7 +795,7 @@ __global__ __launch_bounds__(256) void target_grad_kernel(int32_t k, int32_t voc
   const int64_t at = static_cast<int64_t>(s.row[m]) * k + (e - m * k);
   const int32_t v = s.index[at] - vocab0;
   if (s.index[at] < 0 || v < 0 || v >= columns) return;
-  const float p = __builtin_amdgcn_exp2f(fmaf(s.logit[e], scale, -s.lse2[m]));
+  const float p = __builtin_amdgcn_exp2f((s.logit[e] - s.lse[m]) * scale);
   const float x = coef[m] * (p - s.target[at]);
   const uint16_t rounded = from_f32<T>(x);
   dz[m * ld + v] = rounded;
@@ -993,7 +996,7 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void weight_grad_kernel(
 
 // -------------------------------------------------------- row reductions
 // A workgroup takes 32 rows, 32 threads a row: joins the tiles' maxima and
-// sums to lse2[m], and the row's loss, to row_loss (by i) or into the sum of all
+// sums to lse[m], and the row's loss, to row_loss (by i) or into the sum of all
 // rows. A thread has 8 tiles under way at a time, all of those of 65536 columns.
 // In the loss the target logits are taken from the row's maximum, a difference
 // that is exact where they are close, and not from lse, whose rounding alone
@@ -1004,7 +1007,7 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void weight_grad_kernel(
 __global__ __launch_bounds__(1024) void join_tiles_kernel(const float2* __restrict__ part,
                                                           int32_t vocab, int32_t rest_tile,
                                                           int64_t pad, int32_t k, float scale,
-                                                          float temperature2, bool mean,
+                                                          float temperature, bool mean,
                                                           float* row_loss, float* loss,
                                                           float* partial, Saved s) {
   __shared__ float2 shared[32][33];
@@ -1029,7 +1032,7 @@ __global__ __launch_bounds__(1024) void join_tiles_kernel(const float2* __restri
                                   : make_float2(-__builtin_inff(), 0.0f);
       }
 #pragma unroll
-      for (int u = 0; u < 8; ++u) all = joined(all, x[u]);
+      for (int u = 0; u < 8; ++u) all = joined(all, x[u], scale);
     }
   }
   shared[q][slice] = all;
@@ -1039,7 +1042,8 @@ __global__ __launch_bounds__(1024) void join_tiles_kernel(const float2* __restri
   all = shared[row][lane];
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
-    all = joined(all, make_float2(__shfl_xor(all.x, off, 64), __shfl_xor(all.y, off, 64)));
+    all = joined(all, make_float2(__shfl_xor(all.x, off, 64), __shfl_xor(all.y, off, 64)),
+                 scale);
   }
   // The lanes' orders differ: the first one's result.
   const float top = __shfl(all.x, threadIdx.x & 32, 64);
@@ -1051,7 +1055,7 @@ __global__ __launch_bounds__(1024) void join_tiles_kernel(const float2* __restri
     for (int j = lane; j < k; j += 32) {
       const float p = s.share[i * k + j], z = s.logit[static_cast<int64_t>(mine) * k + j];
       // Absent entries have p = 0; one out of range has z = NaN.
-      if (p != 0.0f || z != z) term = fmaf(p, fmaf(-z, scale, top), term);
+      if (p != 0.0f || z != z) term = fmaf(p, (top - z) * scale, term);
     }
   }
 #pragma unroll
@@ -1061,8 +1065,9 @@ __global__ __launch_bounds__(1024) void join_tiles_kernel(const float2* __restri
     if (mine < count) {
       const float log_sum = __builtin_amdgcn_logf(all.y);
       // A target out of range makes its row NaN in the backward too.
-      s.lse2[mine] = term == term ? top + log_sum : term;
-      value = temperature2 * ((term + log_sum) * kLn2 + s.base[i]);
+      s.lse[mine] = term == term ? top + log_sum / scale : term;
+      // T twice: T^2 by itself can be beyond fp32.
+      value = temperature * (temperature * ((term + log_sum) * kLn2 + s.base[i]));
       if (row_loss != nullptr) row_loss[i] = value;
     }
     losses[row] = value;
@@ -1328,7 +1333,7 @@ int run_forward(const Shape& d, const Source& source, const void* hidden, const 
   });
   hipLaunchKernelGGL(join_tiles_kernel, dim3((d.n + 31) / 32), dim3(1024), 0, stream, w.part,
                      d.vocab, time_of(size_of(d.vocab, d.n)).p, pad, d.k, scale,
-                     temperature * temperature, reduction == FRWKV_REDUCE_MEAN, row_loss,
+                     temperature, reduction == FRWKV_REDUCE_MEAN, row_loss,
                      row_loss == nullptr ? loss : nullptr, w.partial, s);
   return check_launch("linear loss forward");
 }

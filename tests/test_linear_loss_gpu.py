@@ -572,3 +572,18 @@ def test_a_row_weight_beyond_the_others_range_stays_with_its_row(bad, dtype):
     entry = head.labels(targets[keep], 300, -100)
     _check(h[keep], w, entry, (loss[keep], dh[keep], None), row_weight=upstream[keep],
            reduction="none")
+
+
+@pytest.mark.parametrize("t", [1e-25, 1e25])
+def test_losses_at_extreme_temperatures_neither_vanish_nor_overflow(t):
+    """The loss is of the size of T at a small T; one token has the loss 0 at a
+    large T, whose square is beyond fp32. Logits are whole numbers apart."""
+    h = torch.zeros(3, 64, dtype=torch.bfloat16, device=DEV)
+    w = torch.zeros(4 if t < 1 else 1, 64, dtype=torch.bfloat16, device=DEV)
+    h[:, 0] = 1
+    w[:, 0] = torch.arange(w.shape[0], device=DEV)
+    tokens = torch.zeros(3, 1, dtype=torch.int64, device=DEV)
+    loss = pretrain_linear_topk_distillation(h, w, torch.zeros(3, 1, device=DEV), tokens,
+                                             temperature=t, reduction="none")
+    want = 3 * t if t < 1 else 0.0
+    assert ((loss.double() - want).abs() <= 1e-5 * want).all(), loss
