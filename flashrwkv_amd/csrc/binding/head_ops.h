@@ -119,14 +119,15 @@ std::tuple<Tensor, Tensor> linear_cross_entropy_forward(Tensor hidden, Tensor we
   const auto fp32 = hidden.options().dtype(at::kFloat);
   Tensor loss = reduction == FRWKV_REDUCE_NONE ? at::empty(targets.sizes(), fp32)
                                                : at::empty({}, fp32);
+  // Sizes that the call refuses have no bytes; its error says why.
   const size_t saved_bytes = frwkv_linear_loss_saved_bytes(rows, c, 1);
   const size_t work_bytes = frwkv_linear_loss_forward_workspace_bytes(rows, vocab);
   Tensor saved = workspace_like(hidden, saved_bytes), work = workspace_like(hidden, work_bytes);
   check_rc(frwkv_linear_cross_entropy_forward(
       io_code(hidden.scalar_type()), rows, c, vocab, hidden.const_data_ptr(),
       weight.const_data_ptr(), bytes, targets.const_data_ptr(), ignore_index,
-      static_cast<int>(reduction), loss.data_ptr<float>(), saved.data_ptr(), saved_bytes,
-      work.data_ptr(), work_bytes, current_stream(hidden)));
+      static_cast<int>(reduction), loss.data_ptr<float>(), scratch_ptr(saved), saved_bytes,
+      scratch_ptr(work), work_bytes, current_stream(hidden)));
   return {loss, saved};
 }
 
@@ -159,7 +160,7 @@ std::tuple<Tensor, Tensor> linear_topk_distillation_forward(Tensor hidden, Tenso
       weight.const_data_ptr(), io_code(teacher_logits.scalar_type()),
       teacher_logits.const_data_ptr(), bytes, teacher_indices.const_data_ptr(),
       static_cast<float>(temperature), static_cast<int>(reduction), loss.data_ptr<float>(),
-      saved.data_ptr(), saved_bytes, work.data_ptr(), work_bytes, current_stream(hidden)));
+      scratch_ptr(saved), saved_bytes, scratch_ptr(work), work_bytes, current_stream(hidden)));
   return {loss, saved};
 }
 

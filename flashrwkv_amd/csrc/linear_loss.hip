@@ -167,14 +167,15 @@ __host__ __device__ constexpr TileTime time_of(Size s) {
                                  : TileTime{256, 256, 1.65f, 5.0f};
 }
 
-// Fewer than 2^30 tiles, checked at the entry points.
-__host__ __device__ inline int32_t tiles_of(Size s, int32_t p, int32_t q) {
+// kSmall's are fewer than 2^30, checked at the entry points; the narrow ones that
+// size_of counts before it takes them can be four times as many.
+__host__ __device__ inline int64_t tiles_of(Size s, int32_t p, int32_t q) {
   const TileTime t = time_of(s);
-  return (p + t.p - 1) / t.p * ((q + t.q - 1) / t.q);
+  return static_cast<int64_t>((p + t.p - 1) / t.p) * ((q + t.q - 1) / t.q);
 }
 
 __host__ __device__ inline float product_us(Size s, int32_t p, int32_t q, int32_t steps) {
-  const int32_t rounds = (tiles_of(s, p, q) + kCus - 1) / kCus;
+  const int64_t rounds = (tiles_of(s, p, q) + kCus - 1) / kCus;
   return static_cast<float>(rounds) *
          (static_cast<float>(steps) * time_of(s).step_us + time_of(s).fixed_us);
 }
@@ -203,8 +204,8 @@ __host__ __device__ inline Cut cut_of(int32_t vocab, int32_t across, int32_t ste
   if (!sizes.small) return {vocab, large};
   const float small = product_us(Size::kSmall, vocab, across, steps);
   Cut best = small < large ? Cut{0, small} : Cut{vocab, large};
-  const int32_t full = tiles_of(Size::kLarge, vocab, across) / kCus * kCus;
-  const int32_t first = full / ((across + 255) / 256) * 256;
+  const int64_t full = tiles_of(Size::kLarge, vocab, across) / kCus * kCus;
+  const int32_t first = static_cast<int32_t>(full / ((across + 255) / 256) * 256);
   if (first > 0 && first < vocab) {
     const float both = product_us(Size::kLarge, first, across, steps) +
                        product_us(Size::kSmall, vocab - first, across, steps) + 3.0f;
@@ -1260,7 +1261,7 @@ struct Shape {
   int32_t n, c, vocab, k;
 };
 
-int grid_of(int32_t tiles) { return std::min(tiles, kCus); }
+int grid_of(int64_t tiles) { return static_cast<int>(std::min<int64_t>(tiles, kCus)); }
 
 // f(tile type) for a size.
 template <typename T, Major MA, Major MB, typename F>
@@ -1422,6 +1423,17 @@ constexpr int64_t kMostTargets = 1024;
 
 bool within(int64_t x, int64_t most) { return x > 0 && x <= most; }
 
+// What one call takes of rows, channels, vocabulary and targets a row together.
+bool sizes_fit(int64_t n, int64_t c, int64_t vocab, int64_t k) {
+  if (!within(n, kMostRows) || !within(c, kMostChannels) || c % gemm::kStep != 0 ||
+      !within(vocab, kMostVocab) || !within(k, kMostTargets)) {
+    return false;
+  }
+  const int64_t tile = time_of(Size::kSmall).p;  // of the most tiles a product is cut into
+  const int64_t tiles = round_up(vocab, tile) / tile * (round_up(n, tile) / tile);
+  return tiles < (int64_t{1} << 30) && n * k < (int64_t{1} << 31);
+}
+
 int check_shape(const char* what, int io_dtype, int64_t n, int64_t c, int64_t vocab, int64_t k) {
   if (io_dtype != FRWKV_DTYPE_F16 && io_dtype != FRWKV_DTYPE_BF16) {
     return set_error(FRWKV_ERR_UNSUPPORTED, "%s: io dtype must be float16 or bfloat16", what);
@@ -1444,9 +1456,7 @@ int check_shape(const char* what, int io_dtype, int64_t n, int64_t c, int64_t vo
                      "%s: targets of a row must be in [1, 1024], got %lld", what,
                      static_cast<long long>(k));
   }
-  const int64_t tile = time_of(Size::kSmall).p;  // of the most tiles there can be
-  const int64_t tiles = round_up(vocab, tile) / tile * (round_up(n, tile) / tile);
-  if (tiles >= (int64_t{1} << 30) || n * k >= (int64_t{1} << 31)) {
+  if (!sizes_fit(n, c, vocab, k)) {
     return set_error(FRWKV_ERR_UNSUPPORTED,
                      "%s: rows x vocabulary or rows x targets too large for one call", what);
   }
@@ -1525,9 +1535,7 @@ extern "C" {
 
 size_t frwkv_linear_loss_saved_bytes(int64_t rows, int64_t channels, int64_t top) {
   using namespace frwkv;
-  if (!within(rows, kMostRows) || !within(channels, kMostChannels) || !within(top, kMostTargets)) {
-    return 0;
-  }
+  if (!sizes_fit(rows, channels, 1, top)) return 0;
   size_t bytes = 0;
   (void)frwkv::saved_of(nullptr, rows, channels, top, &bytes);
   return bytes;
@@ -1535,7 +1543,7 @@ size_t frwkv_linear_loss_saved_bytes(int64_t rows, int64_t channels, int64_t top
 
 size_t frwkv_linear_loss_forward_workspace_bytes(int64_t rows, int64_t vocab) {
   using namespace frwkv;
-  if (!within(rows, kMostRows) || !within(vocab, kMostVocab)) return 0;
+  if (!sizes_fit(rows, gemm::kStep, vocab, 1)) return 0;
   size_t bytes = 0;
   (void)frwkv::forward_work(nullptr, rows, vocab, &bytes);
   return bytes;
@@ -1544,10 +1552,7 @@ size_t frwkv_linear_loss_forward_workspace_bytes(int64_t rows, int64_t vocab) {
 size_t frwkv_linear_loss_backward_workspace_bytes(int64_t rows, int64_t channels, int64_t vocab,
                                                   int want_grad_hidden) {
   using namespace frwkv;
-  if (!within(rows, kMostRows) || !within(channels, kMostChannels) ||
-      !within(vocab, kMostVocab)) {
-    return 0;
-  }
+  if (!sizes_fit(rows, channels, vocab, 1)) return 0;
   size_t bytes = 0;
   (void)frwkv::backward_work(nullptr, rows, channels, frwkv::plan_of(rows, channels, vocab),
                              want_grad_hidden != 0, &bytes);

@@ -680,7 +680,8 @@ int frwkv_layer_norm_backward(int io_dtype, int64_t rows, int64_t channels, cons
  * through the vocabulary in pieces whose logit gradients (16 bits) fit the
  * workspace. All sums are in a fixed order. Both directions need at least one
  * row. The byte queries give 0 for sizes that the calls refuse: more than 2^23
- * rows, 65536 channels, 2^28 tokens or 1024 targets a row. No counterpart in the
+ * rows, 65536 channels (or no multiple of 64), 2^28 tokens, 1024 targets a row, 2^44
+ * rows x tokens (in tiles of 128) or 2^31 rows x targets. No counterpart in the
  * reference.
  */
 size_t frwkv_linear_loss_saved_bytes(int64_t rows, int64_t channels, int64_t top);

@@ -201,3 +201,14 @@ def test_c_abi_rejects_bad_loss_calls_without_a_gpu():
     assert lib.frwkv_linear_loss_backward(2, n, c, v, 1, p, 1.0, 1, p, p, saved, p, p, p,
                                           back - 1, null) == 1
     assert b"workspace of" in _last()
+
+
+def test_byte_queries_count_tiles_beyond_32_bits_and_give_0_for_refused_products():
+    lib = capi.library()
+    n, v = 1 << 16, 1 << 27  # 2^31 tiles of 64 x 64, 2^29 of 128 x 128
+    assert lib.frwkv_linear_loss_forward_workspace_bytes(n, v) == (v // 128) * n * 8 + n // 32 * 4
+    assert lib.frwkv_linear_loss_forward_workspace_bytes(1 << 22, 1 << 24) == 0
+    assert lib.frwkv_linear_loss_backward_workspace_bytes(1 << 22, 64, 1 << 24, 1) == 0
+    assert lib.frwkv_linear_loss_backward_workspace_bytes(300, 100, 1000, 1) == 0
+    assert lib.frwkv_linear_loss_saved_bytes(1 << 22, 64, 1024) == 0
+    assert lib.frwkv_linear_loss_saved_bytes(300, 100, 1) == 0

@@ -587,3 +587,15 @@ def test_losses_at_extreme_temperatures_neither_vanish_nor_overflow(t):
                                              temperature=t, reduction="none")
     want = 3 * t if t < 1 else 0.0
     assert ((loss.double() - want).abs() <= 1e-5 * want).all(), loss
+
+
+def test_more_rows_than_a_call_takes_are_refused_with_their_count():
+    """Before anything is allocated for them."""
+    n = 2 ** 23 + 1
+    h = torch.zeros(n, 64, dtype=torch.bfloat16, device=DEV)
+    w = torch.zeros(2, 64, dtype=torch.bfloat16, device=DEV)
+    targets = torch.zeros(n, dtype=torch.int32, device=DEV)
+    with pytest.raises(RuntimeError, match=r"rows must be in \[1, 2\^23\], got 8388609"):
+        pretrain_linear_cross_entropy(h, w, targets, reduction="sum")
+    with pytest.raises(RuntimeError, match=r"rows must be in \[1, 2\^23\], got 8388609"):
+        pretrain_linear_topk_distillation(h, w, torch.zeros(n, 1, device=DEV), targets[:, None])
