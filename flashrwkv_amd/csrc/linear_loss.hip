@@ -24,8 +24,9 @@
 // Backward, for one piece of the vocabulary after another: the product again,
 // its epilogue turning logits into dz of the piece (16 bits, [rows][piece]);
 // the target entries are overwritten from the fp32 target logits, so that
-// p - b does not lose digits where the two are close; then dz W into an fp32
-// slab (its sum over slabs, in order, is dh) and dz^T h, which is dW's rows.
+// p - b does not lose digits where the two are close; then dz W into fp32 slabs,
+// one a split of it, to which each piece adds (their sum, in order, is dh), and
+// dz^T h, which is dW's rows.
 // Everything is summed in fp32 in a fixed order; dz is the only rounding to
 // 16 bits before the outputs, as a matrix operand has to be (relative error at
 // most 2^-8 an entry for bf16, independent between entries).
@@ -814,7 +815,7 @@ struct Splitting {
   int32_t across; // tiles over C
   int32_t tile;   // rows of a tile
   float step_us, fixed_us, row_slab_us;
-  int64_t room;   // rows of all slabs of a piece
+  int64_t room;   // rows of all slabs
 };
 
 __host__ __device__ inline float split_us(const Splitting& x, int64_t rows, int32_t s) {
@@ -862,13 +863,14 @@ struct Pieces {
 };
 
 // D[c][m] = sum over a split's vocabulary of W[v][c] dz[m][v], to slab [m][c]
-// of the split (fp32). Bound by the matrix units: 8192 x 32768 x 4096 in 1.64 ms, 1344
+// of the split (fp32), added to what the pieces before left there: they run one
+// after the other, and every element has one owner in each. Bound by the matrix units: 8192 x 32768 x 4096 in 1.64 ms, 1344
 // TFLOP/s, in one split.
 template <typename G, typename T>
 __global__ __launch_bounds__(gemm::kThreads, 2) void hidden_grad_kernel(
     Operand w, Operand dz, const int32_t* __restrict__ count,
     const int32_t* __restrict__ split_count, int32_t steps, int32_t whole_steps, int32_t np,
-    int32_t piece, int32_t c, bool twice, float* __restrict__ slabs) {
+    bool add, int32_t c, bool twice, float* __restrict__ slabs) {
   __shared__ __attribute__((aligned(1024))) char smem[G::kLdsBytes];
   const int rows = *count;
   const int splits = *split_count;
@@ -893,7 +895,7 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void hidden_grad_kernel(
   while (true) {
     tile.multiply(smem);
     const int p0 = tp * G::kBP, q0 = tq * G::kBQ;
-    float* out = slabs + (static_cast<int64_t>(piece) * splits + split) * slab;
+    float* out = slabs + split * slab;
     id += gridDim.x;
     if (id < total) {
       begin();
@@ -914,12 +916,16 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void hidden_grad_kernel(
     for (int j = 0; j < G::TQ; ++j) {
       const int m = q0 + G::column(j);
       if (m >= rows) continue;
+      f32x4* to = reinterpret_cast<f32x4*>(out + static_cast<int64_t>(m) * c + p0 + G::row(0));
+      if (add) {
+#pragma unroll
+        for (int i = 0; i < G::TP; ++i) {
+          if (p0 + G::row(i) < c) tile.acc[i][j] += to[4 * i];
+        }
+      }
 #pragma unroll
       for (int i = 0; i < G::TP; ++i) {
-        const int x = p0 + G::row(i);
-        if (x < c) {
-          *reinterpret_cast<f32x4*>(out + static_cast<int64_t>(m) * c + x) = tile.acc[i][j];
-        }
+        if (p0 + G::row(i) < c) to[4 * i] = tile.acc[i][j];
       }
     }
     if (id >= total) return;
@@ -932,10 +938,10 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void hidden_grad_kernel(
 template <typename T>
 __global__ __launch_bounds__(256) void hidden_grad_rows_kernel(
     const float* __restrict__ slabs, const int32_t* __restrict__ rows,
-    const int32_t* __restrict__ split_count, int32_t pieces, int32_t c, int64_t n,
+    const int32_t* __restrict__ split_count, int32_t c, int64_t n,
     const float* __restrict__ scale, const int32_t* __restrict__ place, uint16_t* __restrict__ dh) {
   const int64_t quads = n * (c / 4), slab = static_cast<int64_t>(*rows) * c;
-  const int count = pieces * *split_count;
+  const int count = *split_count;
   const float by = *scale;
   for (int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; e < quads;
        e += static_cast<int64_t>(gridDim.x) * 256) {
@@ -1154,7 +1160,8 @@ struct Plan {
 // dz of a piece up to kCachedBytes is written and read in the last-level cache;
 // beyond, its traffic is partly hidden by the products (4096 x 65536 x 2048 in
 // pieces of 128, 256 and 512 MB: 2612, 2700, 2675 us; 8192 x 65536 x 4096, whose
-// slabs weigh more: 9784, 9749, 9715 us). A slab is written once and read once.
+// slabs weigh more: 9784, 9749, 9715 us). A slab is written in each piece and read
+// once after it.
 constexpr int64_t kCachedBytes = int64_t{192} << 20;
 constexpr int64_t kMostBytes = int64_t{512} << 20;
 constexpr double kGradBytesPerUs = 20.0e6;
@@ -1212,7 +1219,7 @@ Plan plan_of(int64_t n, int64_t c, int64_t vocab) {
   return best;
 }
 
-// Rows of a piece's slabs: a slab more than all rows want, so that a part of the
+// Rows of the slabs: a slab more than all rows want, so that a part of the
 // rows, which want more splits, can have them.
 int64_t slab_rows(const Plan& plan, int64_t n) {
   return plan.splits == 1 ? n : (plan.splits + 1) * n;
@@ -1250,7 +1257,7 @@ BackwardWork backward_work(char* p, int64_t n, int64_t c, const Plan& plan, bool
   const size_t cuts = l.take(8);
   const size_t dz = l.take(pad * plan.columns * 2);
   const size_t slabs =
-      l.take(hidden ? static_cast<size_t>(plan.pieces) * slab_rows(plan, n) * c * 4 : 0);
+      l.take(hidden ? static_cast<size_t>(slab_rows(plan, n)) * c * 4 : 0);
   *bytes = l.bytes;
   return {reinterpret_cast<float*>(p + coef), reinterpret_cast<float*>(p + scale),
           reinterpret_cast<int32_t*>(p + splits), reinterpret_cast<int32_t*>(p + cuts),
@@ -1367,7 +1374,7 @@ void launch_piece(const Shape& d, const Plan& plan, int piece, const uint16_t* w
       using G = std::remove_pointer_t<decltype(tile)>;
       hipLaunchKernelGGL((hidden_grad_kernel<G, T>), dim3(kCus), dim3(gemm::kThreads), 0, stream,
                          wp, dz, s.count, w.splits, steps, plan.columns / gemm::kStep,
-                         (d.c + G::kBP - 1) / G::kBP, piece, d.c, twice, w.slabs);
+                         (d.c + G::kBP - 1) / G::kBP, piece > 0, d.c, twice, w.slabs);
     });
   }
   if (dw != nullptr) {
@@ -1410,8 +1417,8 @@ int run_backward(const Shape& d, const void* weight, const float* upstream, bool
     const int64_t quads = static_cast<int64_t>(d.n) * (d.c / 4);
     const int64_t blocks = std::min<int64_t>((quads + 255) / 256, 8192);
     hipLaunchKernelGGL((hidden_grad_rows_kernel<T>), dim3(static_cast<unsigned>(blocks)),
-                       dim3(256), 0, stream, w.slabs, s.count, w.splits, plan.pieces,
-                       d.c, d.n, w.scale, s.place, static_cast<uint16_t*>(dh));
+                       dim3(256), 0, stream, w.slabs, s.count, w.splits, d.c, d.n,
+                       w.scale, s.place, static_cast<uint16_t*>(dh));
   }
   return check_launch("linear loss backward");
 }

@@ -212,3 +212,27 @@ def test_byte_queries_count_tiles_beyond_32_bits_and_give_0_for_refused_products
     assert lib.frwkv_linear_loss_backward_workspace_bytes(300, 100, 1000, 1) == 0
     assert lib.frwkv_linear_loss_saved_bytes(1 << 22, 64, 1024) == 0
     assert lib.frwkv_linear_loss_saved_bytes(300, 100, 1) == 0
+
+
+@pytest.mark.parametrize("c,v", [(4096, 65536), (1024, 4096), (64, 300), (2560, 200003)])
+def test_backward_workspace_grows_with_rows_and_not_with_their_square(c, v):
+    """dz of a piece: 512 MB, or 256 columns of all rows where that is more; fp32 slabs
+    of the hidden gradient: one, or one more than the splits of a piece (at most 16).
+    Splits are for products that do not fill the GPU: not for many rows."""
+    lib = capi.library()
+    for n in (1, 100, 4000, 8192, 30000, 65536, 131072, 262144, 1 << 20, 1 << 23):
+        pad = (n + 255) // 256 * 256
+        dz = max(512 << 20, pad * 512)
+        rows = pad * 4 + 4096
+        without = lib.frwkv_linear_loss_backward_workspace_bytes(n, c, v, 0)
+        slabs = lib.frwkv_linear_loss_backward_workspace_bytes(n, c, v, 1) - without
+        assert 0 < without <= dz + rows
+        assert n * c * 4 <= slabs <= 17 * n * c * 4 + 256
+        if n >= 65536:
+            assert slabs <= 4 * n * c * 4 + 256
+
+
+def test_backward_workspace_is_less_than_the_logits_it_avoids():
+    lib = capi.library()
+    for n in (8192, 32768, 65536, 131072, 262144):
+        assert lib.frwkv_linear_loss_backward_workspace_bytes(n, 4096, 65536, 1) < n * 65536 * 2

@@ -599,3 +599,23 @@ def test_more_rows_than_a_call_takes_are_refused_with_their_count():
         pretrain_linear_cross_entropy(h, w, targets, reduction="sum")
     with pytest.raises(RuntimeError, match=r"rows must be in \[1, 2\^23\], got 8388609"):
         pretrain_linear_topk_distillation(h, w, torch.zeros(n, 1, device=DEV), targets[:, None])
+
+
+@pytest.mark.parametrize("n,c,v,masked", [(16500, 128, 20011, 0.0), (17001, 320, 20300, 0.6)])
+def test_many_rows_in_several_pieces(n, c, v, masked):
+    """Each piece of the vocabulary adds to the slabs of the hidden gradient that the
+    pieces before it left; the last piece is ragged, and so is the last row tile."""
+    h, w = _head(n, c, v, torch.bfloat16, seed=50 + n)
+    targets = torch.randint(v, (n,), generator=_gen(n))
+    targets[torch.rand(n, generator=_gen(n + 1)) < masked] = -100
+    targets = targets.to(DEV)
+    upstream = _upstream("none", n, seed=n + 2)
+
+    def call(a, b):
+        return pretrain_linear_cross_entropy(a, b, targets, reduction="none")
+
+    got = _grads(call, h, w, upstream)
+    _check(h, w, head.labels(targets, v, -100), got, row_weight=upstream, reduction="none")
+    assert all(torch.equal(a, b) for a, b in zip(got, _grads(call, h, w, upstream)))
+    frozen = _grads(call, h, w, upstream, weight=False)
+    assert torch.equal(frozen[1], got[1])
