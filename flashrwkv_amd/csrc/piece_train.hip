@@ -323,11 +323,13 @@ __device__ __forceinline__ void piece_rows_to_lds(RowStage& st, const TrainParam
       // LDS access after these loads: the staging area is only read after
       // the column phase's explicit vmcnt(0) wait and the barriers after it.
       // M0 holds the load's LDS base; the block saves and restores it, so a
-      // value the compiler keeps in M0 survives.
+      // value the compiler keeps in M0 survives. A load to LDS reads M0 one wait
+      // state after its write at the earliest.
       uint32_t m0_saved;
       asm volatile(
           "s_mov_b32 %0, m0\n\t"
           "s_mov_b32 m0, %3\n\t"
+          "s_nop 0\n\t"
           "buffer_load_dwordx4 %1, %2, 0 offen lds\n\t"
           "s_mov_b32 m0, %0"
           : "=&s"(m0_saved)

@@ -32,6 +32,16 @@ def test_assembly_that_writes_m0_gives_its_value_back(path):
         assert lines[-1] == f"s_mov_b32 m0, {saved.group(1)}", lines
 
 
+@pytest.mark.parametrize("path", SOURCES, ids=lambda p: p.name)
+def test_loads_to_lds_wait_for_m0(path):
+    """One wait state between a write of m0 and a load to LDS, which the compiler
+    keeps by itself and assembly has to."""
+    for lines in _blocks(path.read_text()):
+        for before, line in zip(lines, lines[1:]):
+            if line.endswith(" lds"):
+                assert not re.match(r"s_\w+ m0,", before), lines
+
+
 def test_the_scan_finds_blocks_and_would_see_a_lost_value():
     blocks = [b for p in SOURCES for b in _blocks(p.read_text())]
     assert sum(any("m0" in line for line in b) for b in blocks) >= 2
