@@ -70,18 +70,16 @@ struct Operand {
 // adds lane * 16 to the address in m0, which is wave-uniform, and writes zeros
 // for lanes whose offset lies beyond the buffer. In asm because the compiler,
 // unable to tell the stages apart, puts a wait for the whole queue before every
-// LDS read that follows the builtin. The block saves and restores m0, so a value that
-// the compiler keeps there survives (the register cannot be declared as written).
+// LDS read that follows the builtin. The compiler writes m0 itself, as the block's
+// operand, so it knows what stands there (saved and restored in the block, as a
+// register that cannot be declared as written, the small tiles were 2% slower); a
+// load reads m0 one wait state after its write at the earliest.
 __device__ __forceinline__ void load_to_lds(u32x4 buffer, uint32_t offset, uint32_t lds) {
-  uint32_t m0_saved;
   asm volatile(
-      "s_mov_b32 %0, m0\n\t"
-      "s_mov_b32 m0, %3\n\t"
       "s_nop 0\n\t"
-      "buffer_load_dwordx4 %1, %2, 0 offen lds\n\t"
-      "s_mov_b32 m0, %0"
-      : "=&s"(m0_saved)
-      : "v"(offset), "s"(buffer), "s"(lds));
+      "buffer_load_dwordx4 %0, %1, 0 offen lds"
+      :
+      : "v"(offset), "s"(buffer), "{m0}"(lds));
 }
 
 // Waits until at most kLeft of this wave's loads are outstanding and its LDS
