@@ -47,7 +47,7 @@ using gemm::Operand;
 constexpr float kLn2 = 0.69314718055994531f;
 constexpr int kRowPad = 256;       // rows of workspaces, and a product's largest tile
 constexpr int kVocabTile = 256;    // pieces of the vocabulary are whole multiples of it
-constexpr int kFewest = 32;        // rows up to here: see Twice below
+constexpr int kFewest = 32;        // rows that take part up to here: see Twice below
 constexpr int kScanThreads = 1024;
 constexpr int kCus = 256;
 constexpr int kMostSplits = 16;
@@ -98,6 +98,14 @@ __device__ __forceinline__ float2 joined(float2 a, float2 b, float scale) {
                               b.y * __builtin_amdgcn_exp2f((b.x - top) * scale));
 }
 
+// Twice: where the two terms of row m of a few stand in dz, 16 rows' first terms
+// and then their second ones, so that a lane of any tile that holds the one holds
+// the other. The hidden rows stand in the same order from kTermRows on.
+constexpr int kTermRows = 2 * kFewest;
+__device__ __forceinline__ int term_row(int m, int term) {
+  return (m & 15) + 2 * (m & ~15) + 16 * term;
+}
+
 // What the forward leaves for the backward. Row indices m count the rows that
 // take part, in order; i is the row's place in the caller's tensors.
 struct Saved {
@@ -113,7 +121,8 @@ struct Saved {
   float* base;      // [N]     sum p log p (by i)
   float* lse;       // [pad]   T log sum exp(z / T), never below the maximum of z (by m)
   float* logit;     // [pad][K] z at the target tokens (by m)
-  uint16_t* hidden; // [pad][C] the rows that take part, zeros after the last up to a tile
+  uint16_t* hidden; // [pad][C] the rows that take part, zeros after the last up to a tile;
+                    // of a few also their term_row order, zeros between, from kTermRows on
 };
 
 struct Layout {
@@ -451,7 +460,7 @@ __device__ __forceinline__ bool own_number(const Source& source, int32_t n, int3
 }
 
 // Copies the hidden rows that take part together (zeros for the rows that fill up
-// the last tile; few rows a second time kFewest rows on) and computes their K > 1
+// the last tile; few rows once more for each term) and computes their K > 1
 // target logits, kGather a workgroup, a wave each (NaN for a token out of range).
 // blockIdx.x: a row i of the caller's, which the workgroup numbers itself (kOwn),
 // or a row m; blockIdx.y: the tokens.
@@ -464,7 +473,7 @@ constexpr int kGather = 4;
 template <typename T, bool kOwn, typename Source>
 __global__ __launch_bounds__(kGatherThreads) void gather_rows_kernel(
     const uint16_t* __restrict__ hidden, const uint16_t* __restrict__ weight, int32_t c,
-    int32_t k, bool twice, Source source, Rows d, Saved s) {
+    int32_t k, Source source, Rows d, Saved s) {
   const int block = blockIdx.x;
   const bool first = blockIdx.y == 0;
   if (!first && block >= d.n) return;
@@ -496,10 +505,16 @@ __global__ __launch_bounds__(kGatherThreads) void gather_rows_kernel(
   };
   const uint16_t* from = hidden + static_cast<int64_t>(i) * c;
   if (first) {
-    const bool copied = twice && block >= kFewest && block < kFewest + count;
+    const bool twice = count <= kFewest;
+    // term_row's inverse: the row whose copy stands in this one.
+    const int at = block - kTermRows;
+    const bool copied = twice && at >= 0 && at < kTermRows && (at & 15) + (at >> 5) * 16 < count;
     if (block >= count && block < round_up(count, kRowPad) && !copied) fill(block, nullptr);
     if (part) fill(m, from);
-    if (part && twice) fill(kFewest + m, from);
+    if (part && twice) {
+      fill(kTermRows + term_row(m, 0), from);
+      fill(kTermRows + term_row(m, 1), from);
+    }
   }
   if (!part) return;
   if (k == 1) {  // one out of range; lse_tiles_kernel writes the others
@@ -698,15 +713,15 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void lse_tiles_kernel(
 // Twice: rounding dz to 16 bits is one error for all elements that a target
 // entry dominates, up to 2^-9 of the entry 1 for bf16. Over many rows such
 // errors average out below the outputs' own rounding; in a few rows one can be
-// twice that. Up to kFewest rows leave half of a tile's columns unused, so there
-// dz has two terms, row m the rounded value and row kFewest + m what is left of
-// it, and the products add both at no cost (bf16 gradients of 3 weighted rows,
+// twice that. Up to kFewest rows that take part leave half of a tile's columns
+// unused, so there dz has two terms, the rounded value and what is left of it, and
+// the products add both at no cost (bf16 gradients of 3 weighted rows,
 // 3001 x 512: up to 3.8e-3 off with one term, 1.7e-3 with two, the outputs' own
 // rounding).
 template <typename G, typename T>
 __global__ __launch_bounds__(gemm::kThreads, 2) void softmax_grad_kernel(
     Operand w, Operand h, const int32_t* __restrict__ cut, int32_t c, float scale,
-    const float* __restrict__ coef, bool twice, uint16_t* __restrict__ dz, int64_t ld, Saved s) {
+    const float* __restrict__ coef, uint16_t* __restrict__ dz, int64_t ld, Saved s) {
   __shared__ __attribute__((aligned(1024))) char smem[G::kLdsBytes];
   int at;
   own_columns<G>(cut, at, w.rows);
@@ -743,39 +758,44 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void softmax_grad_kernel(
     }
     const int left = w.rows - p0;
     const bool all = left >= G::kBP && rows - q0 >= G::kBQ;
-    const bool second = G::kBQ == 2 * kFewest && twice;
+    const bool twice = rows <= kFewest;
 #pragma unroll
     for (int j = 0; j < G::TQ; ++j) {
-      if (second && G::wave_q0() + 16 * j >= kFewest) {  // the second term's
-        if (j == 0) G::arrive();
-        continue;
-      }
       const bool here = q0 + G::column(j) < rows;
-      uint2 out[G::TP], rest[G::TP];
+      const auto term = [&](bool second, uint2 (&out)[G::TP]) {
 #pragma unroll
-      for (int i = 0; i < G::TP; ++i) {
-        float x[4];
+        for (int i = 0; i < G::TP; ++i) {
+          float x[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          x[r] = co[j] * __builtin_amdgcn_exp2f((tile.acc[i][j][r] - from[j]) * scale);
-          if (!all) x[r] = here && G::row(i) + r < left ? x[r] : 0.0f;
+          for (int r = 0; r < 4; ++r) {
+            x[r] = co[j] * __builtin_amdgcn_exp2f((tile.acc[i][j][r] - from[j]) * scale);
+            if (!all) x[r] = here && G::row(i) + r < left ? x[r] : 0.0f;
+          }
+          out[i] = make_uint2(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]));
+          if (second) {
+            out[i] = make_uint2(
+                pack2<T>(x[0] - low<T>(out[i].x), x[1] - high<T>(out[i].x)),
+                pack2<T>(x[2] - low<T>(out[i].y), x[3] - high<T>(out[i].y)));
+          }
         }
-        out[i] = make_uint2(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]));
-        if (second) {
-          rest[i] = make_uint2(
-              pack2<T>(x[0] - low<T>(out[i].x), x[1] - high<T>(out[i].x)),
-              pack2<T>(x[2] - low<T>(out[i].y), x[3] - high<T>(out[i].y)));
-        }
-      }
+      };
+      uint2 out[G::TP];
+      term(false, out);
       // The next tile's loads are waited for before the first store, which
       // would have to be waited for with them.
       if (j == 0) G::arrive();
-      gemm::store_column<G>(dz + q0 * ld + p0, ld, G::kBP, G::kBQ, j, out);
-      if constexpr (G::kBQ == 2 * kFewest) {
-        if (second) {
-          gemm::store_column<G>(dz + (q0 + kFewest) * ld + p0, ld, G::kBP, kFewest, j, rest);
-        }
+      uint16_t* to = dz + q0 * ld + p0;
+      if (!twice) {
+        gemm::store_column<G>(to, ld, G::kBP, G::kBQ, j, out);
+        continue;
       }
+      // Sixteen rows' block of columns, and where their first terms stand from it.
+      const int block = G::wave_q0() + 16 * j;
+      if (block >= kFewest) continue;
+      to += block * ld;
+      gemm::store_column<G>(to, ld, G::kBP, G::kBQ, j, out);
+      term(true, out);
+      gemm::store_column<G>(to + 16 * ld, ld, G::kBP, G::kBQ, j, out);
     }
     if (id >= total) return;
   }
@@ -789,19 +809,25 @@ template <typename T>
 __global__ __launch_bounds__(256) void target_grad_kernel(int32_t k, int32_t vocab0,
                                                           int32_t columns, float scale,
                                                           const float* __restrict__ coef,
-                                                          bool twice, uint16_t* __restrict__ dz,
-                                                          int64_t ld, Saved s) {
+                                                          uint16_t* __restrict__ dz, int64_t ld,
+                                                          Saved s) {
   const int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   const int64_t m = e / k;
-  if (m >= *s.count) return;
+  const int32_t count = *s.count;
+  if (m >= count) return;
   const int64_t at = static_cast<int64_t>(s.row[m]) * k + (e - m * k);
   const int32_t v = s.index[at] - vocab0;
   if (s.index[at] < 0 || v < 0 || v >= columns) return;
   const float p = __builtin_amdgcn_exp2f((s.logit[e] - s.lse[m]) * scale);
   const float x = coef[m] * (p - s.target[at]);
   const uint16_t rounded = from_f32<T>(x);
-  dz[m * ld + v] = rounded;
-  if (twice) dz[(m + kFewest) * ld + v] = from_f32<T>(x - to_f32<T>(rounded));
+  if (count > kFewest) {
+    dz[m * ld + v] = rounded;
+    return;
+  }
+  const int row = static_cast<int>(m);
+  dz[term_row(row, 0) * ld + v] = rounded;
+  dz[term_row(row, 1) * ld + v] = from_f32<T>(x - to_f32<T>(rounded));
 }
 
 // dz W has (C / tile) x (rows / tile) tiles, often fewer than CUs, over a long k:
@@ -870,7 +896,7 @@ template <typename G, typename T>
 __global__ __launch_bounds__(gemm::kThreads, 2) void hidden_grad_kernel(
     Operand w, Operand dz, const int32_t* __restrict__ count,
     const int32_t* __restrict__ split_count, int32_t steps, int32_t whole_steps, int32_t np,
-    bool add, int32_t c, bool twice, float* __restrict__ slabs) {
+    bool add, int32_t c, float* __restrict__ slabs) {
   __shared__ __attribute__((aligned(1024))) char smem[G::kLdsBytes];
   const int rows = *count;
   const int splits = *split_count;
@@ -901,20 +927,19 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void hidden_grad_kernel(
       begin();
       G::arrive();
     }
-    if constexpr (G::kBQ == 2 * kFewest) {
-      static_assert(G::kWQ == 1, "a lane holds both terms");
-      if (twice) {  // both terms of dz
-        constexpr int kHalf = kFewest / 16;
+    static_assert(G::TQ % 2 == 0, "a lane holds both terms");
+    const bool twice = rows <= kFewest;
+    if (twice) {  // both terms of dz
 #pragma unroll
-        for (int j = 0; j < kHalf; ++j) {
+      for (int j = 0; j < G::TQ; j += 2) {
 #pragma unroll
-          for (int i = 0; i < G::TP; ++i) tile.acc[i][j] += tile.acc[i][j + kHalf];
-        }
+        for (int i = 0; i < G::TP; ++i) tile.acc[i][j] += tile.acc[i][j + 1];
       }
     }
 #pragma unroll
     for (int j = 0; j < G::TQ; ++j) {
-      const int m = q0 + G::column(j);
+      int m = q0 + G::column(j);
+      if (twice) m = j % 2 == 0 ? (m & 15) + m / 32 * 16 : rows;
       if (m >= rows) continue;
       f32x4* to = reinterpret_cast<f32x4*>(out + static_cast<int64_t>(m) * c + p0 + G::row(0));
       if (add) {
@@ -968,7 +993,12 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void weight_grad_kernel(
     Operand h, Operand dz, const int32_t* __restrict__ count, int32_t columns, int32_t c,
     const float* __restrict__ scale, uint16_t* __restrict__ dw) {
   __shared__ __attribute__((aligned(1024))) char smem[G::kLdsBytes];
-  const int steps = static_cast<int>(round_up(*count, gemm::kStep) / gemm::kStep);
+  const int rows = *count;
+  const int steps = static_cast<int>(round_up(rows, gemm::kStep) / gemm::kStep);
+  if (rows <= kFewest) {  // both terms of dz, and the hidden rows in their order
+    h.data += kTermRows * h.ld;
+    h.rows -= kTermRows;
+  }
   const int np = tiles_along(c, G::kBP), nq = tiles_along(columns, G::kBQ), total = np * nq;
   int id = blockIdx.x;
   G tile;
@@ -1322,8 +1352,7 @@ int run_forward(const Shape& d, const Source& source, const void* hidden, const 
     const int groups = d.k == 1 ? 1 : (d.k + kGather - 1) / kGather;
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(pad), groups), dim3(kGatherThreads), 0,
                        stream, static_cast<const uint16_t*>(hidden),
-                       static_cast<const uint16_t*>(weight), d.c, d.k, d.n <= kFewest, source,
-                       rows, s);
+                       static_cast<const uint16_t*>(weight), d.c, d.k, source, rows, s);
   };
   if (d.n <= kOwnNumbers) {
     gather(gather_rows_kernel<T, true, Source>);
@@ -1354,7 +1383,6 @@ void launch_piece(const Shape& d, const Plan& plan, int piece, const uint16_t* w
   const int first = piece * plan.columns;
   const int columns = std::min(plan.columns, d.vocab - first);
   const int64_t ld = plan.columns;
-  const bool twice = d.n <= kFewest;
   const uint16_t* from = weight + static_cast<int64_t>(first) * d.c;
   const Operand wp{from, d.c, columns};
   const Operand h{s.hidden, d.c, static_cast<int32_t>(pad)};
@@ -1363,18 +1391,18 @@ void launch_piece(const Shape& d, const Plan& plan, int piece, const uint16_t* w
   for_sizes<T>(columns, d.n, d.c / gemm::kStep, [&](auto* tile, int grid) {
     using G = std::remove_pointer_t<decltype(tile)>;
     hipLaunchKernelGGL((softmax_grad_kernel<G, T>), dim3(grid), dim3(gemm::kThreads), 0, stream,
-                       wp, h, cut, d.c, scale, w.coef, twice, w.dz, ld, s);
+                       wp, h, cut, d.c, scale, w.coef, w.dz, ld, s);
   });
   const int64_t entries = static_cast<int64_t>(d.n) * d.k;
   hipLaunchKernelGGL((target_grad_kernel<T>), dim3(static_cast<unsigned>((entries + 255) / 256)),
-                     dim3(256), 0, stream, d.k, first, columns, scale, w.coef, twice, w.dz, ld, s);
+                     dim3(256), 0, stream, d.k, first, columns, scale, w.coef, w.dz, ld, s);
   if (dh != nullptr) {
     const int steps = static_cast<int>(round_up(columns, gemm::kStep) / gemm::kStep);
     with_tile<T, Major::kX, Major::kK>(plan.hidden, [&](auto* tile) {
       using G = std::remove_pointer_t<decltype(tile)>;
       hipLaunchKernelGGL((hidden_grad_kernel<G, T>), dim3(kCus), dim3(gemm::kThreads), 0, stream,
                          wp, dz, s.count, w.splits, steps, plan.columns / gemm::kStep,
-                         (d.c + G::kBP - 1) / G::kBP, piece > 0, d.c, twice, w.slabs);
+                         (d.c + G::kBP - 1) / G::kBP, piece > 0, d.c, w.slabs);
     });
   }
   if (dw != nullptr) {

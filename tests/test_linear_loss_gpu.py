@@ -619,3 +619,24 @@ def test_many_rows_in_several_pieces(n, c, v, masked):
     assert all(torch.equal(a, b) for a, b in zip(got, _grads(call, h, w, upstream)))
     frozen = _grads(call, h, w, upstream, weight=False)
     assert torch.equal(frozen[1], got[1])
+
+
+@pytest.mark.parametrize("dtype", ROUND)
+@pytest.mark.parametrize("n,c,v,left", [(40, 64, 300, 10), (100, 512, 700, 32), (300, 320, 3001, 1),
+                                        (1030, 512, 3001, 9), (2500, 192, 20011, 20),
+                                        (600, 512, 40000, 31)])
+def test_few_rows_left_by_masks_are_few_rows(n, c, v, left, dtype):
+    """A row's gradient is as exact with masked rows beside it as without them."""
+    h, w = _head(n, c, v, dtype, seed=47 + n)
+    keep = torch.randperm(n, generator=_gen(n))[:left].to(DEV)
+    targets = torch.full((n,), -100, device=DEV)
+    targets[keep] = torch.randint(v, (left,), generator=_gen(n + 1)).to(DEV)
+    upstream = _upstream("none", n, seed=n + 2)
+    entry = head.labels(targets, v, -100)
+
+    def call(a, b):
+        return pretrain_linear_cross_entropy(a, b, targets, reduction="none")
+
+    got = _grads(call, h, w, upstream)
+    _check(h, w, entry, got, row_weight=upstream, reduction="none", terms_of_dz=2)
+    assert all(torch.equal(a, b) for a, b in zip(got, _grads(call, h, w, upstream)))
