@@ -53,8 +53,9 @@ class Model(torch.nn.Module):
         self.head = weight(vocab, c, std=c ** -0.5)
         self.state = torch.nn.Parameter(torch.zeros(1, heads, head_size, head_size))
 
-    def hidden(self, ids: torch.Tensor) -> torch.Tensor:
-        """Normed hidden rows [tokens, C] of one packed sequence."""
+    def recurrence(self, ids: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        """The recurrence's output and the residual stream it joins, [tokens, C] each, of
+        one packed sequence."""
         n = ids.numel()
         stream = self.embedding[ids]
         r, decay, k, v, a, b = (
@@ -65,8 +66,12 @@ class Model(torch.nn.Module):
                                  for x in ([0, 1], [0], [n]))
         out, *_ = statetune_recurrent_fp32io16(self.state, offsets, starts, ends, r, decay, k, v,
                                                -a, (a * torch.sigmoid(b)).contiguous())
-        rows, _ = pretrain_layer_norm(out.reshape(n, -1), self.norm_weight, self.norm_bias,
-                                      residual=stream)
+        return out.reshape(n, -1), stream
+
+    def hidden(self, ids: torch.Tensor) -> torch.Tensor:
+        """Normed hidden rows [tokens, C], for training."""
+        out, stream = self.recurrence(ids)
+        rows, _ = pretrain_layer_norm(out, self.norm_weight, self.norm_bias, residual=stream)
         return rows
 
 
@@ -83,8 +88,9 @@ def step_loss(model: Model, ids, targets, teacher_logits, teacher_tokens, temper
 def token_log_probs(model: Model, ids, targets):
     """Scoring: the log probability of each target, [tokens] fp32 (the rows as a
     serving loop would norm them)."""
-    rows = infer_layer_norm_forward_varlen(model.embedding[ids], model.norm_weight,
-                                           model.norm_bias)
+    out, stream = model.recurrence(ids)
+    rows, _ = infer_layer_norm_forward_varlen(out, model.norm_weight, model.norm_bias,
+                                              residual=stream)
     return -pretrain_linear_cross_entropy(rows, model.head, targets, reduction="none")
 
 

@@ -107,3 +107,20 @@ def test_losses_through_the_c_abi():
                                   grad_weight=dw, **extra)
         want_dh, want_dw = torch.autograd.grad(want, [h, w], one)
         assert torch.equal(loss[0], want) and torch.equal(dh, want_dh) and torch.equal(dw, want_dw)
+
+
+def test_example_scores_with_the_whole_model():
+    """token_log_probs against the model's logits written out in 64 bits, which
+    come from the recurrence and not from the embedding alone."""
+    example = _example()
+    torch.manual_seed(3)
+    model = example.Model(300, 2).to(DEV)
+    ids, targets, _, _ = example.synthetic(300, 96, 8, DEV)
+    targets = targets.clamp_min(0)
+    with torch.no_grad():
+        rows = model.hidden(ids)
+    log_q = torch.log_softmax(rows.double() @ model.head.detach().double().t(), 1)
+    want = log_q.gather(1, targets[:, None])[:, 0]
+    got = example.token_log_probs(model, ids, targets)
+    assert got.dtype == torch.float32 and not got.requires_grad
+    torch.testing.assert_close(got.double(), want, rtol=0, atol=1e-4)
