@@ -275,10 +275,10 @@ __device__ __forceinline__ int32_t as_token(int64_t t, int32_t vocab) {
 
 // Distillation, a wave a row: shares from the teacher's logits. An entry is
 // present where its token is not negative and its logit not -inf; a row
-// without one takes no part. Tokens that occur twice in a row count with the
-// sum of their shares, found by comparing all pairs, four of them a step (2 rows of
-// 116 entries: 5.7 us, one by one 13). Dynamic LDS: K tokens and K shares a wave, rounded
-// up to four.
+// without one takes no part. The gradients of tokens that occur twice in a row take
+// the sum of their shares, found by comparing all pairs, four of them a step (2 rows
+// of 116 entries: 5.7 us, one by one 13); the loss is a sum over the entries. Dynamic
+// LDS: K tokens and K shares a wave, rounded up to four.
 template <typename T, typename Index>
 __global__ __launch_bounds__(256) void teacher_targets_kernel(
     const typename IoTraits<T>::storage* __restrict__ logits, const Index* __restrict__ indices,

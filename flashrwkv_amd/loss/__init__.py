@@ -188,9 +188,12 @@ def pretrain_linear_topk_distillation(
     logit of -inf is absent, a row without entries takes no part. With p =
     softmax(teacher_logits / T) over a row's entries and q = softmax(hidden
     weight^T / T) over the whole vocabulary the loss is
-    ``T^2 sum p (log p - log q)``, reduced as in
-    :func:`pretrain_linear_cross_entropy`. A token listed twice counts with the
-    sum of its p. Gradients for hidden and weight; none for the teacher.
+    ``T^2 sum p (log p - log q)`` over the entries, reduced as in
+    :func:`pretrain_linear_cross_entropy`. A token listed twice pulls with the sum
+    of its p, so the gradients are those of the joined entries; the loss has both
+    entries as they stand, which is less than the joined ones' divergence by
+    ``T^2 sum p log(P / p)`` (P: the token's sum of p) and can be negative.
+    Gradients for hidden and weight; none for the teacher.
     """
     call = C.whole_call("linear_loss_call") if teacher_logits is not None else None
     if call and isinstance(reduction, str) and reduction in REDUCTIONS:

@@ -661,8 +661,9 @@ int frwkv_layer_norm_backward(int io_dtype, int64_t rows, int64_t channels, cons
  * whose target (int32 or int64, target_bytes 4 or 8) is not ignore_index.
  * frwkv_linear_topk_distillation_forward: p = softmax(teacher_logits / T) over
  * a row's present entries (index not negative, logit not -inf), q =
- * softmax(z / T), loss = T^2 sum p (log p - log q). top at most 1024 entries a
- * row; a token that occurs twice counts with the sum of its p.
+ * softmax(z / T), loss = T^2 sum p (log p - log q) over the entries. top at most
+ * 1024 entries a row; the gradient of a token that occurs twice is of the sum of its
+ * p, the loss has its entries one by one (their p log p, not that of their sum).
  *
  * Rows without a target have loss 0 and count nowhere; what they hold is not
  * read by the products. A target at or beyond vocab (for cross entropy: any

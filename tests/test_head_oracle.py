@@ -120,3 +120,13 @@ def test_head_loss_gradients_match_central_differences(mean):
 
     for name, leaf in (("dhidden", h), ("dweight", w)):
         torch.testing.assert_close(got[name], _differences(loss, leaf), rtol=1e-5, atol=1e-8)
+
+
+def test_a_token_listed_four_times_hand_worked():
+    """Entries are summed one by one in the loss, joined in the gradient: a uniform
+    student over 5 tokens and a teacher with its four entries on one of them."""
+    h, w = torch.zeros(1, 2, dtype=torch.float64), _rand(5, 2, seed=18)
+    entry = head.teacher(torch.zeros(1, 4), torch.full((1, 4), 3), 2.0)
+    got = head.head_loss(h, w, *entry, temperature=2.0, row_weight=torch.ones(1))
+    assert got["loss"].item() == pytest.approx(4 * (math.log(5) - math.log(4)), rel=1e-14)
+    assert got["dz"].tolist()[0] == pytest.approx([0.4, 0.4, 0.4, -1.6, 0.4], rel=1e-14)

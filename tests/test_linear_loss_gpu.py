@@ -640,3 +640,24 @@ def test_few_rows_left_by_masks_are_few_rows(n, c, v, left, dtype):
     got = _grads(call, h, w, upstream)
     _check(h, w, entry, got, row_weight=upstream, reduction="none", terms_of_dz=2)
     assert all(torch.equal(a, b) for a, b in zip(got, _grads(call, h, w, upstream)))
+
+
+def test_a_token_listed_four_times_hand_worked():
+    """A uniform student over 5 tokens, four equal entries on one of them: the loss is
+    T^2 (log 5 - log 4), the gradient that of one entry with all of p."""
+    h = torch.zeros(1, 64, dtype=torch.bfloat16, device=DEV)
+    w = torch.zeros(5, 64, dtype=torch.bfloat16, device=DEV)
+    w[:, :5] = 4 * torch.eye(5)
+    four = torch.full((1, 4), 3, device=DEV)
+    loss, dh, dw = _grads(lambda a, b: pretrain_linear_topk_distillation(
+        a, b, torch.zeros(1, 4, device=DEV), four, temperature=2.0, reduction="sum"), h, w,
+        torch.ones((), device=DEV))
+    assert loss.item() == pytest.approx(4 * (math.log(5) - math.log(4)), rel=1e-5)
+    want = torch.tensor([1.6, 1.6, 1.6, -6.4, 1.6], device=DEV)
+    torch.testing.assert_close(dh[0, :5].float(), want, rtol=2.0 ** -8, atol=0)
+    assert not dh[0, 5:].any() and not dw.any()
+    with_far_ahead = h.clone()
+    with_far_ahead[0, 3] = 16  # z = 64 at the token, 0 elsewhere: q is 1 there
+    loss = pretrain_linear_topk_distillation(with_far_ahead, w, torch.zeros(1, 4, device=DEV),
+                                             four, reduction="sum")
+    assert loss.item() == pytest.approx(-math.log(4), rel=1e-5)
