@@ -68,6 +68,7 @@ SIGNATURES = {
     "frwkv_linear_loss_saved_bytes": [_I64] * 3,
     "frwkv_linear_loss_forward_workspace_bytes": [_I64] * 2,
     "frwkv_linear_loss_backward_workspace_bytes": [_I64] * 3 + [_INT],
+    "frwkv_linear_loss_backward_plan": [_I64] * 3 + [_VP] * 4,
     "frwkv_linear_cross_entropy_forward": [_INT] + [_I64] * 3 + [_VP, _VP, _INT, _VP, _I64, _INT]
                                           + [_VP, _VP, _SZ, _VP, _SZ, _VP],
     "frwkv_linear_topk_distillation_forward": [_INT] + [_I64] * 4 + [_VP, _VP, _INT, _VP, _INT]
@@ -379,6 +380,14 @@ def linear_topk_distillation_forward(hidden, weight, teacher_logits, teacher_ind
         _p(teacher_indices), float(temperature), REDUCTIONS[reduction], _p(loss), _p(saved),
         saved.numel(), _p(work), work.numel(), _stream()))
     return saved
+
+
+def linear_loss_backward_plan(rows, channels, vocab):
+    """(columns of a piece, pieces, splits, rows of a tile) of the hidden gradient."""
+    out = [ctypes.c_int32() for _ in range(4)]
+    _check(library().frwkv_linear_loss_backward_plan(rows, channels, vocab,
+                                                     *(ctypes.byref(x) for x in out)))
+    return tuple(x.value for x in out)
 
 
 def linear_loss_backward(grad_loss, weight, saved, *, rows, top, temperature=1.0,

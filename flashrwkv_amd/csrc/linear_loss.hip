@@ -1594,6 +1594,24 @@ size_t frwkv_linear_loss_backward_workspace_bytes(int64_t rows, int64_t channels
   return bytes;
 }
 
+int frwkv_linear_loss_backward_plan(int64_t rows, int64_t channels, int64_t vocab,
+                                    int32_t* columns, int32_t* pieces, int32_t* splits,
+                                    int32_t* tile_rows) {
+  using namespace frwkv;
+  const char* what = "frwkv_linear_loss_backward_plan";
+  if (!columns || !pieces || !splits || !tile_rows) {
+    return set_error(FRWKV_ERR_INVALID_ARGUMENT, "%s: null pointer argument", what);
+  }
+  const int rc = check_shape(what, FRWKV_DTYPE_BF16, rows, channels, vocab, 1);
+  if (rc != FRWKV_OK) return rc;
+  const Plan plan = plan_of(rows, channels, vocab);
+  *columns = plan.columns;
+  *pieces = plan.pieces;
+  *splits = plan.splits;
+  *tile_rows = time_of(plan.hidden).q;
+  return FRWKV_OK;
+}
+
 int frwkv_linear_cross_entropy_forward(int io_dtype, int64_t rows, int64_t channels,
                                        int64_t vocab, const void* hidden, const void* weight,
                                        int target_bytes, const void* targets,

@@ -689,6 +689,12 @@ size_t frwkv_linear_loss_saved_bytes(int64_t rows, int64_t channels, int64_t top
 size_t frwkv_linear_loss_forward_workspace_bytes(int64_t rows, int64_t vocab);
 size_t frwkv_linear_loss_backward_workspace_bytes(int64_t rows, int64_t channels, int64_t vocab,
                                                   int want_grad_hidden);
+/* How the backward of these sizes goes through the vocabulary (a host query):
+ * columns of a piece, pieces, splits of the hidden gradient's product for all rows and
+ * rows of its tiles. */
+int frwkv_linear_loss_backward_plan(int64_t rows, int64_t channels, int64_t vocab,
+                                    int32_t* columns, int32_t* pieces, int32_t* splits,
+                                    int32_t* tile_rows);
 int frwkv_linear_cross_entropy_forward(int io_dtype, int64_t rows, int64_t channels,
                                        int64_t vocab, const void* hidden, const void* weight,
                                        int target_bytes, const void* targets,

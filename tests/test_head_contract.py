@@ -236,3 +236,16 @@ def test_backward_workspace_is_less_than_the_logits_it_avoids():
     lib = capi.library()
     for n in (8192, 32768, 65536, 131072, 262144):
         assert lib.frwkv_linear_loss_backward_workspace_bytes(n, 4096, 65536, 1) < n * 65536 * 2
+
+
+def test_backward_plan_is_a_host_query():
+    columns, pieces, splits, tile_rows = capi.linear_loss_backward_plan(8192, 4096, 65536)
+    assert columns % 256 == 0 and (pieces - 1) * columns < 65536 <= pieces * columns
+    assert 1 <= splits <= 16 and tile_rows in (64, 128, 256)
+    lib = capi.library()
+    null = ctypes.c_void_p()
+    assert lib.frwkv_linear_loss_backward_plan(1, 64, 1, null, null, null, null) == 1
+    assert b"null pointer" in _last()
+    x = [ctypes.byref(ctypes.c_int32()) for _ in range(4)]
+    assert lib.frwkv_linear_loss_backward_plan(1, 100, 1, *x) == 2
+    assert b"multiple of 64" in _last()

@@ -23,6 +23,7 @@ import pytest
 import torch
 
 import flashrwkv_amd
+from flashrwkv_amd import capi
 from flashrwkv_amd.loss import pretrain_linear_cross_entropy, pretrain_linear_topk_distillation
 from oracle import head
 
@@ -661,3 +662,55 @@ def test_a_token_listed_four_times_hand_worked():
     loss = pretrain_linear_topk_distillation(with_far_ahead, w, torch.zeros(1, 4, device=DEV),
                                              four, reduction="sum")
     assert loss.item() == pytest.approx(-math.log(4), rel=1e-5)
+
+
+# Rows, channels, tokens, masked share and whether one piece holds the vocabulary: the
+# hidden gradient goes through 256 x 256 tiles in several splits. Ragged: rows, the last
+# tile of channels, the last split and the last piece.
+LARGE = [(700, 1088, 20011, 0.0, True), (700, 1088, 20011, 0.5, True),
+         (2047, 576, 20011, 0.2, True), (4095, 576, 70001, 0.0, False),
+         (4095, 832, 70001, 0.4, False)]
+
+
+def _require_large_tiles(n, c, v, one_piece):
+    columns, pieces, splits, tile_rows = capi.linear_loss_backward_plan(n, c, v)
+    print(f"pieces of {columns}: {pieces}, splits {splits}, tile rows {tile_rows}", flush=True)
+    assert tile_rows == 256 and splits > 1 and (pieces == 1) == one_piece
+    assert c % 256 and v % columns and n % 256
+
+
+@pytest.mark.parametrize("dtype", ROUND)
+@pytest.mark.parametrize("n,c,v,masked,one_piece", LARGE)
+def test_large_tiles_cross_entropy(n, c, v, masked, one_piece, dtype):
+    _require_large_tiles(n, c, v, one_piece)
+    h, w = _head(n, c, v, dtype, seed=60 + n + c)
+    targets = torch.randint(v, (n,), generator=_gen(n))
+    targets[torch.rand(n, generator=_gen(n + 1)) < masked] = -100
+    targets[-1] = v - 1
+    targets = targets.to(DEV)
+    upstream = _upstream("none", n, seed=n + 2)
+
+    def call(a, b):
+        return pretrain_linear_cross_entropy(a, b, targets, reduction="none")
+
+    got = _grads(call, h, w, upstream)
+    _check(h, w, head.labels(targets, v, -100), got, row_weight=upstream, reduction="none")
+    assert all(torch.equal(a, b) for a, b in zip(got, _grads(call, h, w, upstream)))
+    frozen = _grads(call, h, w, upstream, weight=False)
+    assert torch.equal(frozen[1], got[1])
+
+
+@pytest.mark.parametrize("n,c,v,masked,one_piece", LARGE)
+def test_large_tiles_distillation(n, c, v, masked, one_piece):
+    _require_large_tiles(n, c, v, one_piece)
+    h, w = _head(n, c, v, torch.bfloat16, seed=61 + n + c)
+    gen = torch.Generator(device=DEV).manual_seed(n)
+    first = torch.randint(v, (n, 1), generator=gen, device=DEV)
+    tokens = (first + torch.arange(5, device=DEV) * (v // 5)) % v  # in every piece
+    tokens[torch.rand(n, generator=gen, device=DEV) < masked] = -1
+    logits = torch.randn(n, 5, generator=gen, device=DEV)
+    one = torch.ones((), device=DEV)
+    got = _grads(lambda a, b: pretrain_linear_topk_distillation(
+        a, b, logits, tokens, temperature=1.5, reduction="sum"), h, w, one)
+    _check(h, w, head.teacher(logits, tokens, 1.5), got, temperature=1.5,
+           row_weight=one.expand(n), reduction="sum")
