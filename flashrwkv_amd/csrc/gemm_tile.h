@@ -7,8 +7,8 @@
 // HBM straight into LDS (16 bytes a lane, no registers) up to NS stages ahead.
 //
 // Large products are bound by the matrix units and by the clock that their power
-// allows: 8192 x 65536 x 4096 bf16 in 256 x 256 tiles runs at 1331 TFLOP/s with k-major
-// operands, units busy 74% of the cycles at 1.71 GHz. 256 x 256 by 8 waves of 128 x 64
+// allows: 8192 x 65536 x 4096 bf16 in 256 x 256 tiles runs at 1302 TFLOP/s with k-major
+// operands, units busy 74% of the cycles at 1.67 GHz. 256 x 256 by 8 waves of 128 x 64
 // is the largest tile whose accumulators (128 registers) leave room for two sets
 // of operands; with one set, loads, LDS reads and matrix instructions one after the other,
 // it was 58% at 1.91 GHz. v_mfma_f32_32x32x16 in the same tile was 6 to 8% slower.

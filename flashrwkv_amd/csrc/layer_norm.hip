@@ -18,7 +18,14 @@
 // those in order, so the result does not depend on timing.
 // Measured at 16384 x 4096 bf16: forward with a residual 91 us (5.9 TB/s), backward with
 // a gradient of the stream 115 us (4.7 TB/s), the columns' sums 5 us; a copy of 1 GiB
-// reaches 5.1 TB/s. One row: 5 us, latency of its two reductions and the launch.
+// reaches 5.1 TB/s. fp32 16384 x 4096: forward with a residual 204 us, backward with a
+// gradient of the stream 206 us (5.2 TB/s both). One row: 5 us, latency of its two
+// reductions and the launch. 2311 x 1000 fp32: 8, 11 and 4 us where the bytes take 7 in
+// all, three launches of one row a wave, which are latency as well.
+// The backward with 16 elements a thread, two workgroups a CU at 128 registers, keeps
+// 5 values in scratch for fp32 (C 2049 to 4096), up to 13 for unaligned rows.
+// Unaligned rows of 4097 channels, 16 waves of which half hold nothing, run at half the
+// rate (16384 x 4097 bf16: 164 and 203 us).
 #include <algorithm>
 #include <type_traits>
 

@@ -591,7 +591,7 @@ __device__ __forceinline__ int own_row(int token, int p0, int left) {
 // the sum of 2^(scale (z - maximum)), scale = s log2 e, to part[tile][m]. one: rows
 // have one target each, whose logit goes to s.logit as it stands here, so that
 // it cancels against a maximum that it is.
-// Bound by the matrix units for many rows (8192 x 65536 x 4096 bf16: 3.30 ms, 1331
+// Bound by the matrix units for many rows (8192 x 65536 x 4096 bf16: 3.38 ms, 1302
 // TFLOP/s) and by the weight's read for few (1 row of 2048 channels, 65536 tokens:
 // 44 to 49 us, 5.5 to 6.1 TB/s). A tile's exponentials take 2 of its 5 us beside the
 // product.
@@ -708,7 +708,8 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void lse_tiles_kernel(
 
 // D[v][m] of a piece of the vocabulary: dz[m][v] = coef_m 2^(scale (z - lse_m)),
 // zero for rows and columns that are not there. Bound as the forward is:
-// 8192 x 32768 x 4096 in 1.69 ms, 1304 TFLOP/s.
+// 8192 x 32768 x 4096 in 1.75 ms, 1260 TFLOP/s. The 256 x 256 form has 10 values more
+// than registers: 44 MB of scratch written beside 537 of dz.
 //
 // Twice: rounding dz to 16 bits is one error for all elements that a target
 // entry dominates, up to 2^-9 of the entry 1 for bf16. Over many rows such
@@ -717,7 +718,7 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void lse_tiles_kernel(
 // unused, so there dz has two terms, the rounded value and what is left of it, and
 // the products add both at no cost (bf16 gradients of 3 weighted rows,
 // 3001 x 512: up to 3.8e-3 off with one term, 1.7e-3 with two, the outputs' own
-// rounding).
+// rounding). More rows would need a product of twice as many: they keep one term.
 template <typename G, typename T>
 __global__ __launch_bounds__(gemm::kThreads, 2) void softmax_grad_kernel(
     Operand w, Operand h, const int32_t* __restrict__ cut, int32_t c, float scale,
@@ -890,7 +891,7 @@ struct Pieces {
 
 // D[c][m] = sum over a split's vocabulary of W[v][c] dz[m][v], to slab [m][c]
 // of the split (fp32), added to what the pieces before left there: they run one
-// after the other, and every element has one owner in each. Bound by the matrix units: 8192 x 32768 x 4096 in 1.64 ms, 1344
+// after the other, and every element has one owner in each. Bound by the matrix units: 8192 x 32768 x 4096 in 1.69 ms, 1299
 // TFLOP/s, in one split.
 template <typename G, typename T>
 __global__ __launch_bounds__(gemm::kThreads, 2) void hidden_grad_kernel(
@@ -958,7 +959,7 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void hidden_grad_kernel(
 }
 
 // dh[i][c] = scale x sum of the slabs of row place[i], in order; zeros for
-// rows that took no part. Bound by the slabs' read: two of 8192 x 4096 in 60 us, 5.6
+// rows that took no part. Bound by the slabs' read: one of 8192 x 4096 in 38 us, 5.3
 // TB/s with the output.
 template <typename T>
 __global__ __launch_bounds__(256) void hidden_grad_rows_kernel(
@@ -986,7 +987,7 @@ __global__ __launch_bounds__(256) void hidden_grad_rows_kernel(
 }
 
 // D[c][v] = sum_m h[m][c] dz[m][v]: dW of a piece of the vocabulary. Both operands
-// are x-major, twice the LDS reads of the others: 8192 x 32768 x 4096 in 1.77 ms, 1240
+// are x-major, twice the LDS reads of the others: 8192 x 32768 x 4096 in 1.80 ms, 1223
 // TFLOP/s (a library product of that layout: 1084 to 1136).
 template <typename G, typename T>
 __global__ __launch_bounds__(gemm::kThreads, 2) void weight_grad_kernel(

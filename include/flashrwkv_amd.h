@@ -679,7 +679,8 @@ int frwkv_layer_norm_backward(int io_dtype, int64_t rows, int64_t channels, cons
  * FRWKV_REDUCE_NONE; grad_hidden [rows, channels] and grad_weight [vocab,
  * channels] of the io dtype, either NULL where it is not wanted. It goes
  * through the vocabulary in pieces whose logit gradients (16 bits) fit the
- * workspace. All sums are in a fixed order. Both directions need at least one
+ * workspace: at most 512 MB of them, or 256 tokens' of all rows where that is more,
+ * and for grad_hidden fp32 slabs of [rows, channels], one or at most 17. All sums are in a fixed order. Both directions need at least one
  * row. The byte queries give 0 for sizes that the calls refuse: more than 2^23
  * rows, 65536 channels (or no multiple of 64), 2^28 tokens, 1024 targets a row, 2^44
  * rows x tokens (in tiles of 128) or 2^31 rows x targets. No counterpart in the
