@@ -235,3 +235,61 @@ def linear_loss_backward(grad_loss, weight, saved, rows, top, temperature, reduc
     return ops.linear_loss_backward(grad_loss, weight, saved, int(rows), int(top),
                                     float(temperature), int(reduction), bool(want_hidden),
                                     bool(want_weight))
+
+
+def linear_log_probs_forward(hidden, weight, targets, ignore_index, temperature, entropy):
+    """[log_probs, saved], or [log_probs, entropy, saved]."""
+    return ops.linear_log_probs_forward(hidden, weight, targets, int(ignore_index),
+                                        float(temperature), bool(entropy))
+
+
+def linear_log_probs_backward(grad_log_probs, grad_entropy, weight, saved, rows, temperature,
+                              want_hidden, want_weight):
+    """The gradients asked for, of hidden ([rows, C]) and of weight, in that order."""
+    return ops.linear_log_probs_backward(grad_log_probs, grad_entropy, weight, saved, int(rows),
+                                         float(temperature), bool(want_hidden),
+                                         bool(want_weight))
+
+
+def policy_loss_forward(log_probs, old_log_probs, advantages, reference_log_probs, entropy, mask,
+                        cu_seqlens, clip_low, clip_high, dual_clip, kl_weight, entropy_weight,
+                        reduction, metrics, slopes):
+    """[loss, saved], and the metrics after them; dual_clip 0 for none, reduction 0 none, 1 mean,
+    2 sum, 3 the mean of the sequences' means."""
+    return ops.policy_loss_forward(
+        log_probs, old_log_probs, advantages, reference_log_probs, entropy, mask, cu_seqlens,
+        float(clip_low), float(clip_high), float(dual_clip), float(kl_weight),
+        float(entropy_weight), int(reduction), bool(metrics), bool(slopes))
+
+
+def policy_loss_backward(grad_loss, saved, mask, cu_seqlens, shape, log_probs_dtype,
+                         entropy_dtype, entropy_weight, reduction, want_log_probs, want_entropy):
+    """The gradients asked for, of log_probs and of entropy, in that order."""
+    return ops.policy_loss_backward(
+        grad_loss, saved, mask, cu_seqlens, list(shape), log_probs_dtype, entropy_dtype,
+        float(entropy_weight), int(reduction), bool(want_log_probs), bool(want_entropy))
+
+
+def preference_loss_forward(log_probs, cu_seqlens, reference_log_probs, mask, beta, margin,
+                            label_smoothing, kind, normalize, reduction):
+    """(loss, rewards, saved); kind 0 sigmoid, 1 hinge, 2 squared."""
+    return ops.preference_loss_forward(
+        log_probs, cu_seqlens, reference_log_probs, mask, float(beta), float(margin),
+        float(label_smoothing), int(kind), bool(normalize), int(reduction))
+
+
+def preference_loss_backward(grad_loss, saved, cu_seqlens, mask, shape, log_probs_dtype,
+                             reduction):
+    """The gradient of log_probs."""
+    return ops.preference_loss_backward(grad_loss, saved, cu_seqlens, mask, list(shape),
+                                        log_probs_dtype, int(reduction))
+
+
+def grad_norm(tensors):
+    """The norm of all tensors together."""
+    return ops.grad_norm(list(tensors))
+
+
+def clip_grad_norm(tensors, out, max_norm, eps):
+    """Writes the clipped tensors to out (themselves: in place); their norm from before."""
+    return ops.clip_grad_norm(list(tensors), list(out), float(max_norm), float(eps))

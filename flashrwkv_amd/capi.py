@@ -20,7 +20,8 @@ DTYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 DECAY_LOGITS, DECAY_RAW_W = 0, 1
 
 _INT, _I32, _I64 = ctypes.c_int, ctypes.c_int32, ctypes.c_int64
-_F32, _VP, _SZ = ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t
+_F32, _F64 = ctypes.c_float, ctypes.c_double
+_VP, _SZ = ctypes.c_void_p, ctypes.c_size_t
 
 # name -> argtypes, in the header's parameter order.
 SIGNATURES = {
@@ -75,7 +76,35 @@ SIGNATURES = {
                                               + [_VP, _F32, _INT, _VP, _VP, _SZ, _VP, _SZ, _VP],
     "frwkv_linear_loss_backward": [_INT] + [_I64] * 4 + [_VP, _F32, _INT, _VP, _VP, _SZ]
                                   + [_VP] * 3 + [_SZ, _VP],
+    "frwkv_linear_log_probs_forward_workspace_bytes": [_I64] * 2 + [_INT],
+    "frwkv_linear_log_probs_backward_workspace_bytes": [_I64] * 3 + [_INT] * 2,
+    "frwkv_linear_log_probs_forward": [_INT] + [_I64] * 3 + [_VP, _VP, _INT, _VP, _I64, _F32]
+                                      + [_VP] * 3 + [_SZ, _VP, _SZ, _VP],
+    "frwkv_linear_log_probs_backward": [_INT] + [_I64] * 3 + [_VP, _F32] + [_VP] * 3
+                                       + [_SZ] + [_VP] * 3 + [_SZ, _VP],
+    "frwkv_policy_loss_saved_bytes": [_I64] * 2,
+    "frwkv_preference_loss_saved_bytes": [_I64],
+    "frwkv_sequence_loss_workspace_bytes": [_I64] * 2,
+    "frwkv_policy_loss_forward": [_I64] * 2 + [_VP] * 2 + [_INT, _VP] * 3 + [_INT]
+                                 + [_INT, _VP] * 2 + [_F64] * 3 + [_F32] * 2
+                                 + [_INT, _VP, _VP, _INT, _VP, _SZ, _VP, _SZ, _VP],
+    "frwkv_policy_loss_backward": [_I64] * 2 + [_VP] * 2 + [_F32, _INT, _VP, _VP, _SZ]
+                                  + [_INT, _VP] * 2 + [_VP],
+    "frwkv_preference_loss_forward": [_I64] * 2 + [_VP] * 2 + [_INT, _VP] * 2 + [_F64] * 3
+                                     + [_INT] * 3 + [_VP] * 3 + [_SZ, _VP, _SZ, _VP],
+    "frwkv_preference_loss_backward": [_I64] * 2 + [_VP] * 2 + [_INT, _VP, _VP, _SZ, _INT]
+                                      + [_VP] * 2,
+    "frwkv_grad_norm_workspace_bytes": [_I64, _VP],
+    "frwkv_grad_norm": [_I64, _VP, _VP, _VP, _SZ, _VP],
+    "frwkv_grad_clip": [_I64, _VP, _F64, _F64, _VP, _VP, _SZ, _VP],
 }
+
+
+class Gradient(ctypes.Structure):
+    """``frwkv_gradient``: one tensor of a list."""
+
+    _fields_ = [("data", _VP), ("out", _VP), ("numel", _I64), ("dtype", _I32),
+                ("out_dtype", _I32)]
 
 _LIB = None
 
@@ -401,3 +430,121 @@ def linear_loss_backward(grad_loss, weight, saved, *, rows, top, temperature=1.0
         DTYPE[weight.dtype], rows, c, vocab, top, _p(weight), float(temperature),
         REDUCTIONS[reduction], _p(grad_loss), _p(saved), saved.numel(), _p(grad_hidden),
         _p(grad_weight), _p(work), need, _stream()))
+
+
+def linear_log_probs_forward(hidden, weight, targets, *, log_probs, entropy=None,
+                             temperature=1.0, ignore_index=-100):
+    """Writes ``log_probs`` and, where given, ``entropy`` (fp32); returns the buffer that the
+    backward reads."""
+    vocab, c = weight.shape
+    rows = hidden.numel() // c
+    lib = library()
+    saved = workspace(int(lib.frwkv_linear_loss_saved_bytes(rows, c, 1)), hidden.device)
+    work = workspace(int(lib.frwkv_linear_log_probs_forward_workspace_bytes(
+        rows, vocab, entropy is not None)), hidden.device)
+    _check(lib.frwkv_linear_log_probs_forward(
+        DTYPE[hidden.dtype], rows, c, vocab, _p(hidden), _p(weight), targets.element_size(),
+        _p(targets), int(ignore_index), float(temperature), _p(log_probs), _p(entropy),
+        _p(saved), saved.numel(), _p(work), work.numel(), _stream()))
+    return saved
+
+
+def linear_log_probs_backward(grad_log_probs, grad_entropy, weight, saved, *, rows,
+                              temperature=1.0, grad_hidden=None, grad_weight=None):
+    """Either upstream gradient may be None (zeros), and either gradient (not computed)."""
+    vocab, c = weight.shape
+    need = int(library().frwkv_linear_log_probs_backward_workspace_bytes(
+        rows, c, vocab, grad_hidden is not None, grad_entropy is not None))
+    work = workspace(need, weight.device)
+    _check(library().frwkv_linear_log_probs_backward(
+        DTYPE[weight.dtype], rows, c, vocab, _p(weight), float(temperature), _p(grad_log_probs),
+        _p(grad_entropy), _p(saved), saved.numel(), _p(grad_hidden), _p(grad_weight), _p(work),
+        need, _stream()))
+
+
+POLICY_REDUCTIONS = {**REDUCTIONS, "sequence_mean": 3}
+PREFERENCES = {"sigmoid": 0, "hinge": 1, "squared": 2}
+
+
+def _vector(t):
+    return (0, None) if t is None else (DTYPE[t.dtype], _p(t))
+
+
+def _sequences(cu_seqlens):
+    return 0 if cu_seqlens is None else cu_seqlens.numel() - 1
+
+
+def policy_loss_forward(log_probs, old_log_probs, advantages, *, loss, metrics=None,
+                        reference_log_probs=None, entropy=None, mask=None, cu_seqlens=None,
+                        clip_low=0.2, clip_high=0.2, dual_clip=0.0, kl_weight=0.0,
+                        entropy_weight=0.0, reduction="mean", slopes=True):
+    """Writes ``loss`` and, where given, ``metrics`` (fp32); returns the buffer that the
+    backward reads."""
+    lib, n, b = library(), log_probs.numel(), _sequences(cu_seqlens)
+    saved = workspace(int(lib.frwkv_policy_loss_saved_bytes(n, b)), log_probs.device)
+    work = workspace(int(lib.frwkv_sequence_loss_workspace_bytes(n, b)), log_probs.device)
+    _check(lib.frwkv_policy_loss_forward(
+        n, b, _p(cu_seqlens), _p(mask), *_vector(log_probs), *_vector(old_log_probs),
+        *_vector(advantages), advantages.shape != log_probs.shape,
+        *_vector(reference_log_probs), *_vector(entropy), float(clip_low), float(clip_high),
+        float(dual_clip), float(kl_weight), float(entropy_weight), POLICY_REDUCTIONS[reduction],
+        _p(loss), _p(metrics), int(slopes), _p(saved), saved.numel(), _p(work), work.numel(),
+        _stream()))
+    return saved
+
+
+def policy_loss_backward(grad_loss, saved, *, tokens, mask=None, cu_seqlens=None,
+                         entropy_weight=0.0, reduction="mean", grad_log_probs=None,
+                         grad_entropy=None):
+    """Either gradient may be None: it is then not computed."""
+    _check(library().frwkv_policy_loss_backward(
+        tokens, _sequences(cu_seqlens), _p(cu_seqlens), _p(mask), float(entropy_weight),
+        POLICY_REDUCTIONS[reduction], _p(grad_loss), _p(saved), saved.numel(),
+        *_vector(grad_log_probs), *_vector(grad_entropy), _stream()))
+
+
+def preference_loss_forward(log_probs, cu_seqlens, *, loss, rewards, reference_log_probs=None,
+                            mask=None, beta=0.1, margin=0.0, label_smoothing=0.0, kind="sigmoid",
+                            normalize=False, reduction="mean"):
+    """Writes ``loss`` and ``rewards`` (fp32); returns the buffer that the backward reads."""
+    lib, n, pairs = library(), log_probs.numel(), _sequences(cu_seqlens) // 2
+    saved = workspace(int(lib.frwkv_preference_loss_saved_bytes(pairs)), log_probs.device)
+    work = workspace(int(lib.frwkv_sequence_loss_workspace_bytes(n, 2 * pairs)),
+                     log_probs.device)
+    _check(lib.frwkv_preference_loss_forward(
+        n, pairs, _p(cu_seqlens), _p(mask), *_vector(log_probs), *_vector(reference_log_probs),
+        float(beta), float(margin), float(label_smoothing), PREFERENCES[kind], int(normalize),
+        REDUCTIONS[reduction], _p(loss), _p(rewards), _p(saved), saved.numel(), _p(work),
+        work.numel(), _stream()))
+    return saved
+
+
+def preference_loss_backward(grad_loss, saved, cu_seqlens, *, grad_log_probs, mask=None,
+                             reduction="mean"):
+    _check(library().frwkv_preference_loss_backward(
+        grad_log_probs.numel(), _sequences(cu_seqlens) // 2, _p(cu_seqlens), _p(mask),
+        REDUCTIONS[reduction], _p(grad_loss), _p(saved), saved.numel(),
+        *_vector(grad_log_probs), _stream()))
+
+
+def _gradients(tensors, out):
+    return (Gradient * len(tensors))(*(
+        Gradient(x.data_ptr(), y.data_ptr(), x.numel(), DTYPE[x.dtype], DTYPE[y.dtype])
+        for x, y in zip(tensors, out)))
+
+
+def grad_norm(tensors, *, norm):
+    """Writes ``norm`` (fp32 [1])."""
+    items = _gradients(tensors, tensors)
+    need = int(library().frwkv_grad_norm_workspace_bytes(len(tensors), items))
+    work = workspace(need, norm.device)
+    _check(library().frwkv_grad_norm(len(tensors), items, _p(norm), _p(work), need, _stream()))
+
+
+def grad_clip(tensors, max_norm, *, norm, out=None, eps=1e-6):
+    """Writes ``norm`` and the clipped tensors to ``out`` (None: in place)."""
+    items = _gradients(tensors, tensors if out is None else out)
+    need = int(library().frwkv_grad_norm_workspace_bytes(len(tensors), items))
+    work = workspace(need, norm.device)
+    _check(library().frwkv_grad_clip(len(tensors), items, float(max_norm), float(eps), _p(norm),
+                                     _p(work), need, _stream()))

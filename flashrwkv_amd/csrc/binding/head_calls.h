@@ -17,9 +17,11 @@ using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
 // What a backward returns. Where it is itself recorded, its outputs have no
-// gradient of their own: differentiating them raises.
-variable_list first_order(variable_list grads, const variable_list& upstream, const char* name) {
-  bool recorded = false;
+// gradient of their own: differentiating them raises. always: also where the
+// upstream gradients are constants.
+variable_list first_order(variable_list grads, const variable_list& upstream, const char* name,
+                          bool always = false) {
+  bool recorded = always;
   for (const Tensor& g : upstream) recorded = recorded || (g.defined() && g.requires_grad());
   if (!recorded || !at::GradMode::is_enabled()) return grads;
   std::vector<size_t> at;

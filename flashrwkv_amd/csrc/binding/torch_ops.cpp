@@ -17,6 +17,7 @@
 
 #include <hip/hip_runtime_api.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cmath>
 #include <cstdint>
@@ -1451,6 +1452,7 @@ Tensor recurrent_tmix_fused_forward(Tensor query_start_loc, Tensor state_indices
 }
 
 #include "head_ops.h"
+#include "step_ops.h"
 
 TORCH_LIBRARY(flashrwkv2, m) {
   m.class_<MetadataTicket>("MetadataTicket")
@@ -1531,6 +1533,38 @@ TORCH_LIBRARY(flashrwkv2, m) {
       "linear_loss_backward(Tensor grad_loss, Tensor weight, Tensor saved, int rows, int top, "
       "float temperature, int reduction, bool want_hidden, bool want_weight) -> Tensor[]",
       &linear_loss_backward);
+  m.def(
+      "linear_log_probs_forward(Tensor hidden, Tensor weight, Tensor targets, int ignore_index, "
+      "float temperature, bool entropy) -> Tensor[]",
+      &linear_log_probs_forward);
+  m.def(
+      "linear_log_probs_backward(Tensor? grad_log_probs, Tensor? grad_entropy, Tensor weight, "
+      "Tensor saved, int rows, float temperature, bool want_hidden, bool want_weight) -> Tensor[]",
+      &linear_log_probs_backward);
+  m.def(
+      "policy_loss_forward(Tensor log_probs, Tensor old_log_probs, Tensor advantages, "
+      "Tensor? reference_log_probs, Tensor? entropy, Tensor? mask, Tensor? cu_seqlens, "
+      "float clip_low, float clip_high, float dual_clip, float kl_weight, float entropy_weight, "
+      "int reduction, bool metrics, bool slopes) -> Tensor[]",
+      &policy_loss_forward);
+  m.def(
+      "policy_loss_backward(Tensor grad_loss, Tensor saved, Tensor? mask, Tensor? cu_seqlens, "
+      "int[] shape, ScalarType log_probs_dtype, ScalarType entropy_dtype, float entropy_weight, "
+      "int reduction, bool want_log_probs, bool want_entropy) -> Tensor[]",
+      &policy_loss_backward);
+  m.def(
+      "preference_loss_forward(Tensor log_probs, Tensor cu_seqlens, Tensor? reference_log_probs, "
+      "Tensor? mask, float beta, float margin, float label_smoothing, int kind, bool normalize, "
+      "int reduction) -> (Tensor, Tensor, Tensor)",
+      &preference_loss_forward);
+  m.def(
+      "preference_loss_backward(Tensor grad_loss, Tensor saved, Tensor cu_seqlens, Tensor? mask, "
+      "int[] shape, ScalarType log_probs_dtype, int reduction) -> Tensor",
+      &preference_loss_backward);
+  m.def("grad_norm(Tensor[] tensors) -> Tensor", &grad_norm_op);
+  m.def(
+      "clip_grad_norm(Tensor[] tensors, Tensor(a!)[] out, float max_norm, float eps) -> Tensor",
+      &clip_grad_norm_op);
   m.def("set_recurrent_long_route(int route) -> int", &set_recurrent_long_route);
   m.def("recurrent_long_route() -> int", &recurrent_long_route);
   m.def(
@@ -1874,6 +1908,7 @@ bool advance_varlen_call(const pybind11::object& elapsed, const pybind11::object
 }
 
 #include "head_calls.h"
+#include "step_calls.h"
 
 PYBIND11_MODULE(_flashrwkv_amd_ops, m) {
   namespace py = pybind11;
@@ -1923,6 +1958,11 @@ PYBIND11_MODULE(_flashrwkv_amd_ops, m) {
   m.def("layer_norm_infer_call", &layer_norm_infer_call);
   m.def("layer_norm_train_call", &layer_norm_train_call);
   m.def("linear_loss_call", &linear_loss_call);
+  m.def("linear_log_probs_call", &linear_log_probs_call);
+  m.def("policy_loss_call", &policy_loss_call);
+  m.def("preference_loss_call", &preference_loss_call);
+  m.def("grad_norm_call", &grad_norm_call);
+  m.def("clip_grad_norm_call", &clip_grad_norm_call);
   m.def("recurrent_add_vec_forward_varlen", &recurrent_add_vec_forward_varlen);
   m.def("tmix_kk_a_gate_forward_varlen", &tmix_kk_a_gate_forward_varlen);
   m.def("tmix_lnx_rkvres_xg_forward_varlen", &tmix_lnx_rkvres_xg_forward_varlen);

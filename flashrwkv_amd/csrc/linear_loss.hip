@@ -1,6 +1,7 @@
 // Losses of a language model's head from its hidden rows: softmax cross
-// entropy and distillation from a teacher's top logits, both over the whole
-// vocabulary and both without keeping the logits.
+// entropy, distillation from a teacher's top logits, and the log probability of a
+// token with the entropy beside it, all over the whole vocabulary and without
+// keeping the logits.
 //
 // With z = h W^T (rows i, vocabulary v), s = 1 / T (1 for cross entropy) and a
 // sparse target b_i (one entry 1 for cross entropy; the K shares p_ik =
@@ -9,6 +10,9 @@
 //   loss_i = T^2 (lse_i + sum_k p_ik (log p_ik - s z_i,k))
 //   dL/dz_iv = w_i T (exp(s z_iv - lse_i) - b_iv),  w_i the upstream weight
 //   dh = dz W,  dW = dz^T h.
+// Scores, with log q_iv = s z_iv - lse_i, q = exp(log q) and upstream g_i, e_i:
+//   x_i = log q_i,target,  H_i = -sum_v q_iv log q_iv
+//   dL/dz_iv = s (g_i (b_iv - q_iv) - e_i q_iv (log q_iv + H_i)).
 //
 // Rows that take no part (target = ignore_index; no teacher entry) are left
 // out at the start: the hidden rows of the others are copied together (2 N C
@@ -18,7 +22,8 @@
 // the count end at once.
 //
 // Forward: one product h W^T whose epilogue keeps the maximum and the sum of
-// exponentials of each tile's columns, row by row; a second kernel joins the
+// exponentials of each tile's columns, row by row (for entropies also the sum of
+// exponentials times their exponents); a second kernel joins the
 // tiles. A row's one target logit is taken from the accumulators that hold it;
 // K > 1 of them are dot products of their own (fp32).
 // Backward, for one piece of the vocabulary after another: the product again,
@@ -31,6 +36,7 @@
 // 16 bits before the outputs, as a matrix operand has to be (relative error at
 // most 2^-8 an entry for bf16, independent between entries).
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "capi_internal.h"
@@ -98,6 +104,26 @@ __device__ __forceinline__ float2 joined(float2 a, float2 b, float scale) {
                               b.y * __builtin_amdgcn_exp2f((b.x - top) * scale));
 }
 
+// The same with the sum of 2^d d, d = scale (x - maximum), beside the sum of 2^d:
+// moved to another maximum by t, 2^(d + t) (d + t) = 2^t (2^d d + t 2^d).
+struct Moments {
+  float top, sum, moment;
+};
+
+__device__ __forceinline__ Moments joined(Moments a, Moments b, float scale) {
+  if (b.sum == 0.0f) return a;
+  if (a.sum == 0.0f) return b;
+  const float top = fmaxf(a.top, b.top);
+  const float t = (a.top - top) * scale, u = (b.top - top) * scale;
+  const float x = __builtin_amdgcn_exp2f(t), y = __builtin_amdgcn_exp2f(u);
+  return {top, a.sum * x + b.sum * y,
+          x * fmaf(t, a.sum, a.moment) + y * fmaf(u, b.sum, b.moment)};
+}
+
+// 2^d is 0 in fp32 from here on, and d itself may be -inf: its product with 2^d is
+// taken with this instead.
+constexpr float kLeastExponent = -200.0f;
+
 // Twice: where the two terms of row m of a few stand in dz, 16 rows' first terms
 // and then their second ones, so that a lane of any tile that holds the one holds
 // the other. The hidden rows stand in the same order from kTermRows on.
@@ -121,6 +147,7 @@ struct Saved {
   float* base;      // [N]     sum p log p (by i)
   float* lse;       // [pad]   T log sum exp(z / T), never below the maximum of z (by m)
   float* logit;     // [pad][K] z at the target tokens (by m)
+  float* entropy;   // [pad]   H / log 2, of calls that ask for it (by m)
   uint16_t* hidden; // [pad][C] the rows that take part, zeros after the last up to a tile;
                     // of a few also their term_row order, zeros between, from kTermRows on
 };
@@ -143,6 +170,7 @@ Saved saved_of(char* p, int64_t n, int64_t c, int64_t k, size_t* bytes) {
   const size_t index = l.take(n * k * 4), share = l.take(n * k * 4);
   const size_t target = l.take(n * k * 4), base = l.take(n * 4), lse = l.take(pad * 4);
   const size_t logit = l.take(pad * k * 4), hidden = l.take(pad * c * 2);
+  const size_t entropy = l.take(pad * 4);
   s.count = reinterpret_cast<int32_t*>(p + count);
   s.cut = reinterpret_cast<int32_t*>(p + cut);
   s.done = reinterpret_cast<int32_t*>(p + done);
@@ -156,6 +184,7 @@ Saved saved_of(char* p, int64_t n, int64_t c, int64_t k, size_t* bytes) {
   s.lse = reinterpret_cast<float*>(p + lse);
   s.logit = reinterpret_cast<float*>(p + logit);
   s.hidden = reinterpret_cast<uint16_t*>(p + hidden);
+  s.entropy = reinterpret_cast<float*>(p + entropy);
   *bytes = l.bytes;
   return s;
 }
@@ -382,7 +411,8 @@ struct Teacher {
 struct Rows {
   int32_t n, vocab, steps;
   Sizes sizes;      // launched for it
-  float* row_loss;  // not null: 0 for the rows that take no part
+  float* row_loss;     // not null: 0 for the rows that take no part
+  float* row_entropy;  // the same
 };
 
 __device__ __forceinline__ void note_count(const Rows& d, int32_t count, const Saved& s) {
@@ -415,6 +445,7 @@ __global__ __launch_bounds__(kScanThreads) void number_rows_kernel(Source source
       source.note(i, d.vocab, s);
       s.place[i] = part ? m : -1;
       if (!part && d.row_loss != nullptr) d.row_loss[i] = 0.0f;
+      if (!part && d.row_entropy != nullptr) d.row_entropy[i] = 0.0f;
     }
     if (part) s.row[m] = i;
     before += all;
@@ -488,6 +519,7 @@ __global__ __launch_bounds__(kGatherThreads) void gather_rows_kernel(
         source.note(i, d.vocab, s);
         s.place[i] = part ? m : -1;
         if (!part && d.row_loss != nullptr) d.row_loss[i] = 0.0f;
+        if (!part && d.row_entropy != nullptr) d.row_entropy[i] = 0.0f;
       }
       if (part) s.row[m] = i;
     }
@@ -595,16 +627,19 @@ __device__ __forceinline__ int own_row(int token, int p0, int left) {
 // TFLOP/s) and by the weight's read for few (1 row of 2048 channels, 65536 tokens:
 // 44 to 49 us, 5.5 to 6.1 TB/s). A tile's exponentials take 2 of its 5 us beside the
 // product.
-template <typename G, typename T>
+// kEntropy: also the sum of 2^d d, d = scale (z - maximum), to moments[tile][m].
+template <typename G, typename T, bool kEntropy>
 __global__ __launch_bounds__(gemm::kThreads, 2) void lse_tiles_kernel(
     Operand w, Operand h, int32_t c, float scale, bool one, float2* __restrict__ part,
-    int64_t pad, Saved s) {
+    float* __restrict__ moments, int64_t pad, Saved s) {
   __shared__ __attribute__((aligned(1024))) char smem[G::kLdsBytes];
   __shared__ float maxima[G::kWP][G::kBQ], sums[G::kWP][G::kBQ];
+  __shared__ float weighted[kEntropy ? G::kWP : 1][kEntropy ? G::kBQ : 1];
   int vocab0;
   own_columns<G>(s.cut, vocab0, w.rows);
   w.data += static_cast<int64_t>(vocab0) * w.ld;
   part += vocab0 / 256 * pad;  // behind the large tiles'
+  if constexpr (kEntropy) moments += vocab0 / 256 * pad;
   const int rows = *s.count;
   const int np = tiles_along(w.rows, G::kBP);
   const int nq = tiles_along(rows, G::kBQ), total = np * nq, steps = c / gemm::kStep;
@@ -662,18 +697,27 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void lse_tiles_kernel(
       // -inf everywhere (columns beyond the vocabulary): a sum of 0, not NaN.
       const float from = top == -__builtin_inff() ? 0.0f : top;
       float sum = 0.0f;
+      [[maybe_unused]] float moment = 0.0f;
 #pragma unroll
       for (int i = 0; i < G::TP; ++i) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          sum += __builtin_amdgcn_exp2f((tile.acc[i][j][r] - from) * scale);
+          const float d = (tile.acc[i][j][r] - from) * scale;
+          const float e = __builtin_amdgcn_exp2f(d);
+          sum += e;
+          if constexpr (kEntropy) moment = fmaf(e, fmaxf(d, kLeastExponent), moment);
         }
       }
       sum += __shfl_xor(sum, 16, 64);
       sum += __shfl_xor(sum, 32, 64);
+      if constexpr (kEntropy) {
+        moment += __shfl_xor(moment, 16, 64);
+        moment += __shfl_xor(moment, 32, 64);
+      }
       if ((threadIdx.x & 63) < 16) {
         maxima[wp][G::column(j)] = top;
         sums[wp][G::column(j)] = sum;
+        if constexpr (kEntropy) weighted[wp][G::column(j)] = moment;
       }
     }
     G::arrive();
@@ -701,6 +745,14 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void lse_tiles_kernel(
         if (s != 0.0f) sum += s * __builtin_amdgcn_exp2f((maxima[x][q] - top) * scale);
       }
       part[to + q] = make_float2(top, sum);
+      if constexpr (kEntropy) {
+        Moments all{maxima[0][q], sums[0][q], weighted[0][q]};
+#pragma unroll
+        for (int x = 1; x < G::kWP; ++x) {
+          all = joined(all, Moments{maxima[x][q], sums[x][q], weighted[x][q]}, scale);
+        }
+        moments[to + q] = all.moment;
+      }
     }
     if (id >= total) return;
   }
@@ -710,6 +762,7 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void lse_tiles_kernel(
 // zero for rows and columns that are not there. Bound as the forward is:
 // 8192 x 32768 x 4096 in 1.75 ms, 1260 TFLOP/s. The 256 x 256 form has 10 values more
 // than registers: 44 MB of scratch written beside 537 of dz.
+// kEntropy: dz = 2^l (coef_m + second_m (l log 2 + H_m)), l = scale (z - lse_m).
 //
 // Twice: rounding dz to 16 bits is one error for all elements that a target
 // entry dominates, up to 2^-9 of the entry 1 for bf16. Over many rows such
@@ -719,10 +772,11 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void lse_tiles_kernel(
 // the products add both at no cost (bf16 gradients of 3 weighted rows,
 // 3001 x 512: up to 3.8e-3 off with one term, 1.7e-3 with two, the outputs' own
 // rounding). More rows would need a product of twice as many: they keep one term.
-template <typename G, typename T>
+template <typename G, typename T, bool kEntropy>
 __global__ __launch_bounds__(gemm::kThreads, 2) void softmax_grad_kernel(
     Operand w, Operand h, const int32_t* __restrict__ cut, int32_t c, float scale,
-    const float* __restrict__ coef, uint16_t* __restrict__ dz, int64_t ld, Saved s) {
+    const float* __restrict__ coef, const float* __restrict__ second,
+    uint16_t* __restrict__ dz, int64_t ld, Saved s) {
   __shared__ __attribute__((aligned(1024))) char smem[G::kLdsBytes];
   int at;
   own_columns<G>(cut, at, w.rows);
@@ -741,17 +795,29 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void softmax_grad_kernel(
   while (true) {
     const int p0 = tp * G::kBP, q0 = tq * G::kBQ;
     float from[G::TQ], co[G::TQ];
+    [[maybe_unused]] float slope[G::TQ], entropy[G::TQ];
 #pragma unroll
     for (int j = 0; j < G::TQ; ++j) {
       const int m = q0 + G::column(j);
       from[j] = m < rows ? s.lse[m] : 0.0f;
       co[j] = m < rows ? coef[m] : 0.0f;
+      if constexpr (kEntropy) {
+        slope[j] = m < rows ? second[m] : 0.0f;
+        entropy[j] = m < rows ? s.entropy[m] : 0.0f;
+      }
     }
     tile.multiply(smem);
     // The compiler's wait for these comes here, not behind the loads that
     // begin starts, which it does not count.
 #pragma unroll
-    for (int j = 0; j < G::TQ; ++j) asm volatile("" : "+v"(from[j]), "+v"(co[j]));
+    for (int j = 0; j < G::TQ; ++j) {
+      asm volatile("" : "+v"(from[j]), "+v"(co[j]));
+      if constexpr (kEntropy) {
+        asm volatile("" : "+v"(slope[j]), "+v"(entropy[j]));
+        slope[j] *= kLn2;
+        co[j] = fmaf(slope[j], entropy[j], co[j]);
+      }
+    }
     id += gridDim.x;
     if (id < total) {
       gemm::tile_of(gemm::xcd_run(id, total), np, nq, tp, tq);
@@ -769,7 +835,10 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void softmax_grad_kernel(
           float x[4];
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            x[r] = co[j] * __builtin_amdgcn_exp2f((tile.acc[i][j][r] - from[j]) * scale);
+            const float l = (tile.acc[i][j][r] - from[j]) * scale;
+            float by = co[j];
+            if constexpr (kEntropy) by = fmaf(slope[j], fmaxf(l, kLeastExponent), by);
+            x[r] = by * __builtin_amdgcn_exp2f(l);
             if (!all) x[r] = here && G::row(i) + r < left ? x[r] : 0.0f;
           }
           out[i] = make_uint2(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]));
@@ -806,10 +875,11 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void softmax_grad_kernel(
 // logit, over what the product's epilogue wrote (which as a part of that epilogue
 // costs more, 2 to 4% of a backward, than this launch's 5 us). A thread an entry; equal
 // tokens of a row write the same value.
-template <typename T>
+template <typename T, bool kEntropy>
 __global__ __launch_bounds__(256) void target_grad_kernel(int32_t k, int32_t vocab0,
                                                           int32_t columns, float scale,
                                                           const float* __restrict__ coef,
+                                                          const float* __restrict__ second,
                                                           uint16_t* __restrict__ dz, int64_t ld,
                                                           Saved s) {
   const int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
@@ -819,8 +889,12 @@ __global__ __launch_bounds__(256) void target_grad_kernel(int32_t k, int32_t voc
   const int64_t at = static_cast<int64_t>(s.row[m]) * k + (e - m * k);
   const int32_t v = s.index[at] - vocab0;
   if (s.index[at] < 0 || v < 0 || v >= columns) return;
-  const float p = __builtin_amdgcn_exp2f((s.logit[e] - s.lse[m]) * scale);
-  const float x = coef[m] * (p - s.target[at]);
+  const float l = (s.logit[e] - s.lse[m]) * scale;
+  const float p = __builtin_amdgcn_exp2f(l);
+  float x = coef[m] * (p - s.target[at]);
+  if constexpr (kEntropy) {
+    x = fmaf(second[m] * kLn2 * p, fmaxf(l, kLeastExponent) + s.entropy[m], x);
+  }
   const uint16_t rounded = from_f32<T>(x);
   if (count > kFewest) {
     dz[m * ld + v] = rounded;
@@ -1042,13 +1116,18 @@ __global__ __launch_bounds__(gemm::kThreads, 2) void weight_grad_kernel(
 // The last workgroup to end adds the workgroups' sums, in their order: a launch
 // less than a kernel of its own. Bound by latency: 5 to 7 us up to 1000 rows, 16 us
 // for 8192 rows of 256 tiles (17 MB).
+// kScores: the row's log probability instead of a loss. kEntropy: and its entropy,
+// log sum - sum of 2^d d / sum of 2^d in base 2.
+template <bool kScores, bool kEntropy>
 __global__ __launch_bounds__(1024) void join_tiles_kernel(const float2* __restrict__ part,
+                                                          const float* __restrict__ moments,
                                                           int32_t vocab, int32_t rest_tile,
                                                           int64_t pad, int32_t k, float scale,
                                                           float temperature, bool mean,
-                                                          float* row_loss, float* loss,
-                                                          float* partial, Saved s) {
+                                                          float* row_loss, float* row_entropy,
+                                                          float* loss, float* partial, Saved s) {
   __shared__ float2 shared[32][33];
+  __shared__ float shared_moment[kEntropy ? 32 : 1][33];
   __shared__ float losses[32];
   __shared__ bool last;
   const int q = threadIdx.x & 31, slice = threadIdx.x >> 5;
@@ -1061,27 +1140,43 @@ __global__ __launch_bounds__(1024) void join_tiles_kernel(const float2* __restri
   const int cut = *s.cut;
   const int tiles = tiles_along(cut, 256) + tiles_along(vocab - cut, rest_tile);
   float2 all = make_float2(-__builtin_inff(), 0.0f);
+  [[maybe_unused]] float moment = 0.0f;
+  const auto take = [&](float2 x, float mx) {
+    if constexpr (kEntropy) {
+      const Moments y =
+          joined(Moments{all.x, all.y, moment}, Moments{x.x, x.y, mx}, scale);
+      all = make_float2(y.top, y.sum);
+      moment = y.moment;
+    } else {
+      all = joined(all, x, scale);
+    }
+  };
   if (m < count) {
     for (int t = slice; t < tiles; t += 256) {
       float2 x[8];
+      float mx[8];
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
-        x[u] = t + 32 * u < tiles ? part[(t + 32 * u) * pad + m]
-                                  : make_float2(-__builtin_inff(), 0.0f);
+        const bool here = t + 32 * u < tiles;
+        x[u] = here ? part[(t + 32 * u) * pad + m] : make_float2(-__builtin_inff(), 0.0f);
+        mx[u] = 0.0f;
+        if constexpr (kEntropy) mx[u] = here ? moments[(t + 32 * u) * pad + m] : 0.0f;
       }
 #pragma unroll
-      for (int u = 0; u < 8; ++u) all = joined(all, x[u], scale);
+      for (int u = 0; u < 8; ++u) take(x[u], mx[u]);
     }
   }
   shared[q][slice] = all;
+  if constexpr (kEntropy) shared_moment[q][slice] = moment;
   __syncthreads();
   // 32 rows by 32 slices, turned: 32 lanes join a row's slices.
   const int row = threadIdx.x >> 5, lane = threadIdx.x & 31;
   all = shared[row][lane];
+  if constexpr (kEntropy) moment = shared_moment[row][lane];
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
-    all = joined(all, make_float2(__shfl_xor(all.x, off, 64), __shfl_xor(all.y, off, 64)),
-                 scale);
+    const float2 x = make_float2(__shfl_xor(all.x, off, 64), __shfl_xor(all.y, off, 64));
+    take(x, kEntropy ? __shfl_xor(moment, off, 64) : 0.0f);
   }
   // The lanes' orders differ: the first one's result.
   const float top = __shfl(all.x, threadIdx.x & 32, 64);
@@ -1105,8 +1200,14 @@ __global__ __launch_bounds__(1024) void join_tiles_kernel(const float2* __restri
       // A target out of range makes its row NaN in the backward too.
       s.lse[mine] = term == term ? top + log_sum / scale : term;
       // T twice: T^2 by itself can be beyond fp32.
-      value = temperature * (temperature * ((term + log_sum) * kLn2 + s.base[i]));
+      value = kScores ? (term + log_sum) * -kLn2
+                      : temperature * (temperature * ((term + log_sum) * kLn2 + s.base[i]));
       if (row_loss != nullptr) row_loss[i] = value;
+      if constexpr (kEntropy) {
+        const float entropy = term == term ? log_sum - moment / all.y : term;
+        s.entropy[mine] = entropy;
+        row_entropy[i] = entropy * kLn2;
+      }
     }
     losses[row] = value;
   }
@@ -1131,6 +1232,16 @@ __global__ __launch_bounds__(1024) void join_tiles_kernel(const float2* __restri
   if (threadIdx.x == 0) *loss = mean ? sum / static_cast<float>(count) : sum;
 }
 
+// What the gradients of rows come from: upstream (null: zeros) multiplies (p - b),
+// entropy (null: not asked for) p (log p + H), both by `by` (a score's are -1 / T).
+struct Upstream {
+  const float* loss;
+  const float* entropy;
+  bool per_row, mean;
+  float by;
+  float largest;  // |p (log p + H)| is less than this: log V + 1
+};
+
 // coef[m] multiplies (p - b) of row m in dz, *scale the finished gradients;
 // together they are the row's upstream weight x T (/ count for a mean).
 // One weight for all rows: all of it is in the scale, so that dz is p - b
@@ -1140,9 +1251,9 @@ __global__ __launch_bounds__(1024) void join_tiles_kernel(const float2* __restri
 // 2^up on top of that keeps fp16's small entries normal numbers: |coef (p - b)|
 // is at most 2^14, and 2^-28 of that is the smallest one.
 __global__ __launch_bounds__(kScanThreads) void row_coefficients_kernel(
-    const float* __restrict__ upstream, bool per_row, bool mean, float temperature, int up,
-    Splitting splitting, Pieces pieces, float* __restrict__ coef, float* __restrict__ scale,
-    int32_t* __restrict__ splits, int32_t* __restrict__ cuts, Saved s) {
+    Upstream upstream, int up, Splitting splitting, Pieces pieces, float* __restrict__ coef,
+    float* __restrict__ second, float* __restrict__ scale, int32_t* __restrict__ splits,
+    int32_t* __restrict__ cuts, Saved s) {
   __shared__ float waves[kScanThreads / 64];
   const int n = *s.count;
   if (threadIdx.x < 64) {
@@ -1152,18 +1263,24 @@ __global__ __launch_bounds__(kScanThreads) void row_coefficients_kernel(
     const int which = threadIdx.x - 64;
     cuts[which] = cut_of(pieces.columns[which], n, pieces.steps, pieces.sizes[which]).first;
   }
-  const float by = mean ? temperature / static_cast<float>(n > 0 ? n : 1) : temperature;
+  const float by = upstream.mean ? upstream.by / static_cast<float>(n > 0 ? n : 1) : upstream.by;
   const float lift = ldexpf(1.0f, up);
-  if (!per_row) {
+  if (!upstream.per_row) {
     for (int m = threadIdx.x; m < n; m += kScanThreads) coef[m] = lift;
-    if (threadIdx.x == 0) *scale = *upstream * by / lift;
+    if (threadIdx.x == 0) *scale = *upstream.loss * by / lift;
     return;
   }
+  const auto loss_of = [&](int m) {
+    return upstream.loss != nullptr ? upstream.loss[s.row[m]] * by : 0.0f;
+  };
   // A weight of 1e30 or more, infinite ones among them, has gradients beyond fp16 by
   // itself; the others' power of two is chosen without it, or they would be as well.
   float top = 0.0f;
   for (int m = threadIdx.x; m < n; m += kScanThreads) {
-    const float x = fabsf(upstream[s.row[m]] * by);
+    float x = fabsf(loss_of(m));
+    if (upstream.entropy != nullptr) {
+      x += fabsf(upstream.entropy[s.row[m]] * by) * upstream.largest;
+    }
     top = x < 1e30f ? fmaxf(top, x) : top;
   }
   top = wave_max(top);
@@ -1174,7 +1291,8 @@ __global__ __launch_bounds__(kScanThreads) void row_coefficients_kernel(
   const int exponent = top > 1e-30f ? static_cast<int>(ceilf(__builtin_amdgcn_logf(top))) : 0;
   const float divide = ldexpf(1.0f, up - exponent);
   for (int m = threadIdx.x; m < n; m += kScanThreads) {
-    coef[m] = upstream[s.row[m]] * by * divide;
+    coef[m] = loss_of(m) * divide;
+    if (upstream.entropy != nullptr) second[m] = upstream.entropy[s.row[m]] * by * divide;
   }
   if (threadIdx.x == 0) *scale = ldexpf(1.0f, exponent - up);
 }
@@ -1259,16 +1377,19 @@ int64_t slab_rows(const Plan& plan, int64_t n) {
 struct ForwardWork {
   float2* part;
   float* partial;
+  float* moments;
 };
 
-ForwardWork forward_work(char* p, int64_t n, int64_t vocab, size_t* bytes) {
+ForwardWork forward_work(char* p, int64_t n, int64_t vocab, bool entropy, size_t* bytes) {
   const int64_t pad = round_up(n, kRowPad);
   Layout l;
   const int64_t tile = time_of(size_of(vocab, n)).p;
   const size_t part = l.take((vocab + tile - 1) / tile * pad * 8);
   const size_t partial = l.take(pad / 32 * 4);
+  const size_t moments = l.take(entropy ? (vocab + tile - 1) / tile * pad * 4 : 0);
   *bytes = l.bytes;
-  return {reinterpret_cast<float2*>(p + part), reinterpret_cast<float*>(p + partial)};
+  return {reinterpret_cast<float2*>(p + part), reinterpret_cast<float*>(p + partial),
+          reinterpret_cast<float*>(p + moments)};
 }
 
 struct BackwardWork {
@@ -1278,10 +1399,11 @@ struct BackwardWork {
   int32_t* cuts;
   uint16_t* dz;
   float* slabs;
+  float* second;
 };
 
 BackwardWork backward_work(char* p, int64_t n, int64_t c, const Plan& plan, bool hidden,
-                           size_t* bytes) {
+                           bool entropy, size_t* bytes) {
   const int64_t pad = round_up(n, kRowPad);
   Layout l;
   const size_t coef = l.take(pad * 4), scale = l.take(4), splits = l.take(4);
@@ -1289,10 +1411,12 @@ BackwardWork backward_work(char* p, int64_t n, int64_t c, const Plan& plan, bool
   const size_t dz = l.take(pad * plan.columns * 2);
   const size_t slabs =
       l.take(hidden ? static_cast<size_t>(slab_rows(plan, n)) * c * 4 : 0);
+  const size_t second = l.take(entropy ? pad * 4 : 0);
   *bytes = l.bytes;
   return {reinterpret_cast<float*>(p + coef), reinterpret_cast<float*>(p + scale),
           reinterpret_cast<int32_t*>(p + splits), reinterpret_cast<int32_t*>(p + cuts),
-          reinterpret_cast<uint16_t*>(p + dz), reinterpret_cast<float*>(p + slabs)};
+          reinterpret_cast<uint16_t*>(p + dz), reinterpret_cast<float*>(p + slabs),
+          reinterpret_cast<float*>(p + second)};
 }
 
 struct Shape {
@@ -1340,15 +1464,17 @@ void for_sizes(int32_t vocab, int32_t rows, int32_t steps, F&& f) {
   if (sizes.small) launch(Size::kSmall);
 }
 
-template <typename T, typename Source>
+// kScores: loss takes the log probabilities of rows, entropy their entropies
+// (kEntropy).
+template <typename T, bool kScores, bool kEntropy, typename Source>
 int run_forward(const Shape& d, const Source& source, const void* hidden, const void* weight,
-                float temperature, int reduction, float* loss, const Saved& s,
+                float temperature, int reduction, float* loss, float* entropy, const Saved& s,
                 const ForwardWork& w, hipStream_t stream) {
   const int64_t pad = round_up(d.n, kRowPad);
   const int steps = d.c / gemm::kStep;
   const float scale = kLog2E / temperature;
   float* row_loss = reduction == FRWKV_REDUCE_NONE ? loss : nullptr;
-  const Rows rows{d.n, d.vocab, steps, sizes_of(d.vocab, d.n, steps), row_loss};
+  const Rows rows{d.n, d.vocab, steps, sizes_of(d.vocab, d.n, steps), row_loss, entropy};
   const auto gather = [&](auto* kernel) {
     const int groups = d.k == 1 ? 1 : (d.k + kGather - 1) / kGather;
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(pad), groups), dim3(kGatherThreads), 0,
@@ -1366,17 +1492,17 @@ int run_forward(const Shape& d, const Source& source, const void* hidden, const 
   const Operand b{s.hidden, d.c, static_cast<int32_t>(pad)};
   for_sizes<T>(d.vocab, d.n, steps, [&](auto* tile, int grid) {
     using G = std::remove_pointer_t<decltype(tile)>;
-    hipLaunchKernelGGL((lse_tiles_kernel<G, T>), dim3(grid), dim3(gemm::kThreads), 0, stream, a, b,
-                       d.c, scale, d.k == 1, w.part, pad, s);
+    hipLaunchKernelGGL((lse_tiles_kernel<G, T, kEntropy>), dim3(grid), dim3(gemm::kThreads), 0,
+                       stream, a, b, d.c, scale, d.k == 1, w.part, w.moments, pad, s);
   });
-  hipLaunchKernelGGL(join_tiles_kernel, dim3((d.n + 31) / 32), dim3(1024), 0, stream, w.part,
-                     d.vocab, time_of(size_of(d.vocab, d.n)).p, pad, d.k, scale,
-                     temperature, reduction == FRWKV_REDUCE_MEAN, row_loss,
+  hipLaunchKernelGGL((join_tiles_kernel<kScores, kEntropy>), dim3((d.n + 31) / 32), dim3(1024), 0,
+                     stream, w.part, w.moments, d.vocab, time_of(size_of(d.vocab, d.n)).p, pad,
+                     d.k, scale, temperature, reduction == FRWKV_REDUCE_MEAN, row_loss, entropy,
                      row_loss == nullptr ? loss : nullptr, w.partial, s);
   return check_launch("linear loss forward");
 }
 
-template <typename T>
+template <typename T, bool kEntropy>
 void launch_piece(const Shape& d, const Plan& plan, int piece, const uint16_t* weight,
                   float scale, uint16_t* dh, uint16_t* dw, const Saved& s, const BackwardWork& w,
                   hipStream_t stream) {
@@ -1391,12 +1517,13 @@ void launch_piece(const Shape& d, const Plan& plan, int piece, const uint16_t* w
   const int32_t* cut = w.cuts + (piece + 1 == plan.pieces);
   for_sizes<T>(columns, d.n, d.c / gemm::kStep, [&](auto* tile, int grid) {
     using G = std::remove_pointer_t<decltype(tile)>;
-    hipLaunchKernelGGL((softmax_grad_kernel<G, T>), dim3(grid), dim3(gemm::kThreads), 0, stream,
-                       wp, h, cut, d.c, scale, w.coef, w.dz, ld, s);
+    hipLaunchKernelGGL((softmax_grad_kernel<G, T, kEntropy>), dim3(grid), dim3(gemm::kThreads), 0,
+                       stream, wp, h, cut, d.c, scale, w.coef, w.second, w.dz, ld, s);
   });
   const int64_t entries = static_cast<int64_t>(d.n) * d.k;
-  hipLaunchKernelGGL((target_grad_kernel<T>), dim3(static_cast<unsigned>((entries + 255) / 256)),
-                     dim3(256), 0, stream, d.k, first, columns, scale, w.coef, w.dz, ld, s);
+  hipLaunchKernelGGL((target_grad_kernel<T, kEntropy>),
+                     dim3(static_cast<unsigned>((entries + 255) / 256)), dim3(256), 0, stream, d.k,
+                     first, columns, scale, w.coef, w.second, w.dz, ld, s);
   if (dh != nullptr) {
     const int steps = static_cast<int>(round_up(columns, gemm::kStep) / gemm::kStep);
     with_tile<T, Major::kX, Major::kK>(plan.hidden, [&](auto* tile) {
@@ -1425,22 +1552,29 @@ void launch_piece(const Shape& d, const Plan& plan, int piece, const uint16_t* w
 }
 
 template <typename T>
-int run_backward(const Shape& d, const void* weight, const float* upstream, bool per_row,
-                 bool mean, float temperature, void* dh, void* dw, const Saved& s,
-                 const Plan& plan, const BackwardWork& w, hipStream_t stream) {
+int run_backward(const Shape& d, const void* weight, const Upstream& upstream, float temperature,
+                 void* dh, void* dw, const Saved& s, const Plan& plan, const BackwardWork& w,
+                 hipStream_t stream) {
   const float scale = kLog2E / temperature;
   const int steps = d.c / gemm::kStep, last = d.vocab - (plan.pieces - 1) * plan.columns;
   const Pieces pieces{{plan.columns, last},
                       {sizes_of(plan.columns, d.n, steps), sizes_of(last, d.n, steps)},
                       steps};
   hipLaunchKernelGGL(row_coefficients_kernel, dim3(1), dim3(kScanThreads), 0, stream, upstream,
-                     per_row, mean, temperature, __is_same(T, F16) ? 14 : 0,
+                     __is_same(T, F16) ? 14 : 0,
                      splitting_of(plan.hidden, plan.columns, d.c, slab_rows(plan, d.n)),
-                     pieces,
-                     w.coef, w.scale, w.splits, w.cuts, s);
+                     pieces, w.coef, w.second, w.scale, w.splits, w.cuts, s);
+  const auto piece = [&](auto entropy, int p) {
+    launch_piece<T, decltype(entropy)::value>(d, plan, p, static_cast<const uint16_t*>(weight),
+                                              scale, static_cast<uint16_t*>(dh),
+                                              static_cast<uint16_t*>(dw), s, w, stream);
+  };
   for (int p = 0; p < plan.pieces; ++p) {
-    launch_piece<T>(d, plan, p, static_cast<const uint16_t*>(weight), scale,
-                    static_cast<uint16_t*>(dh), static_cast<uint16_t*>(dw), s, w, stream);
+    if (upstream.entropy != nullptr) {
+      piece(std::true_type{}, p);
+    } else {
+      piece(std::false_type{}, p);
+    }
   }
   if (dh != nullptr) {
     const int64_t quads = static_cast<int64_t>(d.n) * (d.c / 4);
@@ -1528,24 +1662,25 @@ int check_temperature(const char* what, float t) {
   return FRWKV_OK;
 }
 
-template <typename Source>
+template <bool kScores, bool kEntropy, typename Source>
 int forward(int io_dtype, const Shape& d, const Source& source, const void* hidden,
-            const void* weight, float temperature, int reduction, float* loss, const Saved& s,
-            void* workspace, hipStream_t stream) {
+            const void* weight, float temperature, int reduction, float* loss, float* entropy,
+            const Saved& s, void* workspace, hipStream_t stream) {
   size_t need = 0;
-  const ForwardWork w = forward_work(static_cast<char*>(workspace), d.n, d.vocab, &need);
+  const ForwardWork w =
+      forward_work(static_cast<char*>(workspace), d.n, d.vocab, kEntropy, &need);
   return io_dtype == FRWKV_DTYPE_F16
-             ? run_forward<F16>(d, source, hidden, weight, temperature, reduction, loss, s, w,
-                                stream)
-             : run_forward<Bf16>(d, source, hidden, weight, temperature, reduction, loss, s, w,
-                                 stream);
+             ? run_forward<F16, kScores, kEntropy>(d, source, hidden, weight, temperature,
+                                                   reduction, loss, entropy, s, w, stream)
+             : run_forward<Bf16, kScores, kEntropy>(d, source, hidden, weight, temperature,
+                                                    reduction, loss, entropy, s, w, stream);
 }
 
-// The checks that both forwards share, and the layout of what they leave.
+// The checks that the forwards share, and the layout of what they leave.
 int begin_forward(const char* what, int io_dtype, int64_t n, int64_t c, int64_t vocab, int64_t k,
                   const void* hidden, const void* weight, int reduction, const float* loss,
-                  void* saved, size_t saved_bytes, void* workspace, size_t workspace_bytes,
-                  Saved* s) {
+                  bool entropy, void* saved, size_t saved_bytes, void* workspace,
+                  size_t workspace_bytes, Saved* s) {
   if (!hidden || !weight || !loss) {
     return set_error(FRWKV_ERR_INVALID_ARGUMENT, "%s: null pointer argument", what);
   }
@@ -1560,8 +1695,42 @@ int begin_forward(const char* what, int io_dtype, int64_t n, int64_t c, int64_t 
   *s = saved_of(static_cast<char*>(saved), n, c, k, &need);
   rc = check_memory(what, "saved", saved, saved_bytes, need);
   if (rc != FRWKV_OK) return rc;
-  (void)forward_work(nullptr, n, vocab, &need);
+  (void)forward_work(nullptr, n, vocab, entropy, &need);
   return check_memory(what, "workspace", workspace, workspace_bytes, need);
+}
+
+int backward(const char* what, int io_dtype, int64_t rows, int64_t channels, int64_t vocab,
+             int64_t top, const void* weight, float temperature, const Upstream& upstream,
+             const void* saved, size_t saved_bytes, void* grad_hidden, void* grad_weight,
+             void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_shape(what, io_dtype, rows, channels, vocab, top);
+  if (rc == FRWKV_OK) rc = check_temperature(what, temperature);
+  if (rc != FRWKV_OK) return rc;
+  if (!aligned16(weight) || !aligned16(grad_hidden) || !aligned16(grad_weight)) {
+    return set_error(FRWKV_ERR_INVALID_ARGUMENT,
+                     "%s: weight and gradients must be 16-byte aligned", what);
+  }
+  size_t need = 0;
+  // The forward's buffer is only read here.
+  const Saved s = saved_of(const_cast<char*>(static_cast<const char*>(saved)), rows, channels,
+                           top, &need);
+  rc = check_memory(what, "saved", saved, saved_bytes, need);
+  if (rc != FRWKV_OK) return rc;
+  const Plan plan = plan_of(rows, channels, vocab);
+  const BackwardWork w = backward_work(static_cast<char*>(workspace), rows, channels, plan,
+                                       grad_hidden != nullptr, upstream.entropy != nullptr,
+                                       &need);
+  rc = check_memory(what, "workspace", workspace, workspace_bytes, need);
+  if (rc != FRWKV_OK) return rc;
+  if (!grad_hidden && !grad_weight) return FRWKV_OK;
+  const Shape d{static_cast<int32_t>(rows), static_cast<int32_t>(channels),
+                static_cast<int32_t>(vocab), static_cast<int32_t>(top)};
+  const hipStream_t q = static_cast<hipStream_t>(stream);
+  return io_dtype == FRWKV_DTYPE_F16
+             ? run_backward<F16>(d, weight, upstream, temperature, grad_hidden, grad_weight, s,
+                                 plan, w, q)
+             : run_backward<Bf16>(d, weight, upstream, temperature, grad_hidden, grad_weight, s,
+                                  plan, w, q);
 }
 
 }  // namespace
@@ -1581,7 +1750,7 @@ size_t frwkv_linear_loss_forward_workspace_bytes(int64_t rows, int64_t vocab) {
   using namespace frwkv;
   if (!sizes_fit(rows, gemm::kStep, vocab, 1)) return 0;
   size_t bytes = 0;
-  (void)frwkv::forward_work(nullptr, rows, vocab, &bytes);
+  (void)frwkv::forward_work(nullptr, rows, vocab, false, &bytes);
   return bytes;
 }
 
@@ -1591,7 +1760,7 @@ size_t frwkv_linear_loss_backward_workspace_bytes(int64_t rows, int64_t channels
   if (!sizes_fit(rows, channels, vocab, 1)) return 0;
   size_t bytes = 0;
   (void)frwkv::backward_work(nullptr, rows, channels, frwkv::plan_of(rows, channels, vocab),
-                             want_grad_hidden != 0, &bytes);
+                             want_grad_hidden != 0, false, &bytes);
   return bytes;
 }
 
@@ -1623,8 +1792,8 @@ int frwkv_linear_cross_entropy_forward(int io_dtype, int64_t rows, int64_t chann
   const char* what = "frwkv_linear_cross_entropy_forward";
   Saved s;
   const int rc = begin_forward(what, io_dtype, rows, channels, vocab, 1, hidden, weight,
-                               reduction, loss, saved, saved_bytes, workspace, workspace_bytes,
-                               &s);
+                               reduction, loss, false, saved, saved_bytes, workspace,
+                               workspace_bytes, &s);
   if (rc != FRWKV_OK) return rc;
   if (!targets || (target_bytes != 4 && target_bytes != 8)) {
     return set_error(FRWKV_ERR_INVALID_ARGUMENT, "%s: targets must be int32 or int64", what);
@@ -1634,10 +1803,64 @@ int frwkv_linear_cross_entropy_forward(int io_dtype, int64_t rows, int64_t chann
   const Shape d{n, static_cast<int32_t>(channels), v, 1};
   if (target_bytes == 8) {
     const Labels<int64_t> labels{static_cast<const int64_t*>(targets), ignore_index};
-    return forward(io_dtype, d, labels, hidden, weight, 1.0f, reduction, loss, s, workspace, q);
+    return forward<false, false>(io_dtype, d, labels, hidden, weight, 1.0f, reduction, loss,
+                                 nullptr, s, workspace, q);
   }
   const Labels<int32_t> labels{static_cast<const int32_t*>(targets), ignore_index};
-  return forward(io_dtype, d, labels, hidden, weight, 1.0f, reduction, loss, s, workspace, q);
+  return forward<false, false>(io_dtype, d, labels, hidden, weight, 1.0f, reduction, loss, nullptr,
+                               s, workspace, q);
+}
+
+size_t frwkv_linear_log_probs_forward_workspace_bytes(int64_t rows, int64_t vocab,
+                                                      int want_entropy) {
+  using namespace frwkv;
+  if (!sizes_fit(rows, gemm::kStep, vocab, 1)) return 0;
+  size_t bytes = 0;
+  (void)frwkv::forward_work(nullptr, rows, vocab, want_entropy != 0, &bytes);
+  return bytes;
+}
+
+size_t frwkv_linear_log_probs_backward_workspace_bytes(int64_t rows, int64_t channels,
+                                                       int64_t vocab, int want_grad_hidden,
+                                                       int with_grad_entropy) {
+  using namespace frwkv;
+  if (!sizes_fit(rows, channels, vocab, 1)) return 0;
+  size_t bytes = 0;
+  (void)frwkv::backward_work(nullptr, rows, channels, frwkv::plan_of(rows, channels, vocab),
+                             want_grad_hidden != 0, with_grad_entropy != 0, &bytes);
+  return bytes;
+}
+
+int frwkv_linear_log_probs_forward(int io_dtype, int64_t rows, int64_t channels, int64_t vocab,
+                                   const void* hidden, const void* weight, int target_bytes,
+                                   const void* targets, int64_t ignore_index, float temperature,
+                                   float* log_probs, float* entropy, void* saved,
+                                   size_t saved_bytes, void* workspace, size_t workspace_bytes,
+                                   void* stream) {
+  using namespace frwkv;
+  const char* what = "frwkv_linear_log_probs_forward";
+  Saved s;
+  int rc = begin_forward(what, io_dtype, rows, channels, vocab, 1, hidden, weight,
+                         FRWKV_REDUCE_NONE, log_probs, entropy != nullptr, saved, saved_bytes,
+                         workspace, workspace_bytes, &s);
+  if (rc == FRWKV_OK) rc = check_temperature(what, temperature);
+  if (rc != FRWKV_OK) return rc;
+  if (!targets || (target_bytes != 4 && target_bytes != 8)) {
+    return set_error(FRWKV_ERR_INVALID_ARGUMENT, "%s: targets must be int32 or int64", what);
+  }
+  const hipStream_t q = static_cast<hipStream_t>(stream);
+  const Shape d{static_cast<int32_t>(rows), static_cast<int32_t>(channels),
+                static_cast<int32_t>(vocab), 1};
+  const auto run = [&](const auto& labels) {
+    return entropy != nullptr
+               ? forward<true, true>(io_dtype, d, labels, hidden, weight, temperature,
+                                     FRWKV_REDUCE_NONE, log_probs, entropy, s, workspace, q)
+               : forward<true, false>(io_dtype, d, labels, hidden, weight, temperature,
+                                      FRWKV_REDUCE_NONE, log_probs, nullptr, s, workspace, q);
+  };
+  return target_bytes == 8
+             ? run(Labels<int64_t>{static_cast<const int64_t*>(targets), ignore_index})
+             : run(Labels<int32_t>{static_cast<const int32_t*>(targets), ignore_index});
 }
 
 int frwkv_linear_topk_distillation_forward(
@@ -1649,7 +1872,7 @@ int frwkv_linear_topk_distillation_forward(
   const char* what = "frwkv_linear_topk_distillation_forward";
   Saved s;
   int rc = begin_forward(what, io_dtype, rows, channels, vocab, top, hidden, weight, reduction,
-                         loss, saved, saved_bytes, workspace, workspace_bytes, &s);
+                         loss, false, saved, saved_bytes, workspace, workspace_bytes, &s);
   if (rc == FRWKV_OK) rc = check_temperature(what, temperature);
   if (rc != FRWKV_OK) return rc;
   if (!teacher_logits || (teacher_dtype != FRWKV_DTYPE_F32 && teacher_dtype != FRWKV_DTYPE_F16 &&
@@ -1687,8 +1910,9 @@ int frwkv_linear_topk_distillation_forward(
   } else {
     with_index(Bf16{});
   }
-  return forward(io_dtype, Shape{n, static_cast<int32_t>(channels), v, k}, Teacher{s.part},
-                 hidden, weight, temperature, reduction, loss, s, workspace, q);
+  return forward<false, false>(io_dtype, Shape{n, static_cast<int32_t>(channels), v, k},
+                               Teacher{s.part}, hidden, weight, temperature, reduction, loss,
+                               nullptr, s, workspace, q);
 }
 
 int frwkv_linear_loss_backward(int io_dtype, int64_t rows, int64_t channels, int64_t vocab,
@@ -1701,35 +1925,29 @@ int frwkv_linear_loss_backward(int io_dtype, int64_t rows, int64_t channels, int
   if (!weight || !grad_loss) {
     return set_error(FRWKV_ERR_INVALID_ARGUMENT, "%s: null pointer argument", what);
   }
-  int rc = check_shape(what, io_dtype, rows, channels, vocab, top);
-  if (rc == FRWKV_OK) rc = check_reduction(what, reduction);
-  if (rc == FRWKV_OK) rc = check_temperature(what, temperature);
+  const int rc = check_reduction(what, reduction);
   if (rc != FRWKV_OK) return rc;
-  if (!aligned16(weight) || !aligned16(grad_hidden) || !aligned16(grad_weight)) {
-    return set_error(FRWKV_ERR_INVALID_ARGUMENT,
-                     "%s: weight and gradients must be 16-byte aligned", what);
+  const Upstream upstream{grad_loss, nullptr, reduction == FRWKV_REDUCE_NONE,
+                          reduction == FRWKV_REDUCE_MEAN, temperature, 0.0f};
+  return backward(what, io_dtype, rows, channels, vocab, top, weight, temperature, upstream, saved,
+                  saved_bytes, grad_hidden, grad_weight, workspace, workspace_bytes, stream);
+}
+
+int frwkv_linear_log_probs_backward(int io_dtype, int64_t rows, int64_t channels, int64_t vocab,
+                                    const void* weight, float temperature,
+                                    const float* grad_log_probs, const float* grad_entropy,
+                                    const void* saved, size_t saved_bytes, void* grad_hidden,
+                                    void* grad_weight, void* workspace, size_t workspace_bytes,
+                                    void* stream) {
+  using namespace frwkv;
+  const char* what = "frwkv_linear_log_probs_backward";
+  if (!weight || (!grad_log_probs && !grad_entropy)) {
+    return set_error(FRWKV_ERR_INVALID_ARGUMENT, "%s: null pointer argument", what);
   }
-  size_t need = 0;
-  // The forward's buffer is only read here.
-  const Saved s = saved_of(const_cast<char*>(static_cast<const char*>(saved)), rows, channels,
-                           top, &need);
-  rc = check_memory(what, "saved", saved, saved_bytes, need);
-  if (rc != FRWKV_OK) return rc;
-  const Plan plan = plan_of(rows, channels, vocab);
-  const BackwardWork w = backward_work(static_cast<char*>(workspace), rows, channels, plan,
-                                       grad_hidden != nullptr, &need);
-  rc = check_memory(what, "workspace", workspace, workspace_bytes, need);
-  if (rc != FRWKV_OK) return rc;
-  if (!grad_hidden && !grad_weight) return FRWKV_OK;
-  const bool mean = reduction == FRWKV_REDUCE_MEAN, per_row = reduction == FRWKV_REDUCE_NONE;
-  const Shape d{static_cast<int32_t>(rows), static_cast<int32_t>(channels),
-                static_cast<int32_t>(vocab), static_cast<int32_t>(top)};
-  const hipStream_t q = static_cast<hipStream_t>(stream);
-  return io_dtype == FRWKV_DTYPE_F16
-             ? run_backward<F16>(d, weight, grad_loss, per_row, mean, temperature, grad_hidden,
-                                 grad_weight, s, plan, w, q)
-             : run_backward<Bf16>(d, weight, grad_loss, per_row, mean, temperature, grad_hidden,
-                                  grad_weight, s, plan, w, q);
+  const Upstream upstream{grad_log_probs, grad_entropy, true, false, -1.0f / temperature,
+                          std::log(static_cast<float>(vocab)) + 1.0f};
+  return backward(what, io_dtype, rows, channels, vocab, 1, weight, temperature, upstream, saved,
+                  saved_bytes, grad_hidden, grad_weight, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

@@ -1,6 +1,6 @@
-"""Losses of a language model's head, from its hidden rows.
+"""Losses of a language model's head, from its hidden rows, and of its tokens.
 
-Both take the hidden rows ``[..., C]`` (after the last norm) and the head's
+The first three take the hidden rows ``[..., C]`` (after the last norm) and the head's
 weight ``[V, C]`` instead of logits: the product, the softmax over the
 vocabulary and the loss run piece by piece, and the ``[rows, V]`` logits never
 exist in memory, forward or backward.
@@ -10,8 +10,13 @@ exist in memory, forward or backward.
   (minus the log probability of each token).
 * :func:`pretrain_linear_topk_distillation`: the divergence from a teacher that
   is known by its K largest logits a row.
+* :func:`pretrain_linear_log_probs`: the log probability of one token a row at a
+  sampling temperature, and the entropy beside it; not a loss, but what the two
+  below are taken from.
+* :func:`pretrain_policy_loss`, :func:`pretrain_preference_loss`: losses over
+  packed sequences of such log probabilities (:mod:`.sequences`).
 
-float16 and bfloat16, fp32 sums, ``C`` a multiple of 64, any ``V`` and row
+The head's are of float16 and bfloat16, fp32 sums, ``C`` a multiple of 64, any ``V`` and row
 count. Rows that take no part (``ignore_index``; no teacher entry) are left out
 before the products, so they cost nothing there and what they hold, NaN
 included, reaches neither the loss nor a gradient. Only what needs a gradient
@@ -20,7 +25,7 @@ synchronises with the host, so a token out of range cannot be raised as an
 error: it makes its row's loss, and with it the gradients, NaN.
 
 Sums are in a fixed order: the same call gives the same bits. The kernels are
-in ``csrc/linear_loss.hip``; the reference's loss operators are not part of
+in ``csrc/linear_loss.hip`` and ``csrc/sequence_loss.hip``; the reference's loss operators are not part of
 this package, and these do not take their names.
 """
 
@@ -30,6 +35,7 @@ import torch
 
 from .. import _contract as C
 from .._contract import check, is_tensor
+from .sequences import pretrain_policy_loss, pretrain_preference_loss
 
 REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 MAX_TOP = 1024
@@ -51,12 +57,9 @@ HEAD = (
     check("weight", C.same_device_as("hidden"), ValueError, "weight must share hidden's device"),
     check("weight", lambda x, ns: x.ndim == 2 and x.shape[0] > 0
           and x.shape[1] == ns["hidden"].shape[-1], ValueError, "weight must have shape [V,C]"),
-    check("reduction", C.one_of(tuple(REDUCTIONS)), ValueError,
-          "reduction must be one of 'none', 'mean' or 'sum'"),
 )
 
-CROSS_ENTROPY = (
-    *HEAD,
+_TARGETS = (
     is_tensor("targets"),
     check("targets", C.dtype_is(*_INDEX), TypeError, "targets must be int32 or int64"),
     check("targets", C.cuda_contiguous, ValueError, "targets must be CUDA and contiguous"),
@@ -67,8 +70,23 @@ CROSS_ENTROPY = (
     check("ignore_index", C.plain_int, TypeError, "ignore_index must be an int"),
 )
 
+_TEMPERATURE = (
+    check("temperature", lambda x, ns: C.finite_number(x, ns) and not isinstance(x, bool)
+          and 1e-30 < x < 1e30, ValueError, "temperature must be positive and finite"),
+)
+
+_REDUCTION = (
+    check("reduction", C.one_of(tuple(REDUCTIONS)), ValueError,
+          "reduction must be one of 'none', 'mean' or 'sum'"),
+)
+
+CROSS_ENTROPY = (*HEAD, *_REDUCTION, *_TARGETS)
+
+LOG_PROBS = (*HEAD, *_TARGETS, *_TEMPERATURE)
+
 DISTILLATION = (
     *HEAD,
+    *_REDUCTION,
     is_tensor("teacher_logits"),
     check("teacher_logits", C.dtype_is(torch.float32, torch.float16, torch.bfloat16), TypeError,
           "teacher_logits must be float32, float16 or bfloat16"),
@@ -89,8 +107,7 @@ DISTILLATION = (
           "teacher_indices must share hidden's device"),
     check("teacher_indices", C.same_shape_as("teacher_logits"), ValueError,
           "teacher_indices must match teacher_logits"),
-    check("temperature", lambda x, ns: C.finite_number(x, ns) and not isinstance(x, bool)
-          and 1e-30 < x < 1e30, ValueError, "temperature must be positive and finite"),
+    *_TEMPERATURE,
 )
 
 
@@ -133,11 +150,51 @@ class _LinearLoss(torch.autograd.Function):
         return (*grads, None, None, None, None)
 
 
-def _run(name, hidden, weight, launch, top, temperature, reduction):
+class _LinearLogProbs(torch.autograd.Function):
+    """The same for log probabilities and entropies."""
+
+    @staticmethod
+    def forward(ctx, hidden, weight, launch, temperature, entropy):
+        ctx.set_materialize_grads(False)
+        ctx.shape, ctx.temperature = hidden.shape, temperature
+        ctx.rows = hidden.numel() // hidden.shape[-1]
+        if ctx.rows == 0:
+            ctx.save_for_backward(weight)
+            return tuple(torch.zeros(hidden.shape[:-1], device=hidden.device,
+                                     dtype=torch.float32) for _ in range(1 + entropy))
+        *out, saved = launch(hidden, weight)
+        ctx.save_for_backward(weight, saved)
+        return tuple(out)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, *upstream):
+        weight, *saved = ctx.saved_tensors
+        want = ctx.needs_input_grad[:2]
+        grads = [None, None]
+        upstream = [None if g is None else g.contiguous() for g in (*upstream, None)][:2]
+        if ctx.rows == 0:
+            made = [weight.new_empty(ctx.shape), torch.zeros_like(weight)]
+            grads = [g if w else None for g, w in zip(made, want)]
+        elif any(g is not None for g in upstream):
+            made = C.native().linear_log_probs_backward(*upstream, weight, *saved, ctx.rows,
+                                                        ctx.temperature, *want)
+            if want[0]:
+                grads[0] = made[0].view(ctx.shape)
+            if want[1]:
+                grads[1] = made[-1]
+        return (*grads, None, None, None)
+
+
+def _refuse_capture(name):
     C.native()
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError(f"{name} does not run under HIP graph capture: training steps are "
                            "not validated inside a captured graph")
+
+
+def _run(name, hidden, weight, launch, top, temperature, reduction):
+    _refuse_capture(name)
     return _LinearLoss.apply(hidden, weight, launch, top, float(temperature),
                              REDUCTIONS[reduction])
 
@@ -214,4 +271,45 @@ def pretrain_linear_topk_distillation(
                 teacher_logits.shape[-1], temperature, reduction)
 
 
-__all__ = ["pretrain_linear_cross_entropy", "pretrain_linear_topk_distillation"]
+def pretrain_linear_log_probs(
+    hidden: torch.Tensor,
+    weight: torch.Tensor,
+    targets: torch.Tensor,
+    *,
+    temperature: float = 1.0,
+    ignore_index: int = -100,
+    entropy: bool = False,
+) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
+    """Log probability of each row's token under ``q = softmax(hidden weight^T /
+    temperature)``, and with ``entropy=True`` (log_probs, entropy), ``-sum q log q``
+    of each row beside it.
+
+    ``targets`` as in :func:`pretrain_linear_cross_entropy`, whose loss at
+    temperature 1 is minus the first. fp32 in ``targets``' shape; both are 0 for rows
+    with ``ignore_index`` and NaN for a token out of range. Gradients for hidden and weight from
+    either or both.
+    """
+    call = C.whole_call("linear_log_probs_call")
+    if call:
+        got = call(hidden, weight, targets, ignore_index, temperature, bool(entropy))
+        if got is not None:
+            return got if entropy else got[0]
+    C.enforce(LOG_PROBS, {"hidden": hidden, "weight": weight, "targets": targets,
+                          "temperature": temperature, "ignore_index": ignore_index})
+    _refuse_capture("pretrain_linear_log_probs")
+
+    def launch(h, w):
+        return C.native().linear_log_probs_forward(h, w, targets, ignore_index, temperature,
+                                                   entropy)
+
+    got = _LinearLogProbs.apply(hidden, weight, launch, float(temperature), bool(entropy))
+    return got if entropy else got[0]
+
+
+__all__ = [
+    "pretrain_linear_cross_entropy",
+    "pretrain_linear_log_probs",
+    "pretrain_linear_topk_distillation",
+    "pretrain_policy_loss",
+    "pretrain_preference_loss",
+]

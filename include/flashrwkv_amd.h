@@ -53,7 +53,14 @@ enum frwkv_dtype {
 enum frwkv_reduction {
   FRWKV_REDUCE_NONE = 0,
   FRWKV_REDUCE_MEAN = 1,
-  FRWKV_REDUCE_SUM = 2
+  FRWKV_REDUCE_SUM = 2,
+  FRWKV_REDUCE_SEQUENCE_MEAN = 3 /* the policy loss only */
+};
+
+enum frwkv_preference_kind {
+  FRWKV_PREFERENCE_SIGMOID = 0,
+  FRWKV_PREFERENCE_HINGE = 1,
+  FRWKV_PREFERENCE_SQUARED = 2
 };
 
 enum frwkv_decay_mode {
@@ -712,6 +719,123 @@ int frwkv_linear_loss_backward(int io_dtype, int64_t rows, int64_t channels, int
                                const float* grad_loss, const void* saved, size_t saved_bytes,
                                void* grad_hidden, void* grad_weight, void* workspace,
                                size_t workspace_bytes, void* stream);
+
+/*
+ * Log probabilities of a head's tokens from its hidden rows, and the entropies of
+ * its distributions: q = softmax(hidden weight^T / temperature), log_probs[i] =
+ * log q[targets[i]] and, where entropy is not NULL, entropy[i] = -sum q log q
+ * (both fp32 [rows]; 0 for rows whose target is ignore_index, NaN for a target out of
+ * range). Operands, sizes and saved (frwkv_linear_loss_saved_bytes with top 1) as
+ * for frwkv_linear_cross_entropy_forward.
+ *
+ * frwkv_linear_log_probs_backward: grad_log_probs and grad_entropy fp32 [rows],
+ * either NULL for zeros, not both (grad_entropy only where the forward gave
+ * entropies); grad_hidden and grad_weight as in frwkv_linear_loss_backward. No
+ * counterpart in the reference.
+ */
+size_t frwkv_linear_log_probs_forward_workspace_bytes(int64_t rows, int64_t vocab,
+                                                      int want_entropy);
+size_t frwkv_linear_log_probs_backward_workspace_bytes(int64_t rows, int64_t channels,
+                                                       int64_t vocab, int want_grad_hidden,
+                                                       int with_grad_entropy);
+int frwkv_linear_log_probs_forward(int io_dtype, int64_t rows, int64_t channels, int64_t vocab,
+                                   const void* hidden, const void* weight, int target_bytes,
+                                   const void* targets, int64_t ignore_index, float temperature,
+                                   float* log_probs, float* entropy, void* saved,
+                                   size_t saved_bytes, void* workspace, size_t workspace_bytes,
+                                   void* stream);
+int frwkv_linear_log_probs_backward(int io_dtype, int64_t rows, int64_t channels, int64_t vocab,
+                                    const void* weight, float temperature,
+                                    const float* grad_log_probs, const float* grad_entropy,
+                                    const void* saved, size_t saved_bytes, void* grad_hidden,
+                                    void* grad_weight, void* workspace, size_t workspace_bytes,
+                                    void* stream);
+
+/*
+ * Losses over packed sequences of token log probabilities. Vectors are [tokens]
+ * of float32, float16 or bfloat16, each of its own dtype; cu_seqlens int32
+ * [sequences + 1] on the device (0, not falling, at most tokens; tokens behind the
+ * last offset take no part); mask one byte a token (NULL: all take part). What
+ * stands in tokens that take no part, NaN included, reaches nothing; their
+ * gradients are 0. Offsets that may not be make a reduced loss and the gradients
+ * NaN. Sums are in 64 bits and in a fixed order. No counterpart in the reference.
+ *
+ * frwkv_policy_loss_forward: with d = log_probs - old_log_probs, r = exp(d) and
+ * advantage A (one a token or, advantages_per_sequence, one a sequence) a token's
+ * loss is -min(r A, clamp(r, 1 - clip_low, 1 + clip_high) A), for A < 0 and
+ * dual_clip > 1 (0: none) at most -dual_clip A, plus kl_weight k3(reference -
+ * log_probs), k3(x) = exp(x) - 1 - x, minus entropy_weight entropy (reference and
+ * entropy NULL: none). loss: fp32 [tokens] (FRWKV_REDUCE_NONE), or [1] with their
+ * mean or sum over tokens that take part, or FRWKV_REDUCE_SEQUENCE_MEAN, the mean of
+ * each sequence's mean over sequences with such tokens; 0 without any. metrics fp32
+ * [4] (NULL: none): means over those tokens of r, of whether the gradient is clipped,
+ * of k3(d) and of the reference's k3. cu_seqlens may be NULL with 0 sequences.
+ * saved (256-byte aligned) is what the backward reads; want_slopes 0 leaves it
+ * without what a backward needs.
+ *
+ * frwkv_preference_loss_forward: sequences 2p (chosen) and 2p + 1 (rejected) of
+ * pair p; s the sum (normalize: the mean) of log_probs - reference_log_probs (NULL: 0)
+ * over a sequence's tokens, m = beta (s_chosen - s_rejected) - margin, loss by kind:
+ * -(1 - label_smoothing) log sigmoid(m) - label_smoothing log sigmoid(-m),
+ * max(0, 1 - m) or ((m - 1/2) / beta)^2. Pairs of which one side has no token take
+ * no part (loss 0, not counted). loss fp32 [pairs] or [1], rewards fp32 [pairs, 2]:
+ * beta s. The backward's gradients are of the log probabilities alone.
+ */
+size_t frwkv_policy_loss_saved_bytes(int64_t tokens, int64_t sequences);
+size_t frwkv_preference_loss_saved_bytes(int64_t pairs);
+/* Workspace of either forward (a preference loss has 2 pairs sequences). */
+size_t frwkv_sequence_loss_workspace_bytes(int64_t tokens, int64_t sequences);
+int frwkv_policy_loss_forward(int64_t tokens, int64_t sequences, const int32_t* cu_seqlens,
+                              const uint8_t* mask, int log_probs_dtype, const void* log_probs,
+                              int old_dtype, const void* old_log_probs, int advantages_dtype,
+                              const void* advantages, int advantages_per_sequence,
+                              int reference_dtype, const void* reference_log_probs,
+                              int entropy_dtype, const void* entropy, double clip_low,
+                              double clip_high, double dual_clip, float kl_weight,
+                              float entropy_weight, int reduction, float* loss, float* metrics,
+                              int want_slopes, void* saved, size_t saved_bytes, void* workspace,
+                              size_t workspace_bytes, void* stream);
+int frwkv_policy_loss_backward(int64_t tokens, int64_t sequences, const int32_t* cu_seqlens,
+                               const uint8_t* mask, float entropy_weight, int reduction,
+                               const float* grad_loss, const void* saved, size_t saved_bytes,
+                               int log_probs_dtype, void* grad_log_probs, int entropy_dtype,
+                               void* grad_entropy, void* stream);
+int frwkv_preference_loss_forward(int64_t tokens, int64_t pairs, const int32_t* cu_seqlens,
+                                  const uint8_t* mask, int log_probs_dtype,
+                                  const void* log_probs, int reference_dtype,
+                                  const void* reference_log_probs, double beta, double margin,
+                                  double label_smoothing, int kind, int normalize, int reduction,
+                                  float* loss, float* rewards, void* saved, size_t saved_bytes,
+                                  void* workspace, size_t workspace_bytes, void* stream);
+int frwkv_preference_loss_backward(int64_t tokens, int64_t pairs, const int32_t* cu_seqlens,
+                                   const uint8_t* mask, int reduction, const float* grad_loss,
+                                   const void* saved, size_t saved_bytes, int log_probs_dtype,
+                                   void* grad_log_probs, void* stream);
+
+/*
+ * Norm of many gradients together and clipping by it. A list on the host, of any
+ * length (also none), copied into the launches' arguments; the tensors' elements
+ * are contiguous, of float32, float16 or bfloat16 (FRWKV_DTYPE_*) each.
+ *
+ * frwkv_grad_norm: norm fp32 [1] = sqrt(sum x^2), squares and sums in 64 bits, in a
+ * fixed order. frwkv_grad_clip: also out = x min(1, max_norm / (norm + eps)),
+ * rounded to out_dtype; out may be data itself (with its dtype), and no other two
+ * may overlap. Where the norm is not finite, out = x. workspace: 256-byte aligned.
+ * No counterpart in the reference.
+ */
+typedef struct frwkv_gradient {
+  const void* data;
+  void* out;
+  int64_t numel;
+  int32_t dtype;
+  int32_t out_dtype;
+} frwkv_gradient;
+
+size_t frwkv_grad_norm_workspace_bytes(int64_t count, const frwkv_gradient* tensors);
+int frwkv_grad_norm(int64_t count, const frwkv_gradient* tensors, float* norm, void* workspace,
+                    size_t workspace_bytes, void* stream);
+int frwkv_grad_clip(int64_t count, const frwkv_gradient* tensors, double max_norm, double eps,
+                    float* norm, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,221 @@
+"""GPU parity of the gradient norm and clipping against 64 bits.
+
+Bounds, before any run: squares and sums are in 64 bits (relative error far below
+2^-40) and the norm is rounded once to 32: 2^-24 of it, 2 2^-24 allowed. The factor is
+rounded once to 32 bits, the product once to 32 bits and once to the output's type:
+2 2^-24 |y| (1 + u) + u |y| and the type's smallest step.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import flashrwkv_amd
+from flashrwkv_amd import capi, pretrain_clip_grad_norm, pretrain_grad_norm
+from oracle import step
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda")
+E = 2.0 ** -24
+ROUND = {torch.float32: 0.0, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+STEP = {torch.float32: 2.0 ** -149, torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -134}
+TYPES = list(ROUND)
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _require_native():
+    if flashrwkv_amd._C is None:
+        pytest.fail("flashrwkv_amd native library is not built (no fallback exists)")
+
+
+def _tensors(shapes, seed, scale=1.0, types=TYPES):
+    gen = torch.Generator().manual_seed(seed)
+    return [(scale * torch.randn(s, generator=gen)).to(types[i % len(types)]).to(DEV)
+            for i, s in enumerate(shapes)]
+
+
+def _check(tensors, got, norm, max_norm, eps=1e-6):
+    want, clipped = step.clip(tensors, max_norm, eps)
+    assert norm.dtype == torch.float32 and norm.shape == ()
+    assert abs(norm.item() - want) <= 2 * E * want
+    for y, x in zip(got, clipped):
+        u = ROUND[y.dtype]
+        allowed = (2 * E * (1 + u) + u) * x.abs() + STEP[y.dtype]
+        assert ((y.double() - x).abs() <= allowed).all()
+
+
+LISTS = {
+    "one element": [(1,)],
+    "one scalar": [()],
+    "small": [(3,), (64, 5), (1, 1, 1), (0,), (7, 0, 3), (8191,), (8192,), (8193,)],
+    "chunks": [(3 * 8192,), (2, 8192 + 8), (50000,), (77,)],
+    "many": [(1 + (i * 37) % 400,) for i in range(500)],
+    "large": [(5_000_003,), (300, 4096), (17,)],
+}
+
+
+@pytest.mark.parametrize("over", [True, False])
+@pytest.mark.parametrize("name", LISTS)
+def test_clip_in_place_and_into_others(name, over):
+    print(f"case {name} over {over}", flush=True)
+    tensors = _tensors(LISTS[name], seed=1)
+    norm = step.clip(tensors, 1.0, 0.0)[0]
+    most = norm * (0.3 if over else 1.5)
+    assert abs(pretrain_grad_norm(tensors).item() - norm) <= 2 * E * norm
+    before = [t.clone() for t in tensors]
+    for types in ([torch.float32], [torch.bfloat16, torch.float16, torch.float32]):
+        out = [torch.full_like(t, math.nan, dtype=types[i % len(types)])
+               for i, t in enumerate(tensors)]
+        _check(tensors, out, pretrain_clip_grad_norm(tensors, most, out=out), most)
+        assert all(torch.equal(a, b) for a, b in zip(tensors, before))
+    got = pretrain_clip_grad_norm(tensors, most)
+    _check(before, tensors, got, most)
+    if not over:
+        assert all(torch.equal(a, b) for a, b in zip(tensors, before))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("offset", [1, 3, 8])
+def test_views_off_16_byte_places(dtype, offset):
+    """Views of one buffer; what stands between them stays."""
+    gen = torch.Generator().manual_seed(offset)
+    flat = torch.randn(60000, generator=gen).to(dtype).to(DEV)
+    spans = [(offset, 5000), (5000 + offset, 20001), (20003 + offset, 20004 + offset),
+             (30000, 50000 - offset)]
+    views = [flat[a:b] for a, b in spans]
+    before, kept = flat.clone(), torch.ones(60000, dtype=torch.bool, device=DEV)
+    for a, b in spans:
+        kept[a:b] = False
+    norm = pretrain_clip_grad_norm(views, 5.0)
+    _check([before[a:b] for a, b in spans], views, norm, 5.0)
+    assert torch.equal(flat[kept], before[kept])
+
+
+def test_orders_of_dimensions():
+    a = torch.randn(30, 70, device=DEV).t()
+    b = torch.randn(4, 6, 5, 8, device=DEV).to(memory_format=torch.channels_last).bfloat16()
+    before = [a.clone(), b.clone()]
+    out = [torch.empty_strided(t.shape, t.stride(), device=DEV) for t in (a, b)]
+    _check(before, out, pretrain_clip_grad_norm([a, b], 2.0, out=out), 2.0)
+    _check(before, [a, b], pretrain_clip_grad_norm((a, b), 2.0), 2.0)
+
+
+def test_values_whose_squares_32_bits_do_not_hold():
+    for value in (1e25, 1e-30):
+        t = torch.full((10000,), value, device=DEV)
+        want = float(t[0].double()) * 100
+        assert abs(pretrain_grad_norm([t]).item() - want) <= 2 * E * want
+        assert pretrain_clip_grad_norm([t], want / 4, eps=0.0).item() == pytest.approx(want)
+        assert torch.allclose(t, torch.full_like(t, value / 4), rtol=4 * E, atol=0)
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_a_norm_that_is_not_finite_scales_nothing(bad):
+    tensors = _tensors([(100,), (9000,)], seed=3)
+    tensors[1][77] = bad
+    before = [t.clone() for t in tensors]
+    norm = pretrain_clip_grad_norm(tensors, 1e-3)
+    assert not math.isfinite(norm.item())
+    out = [torch.zeros_like(t) for t in tensors]
+    pretrain_clip_grad_norm(tensors, 1e-3, out=out)
+    for x, y, z in zip(before, tensors, out):
+        assert torch.equal(x.nan_to_num(7.0), y.nan_to_num(7.0))
+        assert torch.equal(x.nan_to_num(7.0), z.nan_to_num(7.0))
+
+
+def test_zeros_and_a_maximum_of_zero():
+    t = torch.zeros(100, device=DEV)
+    assert pretrain_clip_grad_norm([t], 1.0).item() == 0.0
+    assert pretrain_clip_grad_norm([t], 0.0, eps=0.0).item() == 0.0 and not t.any()
+    u = torch.ones(100, device=DEV)
+    assert pretrain_clip_grad_norm([u], 0.0).item() == 10.0
+    assert not u.any()
+
+
+def test_writes_count_as_such():
+    t = torch.ones(10, device=DEV)
+    version = t._version
+    pretrain_clip_grad_norm([t], 1.0)
+    assert t._version > version
+    p = torch.ones(10, device=DEV, requires_grad=True)
+    y = p * t
+    pretrain_clip_grad_norm([t], 1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+def test_refusals_that_need_a_gpu():
+    a, b = torch.ones(10, device=DEV), torch.ones(10, device=DEV)
+    assert pretrain_grad_norm([a, a]).item() == pytest.approx(math.sqrt(20))
+    for tensors, out in (([a, a], None), ([a[:6], a[5:]], None), ([a, b], [b, a]),
+                         ([a, b], [a, a]), ([a[:5]], [a[2:7]])):
+        with pytest.raises(ValueError, match="overlap"):
+            pretrain_clip_grad_norm(tensors, 1.0, out=out)
+    assert torch.equal(a, b)
+    with pytest.raises(ValueError, match="gaps"):
+        pretrain_grad_norm([a[::2]])
+    with pytest.raises(ValueError, match="gaps"):
+        pretrain_grad_norm([a[:1].expand(4)])
+    leaf = torch.ones(4, device=DEV, requires_grad=True)
+    with pytest.raises(ValueError, match="must not require gradients"):
+        pretrain_clip_grad_norm([leaf], 1.0)
+    with torch.no_grad():
+        pretrain_clip_grad_norm([leaf], 1.0)
+    assert leaf[0].item() == pytest.approx(0.5)
+    with pytest.raises(ValueError, match="share the first tensor's device|CUDA"):
+        pretrain_grad_norm([a, torch.ones(3)])
+    with pytest.raises(ValueError, match="shape and strides"):
+        pretrain_clip_grad_norm([torch.ones(3, 4, device=DEV)], 1.0,
+                                out=[torch.ones(4, 3, device=DEV).t()])
+
+
+def test_calls_repeat_bitwise_on_any_stream_and_in_graphs():
+    tensors = _tensors([(100_003,), (50, 1000)], seed=5)
+    out = [torch.zeros_like(t) for t in tensors]
+    first = pretrain_clip_grad_norm(tensors, 1.0, out=out)
+    kept = [t.clone() for t in out]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        again = pretrain_clip_grad_norm(tensors, 1.0, out=out)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            norm = pretrain_clip_grad_norm(tensors, 1.0, out=out)
+    torch.cuda.current_stream().wait_stream(stream)
+    assert torch.equal(first, again)
+    for k in range(4):
+        for t in tensors:
+            t.mul_(1.0 + k)
+        graph.replay()
+        torch.cuda.synchronize()
+        got, seen = norm.clone(), [t.clone() for t in out]
+        want = pretrain_clip_grad_norm(tensors, 1.0, out=out)
+        assert torch.equal(got, want) and all(torch.equal(a, b) for a, b in zip(out, seen))
+        if k == 0:
+            assert torch.equal(got, first) and all(torch.equal(a, b) for a, b in zip(kept, seen))
+
+
+def test_c_abi_writes_what_the_operators_return():
+    tensors = _tensors([(5000,), (0,), (33, 3)], seed=6)
+    out = [torch.zeros_like(t) for t in tensors]
+    want = pretrain_clip_grad_norm(tensors, 1.0, out=out)
+    norm, got = torch.empty(1, device=DEV), [torch.zeros_like(t) for t in tensors]
+    capi.grad_norm(tensors, norm=norm)
+    assert torch.equal(norm[0], want)
+    capi.grad_clip(tensors, 1.0, norm=norm, out=got)
+    assert torch.equal(norm[0], want) and all(torch.equal(a, b) for a, b in zip(got, out))
+    capi.grad_norm([], norm=norm)
+    assert norm.item() == 0.0
+
+
+def test_subclasses_take_the_tables():
+    class Wrapped(torch.Tensor):
+        pass
+
+    t = torch.ones(100, device=DEV).as_subclass(Wrapped)
+    assert pretrain_grad_norm([t]).item() == 10.0
+    assert pretrain_clip_grad_norm([t], 5.0, eps=0.0).item() == 10.0
+    assert torch.equal(t.as_subclass(torch.Tensor), torch.full((100,), 0.5, device=DEV))
