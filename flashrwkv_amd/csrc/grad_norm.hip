@@ -6,15 +6,24 @@
 // the norm tells the caller.
 //
 // Memory bounds both passes: each tensor is read once for the norm and once more
-// to be scaled. Tensors are cut into chunks of kChunk elements that workgroups
-// take in turn, so that a list of small tensors and one large one are the same
-// work; which tensor a chunk is of stands in the kernel's arguments, kEntries
-// tensors a launch, and no table is copied to the device. Squares are summed in
-// 64 bits: gradients beyond 1.8e19 or below 1e-23 have squares that 32 bits do not
-// hold, and the sum of many of them loses nothing. Workgroups leave one sum each, added in their
-// order: two calls give the same bits.
+// to be scaled. Tensors are cut into units of kUnit elements, so that a list of small
+// tensors and one large one are the same work. Squares are summed in 64 bits: gradients
+// beyond 1.8e19 or below 1e-23 have squares that 32 bits do not hold, and the sum
+// of many of them loses nothing. Workgroups leave one sum each, added in a fixed order:
+// two calls give the same bits. Two forms, by plan_of's rule:
+//
+// Short lists of few elements stand in the kernels' arguments. A workgroup takes a
+// run of consecutive chunks and searches the list for the first of them. All workgroups
+// that scale add up the sums by themselves, which saves the launch that would.
+//
+// Others are written to the workspace by small kernels that take the list in their
+// arguments (nothing is copied from the host, and a captured call keeps its
+// list), with the tensor of each unit beside it. Each unit is scaled by a workgroup
+// of its own, in the order of memory, which the DRAM answers best: bf16 to fp32, 449M
+// elements, 450 us, and 542 in 2048 runs of their own.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "capi_internal.h"
 #include "wkv7_device.h"
@@ -23,23 +32,34 @@ namespace frwkv {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kChunk = 8192;        // elements
-constexpr int kEntries = 112;       // of a launch: 3.5 KB of arguments
-constexpr int kMostGroups = 2048;   // workgroups of a launch
-constexpr int kJoinThreads = 1024;
+constexpr int kUnit = 8 * kThreads;  // elements: eight a thread
+constexpr int kMany = 4;             // units that are read together
+constexpr int kEntries = 112;        // tensors in a launch's arguments: 3.5 KB
+constexpr int kMostGroups = 2048;    // workgroups that sum, eight a CU
 
 struct Entry {
   const void* from;
   void* to;
   int64_t numel;
-  int32_t first;  // chunk
+  int32_t first;  // chunk, or unit
   uint8_t dtype, to_dtype;
   bool aligned, to_aligned;  // to 16 bytes
 };
 
-struct Table {
+struct Entries {
   Entry entry[kEntries];
-  int32_t count, chunks;
+};
+
+// The whole list as a launch sees it.
+struct List {
+  int32_t count, chunks;  // or units
+  bool in_place;  // all of them
+};
+
+// The list in the workspace.
+struct Places {
+  Entry* entry;   // [count]
+  int32_t* owner; // [units]  the entry of a unit
 };
 
 __device__ __forceinline__ double wave_sum(double x) {
@@ -60,26 +80,57 @@ __device__ __forceinline__ double workgroup_sum(double x, double* shared) {
   return sum;
 }
 
-// Eight consecutive elements.
-template <typename T>
-struct Eight {
+typedef uint32_t Word2 __attribute__((ext_vector_type(2)));
+typedef uint32_t Word4 __attribute__((ext_vector_type(4)));
+
+// kPer consecutive elements.
+template <typename T, int kPer>
+struct Pack {
   using S = typename IoTraits<T>::storage;
-  static constexpr int kParts = 8 * sizeof(S) / 16;
-  uint4 part[kParts];
+  static constexpr int kBytes = kPer * sizeof(S);
+  static_assert(kEntries <= kThreads && (kBytes == 8 || kBytes == 16), "one load, one thread an entry");
+  using Word = std::conditional_t<kBytes == 16, Word4, Word2>;
+  Word word;
+  // kStream: past the caches, for what is not read again soon.
+  template <bool kStream>
   __device__ __forceinline__ void load(const void* from, int64_t i) {
-    const uint4* p = reinterpret_cast<const uint4*>(static_cast<const S*>(from) + i);
-#pragma unroll
-    for (int q = 0; q < kParts; ++q) part[q] = p[q];
+    const Word* p = reinterpret_cast<const Word*>(static_cast<const S*>(from) + i);
+    word = kStream ? __builtin_nontemporal_load(p) : *p;
   }
   __device__ __forceinline__ void load_unaligned(const void* from, int64_t i, int64_t left) {
-    S* e = reinterpret_cast<S*>(part);
+    S* e = reinterpret_cast<S*>(&word);
 #pragma unroll
-    for (int q = 0; q < 8; ++q) e[q] = q < left ? static_cast<const S*>(from)[i + q] : S{0};
+    for (int q = 0; q < kPer; ++q) e[q] = q < left ? static_cast<const S*>(from)[i + q] : S{0};
   }
   __device__ __forceinline__ float at(int e) const {
-    return to_f32<T>(reinterpret_cast<const S*>(part)[e]);
+    return to_f32<T>(reinterpret_cast<const S*>(&word)[e]);
+  }
+  __device__ __forceinline__ void set(int e, float x) {
+    reinterpret_cast<S*>(&word)[e] = from_f32<T>(x);
+  }
+  template <bool kStream>
+  __device__ __forceinline__ void store(void* to, int64_t i) const {
+    Word* p = reinterpret_cast<Word*>(static_cast<S*>(to) + i);
+    if constexpr (kStream) {
+      __builtin_nontemporal_store(word, p);
+    } else {
+      *p = word;
+    }
+  }
+  __device__ __forceinline__ void store_unaligned(void* to, int64_t i, int64_t left) const {
+    const S* e = reinterpret_cast<const S*>(&word);
+#pragma unroll
+    for (int q = 0; q < kPer; ++q) {
+      if (q < left) static_cast<S*>(to)[i + q] = e[q];
+    }
   }
 };
+
+// Elements that a lane takes at a time: 16 bytes, and where an fp32 tensor is read or
+// written 4 elements, so that a wave's accesses to it are without gaps (bf16 to
+// fp32 with 8, whose stores have gaps of 16 bytes: 4.0 TB/s).
+template <typename T, typename To>
+constexpr int kPerLane = std::is_same_v<T, float> || std::is_same_v<To, float> ? 4 : 8;
 
 // f(type) for a dtype code.
 template <typename F>
@@ -93,37 +144,83 @@ __device__ __forceinline__ void with_dtype(uint8_t dtype, F&& f) {
   }
 }
 
-template <typename T>
-__device__ __forceinline__ void chunk_squares(const Entry& e, int64_t first, double (&sum)[4]) {
-  constexpr int kEach = kChunk / (8 * kThreads);
-  const int64_t left = e.numel - first;
-  Eight<T> x[kEach];
+// Place of a thread's pack j of a chunk.
+template <int kPer>
+__device__ __forceinline__ int64_t place(int64_t first, int j) {
+  return first + (j * kThreads + static_cast<int>(threadIdx.x)) * kPer;
+}
+
+template <bool kStream, typename T, int kPer, int kPacks>
+__device__ __forceinline__ void load_chunk(const Entry& e, int64_t first,
+                                           Pack<T, kPer> (&x)[kPacks]) {
+  if (e.aligned && e.numel - first >= kPacks * kThreads * kPer) {
 #pragma unroll
-  for (int j = 0; j < kEach; ++j) {
-    const int64_t i = first + (j * kThreads + threadIdx.x) * 8;
-    const int64_t here = e.numel - i;
-    if (e.aligned && (left >= kChunk || here >= 8)) {
-      x[j].load(e.from, i);
-    } else {
-      x[j].load_unaligned(e.from, i, here);
-    }
+    for (int j = 0; j < kPacks; ++j) x[j].template load<kStream>(e.from, place<kPer>(first, j));
+    return;
   }
 #pragma unroll
-  for (int j = 0; j < kEach; ++j) {
-#pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      const double v = x[j].at(q);
-      sum[q & 3] = fma(v, v, sum[q & 3]);
+  for (int j = 0; j < kPacks; ++j) {
+    const int64_t i = place<kPer>(first, j);
+    if (e.aligned && e.numel - i >= kPer) {
+      x[j].template load<kStream>(e.from, i);
+    } else {
+      x[j].load_unaligned(e.from, i, e.numel - i);
     }
   }
 }
 
-// The entry of a chunk, from the last one on.
-__device__ __forceinline__ int entry_of(const Table& t, int32_t chunk) {
-  int at = 0, left = t.count;
+// Squares of kEach units of a tensor from `first` on, as far as they go.
+template <int kEach, bool kStream>
+__device__ __forceinline__ void add_squares(const Entry& e, int64_t first, double (&sum)[4]) {
+  with_dtype(e.dtype, [&](auto type) {
+    using T = decltype(type);
+    constexpr int kPer = kPerLane<T, T>, kPacks = kEach * 8 / kPer;
+    Pack<T, kPer> x[kPacks];
+    load_chunk<kStream>(e, first, x);
+#pragma unroll
+    for (int j = 0; j < kPacks; ++j) {
+#pragma unroll
+      for (int q = 0; q < kPer; ++q) {
+        const double v = x[j].at(q);
+        sum[q & 3] = fma(v, v, sum[q & 3]);
+      }
+    }
+  });
+}
+
+// kEach units of a tensor, scaled.
+template <int kEach, bool kStream>
+__device__ __forceinline__ void scale_units(const Entry& e, int64_t first, float by) {
+  with_dtype(e.dtype, [&](auto type) {
+    with_dtype(e.to_dtype, [&](auto to_type) {
+      using T = decltype(type);
+      using To = decltype(to_type);
+      constexpr int kPer = kPerLane<T, To>, kPacks = kEach * 8 / kPer;
+      Pack<T, kPer> x[kPacks];
+      load_chunk<kStream>(e, first, x);
+      const bool whole = e.to_aligned && e.numel - first >= kEach * kUnit;
+#pragma unroll
+      for (int j = 0; j < kPacks; ++j) {
+        const int64_t i = place<kPer>(first, j);
+        Pack<To, kPer> y;
+#pragma unroll
+        for (int q = 0; q < kPer; ++q) y.set(q, x[j].at(q) * by);
+        if (whole || (e.to_aligned && e.numel - i >= kPer)) {
+          y.template store<kStream>(e.to, i);
+        } else {
+          y.store_unaligned(e.to, i, e.numel - i);
+        }
+      }
+    });
+  });
+}
+
+// The entry of a chunk.
+__device__ __forceinline__ int entry_of(const Entry* entries, int count, int32_t chunk) {
+  int at = 0, left = count;
   while (left > 1) {
     const int half = left / 2;
-    if (t.entry[at + half].first <= chunk) {
+    if (entries[at + half].first <= chunk) {
       at += half;
       left -= half;
     } else {
@@ -133,17 +230,94 @@ __device__ __forceinline__ int entry_of(const Table& t, int32_t chunk) {
   return at;
 }
 
-__global__ __launch_bounds__(kThreads) void squares_kernel(Table t, double* __restrict__ sums) {
+// A workgroup's run of chunks.
+struct Run {
+  int32_t from, to;
+};
+
+__device__ __forceinline__ Run run_of(int32_t chunks) {
+  const int64_t g = blockIdx.x, n = gridDim.x;
+  return {static_cast<int32_t>(g * chunks / n), static_cast<int32_t>((g + 1) * chunks / n)};
+}
+
+template <int kEach>
+__global__ __launch_bounds__(kThreads) void run_squares_kernel(Entries entries, List list,
+                                                               double* __restrict__ sums) {
   __shared__ double shared[kThreads / 64];
+  const Run run = run_of(list.chunks);
   double sum[4] = {};
-  for (int32_t c = blockIdx.x; c < t.chunks; c += gridDim.x) {
-    const Entry& e = t.entry[entry_of(t, c)];
-    with_dtype(e.dtype, [&](auto type) {
-      chunk_squares<decltype(type)>(e, static_cast<int64_t>(c - e.first) * kChunk, sum);
-    });
+  int at = entry_of(entries.entry, list.count, run.from);
+  for (int32_t c = run.from; c < run.to; ++c) {
+    while (at + 1 < list.count && entries.entry[at + 1].first <= c) ++at;
+    const Entry e = entries.entry[at];
+    add_squares<kEach, false>(e, static_cast<int64_t>(c - e.first) * (kEach * kUnit), sum);
   }
   const double all = workgroup_sum<kThreads>((sum[0] + sum[1]) + (sum[2] + sum[3]), shared);
   if (threadIdx.x == 0) sums[blockIdx.x] = all;
+}
+
+// A part of the list to the workspace, and its units' owners.
+__global__ __launch_bounds__(kThreads) void list_kernel(Entries part, int32_t count,
+                                                        int32_t index, int32_t units,
+                                                        Places to) {
+  __shared__ int32_t firsts[kEntries];
+  if (threadIdx.x < count) firsts[threadIdx.x] = part.entry[threadIdx.x].first;
+  if (blockIdx.x == 0 && threadIdx.x < count) to.entry[index + threadIdx.x] = part.entry[threadIdx.x];
+  __syncthreads();
+  const int32_t thread = static_cast<int32_t>(blockIdx.x) * kThreads + threadIdx.x;
+  for (int64_t u = thread; u < units; u += static_cast<int64_t>(gridDim.x) * kThreads) {
+    const int32_t unit = firsts[0] + static_cast<int32_t>(u);
+    int at = 0, left = count;
+    while (left > 1) {
+      const int half = left / 2;
+      const bool behind = firsts[at + half] <= unit;
+      at += behind ? half : 0;
+      left = behind ? left - half : half;
+    }
+    to.owner[unit] = index + at;
+  }
+}
+
+// kMany consecutive units at a time, in turns: read together where they are of one tensor.
+// kStream: 449M bf16 elements in 135 us, 150 through the caches.
+template <bool kStream>
+__global__ __launch_bounds__(kThreads) void squares_kernel(Places places, List list,
+                                                           double* __restrict__ sums) {
+  __shared__ double shared[kThreads / 64];
+  double sum[4] = {};
+  const int32_t step = static_cast<int32_t>(gridDim.x) * kMany;
+  for (int64_t u = static_cast<int64_t>(blockIdx.x) * kMany; u < list.chunks; u += step) {
+    const int32_t last = static_cast<int32_t>(min(u + kMany, static_cast<int64_t>(list.chunks))) - 1;
+    int32_t unit = static_cast<int32_t>(u);
+    const int32_t at = places.owner[unit];
+    if (places.owner[last] == at) {
+      const Entry e = places.entry[at];
+      add_squares<kMany, kStream>(e, static_cast<int64_t>(unit - e.first) * kUnit, sum);
+      continue;
+    }
+    for (; unit <= last; ++unit) {
+      const Entry e = places.entry[places.owner[unit]];
+      add_squares<1, kStream>(e, static_cast<int64_t>(unit - e.first) * kUnit, sum);
+    }
+  }
+  const double all = workgroup_sum<kThreads>((sum[0] + sum[1]) + (sum[2] + sum[3]), shared);
+  if (threadIdx.x == 0) sums[blockIdx.x] = all;
+}
+
+// The sum of all workgroups' sums, the same one for every caller.
+template <int kBlock>
+__device__ __forceinline__ double total_of(const double* __restrict__ sums, int32_t groups,
+                                           double* shared) {
+  constexpr int kEach = kMostGroups / kBlock;
+  double x[kEach];
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    const int32_t g = j * kBlock + static_cast<int32_t>(threadIdx.x);
+    x[j] = g < groups ? sums[g] : 0.0;
+  }
+#pragma unroll
+  for (int j = 1; j < kEach; ++j) x[0] += x[j];
+  return workgroup_sum<kBlock>(x[0], shared);
 }
 
 __device__ __forceinline__ float factor_of(double total, double most, double eps) {
@@ -152,89 +326,54 @@ __device__ __forceinline__ float factor_of(double total, double most, double eps
   return static_cast<float>(fmin(1.0, most / (norm + eps)));
 }
 
-__global__ __launch_bounds__(kJoinThreads) void norm_join_kernel(const double* __restrict__ sums,
-                                                                 int32_t groups, double most,
-                                                                 double eps,
-                                                                 float* __restrict__ norm,
-                                                                 float* __restrict__ factor) {
-  __shared__ double shared[kJoinThreads / 64];
-  double sum = 0.0;
-  for (int32_t g = threadIdx.x; g < groups; g += kJoinThreads) sum += sums[g];
-  sum = workgroup_sum<kJoinThreads>(sum, shared);
-  if (threadIdx.x == 0) {
-    *norm = static_cast<float>(sqrt(sum));
-    if (factor != nullptr) *factor = factor_of(sum, most, eps);
+// factor: null for the norm alone.
+__global__ __launch_bounds__(kThreads) void norm_kernel(const double* __restrict__ sums,
+                                                        int32_t groups, double most, double eps,
+                                                        float* norm, float* factor) {
+  __shared__ double shared[kThreads / 64];
+  const double total = total_of<kThreads>(sums, groups, shared);
+  if (threadIdx.x != 0) return;
+  *norm = static_cast<float>(sqrt(total));
+  if (factor != nullptr) *factor = factor_of(total, most, eps);
+}
+
+// From a run's last chunk to its first: what the norm read last is still in the cache.
+template <int kEach>
+__global__ __launch_bounds__(kThreads) void run_scale_kernel(Entries entries, List list,
+                                                             const double* __restrict__ sums,
+                                                             int32_t groups, double most,
+                                                             double eps,
+                                                             float* __restrict__ norm) {
+  __shared__ double shared[kThreads / 64];
+  const double total = total_of<kThreads>(sums, groups, shared);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *norm = static_cast<float>(sqrt(total));
+  const float by = factor_of(total, most, eps);
+  if (list.in_place && by == 1.0f) return;
+  const Run run = run_of(list.chunks);
+  int at = entry_of(entries.entry, list.count, run.to - 1);
+  for (int32_t c = run.to - 1; c >= run.from; --c) {
+    while (entries.entry[at].first > c) --at;
+    const Entry e = entries.entry[at];
+    scale_units<kEach, false>(e, static_cast<int64_t>(c - e.first) * (kEach * kUnit), by);
   }
 }
 
-template <typename T>
-__device__ __forceinline__ void store_eight(void* to, int64_t i, int64_t left, bool aligned,
-                                            const float (&y)[8]) {
-  using S = typename IoTraits<T>::storage;
-  S out[8];
-#pragma unroll
-  for (int q = 0; q < 8; ++q) out[q] = from_f32<T>(y[q]);
-  S* p = static_cast<S*>(to) + i;
-  if (aligned && left >= 8) {
-    constexpr int kParts = 8 * sizeof(S) / 16;
-#pragma unroll
-    for (int q = 0; q < kParts; ++q) {
-      reinterpret_cast<uint4*>(p)[q] = reinterpret_cast<const uint4*>(out)[q];
-    }
-    return;
-  }
-#pragma unroll
-  for (int q = 0; q < 8; ++q) {
-    if (q < left) p[q] = out[q];
-  }
-}
+// A unit a workgroup, from the last one (and again, beyond what a launch has).
+constexpr int kMostScalers = 1 << 22;
 
-template <typename T, typename To>
-__device__ __forceinline__ void scale_chunk(const Entry& e, int64_t first, float by) {
-  constexpr int kEach = kChunk / (8 * kThreads);
-  Eight<T> x[kEach];
-#pragma unroll
-  for (int j = 0; j < kEach; ++j) {
-    const int64_t i = first + (j * kThreads + threadIdx.x) * 8;
-    const int64_t here = e.numel - i;
-    if (e.aligned && here >= 8) {
-      x[j].load(e.from, i);
-    } else {
-      x[j].load_unaligned(e.from, i, here);
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < kEach; ++j) {
-    const int64_t i = first + (j * kThreads + threadIdx.x) * 8;
-    float y[8];
-#pragma unroll
-    for (int q = 0; q < 8; ++q) y[q] = x[j].at(q) * by;
-    store_eight<To>(e.to, i, e.numel - i, e.to_aligned, y);
-  }
-}
-
-// From the last chunk to the first: what the norm read last is still in the cache.
-__global__ __launch_bounds__(kThreads) void scale_kernel(Table t,
-                                                         const float* __restrict__ factor,
-                                                         bool in_place) {
+template <bool kStream>
+__global__ __launch_bounds__(kThreads) void scale_kernel(Places places, List list,
+                                                         const float* __restrict__ factor) {
   const float by = *factor;
-  if (in_place && by == 1.0f) return;
-  for (int32_t c = t.chunks - 1 - static_cast<int32_t>(blockIdx.x); c >= 0; c -= gridDim.x) {
-    const Entry& e = t.entry[entry_of(t, c)];
-    const int64_t first = static_cast<int64_t>(c - e.first) * kChunk;
-    with_dtype(e.dtype, [&](auto type) {
-      with_dtype(e.to_dtype, [&](auto to) {
-        scale_chunk<decltype(type), decltype(to)>(e, first, by);
-      });
-    });
+  if (list.in_place && by == 1.0f) return;
+  for (int32_t unit = list.chunks - 1 - static_cast<int32_t>(blockIdx.x); unit >= 0;
+       unit -= static_cast<int32_t>(gridDim.x)) {
+    const Entry e = places.entry[places.owner[unit]];
+    scale_units<1, kStream>(e, static_cast<int64_t>(unit - e.first) * kUnit, by);
   }
 }
 
 constexpr int64_t kMostElements = int64_t{1} << 40;  // of a tensor
-
-int64_t chunks_of(int64_t numel) { return (numel + kChunk - 1) / kChunk; }
-
-int groups_of(int32_t chunks) { return std::min(chunks, kMostGroups); }
 
 bool known_dtype(int dtype) {
   return dtype == FRWKV_DTYPE_F32 || dtype == FRWKV_DTYPE_F16 || dtype == FRWKV_DTYPE_BF16;
@@ -242,30 +381,89 @@ bool known_dtype(int dtype) {
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
-// f(table) for every launch over the tensors, those without elements left out.
+// How a list is cut and where it stands.
+struct Plan {
+  int64_t count;  // tensors with elements
+  int64_t units;
+  int64_t chunks; // of kMany units each, or of one; in the list's form, of one
+  int each;       // units of a chunk; 0: the list stands in the workspace
+  bool stream;
+
+  int groups() const {
+    const int64_t turns = each == 0 ? (units + kMany - 1) / kMany : chunks;
+    return static_cast<int>(std::min<int64_t>(turns, kMostGroups));
+  }
+  // Workspace: sums, factor, entries, owners.
+  size_t sums_bytes() const { return (static_cast<size_t>(groups()) * 8 + 255) / 256 * 256; }
+  size_t entry_bytes() const {
+    return each != 0 ? 0 : (static_cast<size_t>(count) * sizeof(Entry) + 255) / 256 * 256;
+  }
+  size_t bytes() const {
+    const size_t owners = each != 0 ? 0 : (static_cast<size_t>(units) * 4 + 255) / 256 * 256;
+    return 256 + sums_bytes() + entry_bytes() + owners;
+  }
+};
+
+int64_t chunks_of(int64_t numel, int64_t each) {
+  return (numel + each * kUnit - 1) / (each * kUnit);
+}
+
+// Most chunks of a list in the arguments: runs of eight, beyond which the order of
+// memory makes up for the launches that the other form has more.
+constexpr int64_t kMostRuns = 8 * kMostGroups;
+// The last-level cache's size: what is read twice and is larger passes by it.
+constexpr int64_t kCacheBytes = int64_t{256} << 20;
+
+Plan plan_of(int64_t count, const frwkv_gradient* tensors) {
+  Plan p{0, 0, 0, 1, false};
+  int64_t bytes = 0;
+  for (int64_t i = 0; i < count; ++i) {
+    const int64_t numel = tensors[i].numel;
+    if (numel == 0) continue;
+    ++p.count;
+    p.units += chunks_of(numel, 1);
+    p.chunks += chunks_of(numel, kMany);
+    bytes += numel * (tensors[i].dtype == FRWKV_DTYPE_F32 ? 4 : 2);
+  }
+  p.stream = bytes > kCacheBytes;
+  if (p.count > kEntries || p.chunks > kMostRuns) {
+    p.each = 0;
+    p.chunks = p.units;
+  } else if (p.units > kMostGroups) {
+    p.each = kMany;
+  } else {
+    p.chunks = p.units;
+  }
+  return p;
+}
+
+// f(entries, how many, index of the first, chunks) for every kEntries tensors with
+// elements; chunks are of `each` units.
 template <typename F>
-void for_tables(int64_t count, const frwkv_gradient* tensors, F&& f) {
-  Table t;
-  t.count = t.chunks = 0;
+void for_entries(int64_t count, const frwkv_gradient* tensors, int each, F&& f) {
+  Entries part;
+  int32_t have = 0, first = 0, done = 0, before = 0;
+  const auto flush = [&] {
+    if (have > 0) f(part, have, done, first - before);
+    done += have;
+    before = first;
+    have = 0;
+  };
   for (int64_t i = 0; i < count; ++i) {
     const frwkv_gradient& x = tensors[i];
     if (x.numel == 0) continue;
-    const int64_t chunks = chunks_of(x.numel);
-    if (t.count == kEntries || t.chunks + chunks > INT32_MAX / 2) {
-      f(t);
-      t.count = t.chunks = 0;
-    }
-    t.entry[t.count++] = {x.data,
+    if (have == kEntries) flush();
+    part.entry[have++] = {x.data,
                           x.out,
                           x.numel,
-                          t.chunks,
+                          first,
                           static_cast<uint8_t>(x.dtype),
                           static_cast<uint8_t>(x.out_dtype),
                           aligned16(x.data),
                           aligned16(x.out)};
-    t.chunks += static_cast<int32_t>(chunks);
+    first += static_cast<int32_t>(chunks_of(x.numel, each));
   }
-  if (t.count > 0) f(t);
+  flush();
 }
 
 int check_tensors(const char* what, int64_t count, const frwkv_gradient* tensors, bool out) {
@@ -298,31 +496,83 @@ int check_tensors(const char* what, int64_t count, const frwkv_gradient* tensors
   return FRWKV_OK;
 }
 
-size_t workspace_of(int64_t count, const frwkv_gradient* tensors) {
-  size_t groups = 0;
-  for_tables(count, tensors, [&](const Table& t) { groups += groups_of(t.chunks); });
-  return 256 + (groups * 8 + 255) / 256 * 256;
+// f(streaming) as a constant.
+template <typename F>
+void with_stream(bool stream, F&& f) {
+  if (stream) {
+    f(std::true_type{});
+  } else {
+    f(std::false_type{});
+  }
 }
 
-// factor: null for the norm alone.
-void launch_norm(int64_t count, const frwkv_gradient* tensors, double most, double eps,
-                 float* norm, float* factor, double* sums, hipStream_t stream) {
-  int32_t groups = 0;
-  for_tables(count, tensors, [&](const Table& t) {
-    const int own = groups_of(t.chunks);
-    hipLaunchKernelGGL(squares_kernel, dim3(own), dim3(kThreads), 0, stream, t, sums + groups);
-    groups += own;
-  });
-  hipLaunchKernelGGL(norm_join_kernel, dim3(1), dim3(kJoinThreads), 0, stream, sums, groups, most,
-                     eps, norm, factor);
+// Launches the norm, with the scaling behind it (scale) or without.
+void launch(const Plan& plan, int64_t count, const frwkv_gradient* tensors, bool scale,
+            double most, double eps, float* norm, char* workspace, hipStream_t stream) {
+  float* factor = scale ? reinterpret_cast<float*>(workspace) : nullptr;
+  double* sums = reinterpret_cast<double*>(workspace + 256);
+  const int groups = plan.groups();
+  List list{static_cast<int32_t>(plan.count), static_cast<int32_t>(plan.chunks), scale};
+  for (int64_t i = 0; i < count && list.in_place; ++i) {
+    list.in_place = tensors[i].numel == 0 || tensors[i].data == tensors[i].out;
+  }
+  const auto norm_of = [&] {
+    hipLaunchKernelGGL(norm_kernel, dim3(1), dim3(kThreads), 0, stream, sums, groups, most, eps,
+                       norm, factor);
+  };
+  if (plan.count == 0) return norm_of();
+  if (plan.each == 0) {
+    char* at = workspace + 256 + plan.sums_bytes();
+    const Places places{reinterpret_cast<Entry*>(at),
+                        reinterpret_cast<int32_t*>(at + plan.entry_bytes())};
+    for_entries(count, tensors, 1, [&](const Entries& part, int32_t have, int32_t first,
+                                       int32_t units) {
+      const int blocks = std::clamp<int>(units / (4 * kThreads), 1, 256);
+      hipLaunchKernelGGL(list_kernel, dim3(blocks), dim3(kThreads), 0, stream, part, have, first,
+                         units, places);
+    });
+    with_stream(plan.stream, [&](auto streaming) {
+      constexpr bool kStream = decltype(streaming)::value;
+      hipLaunchKernelGGL((squares_kernel<kStream>), dim3(groups), dim3(kThreads), 0, stream,
+                         places, list, sums);
+      norm_of();
+      if (scale) {
+        hipLaunchKernelGGL((scale_kernel<kStream>), dim3(std::min(list.chunks, kMostScalers)),
+                           dim3(kThreads), 0, stream,
+                           places, list, factor);
+      }
+    });
+    return;
+  }
+  const auto run = [&](auto each) {
+    constexpr int kEach = decltype(each)::value;
+    for_entries(count, tensors, kEach, [&](const Entries& entries, int32_t, int32_t, int32_t) {
+      hipLaunchKernelGGL((run_squares_kernel<kEach>), dim3(groups), dim3(kThreads), 0, stream,
+                         entries, list, sums);
+      if (scale) {
+        hipLaunchKernelGGL((run_scale_kernel<kEach>), dim3(groups), dim3(kThreads), 0, stream,
+                           entries, list, sums, groups, most, eps, norm);
+      }
+    });
+  };
+  if (plan.each == 1) {
+    run(std::integral_constant<int, 1>{});
+  } else {
+    run(std::integral_constant<int, kMany>{});
+  }
+  if (!scale) norm_of();
 }
 
 int begin(const char* what, int64_t count, const frwkv_gradient* tensors, bool out,
-          const float* norm, void* workspace, size_t workspace_bytes) {
+          const float* norm, void* workspace, size_t workspace_bytes, Plan* plan) {
   const int rc = check_tensors(what, count, tensors, out);
   if (rc != FRWKV_OK) return rc;
+  *plan = plan_of(count, tensors);
+  if (plan->units > INT32_MAX / 2 || plan->count > INT32_MAX / 2) {
+    return set_error(FRWKV_ERR_UNSUPPORTED, "%s: too many elements for one call", what);
+  }
   if (!norm) return set_error(FRWKV_ERR_INVALID_ARGUMENT, "%s: norm is null", what);
-  const size_t need = workspace_of(count, tensors);
+  const size_t need = plan->bytes();
   if (workspace == nullptr || workspace_bytes < need) {
     return set_error(FRWKV_ERR_INVALID_ARGUMENT, "%s: workspace of %zu bytes given, %zu needed",
                      what, workspace == nullptr ? size_t{0} : workspace_bytes, need);
@@ -343,18 +593,18 @@ size_t frwkv_grad_norm_workspace_bytes(int64_t count, const frwkv_gradient* tens
   if (check_tensors("frwkv_grad_norm_workspace_bytes", count, tensors, false) != FRWKV_OK) {
     return 0;
   }
-  return workspace_of(count, tensors);
+  return plan_of(count, tensors).bytes();
 }
 
 int frwkv_grad_norm(int64_t count, const frwkv_gradient* tensors, float* norm, void* workspace,
                     size_t workspace_bytes, void* stream) {
   using namespace frwkv;
+  Plan plan;
   const int rc = begin("frwkv_grad_norm", count, tensors, false, norm, workspace,
-                       workspace_bytes);
+                       workspace_bytes, &plan);
   if (rc != FRWKV_OK) return rc;
-  launch_norm(count, tensors, 0.0, 0.0, norm, nullptr,
-              reinterpret_cast<double*>(static_cast<char*>(workspace) + 256),
-              static_cast<hipStream_t>(stream));
+  launch(plan, count, tensors, false, 0.0, 0.0, norm, static_cast<char*>(workspace),
+         static_cast<hipStream_t>(stream));
   return check_launch("gradient norm");
 }
 
@@ -362,23 +612,15 @@ int frwkv_grad_clip(int64_t count, const frwkv_gradient* tensors, double max_nor
                     float* norm, void* workspace, size_t workspace_bytes, void* stream) {
   using namespace frwkv;
   const char* what = "frwkv_grad_clip";
-  const int rc = begin(what, count, tensors, true, norm, workspace, workspace_bytes);
+  Plan plan;
+  const int rc = begin(what, count, tensors, true, norm, workspace, workspace_bytes, &plan);
   if (rc != FRWKV_OK) return rc;
   if (!(max_norm >= 0.0) || !std::isfinite(max_norm) || !(eps >= 0.0) || !std::isfinite(eps)) {
     return set_error(FRWKV_ERR_INVALID_ARGUMENT,
                      "%s: max_norm and eps must be finite and not negative", what);
   }
-  float* factor = static_cast<float*>(workspace);
-  const hipStream_t q = static_cast<hipStream_t>(stream);
-  launch_norm(count, tensors, max_norm, eps, norm, factor,
-              reinterpret_cast<double*>(static_cast<char*>(workspace) + 256), q);
-  // A launch's tensors are in place or are not; mixed lists are written as a whole.
-  for_tables(count, tensors, [&](const Table& t) {
-    bool in_place = true;
-    for (int i = 0; i < t.count; ++i) in_place = in_place && t.entry[i].from == t.entry[i].to;
-    hipLaunchKernelGGL(scale_kernel, dim3(groups_of(t.chunks)), dim3(kThreads), 0, q, t, factor,
-                       in_place);
-  });
+  launch(plan, count, tensors, true, max_norm, eps, norm, static_cast<char*>(workspace),
+         static_cast<hipStream_t>(stream));
   return check_launch("gradient clipping");
 }
 

@@ -17,8 +17,9 @@
 //       ((m - 1/2) / beta)^2,
 //   dl/dx_i = dl/dm beta (+ or -) (/ count).
 //
-// d and t are differences of logs that may both be large, and decide on which
-// side of a border a token is: they are taken in 64 bits, as all sums are.
+// d decides on which side of a border a token is. Differences of logs are exact up
+// to one rounding; where a rounded one falls on a rounded border, both are taken in
+// 64 bits. A lane adds its few tokens up in 32 bits, everything beyond is in 64.
 //
 // A wave takes a tile of 64 x kRounds consecutive tokens with all loads under
 // way at once, and finds the sequence of its first token by itself, 64 offsets a
@@ -30,6 +31,7 @@
 // token make the loss, and with it the gradients, NaN.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "capi_internal.h"
 #include "wkv7_device.h"
@@ -41,16 +43,44 @@ constexpr int kWaves = 4;           // of a workgroup of the token kernels
 constexpr int kJoinThreads = 1024;
 constexpr int kJoinWaves = kJoinThreads / 64;
 constexpr int kMostJoins = 64;      // workgroups that join
-constexpr int kMany = 8;            // rounds of a tile of a large call
+constexpr int kMany = 4;            // rounds of a tile of a large call
 constexpr int kFew = 2;
 constexpr int kNone = -1;           // a column that is not there
 
 __device__ __forceinline__ int lane_id() { return threadIdx.x & 63; }
 
+// A lane's 32 bits moved by a DPP pattern, 0 where it has no source.
+template <int kPattern, int kRows>
+__device__ __forceinline__ int32_t moved(int32_t x) {
+  return __builtin_amdgcn_update_dpp(0, x, kPattern, kRows, 0xf, true);
+}
+
+template <int kPattern, int kRows, typename T>
+__device__ __forceinline__ T moved_of(T x) {
+  int32_t part[sizeof(T) / 4];
+  __builtin_memcpy(part, &x, sizeof(T));
+#pragma unroll
+  for (size_t i = 0; i < sizeof(T) / 4; ++i) part[i] = moved<kPattern, kRows>(part[i]);
+  __builtin_memcpy(&x, part, sizeof(T));
+  return x;
+}
+
+// The sum over the wave, the same for all lanes. By row shifts and row broadcasts,
+// which stay in the vector unit: through LDS the six steps of a 64-bit sum are
+// twelve dependent trips.
 template <typename T>
 __device__ __forceinline__ T wave_sum(T x) {
+  x += moved_of<0x111, 0xf>(x);  // row_shr 1, 2, 4, 8: lane 15 of a row of 16 has its sum
+  x += moved_of<0x112, 0xf>(x);
+  x += moved_of<0x114, 0xf>(x);
+  x += moved_of<0x118, 0xf>(x);
+  x += moved_of<0x142, 0xa>(x);  // row_bcast 15 into rows 1 and 3, 31 into rows 2 and 3
+  x += moved_of<0x143, 0xc>(x);
+  int32_t part[sizeof(T) / 4];
+  __builtin_memcpy(part, &x, sizeof(T));
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
+  for (size_t i = 0; i < sizeof(T) / 4; ++i) part[i] = __builtin_amdgcn_readlane(part[i], 63);
+  __builtin_memcpy(&x, part, sizeof(T));
   return x;
 }
 
@@ -59,6 +89,48 @@ struct Column {
   const void* data;
   int dtype;  // FRWKV_DTYPE_*, or kNone
   __host__ __device__ bool given() const { return dtype != kNone; }
+};
+
+// log2 of a tile's tokens.
+__host__ __device__ constexpr int shift_of(int rounds) { return rounds == 1 ? 6 : 1 + shift_of(rounds / 2); }
+
+// A tile of 64 x kRounds tokens: where it begins and how many there are.
+template <int kRounds>
+struct Tile {
+  int64_t first;
+  int32_t left;
+  __device__ __forceinline__ Tile(int64_t tile, int64_t tokens) {
+    first = tile * (64 * kRounds);
+    left = static_cast<int32_t>(min(tokens - first, int64_t{64 * kRounds}));
+  }
+  __device__ __forceinline__ bool empty() const { return left <= 0; }
+  __device__ __forceinline__ bool has(int r) const { return 64 * r + lane_id() < left; }
+  // to[r] = from[token of round r], the last one for those beyond it. Whole tiles are
+  // read at constant distances from one address.
+  template <typename S, typename D>
+  __device__ __forceinline__ void fetch(const S* from, D (&to)[kRounds]) const {
+    from += first;
+    if (left == 64 * kRounds) {
+#pragma unroll
+      for (int r = 0; r < kRounds; ++r) to[r] = from[64 * r + lane_id()];
+    } else {
+#pragma unroll
+      for (int r = 0; r < kRounds; ++r) to[r] = from[min(64 * r + lane_id(), left - 1)];
+    }
+  }
+  __device__ __forceinline__ void fetch(const Column& from, uint32_t (&to)[kRounds]) const {
+    if (from.dtype == FRWKV_DTYPE_F32) {
+      fetch(static_cast<const uint32_t*>(from.data), to);
+    } else {
+      fetch(static_cast<const uint16_t*>(from.data), to);
+    }
+  }
+  __device__ __forceinline__ void fetch_part(const uint8_t* mask, bool (&part)[kRounds]) const {
+    uint32_t here[kRounds];
+    if (mask != nullptr) fetch(mask, here);
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) part[r] = has(r) && (mask == nullptr || here[r] != 0);
+  }
 };
 
 __device__ __forceinline__ uint32_t bits_at(const Column& c, int64_t i) {
@@ -195,24 +267,29 @@ __device__ __forceinline__ bool in_order(const Packed& p, int32_t b) {
 
 // Sum of a sequence's pieces: up to kOwnPieces by the lane that asks, others by
 // the wave. All lanes call; b < 0 asks for none.
-constexpr int kOwnPieces = 4;
+constexpr int kOwnPieces = 64;
+constexpr int kAtOnce = 8;  // of them under way
 
-__device__ __forceinline__ Piece sum_of(const Packed& p, const Piece* pieces, int tile_tokens,
+__device__ __forceinline__ Piece sum_of(const Packed& p, const Piece* pieces, int tile_shift,
                                         int64_t tiles, int32_t b) {
   Piece out{0.0, 0};
   int64_t from = 0, to = 0;  // tiles
   if (b >= 0 && in_order(p, b) && p.cu[b] < p.cu[b + 1]) {
-    from = p.cu[b] / tile_tokens;
-    to = min(static_cast<int64_t>(p.cu[b + 1] - 1) / tile_tokens + 1, tiles);
+    from = p.cu[b] >> tile_shift;
+    to = min(static_cast<int64_t>((p.cu[b + 1] - 1) >> tile_shift) + 1, tiles);
   }
   const bool own = to - from <= kOwnPieces;
   if (own) {
+    for (int64_t t = from; t < to; t += kAtOnce) {
+      Piece x[kAtOnce];
 #pragma unroll
-    for (int t = 0; t < kOwnPieces; ++t) {
-      if (from + t < to) {
-        const Piece x = pieces[from + t + b];
-        out.sum += x.sum;
-        out.count += x.count;
+      for (int u = 0; u < kAtOnce; ++u) x[u] = pieces[min(t + u, to - 1) + b];
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) {
+        if (t + u < to) {
+          out.sum += x[u].sum;
+          out.count += x[u].count;
+        }
       }
     }
   }
@@ -241,54 +318,70 @@ __device__ __forceinline__ Piece sum_of(const Packed& p, const Piece* pieces, in
 struct Policy {
   Column x, old, advantage, reference, entropy;
   bool per_sequence;  // advantages are
-  double above, below, far;  // log(1 + high), log(1 - low), log dual
+  float above, below, far;   // borders: log(1 + high), log(1 - low), log dual
+  double above_exact, below_exact, far_exact;
   float most, least, dual;   // 1 + high, 1 - low; dual 0: none
   float kl, ew;
 };
 
 // Sums over a workgroup's tokens, and what the call returns of them.
-enum { kLoss, kCount, kRatio, kClipped, kOld, kReference, kSums };
+enum { kLoss, kCount, kBad, kRatio, kClipped, kOld, kReference, kSums };
 constexpr int kMetrics = 4;  // the last of them, over the count
 
-// e^t and e^t - 1; k3 = e^t - 1 - t. Up to |t| = 1 by k3's series, whose terms are
-// positive or fall quickly, since the differences lose all digits near 0 (nine
-// terms: 5e-8 of the sum at 1).
+// e^t, e^t - 1 and k3 = e^t - 1 - t, without a branch. e^t = 2^n (1 + r log 2), n the
+// rounded t log2 e and r what that left out; the differences lose all digits near 0
+// and are taken up to |t| = 1 from k3's series, whose terms fall quickly (nine of them: 5e-8 of
+// the sum at 1).
 struct Exponential {
   float e, less_one, k3;
 };
 
 __device__ __forceinline__ Exponential exponential(float t) {
-  if (fabsf(t) < 1.0f) {
-    float s = 1.0f / 3628800.0f;
-    s = fmaf(s, t, 1.0f / 362880.0f);
-    s = fmaf(s, t, 1.0f / 40320.0f);
-    s = fmaf(s, t, 1.0f / 5040.0f);
-    s = fmaf(s, t, 1.0f / 720.0f);
-    s = fmaf(s, t, 1.0f / 120.0f);
-    s = fmaf(s, t, 1.0f / 24.0f);
-    s = fmaf(s, t, 1.0f / 6.0f);
-    s = fmaf(s, t, 0.5f);
-    const float k3 = t * t * s;
-    return {1.0f + (t + k3), t + k3, k3};
-  }
-  const float e = expf(t);
-  return {e, e - 1.0f, e - 1.0f - t};
+  constexpr float kLog2ELow = 1.9259629911266175e-8f;  // log2 e - kLog2E
+  const float n = t * kLog2E;
+  const float r = fmaf(t, kLog2ELow, fmaf(t, kLog2E, -n));
+  const float power = __builtin_amdgcn_exp2f(n);
+  // Beyond, the power is 0 or infinite and r may be NaN.
+  const float e = fabsf(n) < 128.0f ? fmaf(power * 0.69314718f, r, power) : power;
+  float s = 1.0f / 3628800.0f;
+  s = fmaf(s, t, 1.0f / 362880.0f);
+  s = fmaf(s, t, 1.0f / 40320.0f);
+  s = fmaf(s, t, 1.0f / 5040.0f);
+  s = fmaf(s, t, 1.0f / 720.0f);
+  s = fmaf(s, t, 1.0f / 120.0f);
+  s = fmaf(s, t, 1.0f / 24.0f);
+  s = fmaf(s, t, 1.0f / 6.0f);
+  s = fmaf(s, t, 0.5f);
+  const float near = t * t * s;
+  const bool small = fabsf(t) < 1.0f;
+  const float less_one = small ? t + near : e - 1.0f;
+  return {small ? 1.0f + less_one : e, less_one, small ? near : less_one - t};
 }
 
+// A token's surrogate, as a loss and its slope in x.
 struct Term {
   float loss, slope;
-  float ratio, old, reference;
+  float ratio, k3;
   bool clipped;
 };
 
-__device__ __forceinline__ Term policy_term(const Policy& a, float x, float old, float advantage,
-                                            float reference, float entropy) {
+__device__ __forceinline__ Term policy_term(const Policy& a, float x, float old,
+                                            float advantage) {
   Term out;
-  const double d = static_cast<double>(x) - static_cast<double>(old);
-  const Exponential r = exponential(static_cast<float>(d));
-  const bool dual = a.dual > 0.0f && advantage < 0.0f;
-  out.clipped = (advantage > 0.0f && d > a.above) || (advantage < 0.0f && d < a.below) ||
-                (dual && d > a.far);
+  const float d = x - old;
+  const bool gains = advantage > 0.0f, loses = advantage < 0.0f;
+  const bool dual = a.dual > 0.0f && loses;
+  out.clipped = (gains && d > a.above) || (loses && d < a.below) || (dual && d > a.far);
+  // Rounding keeps the order, so a rounded d beside a rounded border decides; d on
+  // it is compared in 64 bits.
+  const bool on = d == a.above || d == a.below || d == a.far;
+  if (__builtin_expect(__ballot(on) != 0, 0)) {
+    const double exact = static_cast<double>(x) - static_cast<double>(old);
+    const bool clipped = (gains && exact > a.above_exact) || (loses && exact < a.below_exact) ||
+                         (dual && exact > a.far_exact);
+    if (on) out.clipped = clipped;
+  }
+  const Exponential r = exponential(d);
   const float plain = r.e * advantage;
   const float bounded = fminf(fmaxf(r.e, a.least), a.most) * advantage;
   // NaN stays NaN.
@@ -297,16 +390,7 @@ __device__ __forceinline__ Term policy_term(const Policy& a, float x, float old,
   out.loss = -gain;
   out.slope = out.clipped ? 0.0f : -plain;
   out.ratio = r.e;
-  out.old = r.k3;
-  out.reference = 0.0f;
-  if (a.reference.given()) {
-    const double t = static_cast<double>(reference) - static_cast<double>(x);
-    const Exponential q = exponential(static_cast<float>(t));
-    out.loss = fmaf(a.kl, q.k3, out.loss);
-    out.slope = fmaf(-a.kl, q.less_one, out.slope);
-    out.reference = q.k3;
-  }
-  if (a.entropy.given()) out.loss = fmaf(-a.ew, entropy, out.loss);
+  out.k3 = r.k3;
   return out;
 }
 
@@ -331,23 +415,20 @@ struct PolicyOut {
   bool slopes;
 };
 
-// Adds `values` up over the workgroup; the result is thread 0's.
+// Adds `values` up over the workgroup; the result is the first wave's.
 template <int kBlockWaves, int kValues>
 __device__ __forceinline__ void workgroup_sum(double (&values)[kValues], double* shared) {
   const int wave = threadIdx.x >> 6;
 #pragma unroll
   for (int v = 0; v < kValues; ++v) {
     const double x = wave_sum(values[v]);
-    if (lane_id() == 0) shared[wave * kValues + v] = x;
+    if (lane_id() == 0) shared[v * kBlockWaves + wave] = x;
   }
   __syncthreads();
-  if (threadIdx.x == 0) {
+  if (wave == 0) {
 #pragma unroll
     for (int v = 0; v < kValues; ++v) {
-      double x = 0.0;
-#pragma unroll
-      for (int w = 0; w < kBlockWaves; ++w) x += shared[w * kValues + v];
-      values[v] = x;
+      values[v] = wave_sum(lane_id() < kBlockWaves ? shared[v * kBlockWaves + lane_id()] : 0.0);
     }
   }
   __syncthreads();
@@ -355,30 +436,22 @@ __device__ __forceinline__ void workgroup_sum(double (&values)[kValues], double*
 
 template <int kRounds>
 __device__ __forceinline__ void policy_tile(const Policy& a, const Packed& p, const PolicyOut& o,
-                                            const Saved& s, const Scratch& w, int64_t tile,
+                                            const Saved& s, const Scratch& w, int64_t index,
                                             double (&sums)[kSums]) {
-  const int64_t first = tile * (64 * kRounds);
-  if (first >= p.n) return;
-  const int lane = lane_id();
+  const Tile<kRounds> tile(index, p.n);
+  if (tile.empty()) return;
   uint32_t x[kRounds], old[kRounds], advantage[kRounds], reference[kRounds], entropy[kRounds];
   bool part[kRounds];
-  const auto fetch = [&](const Column& c, uint32_t (&to)[kRounds]) {
-#pragma unroll
-    for (int r = 0; r < kRounds; ++r) to[r] = bits_at(c, min(first + 64 * r + lane, p.n - 1));
-  };
-  fetch(a.x, x);
-  fetch(a.old, old);
-  if (!a.per_sequence) fetch(a.advantage, advantage);
-  if (a.reference.given()) fetch(a.reference, reference);
-  if (a.entropy.given()) fetch(a.entropy, entropy);
-#pragma unroll
-  for (int r = 0; r < kRounds; ++r) {
-    const int64_t i = first + 64 * r + lane;
-    part[r] = i < p.n && (p.mask == nullptr || p.mask[min(i, p.n - 1)] != 0);
-  }
+  tile.fetch(a.x, x);
+  tile.fetch(a.old, old);
+  if (!a.per_sequence) tile.fetch(a.advantage, advantage);
+  if (a.reference.given()) tile.fetch(a.reference, reference);
+  if (a.entropy.given()) tile.fetch(a.entropy, entropy);
+  tile.fetch_part(p.mask, part);
+  const bool by_sequence = o.reduction == FRWKV_REDUCE_SEQUENCE_MEAN;
   int32_t id[kRounds];
-  if (p.cu != nullptr) {
-    sequences_of<kRounds>(p, first, id);
+  if (by_sequence || a.per_sequence) {
+    sequences_of<kRounds>(p, tile.first, id);
 #pragma unroll
     for (int r = 0; r < kRounds; ++r) part[r] = part[r] && id[r] < p.sequences;
     if (a.per_sequence) {
@@ -387,56 +460,103 @@ __device__ __forceinline__ void policy_tile(const Policy& a, const Packed& p, co
         advantage[r] = bits_at(a.advantage, min(id[r], p.sequences - 1));
       }
     }
+  } else if (p.cu != nullptr) {  // which sequence does not matter, only whether one
+    const int64_t end = p.cu[p.sequences] - tile.first;
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) part[r] = part[r] && 64 * r + lane_id() < end;
   }
-  const bool by_sequence = o.reduction == FRWKV_REDUCE_SEQUENCE_MEAN;
-  Pieces pieces;
-  if (by_sequence) {
-    pieces.at = w.pieces + tile;
-    pieces.sequences = p.sequences;
-    pieces.open = __builtin_amdgcn_readfirstlane(id[0]);
-  }
+  // Vector by vector: what is the same for all tokens is asked once a tile.
+  float losses[kRounds], slopes[kRounds];
+  float ratio = 0.0f, old_kl = 0.0f, reference_kl = 0.0f;
+  int32_t count = 0, clipped = 0;
 #pragma unroll
   for (int r = 0; r < kRounds; ++r) {
-    const int64_t i = first + 64 * r + lane;
-    Term t = policy_term(a, value_of(a.x, x[r]), value_of(a.old, old[r]),
-                         value_of(a.advantage, advantage[r]),
-                         a.reference.given() ? value_of(a.reference, reference[r]) : 0.0f,
-                         a.entropy.given() ? value_of(a.entropy, entropy[r]) : 0.0f);
+    const Term t = policy_term(a, value_of(a.x, x[r]), value_of(a.old, old[r]),
+                               value_of(a.advantage, advantage[r]));
+    losses[r] = t.loss;
+    slopes[r] = t.slope;
     // What stands in a token that takes no part, NaN included, ends here.
-    if (!part[r]) t = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, false};
-    if (i < p.n) {
-      if (o.slopes) s.slope[i] = t.slope;
-      if (o.reduction == FRWKV_REDUCE_NONE) o.loss[i] = t.loss;
-    }
-    sums[kLoss] += t.loss;
-    sums[kCount] += part[r] ? 1.0 : 0.0;
-    if (o.metrics != nullptr) {
-      sums[kRatio] += t.ratio;
-      sums[kClipped] += t.clipped ? 1.0 : 0.0;
-      sums[kOld] += t.old;
-      sums[kReference] += t.reference;
-    }
-    if (by_sequence) pieces.add(id[r], t.loss, part[r]);
+    ratio += part[r] ? t.ratio : 0.0f;
+    old_kl += part[r] ? t.k3 : 0.0f;
+    clipped += part[r] && t.clipped ? 1 : 0;
+    count += part[r] ? 1 : 0;
   }
-  if (by_sequence) pieces.end();
+  if (a.reference.given()) {
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) {
+      const Exponential q =
+          exponential(value_of(a.reference, reference[r]) - value_of(a.x, x[r]));
+      losses[r] = fmaf(a.kl, q.k3, losses[r]);
+      slopes[r] = fmaf(-a.kl, q.less_one, slopes[r]);
+      reference_kl += part[r] ? q.k3 : 0.0f;
+    }
+  }
+  if (a.entropy.given()) {
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) {
+      losses[r] = fmaf(-a.ew, value_of(a.entropy, entropy[r]), losses[r]);
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) losses[r] = part[r] ? losses[r] : 0.0f;
+  if (o.slopes) {
+    float* to = s.slope + tile.first;
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) {
+      if (tile.has(r)) to[64 * r + lane_id()] = part[r] ? slopes[r] : 0.0f;
+    }
+  }
+  if (o.reduction == FRWKV_REDUCE_NONE) {
+    float* to = o.loss + tile.first;
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) {
+      if (tile.has(r)) to[64 * r + lane_id()] = losses[r];
+    }
+  }
+  float loss = 0.0f;
+  if (by_sequence) {
+    Pieces pieces;
+    pieces.at = w.pieces + index;
+    pieces.sequences = p.sequences;
+    pieces.open = __builtin_amdgcn_readfirstlane(id[0]);
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) pieces.add(id[r], losses[r], part[r]);
+    pieces.end();
+  } else {
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) loss += losses[r];
+  }
+  sums[kLoss] = loss;
+  sums[kCount] = count;
+  sums[kRatio] = ratio;
+  sums[kClipped] = clipped;
+  sums[kOld] = old_kl;
+  sums[kReference] = reference_kl;
 }
 
-// A workgroup's part of the sequences: {sum of their means, how many have
-// tokens, how many have offsets that may not be}.
+// Offsets that may not be, of a thread's share of the sequences.
+__device__ __forceinline__ double bad_offsets(const Packed& p, int64_t thread, int64_t threads) {
+  if (p.cu == nullptr) return 0.0;
+  double bad = 0.0;
+  for (int64_t b = thread; b < p.sequences; b += threads) {
+    if (!in_order(p, static_cast<int32_t>(b))) bad = 1.0;
+  }
+  return bad;
+}
+
+// A workgroup's part of the sequences, for the mean over them: {sum of their means,
+// how many have tokens}.
 __device__ __forceinline__ void join_sequences(const Packed& p, const PolicyOut& o,
-                                               const Saved& s, const Scratch& w, int tile_tokens,
+                                               const Saved& s, const Scratch& w, int tile_shift,
                                                int64_t tiles, int64_t wave, int64_t waves,
-                                               double (&found)[3]) {
-  if (p.cu == nullptr) return;
-  const bool by_sequence = o.reduction == FRWKV_REDUCE_SEQUENCE_MEAN;
+                                               double (&found)[2]) {
+  if (o.reduction != FRWKV_REDUCE_SEQUENCE_MEAN) return;
   // Few sequences are one a wave, many 64.
   const int64_t each = min(max((p.sequences + waves - 1) / waves, int64_t{1}), int64_t{64});
   for (int64_t at = wave * each; at < p.sequences; at += waves * each) {
     const bool mine = lane_id() < each && at + lane_id() < p.sequences;
     const int32_t b = mine ? static_cast<int32_t>(at) + lane_id() : -1;
-    if (mine && !in_order(p, b)) found[2] += 1.0;
-    if (!by_sequence) continue;
-    const Piece x = sum_of(p, w.pieces, tile_tokens, tiles, b);
+    const Piece x = sum_of(p, w.pieces, tile_shift, tiles, b);
     if (mine) {
       s.weight[b] = x.count > 0 ? static_cast<float>(1.0 / static_cast<double>(x.count)) : 0.0f;
       if (x.count > 0) {
@@ -449,9 +569,9 @@ __device__ __forceinline__ void join_sequences(const Packed& p, const PolicyOut&
 
 __device__ __forceinline__ void write_policy(const PolicyOut& o, const Saved& s,
                                              const double (&sums)[kSums],
-                                             const double (&found)[3]) {
+                                             const double (&found)[2]) {
   const bool by_sequence = o.reduction == FRWKV_REDUCE_SEQUENCE_MEAN;
-  const float bad = found[2] > 0.0 ? __builtin_nanf("") : 0.0f;
+  const float bad = sums[kBad] > 0.0 ? __builtin_nanf("") : 0.0f;
   const double over = by_sequence ? found[1] : sums[kCount];
   const bool mean = by_sequence || o.reduction == FRWKV_REDUCE_MEAN;
   const double share = mean ? (over > 0.0 ? 1.0 / over : 0.0) : 1.0;
@@ -470,21 +590,31 @@ __device__ __forceinline__ void write_policy(const PolicyOut& o, const Saved& s,
 }
 
 // Losses and slopes of all tokens. kAlone: one workgroup takes them all and
-// joins them, which saves the second launch.
-template <int kRounds, int kBlockWaves, bool kAlone>
+// joins them, which saves the second launch. kPlain: all vectors are fp32, known to the
+// compiler; a type that is looked at for each value costs as many scalar
+// instructions as there are vector ones (4M tokens: 32 us).
+template <int kRounds, int kBlockWaves, bool kAlone, bool kPlain>
 __global__ __launch_bounds__(kBlockWaves * 64) void policy_tokens_kernel(Policy a, Packed p,
                                                                          PolicyOut o, Saved s,
                                                                          Scratch w,
                                                                          int64_t tiles) {
   __shared__ double shared[kBlockWaves * kSums];
+  constexpr int kThreads = kBlockWaves * 64;
   const int64_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if constexpr (kPlain) {
+    a.x.dtype = a.old.dtype = a.advantage.dtype = FRWKV_DTYPE_F32;
+    if (a.reference.given()) a.reference.dtype = FRWKV_DTYPE_F32;
+    if (a.entropy.given()) a.entropy.dtype = FRWKV_DTYPE_F32;
+  }
   double sums[kSums] = {};
   policy_tile<kRounds>(a, p, o, s, w,
                        static_cast<int64_t>(blockIdx.x) * kBlockWaves + wave, sums);
+  sums[kBad] = bad_offsets(p, static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x,
+                           static_cast<int64_t>(gridDim.x) * kThreads);
   workgroup_sum<kBlockWaves>(sums, shared);
   if constexpr (kAlone) {
-    double found[3] = {};
-    join_sequences(p, o, s, w, 64 * kRounds, tiles, wave, kBlockWaves, found);
+    double found[2] = {};
+    join_sequences(p, o, s, w, shift_of(kRounds), tiles, wave, kBlockWaves, found);
     workgroup_sum<kBlockWaves>(found, shared);
     if (threadIdx.x == 0) write_policy(o, s, sums, found);
   } else if (threadIdx.x == 0) {
@@ -494,38 +624,48 @@ __global__ __launch_bounds__(kBlockWaves * 64) void policy_tokens_kernel(Policy 
   }
 }
 
+// Whether this is the last of the launch's workgroups to end, which then has all of
+// their sums.
+template <int kValues>
+__device__ __forceinline__ bool last_with_all(double (&found)[kValues], const Scratch& w,
+                                              double* shared) {
+  __shared__ bool last;
+  if (gridDim.x == 1) return true;
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int v = 0; v < kValues; ++v) {
+      __hip_atomic_store(w.joins + blockIdx.x * kValues + v, found[v], __ATOMIC_RELAXED,
+                         __HIP_MEMORY_SCOPE_AGENT);
+    }
+    last = __hip_atomic_fetch_add(w.done, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) ==
+           static_cast<int32_t>(gridDim.x) - 1;
+  }
+  __syncthreads();
+  if (!last) return false;
+#pragma unroll
+  for (int v = 0; v < kValues; ++v) {
+    found[v] = threadIdx.x < gridDim.x
+                   ? __hip_atomic_load(w.joins + threadIdx.x * kValues + v, __ATOMIC_RELAXED,
+                                       __HIP_MEMORY_SCOPE_AGENT)
+                   : 0.0;
+  }
+  workgroup_sum<kJoinWaves>(found, shared);
+  return true;
+}
+
 __global__ __launch_bounds__(kJoinThreads) void policy_join_kernel(Packed p, PolicyOut o, Saved s,
-                                                                   Scratch w, int tile_tokens,
+                                                                   Scratch w, int tile_shift,
                                                                    int64_t tiles,
                                                                    int32_t blocks) {
   __shared__ double shared[kJoinWaves * kSums];
-  __shared__ bool last;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  double found[3] = {};
-  join_sequences(p, o, s, w, tile_tokens, tiles,
+  double found[2] = {};
+  join_sequences(p, o, s, w, tile_shift, tiles,
                  static_cast<int64_t>(blockIdx.x) * kJoinWaves + wave,
                  static_cast<int64_t>(gridDim.x) * kJoinWaves, found);
-  workgroup_sum<kJoinWaves>(found, shared);
-  if (gridDim.x > 1) {
-    if (threadIdx.x == 0) {
-#pragma unroll
-      for (int v = 0; v < 3; ++v) {
-        __hip_atomic_store(w.joins + blockIdx.x * 3 + v, found[v], __ATOMIC_RELAXED,
-                           __HIP_MEMORY_SCOPE_AGENT);
-      }
-      last = __hip_atomic_fetch_add(w.done, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) ==
-             static_cast<int32_t>(gridDim.x) - 1;
-    }
-    __syncthreads();
-    if (!last) return;
-#pragma unroll
-    for (int v = 0; v < 3; ++v) {
-      found[v] = threadIdx.x < gridDim.x
-                     ? __hip_atomic_load(w.joins + threadIdx.x * 3 + v, __ATOMIC_RELAXED,
-                                         __HIP_MEMORY_SCOPE_AGENT)
-                     : 0.0;
-    }
+  if (o.reduction == FRWKV_REDUCE_SEQUENCE_MEAN) {
     workgroup_sum<kJoinWaves>(found, shared);
+    if (!last_with_all(found, w, shared)) return;
   }
   double sums[kSums] = {};
   for (int32_t b = threadIdx.x; b < blocks; b += kJoinThreads) {
@@ -551,42 +691,43 @@ template <int kRounds>
 __global__ __launch_bounds__(kWaves * 64) void policy_grad_kernel(Packed p, PolicyGrad g,
                                                                   Saved s) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t first = (static_cast<int64_t>(blockIdx.x) * kWaves + wave) * (64 * kRounds);
-  if (first >= p.n) return;
+  const Tile<kRounds> tile(static_cast<int64_t>(blockIdx.x) * kWaves + wave, p.n);
+  if (tile.empty()) return;
   float slope[kRounds], up[kRounds];
   bool part[kRounds];
-  const bool per_token = g.reduction == FRWKV_REDUCE_NONE;
+  if (g.x != nullptr) tile.fetch(s.slope, slope);
+  if (g.reduction == FRWKV_REDUCE_NONE) {
+    tile.fetch(g.upstream, up);
+  } else {
 #pragma unroll
-  for (int r = 0; r < kRounds; ++r) {
-    const int64_t i = min(first + 64 * r + lane_id(), p.n - 1);
-    slope[r] = g.x != nullptr ? s.slope[i] : 0.0f;
-    up[r] = g.upstream[per_token ? i : 0];
-    part[r] = g.entropy == nullptr || p.mask == nullptr || p.mask[i] != 0;
+    for (int r = 0; r < kRounds; ++r) up[r] = *g.upstream;
   }
+  tile.fetch_part(g.entropy != nullptr ? p.mask : nullptr, part);
   const float share = *s.share;
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) up[r] *= share;
   const bool by_sequence = g.reduction == FRWKV_REDUCE_SEQUENCE_MEAN;
-  int32_t id[kRounds];
-  float weight[kRounds];
+  if (by_sequence) {
+    int32_t id[kRounds];
+    sequences_of<kRounds>(p, tile.first, id);
 #pragma unroll
-  for (int r = 0; r < kRounds; ++r) weight[r] = share;
-  if (by_sequence || (g.entropy != nullptr && p.cu != nullptr)) {
-    sequences_of<kRounds>(p, first, id);
-#pragma unroll
-    for (int r = 0; r < kRounds; ++r) part[r] = part[r] && id[r] < p.sequences;
-    if (by_sequence) {
-#pragma unroll
-      for (int r = 0; r < kRounds; ++r) weight[r] *= s.weight[min(id[r], p.sequences - 1)];
+    for (int r = 0; r < kRounds; ++r) {
+      part[r] = part[r] && id[r] < p.sequences;
+      up[r] *= s.weight[min(id[r], p.sequences - 1)];
     }
+  } else if (g.entropy != nullptr && p.cu != nullptr) {
+    const int64_t end = p.cu[p.sequences] - tile.first;
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) part[r] = part[r] && 64 * r + lane_id() < end;
   }
 #pragma unroll
   for (int r = 0; r < kRounds; ++r) {
-    const int64_t i = first + 64 * r + lane_id();
-    if (i >= p.n) continue;
-    const float by = up[r] * weight[r];
+    if (!tile.has(r)) continue;
+    const int64_t i = tile.first + 64 * r + lane_id();
     // A slope of 0, as a token without part has, stays 0 under any upstream.
-    if (g.x != nullptr) store_at(g.x, g.x_dtype, i, slope[r] == 0.0f ? 0.0f : slope[r] * by);
+    if (g.x != nullptr) store_at(g.x, g.x_dtype, i, slope[r] == 0.0f ? 0.0f : slope[r] * up[r]);
     if (g.entropy != nullptr) {
-      store_at(g.entropy, g.entropy_dtype, i, part[r] ? -g.ew * by : 0.0f);
+      store_at(g.entropy, g.entropy_dtype, i, part[r] ? -g.ew * up[r] : 0.0f);
     }
   }
 }
@@ -613,22 +754,18 @@ struct PreferenceSaved {
 
 template <int kRounds>
 __device__ __forceinline__ void preference_tile(const Preference& a, const Packed& p, Piece* all,
-                                                int64_t tile) {
-  const int64_t first = tile * (64 * kRounds);
-  if (first >= p.n) return;
+                                                int64_t index) {
+  const Tile<kRounds> tile(index, p.n);
+  if (tile.empty()) return;
   uint32_t x[kRounds], reference[kRounds];
   bool part[kRounds];
-#pragma unroll
-  for (int r = 0; r < kRounds; ++r) {
-    const int64_t i = first + 64 * r + lane_id(), at = min(i, p.n - 1);
-    x[r] = bits_at(a.x, at);
-    if (a.reference.given()) reference[r] = bits_at(a.reference, at);
-    part[r] = i < p.n && (p.mask == nullptr || p.mask[at] != 0);
-  }
+  tile.fetch(a.x, x);
+  if (a.reference.given()) tile.fetch(a.reference, reference);
+  tile.fetch_part(p.mask, part);
   int32_t id[kRounds];
-  sequences_of<kRounds>(p, first, id);
+  sequences_of<kRounds>(p, tile.first, id);
   Pieces pieces;
-  pieces.at = all + tile;
+  pieces.at = all + index;
   pieces.sequences = p.sequences;
   pieces.open = __builtin_amdgcn_readfirstlane(id[0]);
 #pragma unroll
@@ -665,7 +802,7 @@ __device__ __forceinline__ void preference_term(const Preference& a, double m, d
 // offsets}. A lane has one sequence, even ones the chosen.
 __device__ __forceinline__ void join_pairs(const Preference& a, const Packed& p,
                                            const PreferenceOut& o, const PreferenceSaved& s,
-                                           const Piece* pieces, int tile_tokens, int64_t tiles,
+                                           const Piece* pieces, int tile_shift, int64_t tiles,
                                            int64_t wave, int64_t waves, double (&found)[3]) {
   int64_t each = (p.sequences / 2 + waves - 1) / waves;
   each = 2 * min(max(each, int64_t{1}), int64_t{32});
@@ -673,7 +810,7 @@ __device__ __forceinline__ void join_pairs(const Preference& a, const Packed& p,
     const bool mine = lane_id() < each && at + lane_id() < p.sequences;
     const int32_t b = mine ? static_cast<int32_t>(at) + lane_id() : -1;
     if (mine && !in_order(p, b)) found[2] += 1.0;
-    const Piece x = sum_of(p, pieces, tile_tokens, tiles, b);
+    const Piece x = sum_of(p, pieces, tile_shift, tiles, b);
     const double by = a.normalize && x.count > 0 ? 1.0 / static_cast<double>(x.count) : 1.0;
     const double reward = a.beta * (x.sum * by);
     const double other = __shfl_xor(reward, 1, 64);
@@ -716,7 +853,7 @@ __global__ __launch_bounds__(kBlockWaves * 64) void preference_tokens_kernel(
     __shared__ double shared[kBlockWaves * 3];
     __syncthreads();
     double found[3] = {};
-    join_pairs(a, p, o, s, w.pieces, 64 * kRounds, tiles, wave, kBlockWaves, found);
+    join_pairs(a, p, o, s, w.pieces, shift_of(kRounds), tiles, wave, kBlockWaves, found);
     workgroup_sum<kBlockWaves>(found, shared);
     if (threadIdx.x == 0) write_preference(o, s, found);
   } else if (blockIdx.x == 0 && threadIdx.x == 0) {
@@ -725,37 +862,16 @@ __global__ __launch_bounds__(kBlockWaves * 64) void preference_tokens_kernel(
 }
 
 __global__ __launch_bounds__(kJoinThreads) void preference_join_kernel(
-    Preference a, Packed p, PreferenceOut o, PreferenceSaved s, Scratch w, int tile_tokens,
+    Preference a, Packed p, PreferenceOut o, PreferenceSaved s, Scratch w, int tile_shift,
     int64_t tiles) {
   __shared__ double shared[kJoinWaves * 3];
-  __shared__ bool last;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   double found[3] = {};
-  join_pairs(a, p, o, s, w.pieces, tile_tokens, tiles,
+  join_pairs(a, p, o, s, w.pieces, tile_shift, tiles,
              static_cast<int64_t>(blockIdx.x) * kJoinWaves + wave,
              static_cast<int64_t>(gridDim.x) * kJoinWaves, found);
   workgroup_sum<kJoinWaves>(found, shared);
-  if (gridDim.x > 1) {
-    if (threadIdx.x == 0) {
-#pragma unroll
-      for (int v = 0; v < 3; ++v) {
-        __hip_atomic_store(w.joins + blockIdx.x * 3 + v, found[v], __ATOMIC_RELAXED,
-                           __HIP_MEMORY_SCOPE_AGENT);
-      }
-      last = __hip_atomic_fetch_add(w.done, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) ==
-             static_cast<int32_t>(gridDim.x) - 1;
-    }
-    __syncthreads();
-    if (!last) return;
-#pragma unroll
-    for (int v = 0; v < 3; ++v) {
-      found[v] = threadIdx.x < gridDim.x
-                     ? __hip_atomic_load(w.joins + threadIdx.x * 3 + v, __ATOMIC_RELAXED,
-                                         __HIP_MEMORY_SCOPE_AGENT)
-                     : 0.0;
-    }
-    workgroup_sum<kJoinWaves>(found, shared);
-  }
+  if (!last_with_all(found, w, shared)) return;
   if (threadIdx.x == 0) write_preference(o, s, found);
 }
 
@@ -764,26 +880,22 @@ __global__ __launch_bounds__(kWaves * 64) void preference_grad_kernel(
     Packed p, PreferenceSaved s, const float* __restrict__ upstream, bool per_pair,
     void* grad_x, int x_dtype) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t first = (static_cast<int64_t>(blockIdx.x) * kWaves + wave) * (64 * kRounds);
-  if (first >= p.n) return;
+  const Tile<kRounds> tile(static_cast<int64_t>(blockIdx.x) * kWaves + wave, p.n);
+  if (tile.empty()) return;
   bool part[kRounds];
-#pragma unroll
-  for (int r = 0; r < kRounds; ++r) {
-    const int64_t i = min(first + 64 * r + lane_id(), p.n - 1);
-    part[r] = p.mask == nullptr || p.mask[i] != 0;
-  }
+  tile.fetch_part(p.mask, part);
   const float share = *s.share;
   int32_t id[kRounds];
-  sequences_of<kRounds>(p, first, id);
+  sequences_of<kRounds>(p, tile.first, id);
 #pragma unroll
   for (int r = 0; r < kRounds; ++r) {
-    const int64_t i = first + 64 * r + lane_id();
-    if (i >= p.n) continue;
     const int32_t b = min(id[r], p.sequences - 1);
     const float c = s.coefficient[b];
     const bool here = part[r] && id[r] < p.sequences && c != 0.0f;
     const float up = upstream[per_pair ? b / 2 : 0] * share;
-    store_at(grad_x, x_dtype, i, here ? c * up : 0.0f);
+    if (tile.has(r)) {
+      store_at(grad_x, x_dtype, tile.first + 64 * r + lane_id(), here ? c * up : 0.0f);
+    }
   }
 }
 
@@ -837,10 +949,11 @@ Scratch scratch_of(char* p, int64_t tokens, int64_t sequences, size_t* bytes) {
           reinterpret_cast<double*>(p + joins), reinterpret_cast<Piece*>(p + pieces)};
 }
 
-// Workgroups of a join: a wave for each sequence, or 64 a wave of many.
+// Workgroups of a join, 64 sequences a wave: up to 1024 need no other workgroup,
+// whose sums would take two trips through memory.
 unsigned joins_of(int64_t sequences) {
   return static_cast<unsigned>(
-      std::clamp<int64_t>((sequences + kJoinWaves - 1) / kJoinWaves, 1, kMostJoins));
+      std::clamp<int64_t>((sequences + kJoinThreads - 1) / kJoinThreads, 1, kMostJoins));
 }
 
 bool known_dtype(int dtype) {
@@ -981,9 +1094,12 @@ int frwkv_policy_loss_forward(int64_t tokens, int64_t sequences, const int32_t* 
   rc = check_memory(what, "workspace", workspace, workspace_bytes, need);
   if (rc != FRWKV_OK) return rc;
   a.per_sequence = advantages_per_sequence != 0;
-  a.above = std::log1p(clip_high);
-  a.below = std::log1p(-clip_low);
-  a.far = dual_clip > 0.0 ? std::log(dual_clip) : 0.0;
+  a.above_exact = std::log1p(clip_high);
+  a.below_exact = std::log1p(-clip_low);
+  a.far_exact = dual_clip > 0.0 ? std::log(dual_clip) : a.above_exact;
+  a.above = static_cast<float>(a.above_exact);
+  a.below = static_cast<float>(a.below_exact);
+  a.far = static_cast<float>(a.far_exact);
   a.most = static_cast<float>(1.0 + clip_high);
   a.least = static_cast<float>(1.0 - clip_low);
   a.dual = static_cast<float>(dual_clip);
@@ -993,18 +1109,31 @@ int frwkv_policy_loss_forward(int64_t tokens, int64_t sequences, const int32_t* 
   const PolicyOut o{loss, metrics, reduction, want_slopes != 0};
   const int64_t tiles = tiles_of(tokens);
   const hipStream_t q = static_cast<hipStream_t>(stream);
-  with_rounds(tokens, [&](auto rounds) {
+  bool plain = true;
+  for (const Column* c : {&a.x, &a.old, &a.advantage, &a.reference, &a.entropy}) {
+    plain = plain && (!c->given() || c->dtype == FRWKV_DTYPE_F32);
+  }
+  const auto run = [&](auto rounds, auto all_plain) {
     constexpr int kRounds = decltype(rounds)::value;
+    constexpr bool kPlain = decltype(all_plain)::value;
     if (tiles <= kJoinWaves) {
-      hipLaunchKernelGGL((policy_tokens_kernel<kRounds, kJoinWaves, true>), dim3(1),
+      hipLaunchKernelGGL((policy_tokens_kernel<kRounds, kJoinWaves, true, kPlain>), dim3(1),
                          dim3(kJoinThreads), 0, q, a, p, o, s, w, tiles);
       return;
     }
     const unsigned blocks = blocks_of(tiles);
-    hipLaunchKernelGGL((policy_tokens_kernel<kRounds, kWaves, false>), dim3(blocks),
+    hipLaunchKernelGGL((policy_tokens_kernel<kRounds, kWaves, false, kPlain>), dim3(blocks),
                        dim3(kWaves * 64), 0, q, a, p, o, s, w, tiles);
-    hipLaunchKernelGGL(policy_join_kernel, dim3(joins_of(sequences)), dim3(kJoinThreads), 0, q, p,
-                       o, s, w, 64 * kRounds, tiles, static_cast<int32_t>(blocks));
+    const unsigned joins = reduction == FRWKV_REDUCE_SEQUENCE_MEAN ? joins_of(sequences) : 1;
+    hipLaunchKernelGGL(policy_join_kernel, dim3(joins), dim3(kJoinThreads), 0, q, p, o, s, w,
+                       shift_of(kRounds), tiles, static_cast<int32_t>(blocks));
+  };
+  with_rounds(tokens, [&](auto rounds) {
+    if (plain) {
+      run(rounds, std::true_type{});
+    } else {
+      run(rounds, std::false_type{});
+    }
   });
   return check_launch("policy loss forward");
 }
@@ -1110,7 +1239,7 @@ int frwkv_preference_loss_forward(int64_t tokens, int64_t pairs, const int32_t* 
     hipLaunchKernelGGL((preference_tokens_kernel<kRounds, kWaves, false>), dim3(blocks_of(tiles)),
                        dim3(kWaves * 64), 0, q, a, p, o, s, w, tiles);
     hipLaunchKernelGGL(preference_join_kernel, dim3(joins_of(sequences)), dim3(kJoinThreads), 0, q,
-                       a, p, o, s, w, 64 * kRounds, tiles);
+                       a, p, o, s, w, shift_of(kRounds), tiles);
   });
   return check_launch("preference loss forward");
 }

@@ -245,6 +245,30 @@ def test_small_kl_keeps_its_digits():
     torch.testing.assert_close(grad.double(), -torch.expm1(t), rtol=8 * E, atol=0)
 
 
+def test_policy_ratios_far_out_stay_what_the_formula_says():
+    """Ratios that are 0 or infinite in 32 bits: clipped where the clip bounds them."""
+    old = torch.tensor([-200.0, 0.0, -math.inf, 0.0, -100.0, 0.0], device=DEV)
+    x = torch.tensor([0.0, -200.0, 0.0, -math.inf, 0.0, -100.0], device=DEV)
+    leaf = x.clone().requires_grad_()
+    loss = pretrain_policy_loss(leaf, old, torch.ones_like(x), reduction="none")
+    grad, = torch.autograd.grad(loss.sum(), [leaf])
+    assert loss.tolist() == pytest.approx([-1.2, 0.0, -1.2, 0.0, -1.2, 0.0])
+    assert not grad.any()
+    loss = pretrain_policy_loss(leaf, old, -torch.ones_like(x), reduction="none")
+    grad, = torch.autograd.grad(loss.sum(), [leaf])
+    for t in (loss, grad):
+        assert t.tolist() == pytest.approx([math.inf, 0.8, math.inf, 0.8, math.inf, 0.8]
+                                           if t is loss else
+                                           [math.inf, 0.0, math.inf, 0.0, math.inf, 0.0])
+    loss = pretrain_policy_loss(leaf, x, -torch.ones_like(x), reduction="none", kl_weight=1.0,
+                                reference_log_probs=torch.tensor(
+                                    [-300.0, 0.0, 0.0, 0.0, 60.0, -190.0], device=DEV))
+    assert loss[0].item() == 300.0 - 1.0 + 1.0
+    assert loss[1].item() == math.inf and loss[2].item() == 1.0
+    assert loss[4].item() == pytest.approx(math.exp(60.0) - 61.0 + 1.0, rel=64 * E)
+    assert loss[5].item() == pytest.approx(90.0 - 1.0 + 1.0)
+
+
 def test_policy_tokens_without_part_may_hold_anything():
     for reduction in ("mean", "sequence_mean", "none"):
         x, old, a, args, up = _policy([500, 40, 700], reduction=reduction, tail=30, seed=10)
