@@ -237,10 +237,12 @@ def linear_loss_backward(grad_loss, weight, saved, rows, top, temperature, reduc
                                     bool(want_weight))
 
 
-def linear_log_probs_forward(hidden, weight, targets, ignore_index, temperature, entropy):
+def linear_log_probs_forward(hidden, weight, targets, ignore_index, temperature, entropy,
+                             backward_follows=True):
     """[log_probs, saved], or [log_probs, entropy, saved]."""
     return ops.linear_log_probs_forward(hidden, weight, targets, int(ignore_index),
-                                        float(temperature), bool(entropy))
+                                        float(temperature), bool(entropy),
+                                        bool(backward_follows))
 
 
 def linear_log_probs_backward(grad_log_probs, grad_entropy, weight, saved, rows, temperature,

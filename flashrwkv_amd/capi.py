@@ -79,7 +79,7 @@ SIGNATURES = {
     "frwkv_linear_log_probs_forward_workspace_bytes": [_I64] * 2 + [_INT],
     "frwkv_linear_log_probs_backward_workspace_bytes": [_I64] * 3 + [_INT] * 2,
     "frwkv_linear_log_probs_forward": [_INT] + [_I64] * 3 + [_VP, _VP, _INT, _VP, _I64, _F32]
-                                      + [_VP] * 3 + [_SZ, _VP, _SZ, _VP],
+                                      + [_INT] + [_VP] * 3 + [_SZ, _VP, _SZ, _VP],
     "frwkv_linear_log_probs_backward": [_INT] + [_I64] * 3 + [_VP, _F32] + [_VP] * 3
                                        + [_SZ] + [_VP] * 3 + [_SZ, _VP],
     "frwkv_policy_loss_saved_bytes": [_I64] * 2,
@@ -433,7 +433,7 @@ def linear_loss_backward(grad_loss, weight, saved, *, rows, top, temperature=1.0
 
 
 def linear_log_probs_forward(hidden, weight, targets, *, log_probs, entropy=None,
-                             temperature=1.0, ignore_index=-100):
+                             temperature=1.0, ignore_index=-100, backward_follows=True):
     """Writes ``log_probs`` and, where given, ``entropy`` (fp32); returns the buffer that the
     backward reads."""
     vocab, c = weight.shape
@@ -444,8 +444,8 @@ def linear_log_probs_forward(hidden, weight, targets, *, log_probs, entropy=None
         rows, vocab, entropy is not None)), hidden.device)
     _check(lib.frwkv_linear_log_probs_forward(
         DTYPE[hidden.dtype], rows, c, vocab, _p(hidden), _p(weight), targets.element_size(),
-        _p(targets), int(ignore_index), float(temperature), _p(log_probs), _p(entropy),
-        _p(saved), saved.numel(), _p(work), work.numel(), _stream()))
+        _p(targets), int(ignore_index), float(temperature), int(backward_follows),
+        _p(log_probs), _p(entropy), _p(saved), saved.numel(), _p(work), work.numel(), _stream()))
     return saved
 
 

@@ -149,7 +149,8 @@ pybind11::object linear_log_probs_call(const pybind11::object& hidden_,
   variable_list out;
   {
     pybind11::gil_scoped_release release;
-    out = linear_log_probs_forward(hidden, weight, targets, ignore_index, temperature, entropy);
+    out = linear_log_probs_forward(hidden, weight, targets, ignore_index, temperature, entropy,
+                                   torch::autograd::compute_requires_grad(hidden, weight));
     const Tensor saved = std::move(out.back());
     out.pop_back();
     record<LinearLogProbsNode>(

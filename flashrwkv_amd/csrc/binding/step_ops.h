@@ -9,7 +9,7 @@ namespace {
 // {log_probs}, {log_probs, entropy}, and what the backward reads after them.
 std::vector<Tensor> linear_log_probs_forward(Tensor hidden, Tensor weight, Tensor targets,
                                              int64_t ignore_index, double temperature,
-                                             bool entropy) {
+                                             bool entropy, bool backward_follows) {
   const int64_t rows = check_head(hidden, weight, FRWKV_REDUCE_NONE);
   check_device_contiguous(targets, "targets");
   const int bytes = index_bytes(targets, "targets");
@@ -27,7 +27,7 @@ std::vector<Tensor> linear_log_probs_forward(Tensor hidden, Tensor weight, Tenso
   check_rc(frwkv_linear_log_probs_forward(
       io_code(hidden.scalar_type()), rows, c, vocab, hidden.const_data_ptr(),
       weight.const_data_ptr(), bytes, targets.const_data_ptr(), ignore_index,
-      static_cast<float>(temperature), out[0].data_ptr<float>(),
+      static_cast<float>(temperature), backward_follows, out[0].data_ptr<float>(),
       entropy ? out[1].data_ptr<float>() : nullptr, scratch_ptr(saved), saved_bytes,
       scratch_ptr(work), work_bytes, current_stream(hidden)));
   out.push_back(saved);

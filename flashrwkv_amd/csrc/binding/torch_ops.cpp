@@ -1535,7 +1535,7 @@ TORCH_LIBRARY(flashrwkv2, m) {
       &linear_loss_backward);
   m.def(
       "linear_log_probs_forward(Tensor hidden, Tensor weight, Tensor targets, int ignore_index, "
-      "float temperature, bool entropy) -> Tensor[]",
+      "float temperature, bool entropy, bool backward_follows) -> Tensor[]",
       &linear_log_probs_forward);
   m.def(
       "linear_log_probs_backward(Tensor? grad_log_probs, Tensor? grad_entropy, Tensor weight, "

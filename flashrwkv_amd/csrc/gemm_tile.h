@@ -74,12 +74,22 @@ struct Operand {
 // operand, so it knows what stands there (saved and restored in the block, as a
 // register that cannot be declared as written, the small tiles were 2% slower); a
 // load reads m0 one wait state after its write at the earliest.
+// kStream: not kept in the caches.
+template <bool kStream>
 __device__ __forceinline__ void load_to_lds(u32x4 buffer, uint32_t offset, uint32_t lds) {
-  asm volatile(
-      "s_nop 0\n\t"
-      "buffer_load_dwordx4 %0, %1, 0 offen lds"
-      :
-      : "v"(offset), "s"(buffer), "{m0}"(lds));
+  if constexpr (kStream) {
+    asm volatile(
+        "s_nop 0\n\t"
+        "buffer_load_dwordx4 %0, %1, 0 offen nt lds"
+        :
+        : "v"(offset), "s"(buffer), "{m0}"(lds));
+  } else {
+    asm volatile(
+        "s_nop 0\n\t"
+        "buffer_load_dwordx4 %0, %1, 0 offen lds"
+        :
+        : "v"(offset), "s"(buffer), "{m0}"(lds));
+  }
 }
 
 // Waits until at most kLeft of this wave's loads are outstanding and its LDS
@@ -92,7 +102,7 @@ __device__ __forceinline__ void wait_and_barrier() {
 // The loads of one operand's stages by the whole workgroup: 16-byte pieces, one
 // a thread and round. A thread's offset from the round's first row never
 // changes; the rounds' and stages' first rows are scalars.
-template <Major M, int BX, bool kTurn>
+template <Major M, int BX, bool kTurn, bool kStream = false>
 struct Loader {
   static constexpr int kRounds = BX * 8 / kThreads;
   static constexpr int kBytes = BX * kStep * 2;
@@ -146,7 +156,7 @@ struct Loader {
     const uint64_t address = reinterpret_cast<uint64_t>(from);
     const u32x4 buffer = {static_cast<uint32_t>(address), static_cast<uint32_t>(address >> 32),
                           static_cast<uint32_t>(bytes), 0x00020000u};
-    load_to_lds(buffer, offset, lds + j * (kThreads * 16u) + wave_lds);
+    load_to_lds<kStream>(buffer, offset, lds + j * (kThreads * 16u) + wave_lds);
   }
   // Moves on to the stage after it.
   __device__ __forceinline__ void next() {
@@ -205,9 +215,11 @@ struct Reader {
 // acc[i][j] of lane (g, n) is D[p0 + 16 i + 4 g + r][q0 + 16 j + n], r = 0..3,
 // p0 = BP / WP * (wave / WQ), q0 = BQ / WQ * (wave % WQ).
 template <typename T, Major MA, Major MB, int BP, int BQ, int WP, int WQ, int NS,
-          bool kTurn = false>
+          bool kTurn = false, bool kStream = false>
 struct Tile {
   static constexpr bool kTurns = kTurn;
+  // The same with A's loads past the caches.
+  using Streaming = Tile<T, MA, MB, BP, BQ, WP, WQ, NS, kTurn, true>;
   static constexpr int kBP = BP, kBQ = BQ, kWP = WP, kWQ = WQ;
   static constexpr int TP = BP / WP / 16;
   static constexpr int TQ = BQ / WQ / 16;
@@ -216,7 +228,7 @@ struct Tile {
   static_assert(WP * WQ * 64 == kThreads, "8 waves");
   static_assert(kLdsBytes <= 160 * 1024, "LDS of a CU");
 
-  using LoadA = Loader<MA, BP, kTurn>;
+  using LoadA = Loader<MA, BP, kTurn, kStream>;
   using LoadB = Loader<MB, BQ, kTurn>;
   static constexpr int kLoads = LoadA::kRounds + LoadB::kRounds;
 

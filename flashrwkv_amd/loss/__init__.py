@@ -162,7 +162,7 @@ class _LinearLogProbs(torch.autograd.Function):
             ctx.save_for_backward(weight)
             return tuple(torch.zeros(hidden.shape[:-1], device=hidden.device,
                                      dtype=torch.float32) for _ in range(1 + entropy))
-        *out, saved = launch(hidden, weight)
+        *out, saved = launch(hidden, weight, any(ctx.needs_input_grad))
         ctx.save_for_backward(weight, saved)
         return tuple(out)
 
@@ -298,9 +298,9 @@ def pretrain_linear_log_probs(
                           "temperature": temperature, "ignore_index": ignore_index})
     _refuse_capture("pretrain_linear_log_probs")
 
-    def launch(h, w):
+    def launch(h, w, backward_follows):
         return C.native().linear_log_probs_forward(h, w, targets, ignore_index, temperature,
-                                                   entropy)
+                                                   entropy, backward_follows)
 
     got = _LinearLogProbs.apply(hidden, weight, launch, float(temperature), bool(entropy))
     return got if entropy else got[0]

@@ -726,7 +726,8 @@ int frwkv_linear_loss_backward(int io_dtype, int64_t rows, int64_t channels, int
  * log q[targets[i]] and, where entropy is not NULL, entropy[i] = -sum q log q
  * (both fp32 [rows]; 0 for rows whose target is ignore_index, NaN for a target out of
  * range). Operands, sizes and saved (frwkv_linear_loss_saved_bytes with top 1) as
- * for frwkv_linear_cross_entropy_forward.
+ * for frwkv_linear_cross_entropy_forward. backward_follows 0: the weight is not read
+ * again soon (a hint; saved is written either way).
  *
  * frwkv_linear_log_probs_backward: grad_log_probs and grad_entropy fp32 [rows],
  * either NULL for zeros, not both (grad_entropy only where the forward gave
@@ -741,9 +742,9 @@ size_t frwkv_linear_log_probs_backward_workspace_bytes(int64_t rows, int64_t cha
 int frwkv_linear_log_probs_forward(int io_dtype, int64_t rows, int64_t channels, int64_t vocab,
                                    const void* hidden, const void* weight, int target_bytes,
                                    const void* targets, int64_t ignore_index, float temperature,
-                                   float* log_probs, float* entropy, void* saved,
-                                   size_t saved_bytes, void* workspace, size_t workspace_bytes,
-                                   void* stream);
+                                   int backward_follows, float* log_probs, float* entropy,
+                                   void* saved, size_t saved_bytes, void* workspace,
+                                   size_t workspace_bytes, void* stream);
 int frwkv_linear_log_probs_backward(int io_dtype, int64_t rows, int64_t channels, int64_t vocab,
                                     const void* weight, float temperature,
                                     const float* grad_log_probs, const float* grad_entropy,

@@ -164,6 +164,18 @@ def test_a_large_vocabulary_in_pieces(dtype):
     _check(h, w, targets, _run(h, w, targets, g, e), temperature=1.0, g=g, e=e)
 
 
+@pytest.mark.parametrize("n", [1, 40])
+def test_a_weight_beyond_the_caches_is_read_alike(n):
+    """Without a backward to follow few rows read a large weight past the caches."""
+    c, v = 2048, 50000
+    assert 2 * c * v > 192 << 20
+    h, w, targets, _, _ = _case(n, c, v, torch.bfloat16, seed=12, masked=0.0)
+    alone = pretrain_linear_log_probs(h, w, targets, entropy=True)
+    followed = pretrain_linear_log_probs(h.clone().requires_grad_(), w, targets, entropy=True)
+    assert all(torch.equal(a, b) for a, b in zip(alone, followed))
+    _check(h, w, targets, dict(zip(("log_probs", "entropy"), alone)), temperature=1.0)
+
+
 @pytest.mark.parametrize("shape", [(), (6,), (2, 3)])
 @pytest.mark.parametrize("index", [torch.int32, torch.int64])
 def test_leading_shapes_and_index_types(shape, index):

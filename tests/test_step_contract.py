@@ -209,7 +209,7 @@ def test_c_abi_refuses_before_any_launch():
                                           null, null) == 1 and "grad_loss" in error()
     assert lib.frwkv_linear_log_probs_backward(2, 1, 64, 5, p, 1.0, null, null, p, 1 << 20, p, p,
                                                p, 1 << 20, null) == 1
-    assert lib.frwkv_linear_log_probs_forward(2, 1, 64, 5, p, p, 4, p, -100, 0.0, p, null, p,
+    assert lib.frwkv_linear_log_probs_forward(2, 1, 64, 5, p, p, 4, p, -100, 0.0, 1, p, null, p,
                                               1 << 20, p, 1 << 20, null) == 1
     assert "temperature" in error()
 
