@@ -43,6 +43,8 @@ def _list_of(name):
               f"{name} must be CUDA and strided"),
         check(name, _each(lambda t, ns: t.device == ns["tensors"][0].device), ValueError,
               f"{name} must share the first tensor's device"),
+        check(name, _each(lambda t, ns: not t.is_neg()), ValueError,
+              f"{name} must hold their values, not be negated views"),
         check(name, _each(lambda t, ns: _dense(t)), ValueError,
               f"{name} must leave no gaps in memory"),
     )

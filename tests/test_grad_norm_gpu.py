@@ -54,6 +54,10 @@ LISTS = {
     "chunks": [(3 * 8192,), (2, 8192 + 8), (50000,), (77,)],
     "many": [(1 + (i * 37) % 400,) for i in range(500)],
     "large": [(5_000_003,), (300, 4096), (17,)],
+    # Lists that stand in memory: units that are read together and alone, and a tensor
+    # of more units than are summed at a time.
+    "long list": [(1 + (i * 2477) % 30000,) for i in range(230)],
+    "one of many units": [(40_000_001,), (2048,), (2049,)],
 }
 
 
@@ -75,6 +79,18 @@ def test_clip_in_place_and_into_others(name, over):
     _check(before, tensors, got, most)
     if not over:
         assert all(torch.equal(a, b) for a, b in zip(tensors, before))
+
+
+def test_more_than_the_last_level_cache():
+    """300 MB in bf16 and fp32, read past the caches, 16-byte places or not."""
+    gen = torch.Generator(device=DEV).manual_seed(8)
+    flat = torch.randn(40_000_007, generator=gen, device=DEV)
+    tensors = [flat[3:], torch.randn(70_000_001, generator=gen, device=DEV).bfloat16()]
+    before = [t.clone() for t in tensors]
+    out = [torch.empty_like(t, dtype=torch.float32) for t in tensors]
+    most = 0.1 * math.sqrt(110_000_005)
+    _check(before, out, pretrain_clip_grad_norm(tensors, most, out=out), most)
+    _check(before, tensors, pretrain_clip_grad_norm(tensors, most), most)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -159,6 +175,8 @@ def test_refusals_that_need_a_gpu():
         pretrain_grad_norm([a[::2]])
     with pytest.raises(ValueError, match="gaps"):
         pretrain_grad_norm([a[:1].expand(4)])
+    with pytest.raises(ValueError, match="negated"):
+        pretrain_clip_grad_norm([torch._neg_view(a)], 1.0)
     leaf = torch.ones(4, device=DEV, requires_grad=True)
     with pytest.raises(ValueError, match="must not require gradients"):
         pretrain_clip_grad_norm([leaf], 1.0)

@@ -488,6 +488,49 @@ def test_subclasses_take_the_tables():
         assert torch.equal(got[name].as_subclass(torch.Tensor), want[name]), name
 
 
+def test_the_graph_is_kept_or_freed_as_asked():
+    x, old, _ = _logs(20, seed=27)
+    cu = torch.tensor([0, 11, 20], dtype=torch.int32, device=DEV)
+    leaf = x.clone().requires_grad_()
+    for loss in (pretrain_policy_loss(leaf, old, old), pretrain_preference_loss(leaf, cu)[0]):
+        first, = torch.autograd.grad(loss, [leaf], retain_graph=True)
+        assert torch.equal(torch.autograd.grad(loss, [leaf])[0], first)
+        with pytest.raises(RuntimeError, match="second time"):
+            torch.autograd.grad(loss, [leaf])
+    # A tensor of the caller's that the backward reads and that has changed since.
+    mask = torch.ones(20, dtype=torch.bool, device=DEV)
+    loss, _ = pretrain_preference_loss(leaf, cu, mask=mask)
+    mask[3] = False
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+def test_forward_mode_is_refused():
+    x, old, _ = _logs(20, seed=27)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            pretrain_policy_loss(dual, old, old)
+
+
+def test_backward_on_a_capturing_stream_is_refused():
+    x, old, _ = _logs(20, seed=27)
+    leaf = x.clone().requires_grad_()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        loss = pretrain_policy_loss(leaf, old, old)
+        one = torch.ones((), device=DEV)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        graph.capture_begin()
+        try:
+            with pytest.raises(RuntimeError, match="graph capture"):
+                torch.autograd.grad(loss, [leaf], one)
+        finally:
+            graph.capture_end()
+
+
 def test_second_derivatives_and_captures_are_refused():
     x, old, _ = _logs(20, seed=27)
     cu = torch.tensor([0, 11, 20], dtype=torch.int32, device=DEV)
