@@ -56,6 +56,20 @@ struct List {
   bool in_place;  // all of them
 };
 
+// A tensor on its way to the list in the workspace: its data, and its elements with the
+// types above them; where it is not written in place, its output beside it.
+struct Item {
+  uint64_t from, size;
+};
+constexpr int kTypeBit = 48, kToTypeBit = 52;
+
+template <bool kInPlace>
+struct Items {
+  static constexpr int kCount = kInPlace ? 240 : 160;  // 3.8 KB of arguments
+  Item item[kCount];
+  uint64_t to[kInPlace ? 1 : kCount];
+};
+
 // The list in the workspace.
 struct Places {
   Entry* entry;   // [count]
@@ -256,17 +270,46 @@ __global__ __launch_bounds__(kThreads) void run_squares_kernel(Entries entries, 
   if (threadIdx.x == 0) sums[blockIdx.x] = all;
 }
 
-// A part of the list to the workspace, and its units' owners.
-__global__ __launch_bounds__(kThreads) void list_kernel(Entries part, int32_t count,
-                                                        int32_t index, int32_t units,
-                                                        Places to) {
-  __shared__ int32_t firsts[kEntries];
-  if (threadIdx.x < count) firsts[threadIdx.x] = part.entry[threadIdx.x].first;
-  if (blockIdx.x == 0 && threadIdx.x < count) to.entry[index + threadIdx.x] = part.entry[threadIdx.x];
+// A part of the list to the workspace, and its units' owners. Each workgroup finds the
+// tensors' first units for itself: a launch takes 5 us, of which its arguments' way over
+// the host's link is most, and fewer of them are what counts.
+template <bool kInPlace>
+__global__ __launch_bounds__(kThreads) void list_kernel(Items<kInPlace> part, int32_t count,
+                                                        int32_t index, int32_t first,
+                                                        int32_t units, Places to) {
+  static_assert(Items<kInPlace>::kCount <= kThreads, "a thread a tensor");
+  __shared__ int32_t firsts[kThreads], waves[kThreads / 64];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  Entry e{};
+  int32_t own = 0;
+  if (t < count) {
+    const uint64_t size = part.item[t].size;
+    e.from = reinterpret_cast<const void*>(part.item[t].from);
+    e.to = reinterpret_cast<void*>(kInPlace ? part.item[t].from : part.to[kInPlace ? 0 : t]);
+    e.numel = static_cast<int64_t>(size & ((uint64_t{1} << kTypeBit) - 1));
+    e.dtype = static_cast<uint8_t>(size >> kTypeBit & 3);
+    e.to_dtype = static_cast<uint8_t>(size >> kToTypeBit & 3);
+    e.aligned = reinterpret_cast<uintptr_t>(e.from) % 16 == 0;
+    e.to_aligned = reinterpret_cast<uintptr_t>(e.to) % 16 == 0;
+    own = static_cast<int32_t>((e.numel + kUnit - 1) / kUnit);
+  }
+  int32_t before = own;  // units up to this tensor's end
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int32_t other = __shfl_up(before, off, 64);
+    if (lane >= off) before += other;
+  }
+  if (lane == 63) waves[wave] = before;
   __syncthreads();
-  const int32_t thread = static_cast<int32_t>(blockIdx.x) * kThreads + threadIdx.x;
-  for (int64_t u = thread; u < units; u += static_cast<int64_t>(gridDim.x) * kThreads) {
-    const int32_t unit = firsts[0] + static_cast<int32_t>(u);
+  before += first - own;
+  for (int w = 0; w < wave; ++w) before += waves[w];
+  firsts[t] = before;
+  e.first = before;
+  if (blockIdx.x == 0 && t < count) to.entry[index + t] = e;
+  __syncthreads();
+  for (int64_t u = static_cast<int64_t>(blockIdx.x) * kThreads + t; u < units;
+       u += static_cast<int64_t>(gridDim.x) * kThreads) {
+    const int32_t unit = first + static_cast<int32_t>(u);
     int at = 0, left = count;
     while (left > 1) {
       const int half = left / 2;
@@ -437,22 +480,42 @@ Plan plan_of(int64_t count, const frwkv_gradient* tensors) {
   return p;
 }
 
-// f(entries, how many, index of the first, chunks) for every kEntries tensors with
-// elements; chunks are of `each` units.
-template <typename F>
-void for_entries(int64_t count, const frwkv_gradient* tensors, int each, F&& f) {
-  Entries part;
-  int32_t have = 0, first = 0, done = 0, before = 0;
+// f(items, how many, index of the first, its unit, units) for as many tensors with
+// elements as a launch takes.
+template <bool kInPlace, typename F>
+void for_items(int64_t count, const frwkv_gradient* tensors, F&& f) {
+  Items<kInPlace> part;
+  int32_t have = 0, done = 0, units = 0, before = 0;
   const auto flush = [&] {
-    if (have > 0) f(part, have, done, first - before);
+    if (have > 0) f(part, have, done, before, units - before);
     done += have;
-    before = first;
+    before = units;
     have = 0;
   };
   for (int64_t i = 0; i < count; ++i) {
     const frwkv_gradient& x = tensors[i];
     if (x.numel == 0) continue;
-    if (have == kEntries) flush();
+    if (have == Items<kInPlace>::kCount) flush();
+    part.item[have] = {reinterpret_cast<uint64_t>(x.data),
+                       static_cast<uint64_t>(x.numel) |
+                           static_cast<uint64_t>(x.dtype) << kTypeBit |
+                           static_cast<uint64_t>(x.out_dtype) << kToTypeBit};
+    if constexpr (!kInPlace) part.to[have] = reinterpret_cast<uint64_t>(x.out);
+    ++have;
+    units += static_cast<int32_t>(chunks_of(x.numel, 1));
+  }
+  flush();
+}
+
+// f(entries) of a list of at most kEntries tensors with elements; chunks are of `each`
+// units.
+template <typename F>
+void with_entries(int64_t count, const frwkv_gradient* tensors, int each, F&& f) {
+  Entries part;
+  int32_t have = 0, first = 0;
+  for (int64_t i = 0; i < count; ++i) {
+    const frwkv_gradient& x = tensors[i];
+    if (x.numel == 0) continue;
     part.entry[have++] = {x.data,
                           x.out,
                           x.numel,
@@ -463,7 +526,7 @@ void for_entries(int64_t count, const frwkv_gradient* tensors, int each, F&& f) 
                           aligned16(x.out)};
     first += static_cast<int32_t>(chunks_of(x.numel, each));
   }
-  flush();
+  f(part);
 }
 
 int check_tensors(const char* what, int64_t count, const frwkv_gradient* tensors, bool out) {
@@ -525,12 +588,20 @@ void launch(const Plan& plan, int64_t count, const frwkv_gradient* tensors, bool
     char* at = workspace + 256 + plan.sums_bytes();
     const Places places{reinterpret_cast<Entry*>(at),
                         reinterpret_cast<int32_t*>(at + plan.entry_bytes())};
-    for_entries(count, tensors, 1, [&](const Entries& part, int32_t have, int32_t first,
-                                       int32_t units) {
-      const int blocks = std::clamp<int>(units / (4 * kThreads), 1, 256);
-      hipLaunchKernelGGL(list_kernel, dim3(blocks), dim3(kThreads), 0, stream, part, have, first,
-                         units, places);
-    });
+    const auto write = [&](auto in_place) {
+      constexpr bool kInPlace = decltype(in_place)::value;
+      for_items<kInPlace>(count, tensors, [&](const Items<kInPlace>& part, int32_t have,
+                                              int32_t index, int32_t first, int32_t units) {
+        const int blocks = std::clamp<int>(units / (4 * kThreads), 1, 256);
+        hipLaunchKernelGGL((list_kernel<kInPlace>), dim3(blocks), dim3(kThreads), 0, stream, part,
+                           have, index, first, units, places);
+      });
+    };
+    if (list.in_place || !scale) {  // the norm alone writes nothing
+      write(std::true_type{});
+    } else {
+      write(std::false_type{});
+    }
     with_stream(plan.stream, [&](auto streaming) {
       constexpr bool kStream = decltype(streaming)::value;
       hipLaunchKernelGGL((squares_kernel<kStream>), dim3(groups), dim3(kThreads), 0, stream,
@@ -546,7 +617,7 @@ void launch(const Plan& plan, int64_t count, const frwkv_gradient* tensors, bool
   }
   const auto run = [&](auto each) {
     constexpr int kEach = decltype(each)::value;
-    for_entries(count, tensors, kEach, [&](const Entries& entries, int32_t, int32_t, int32_t) {
+    with_entries(count, tensors, kEach, [&](const Entries& entries) {
       hipLaunchKernelGGL((run_squares_kernel<kEach>), dim3(groups), dim3(kThreads), 0, stream,
                          entries, list, sums);
       if (scale) {
