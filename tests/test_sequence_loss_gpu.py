@@ -1,12 +1,14 @@
 """GPU parity of the policy and preference losses against oracle/step.py (64 bits).
 
-Bounds, before any run. A token's log ratio is exact in 64 bits and rounded once to
-32, so its exponential is off by 2^-24 |d| and that of the function (2 units), and a token's
-terms by K 2^-24 of their sizes, K = 16 + |d|; sums are in 64 bits and rounded once:
-  loss:      K 2^-24 sum |terms| share + 2^-24 |ref|
+Bounds, before any run. A token's log ratio is rounded once to 32 bits, so its
+exponential is off by 2^-24 |d| and that of the function and of the products after it
+(8 units in all), and up to 256 tokens are added up in 32 bits (10 roundings), the rest in 64:
+K 2^-24 of the sizes of the terms, K = 16 + |d|, with 4 (loss) or 2 (metrics) more
+where sums are made:
+  loss:      (K + 4) 2^-24 sum |terms| share + 2^-24 |ref|
   gradient:  K 2^-24 |terms of the slope| share + 4 2^-24 |ref| + u |ref|, u of the type
              of log_probs (its smallest step beside it)
-  metrics:   K 2^-24 of the mean of their terms
+  metrics:   (K + 2) 2^-24 of the mean of their terms
 A preference's sums are of differences that are exact in 64 bits, and everything of
 a pair is in 64 bits until its one rounding: rewards 2 2^-24 |ref|, losses and
 gradients 4 2^-24 |ref| and the rounding of their type.
