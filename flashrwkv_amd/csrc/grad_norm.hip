@@ -112,16 +112,26 @@ struct Pack {
     word = kStream ? __builtin_nontemporal_load(p) : *p;
   }
   __device__ __forceinline__ void load_unaligned(const void* from, int64_t i, int64_t left) {
-    S* e = reinterpret_cast<S*>(&word);
 #pragma unroll
-    for (int q = 0; q < kPer; ++q) e[q] = q < left ? static_cast<const S*>(from)[i + q] : S{0};
+    for (int q = 0; q < kPer; ++q) put(q, q < left ? static_cast<const S*>(from)[i + q] : S{0});
   }
-  __device__ __forceinline__ float at(int e) const {
-    return to_f32<T>(reinterpret_cast<const S*>(&word)[e]);
+  __device__ __forceinline__ S get(int e) const {
+    if constexpr (sizeof(S) == 4) {
+      return __uint_as_float(word[e]);
+    } else {
+      return static_cast<S>(word[e / 2] >> (16 * (e % 2)));
+    }
   }
-  __device__ __forceinline__ void set(int e, float x) {
-    reinterpret_cast<S*>(&word)[e] = from_f32<T>(x);
+  // In ascending order: the first half of a word clears the second.
+  __device__ __forceinline__ void put(int e, S x) {
+    if constexpr (sizeof(S) == 4) {
+      word[e] = __float_as_uint(x);
+    } else {
+      word[e / 2] = e % 2 == 0 ? uint32_t{x} : word[e / 2] | uint32_t{x} << 16;
+    }
   }
+  __device__ __forceinline__ float at(int e) const { return to_f32<T>(get(e)); }
+  __device__ __forceinline__ void set(int e, float x) { put(e, from_f32<T>(x)); }
   template <bool kStream>
   __device__ __forceinline__ void store(void* to, int64_t i) const {
     Word* p = reinterpret_cast<Word*>(static_cast<S*>(to) + i);
@@ -132,10 +142,9 @@ struct Pack {
     }
   }
   __device__ __forceinline__ void store_unaligned(void* to, int64_t i, int64_t left) const {
-    const S* e = reinterpret_cast<const S*>(&word);
 #pragma unroll
     for (int q = 0; q < kPer; ++q) {
-      if (q < left) static_cast<S*>(to)[i + q] = e[q];
+      if (q < left) static_cast<S*>(to)[i + q] = get(q);
     }
   }
 };

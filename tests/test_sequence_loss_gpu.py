@@ -297,6 +297,22 @@ def test_policy_calls_repeat_bitwise_on_any_stream():
     assert all(torch.equal(first[name], other[name]) for name in first)
 
 
+def test_calls_on_two_streams_at_once():
+    cases = [_policy(LAYOUTS["many pieces"], reduction="sequence_mean", seed=30),
+             _policy(LAYOUTS["tiny"], reduction="mean", seed=31)]
+    want = [_run_policy(*case) for case in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for case, stream, out in zip(cases, streams, got):
+            with torch.cuda.stream(stream):
+                out.append(_run_policy(*case))
+    torch.cuda.synchronize()
+    for first, runs in zip(want, got):
+        assert all(torch.equal(run[name], first[name]) for run in runs for name in first)
+
+
 def test_policy_gradient_of_either_input_alone():
     x, old, a, args, up = _policy([100, 200], seed=12)
     full = _run_policy(x, old, a, args, up)
