@@ -376,9 +376,10 @@ __device__ __forceinline__ double total_of(const double* __restrict__ sums, int3
   return workgroup_sum<kBlock>(x[0], shared);
 }
 
+// 1 where the norm as it is returned, in 32 bits, is not finite.
 __device__ __forceinline__ float factor_of(double total, double most, double eps) {
   const double norm = sqrt(total);
-  if (!(norm < __builtin_inf())) return 1.0f;
+  if (!(static_cast<float>(norm) < __builtin_inff())) return 1.0f;
   return static_cast<float>(fmin(1.0, most / (norm + eps)));
 }
 

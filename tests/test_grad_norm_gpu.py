@@ -142,6 +142,16 @@ def test_a_norm_that_is_not_finite_scales_nothing(bad):
         assert torch.equal(x.nan_to_num(7.0), z.nan_to_num(7.0))
 
 
+@pytest.mark.parametrize("count", [4, 300])
+def test_a_norm_beyond_32_bits_scales_nothing(count):
+    """Each value is fp32's, their norm (2e38 sqrt(count)) is not: the returned norm is
+    infinite, by which a caller skips the step, so the tensors are left alone too."""
+    tensors = [torch.full((1,), 2e38, device=DEV) for _ in range(count)]
+    norm = pretrain_clip_grad_norm(tensors, 1.0)
+    assert norm.item() == math.inf == pretrain_grad_norm(tensors).item()
+    assert all(t.item() == torch.tensor(2e38).item() for t in tensors)
+
+
 def test_zeros_and_a_maximum_of_zero():
     t = torch.zeros(100, device=DEV)
     assert pretrain_clip_grad_norm([t], 1.0).item() == 0.0
