@@ -71,6 +71,12 @@ def tensor(x, ns) -> bool:
     return isinstance(x, torch.Tensor)
 
 
+def constant(x, ns) -> bool:
+    """Whether nothing is to be differentiated by it, backward or forward."""
+    return (not (x.requires_grad and torch.is_grad_enabled())
+            and torch.autograd.forward_ad.unpack_dual(x).tangent is None)
+
+
 def contiguous(x, ns) -> bool:
     return x.is_contiguous()
 

@@ -48,10 +48,6 @@ void record(const variable_list& outputs, F&& fill, const Inputs&... inputs) {
   for (const Tensor& t : outputs) torch::autograd::set_history(t, node);
 }
 
-// Without a node of torch::autograd::Function nothing refuses forward-mode
-// derivatives: calls with tangents are declined.
-bool has_tangent(const Tensor& t) { return t._fw_grad(0).defined(); }
-
 struct LinearLogProbsNode : StepNode {  // saved: weight, the forward's buffer
   std::vector<int64_t> shape;
   double temperature = 1.0;
@@ -178,7 +174,7 @@ struct SequenceArgs : HeadArgs {
   std::optional<Tensor> column(const pybind11::object& x, bool constant) {
     const std::optional<Tensor> t = optional_tensor(x);
     require(ok && (!t.has_value() || (is_column(*t) && t->sizes() == log_probs.sizes() &&
-                                      !(constant && wants_grad(*t)))));
+                                      !has_tangent(*t) && !(constant && wants_grad(*t)))));
     return t;
   }
   std::optional<Tensor> mask(const pybind11::object& x) {
@@ -218,6 +214,7 @@ pybind11::object policy_loss_call(
   const std::optional<Tensor> cu = args.offsets(cu_seqlens_);
   const Tensor advantages = args.tensor(advantages_);
   args.require(args.ok && args.is_column(advantages) && !args.wants_grad(advantages) &&
+               !has_tangent(advantages) &&
                (advantages.sizes() == args.log_probs.sizes() ||
                 (cu.has_value() && advantages.dim() == 1 &&
                  advantages.size(0) == cu->size(0) - 1)));
@@ -230,7 +227,7 @@ pybind11::object policy_loss_call(
                (ew == 0.0 || entropy.has_value()) &&
                (cu.has_value() || reduction != FRWKV_REDUCE_SEQUENCE_MEAN));
   const Tensor& x = args.log_probs;
-  args.require(args.ok && !has_tangent(x) && !(entropy.has_value() && has_tangent(*entropy)));
+  args.require(args.ok && !has_tangent(x));
   if (!args.ok || stream_is_capturing(x)) return pybind11::none();
   variable_list out;
   {
@@ -323,7 +320,7 @@ pybind11::object grad_norm_call(const pybind11::object& tensors_) {
   const std::vector<Tensor> tensors = plain_list(args, tensors_);
   args.require(!tensors.empty());
   for (size_t i = 0; i < tensors.size() && args.ok; ++i) {
-    args.require(is_gradient(tensors[i], tensors[0]));
+    args.require(is_gradient(tensors[i], tensors[0]) && is_constant(tensors[i]));
   }
   if (!args.ok) return pybind11::none();
   return pybind11::cast(grad_norm(tensors));

@@ -257,6 +257,15 @@ Tensor preference_loss_backward(Tensor grad_loss, Tensor saved, Tensor cu_seqlen
 }
 
 // ------------------------------------------------------------------ gradients
+// Without a node of torch::autograd::Function nothing refuses forward-mode
+// derivatives: calls with tangents are declined.
+bool has_tangent(const Tensor& t) { return t._fw_grad(0).defined(); }
+
+// Whether nothing is to be differentiated by it: norms and clipped tensors have no history.
+bool is_constant(const Tensor& t) {
+  return !(t.requires_grad() && at::GradMode::is_enabled()) && !has_tangent(t);
+}
+
 bool gradient_dtype(const Tensor& t) {
   return t.scalar_type() == at::kFloat || t.scalar_type() == at::kHalf ||
          t.scalar_type() == at::kBFloat16;
@@ -327,14 +336,12 @@ Tensor grad_norm(const std::vector<Tensor>& tensors) {
   return norm;
 }
 
-bool may_write(const Tensor& t) { return !(t.requires_grad() && at::GradMode::is_enabled()); }
-
 bool may_clip(const std::vector<Tensor>& tensors, const std::vector<Tensor>& out) {
   if (tensors.empty() || out.size() != tensors.size()) return false;
   for (size_t i = 0; i < tensors.size(); ++i) {
     const Tensor &x = tensors[i], &y = out[i];
-    if (!is_gradient(x, tensors[0]) || !is_gradient(y, tensors[0]) || !may_write(y) ||
-        y.sizes() != x.sizes() || y.strides() != x.strides()) {
+    if (!is_gradient(x, tensors[0]) || !is_gradient(y, tensors[0]) || !is_constant(x) ||
+        !is_constant(y) || y.sizes() != x.sizes() || y.strides() != x.strides()) {
       return false;
     }
   }
@@ -361,7 +368,7 @@ Tensor clip_grad_norm_op(std::vector<Tensor> tensors, std::vector<Tensor> out, d
                          double eps) {
   TORCH_CHECK(may_clip(tensors, out),
               "tensors and out must be CUDA float32, float16 or bfloat16 without gaps, on one "
-              "device, pairwise of one layout, and out must not require gradients");
+              "device, pairwise of one layout, and must not require gradients");
   const std::vector<frwkv_gradient> list = gradient_list(tensors, &out);
   TORCH_CHECK(apart(list), "tensors that are written must not overlap others");
   return clip_gradients(tensors, out, list, max_norm, eps);

@@ -47,6 +47,8 @@ def _list_of(name):
               f"{name} must hold their values, not be negated views"),
         check(name, _each(lambda t, ns: _dense(t)), ValueError,
               f"{name} must leave no gaps in memory"),
+        check(name, _each(C.constant), ValueError,
+              f"{name} must not require gradients: the norm has none (detach them)"),
     )
 
 
@@ -84,8 +86,6 @@ CLIP = (
     check("out", _pairwise(lambda a, b: a.data_ptr() != b.data_ptr() or a.dtype == b.dtype
                            or a.numel() == 0), ValueError,
           "a tensor that is written in place must keep its dtype"),
-    check("out", _each(lambda t, ns: not (t.requires_grad and torch.is_grad_enabled())),
-          ValueError, "tensors that are written must not require gradients"),
     check("out", _apart, ValueError, "tensors that are written must not overlap others"),
     check("max_norm", _amount, ValueError, "max_norm must be a finite number, not negative"),
     check("eps", _amount, ValueError, "eps must be a finite number, not negative"),
@@ -94,7 +94,8 @@ CLIP = (
 
 def pretrain_grad_norm(tensors: Sequence[torch.Tensor]) -> torch.Tensor:
     """``sqrt(sum x^2)`` over all elements of all tensors, an fp32 scalar on their
-    device. A tensor that is listed twice counts twice."""
+    device, without gradients: the tensors must not require any. A tensor that is listed
+    twice counts twice."""
     call = C.whole_call("grad_norm_call")
     norm = call(tensors) if call else None
     if norm is not None:

@@ -38,10 +38,6 @@ def _given(name):
     return lambda ns: ns[name] is not None
 
 
-def _constant(x, ns):
-    return not (x.requires_grad and torch.is_grad_enabled())
-
-
 def _vector(name, *, constant, shaped=True):
     rules = [
         is_tensor(name),
@@ -56,7 +52,7 @@ def _vector(name, *, constant, shaped=True):
             rules.append(check(name, C.same_shape_as("log_probs"), ValueError,
                                f"{name} must match log_probs"))
     if constant:
-        rules.append(check(name, _constant, ValueError,
+        rules.append(check(name, C.constant, ValueError,
                            f"{name} must not require gradients: it has none here (detach it)"))
     return rules
 
@@ -264,7 +260,7 @@ def pretrain_policy_loss(
     def launch(x, h, slopes):
         return C.native().policy_loss_forward(
             x, old_log_probs, advantages, reference_log_probs, h, mask, cu_seqlens, clip_low,
-            clip_high, dual, kl_weight, entropy_weight, POLICY_REDUCTIONS[reduction], metrics,
+            clip_high, dual, kl_weight, entropy_weight, POLICY_REDUCTIONS[reduction], bool(metrics),
             slopes)
 
     got = _PolicyLoss.apply(log_probs, entropy, mask, cu_seqlens, float(entropy_weight),
@@ -323,7 +319,7 @@ def pretrain_preference_loss(
     def launch(x):
         return C.native().preference_loss_forward(
             x, cu_seqlens, reference_log_probs, mask, beta, margin, label_smoothing, KINDS[kind],
-            normalize, PAIR_REDUCTIONS[reduction])
+            bool(normalize), PAIR_REDUCTIONS[reduction])
 
     return _PreferenceLoss.apply(log_probs, mask, cu_seqlens, PAIR_REDUCTIONS[reduction], launch)
 

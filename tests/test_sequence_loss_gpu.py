@@ -529,6 +529,17 @@ def test_forward_mode_is_refused():
         dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
         with pytest.raises((RuntimeError, NotImplementedError)):
             pretrain_policy_loss(dual, old, old)
+        cu = torch.tensor([0, 11, 20], dtype=torch.int32, device=DEV)
+        for call in (lambda: pretrain_policy_loss(x, dual, old),
+                     lambda: pretrain_policy_loss(x, old, dual),
+                     lambda: pretrain_policy_loss(x, old, old, reference_log_probs=dual),
+                     lambda: pretrain_preference_loss(x, cu, reference_log_probs=dual),
+                     lambda: flashrwkv_amd.pretrain_grad_norm([x, dual]),
+                     lambda: flashrwkv_amd.pretrain_clip_grad_norm([dual], 1.0, out=[old])):
+            with pytest.raises(ValueError, match="must not require gradients"):
+                call()
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            pretrain_policy_loss(x, old, old, entropy=dual, entropy_weight=0.1)
 
 
 def test_backward_on_a_capturing_stream_is_refused():

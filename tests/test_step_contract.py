@@ -165,6 +165,12 @@ def test_gradient_refusals():
         pretrain_clip_grad_norm([a], 1.0, out=[_fake(2, 2)])
     with pytest.raises(ValueError, match="must not require gradients"):
         pretrain_clip_grad_norm([_fake(4).requires_grad_()], 1.0)
+    with pytest.raises(ValueError, match="tensors must not require gradients"):
+        pretrain_grad_norm([a, _fake(4).requires_grad_()])
+    with pytest.raises(ValueError, match="tensors must not require gradients"):
+        pretrain_clip_grad_norm([_fake(4).requires_grad_()], 1.0, out=[a])
+    with pytest.raises(ValueError, match="out must not require gradients"):
+        pretrain_clip_grad_norm([a], 1.0, out=[_fake(4).requires_grad_()])
     flat = _fake(10)
     for tensors, out in (([a, a], None), ([flat[:6], flat[5:]], None), ([flat[:4]], [flat[2:6]]),
                          ([a, _fake(4)], [flat[:4]] * 2)):
