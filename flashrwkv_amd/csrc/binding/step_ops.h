@@ -115,6 +115,12 @@ const int32_t* check_offsets(const std::optional<Tensor>& cu, const Tensor& like
   return cu->const_data_ptr<int32_t>();
 }
 
+// One of the codes up to `last`: shapes are chosen by it before it is narrowed.
+int reduction_code(int64_t reduction, int last) {
+  TORCH_CHECK(reduction >= FRWKV_REDUCE_NONE && reduction <= last, "unknown reduction ", reduction);
+  return static_cast<int>(reduction);
+}
+
 // What the backward reads and the call's scratch, small beside it, as one allocation:
 // one takes 1.3 us of a call's 8.
 struct Buffers {
@@ -137,6 +143,7 @@ std::vector<Tensor> policy_loss_forward(Tensor log_probs, Tensor old_log_probs, 
                                         bool slopes) {
   const int64_t tokens = log_probs.numel();
   TORCH_CHECK(tokens > 0, "log_probs must hold at least one token");
+  const int reduce = reduction_code(reduction, FRWKV_REDUCE_SEQUENCE_MEAN);
   const TokenColumn x = token_column(log_probs, log_probs, "log_probs");
   const TokenColumn old = token_column(old_log_probs, log_probs, "old_log_probs");
   const TokenColumn reference =
@@ -153,8 +160,8 @@ std::vector<Tensor> policy_loss_forward(Tensor log_probs, Tensor old_log_probs, 
               "advantages must have log_probs' shape, or one entry a sequence of cu_seqlens");
   c10::DeviceGuard guard(log_probs.device());
   const auto fp32 = log_probs.options().dtype(at::kFloat);
-  Tensor loss = reduction == FRWKV_REDUCE_NONE ? at::empty(log_probs.sizes(), fp32)
-                                               : at::empty({}, fp32);
+  Tensor loss = reduce == FRWKV_REDUCE_NONE ? at::empty(log_probs.sizes(), fp32)
+                                            : at::empty({}, fp32);
   Tensor found;
   if (metrics) found = at::empty({4}, fp32);
   const Buffers buffers(log_probs, frwkv_policy_loss_saved_bytes(tokens, sequences),
@@ -163,9 +170,8 @@ std::vector<Tensor> policy_loss_forward(Tensor log_probs, Tensor old_log_probs, 
       tokens, sequences, cu, m, x.dtype, x.data, old.dtype, old.data,
       io_code(advantages.scalar_type()), advantages.const_data_ptr(), per_sequence,
       reference.dtype, reference.data, h.dtype, h.data, clip_low, clip_high, dual_clip,
-      static_cast<float>(kl_weight), static_cast<float>(entropy_weight),
-      static_cast<int>(reduction), loss.data_ptr<float>(),
-      metrics ? found.data_ptr<float>() : nullptr, slopes, buffers.saved(), buffers.saved_bytes,
+      static_cast<float>(kl_weight), static_cast<float>(entropy_weight), reduce,
+      loss.data_ptr<float>(), metrics ? found.data_ptr<float>() : nullptr, slopes, buffers.saved(), buffers.saved_bytes,
       buffers.work(), buffers.work_bytes, current_stream(log_probs)));
   if (metrics) return {loss, buffers.all, found};
   return {loss, buffers.all};
@@ -182,9 +188,10 @@ std::vector<Tensor> policy_loss_backward(Tensor grad_loss, Tensor saved,
                                          bool want_entropy) {
   check_device_contiguous(saved, "saved");
   refuse_capture(saved, "the policy loss's backward");
+  const int reduce = reduction_code(reduction, FRWKV_REDUCE_SEQUENCE_MEAN);
   const int64_t tokens = c10::multiply_integers(shape);
   const float* up = check_upstream(
-      grad_loss, reduction == FRWKV_REDUCE_NONE ? tokens : 1, saved, "grad_loss");
+      grad_loss, reduce == FRWKV_REDUCE_NONE ? tokens : 1, saved, "grad_loss");
   const uint8_t* m = check_mask(mask, tokens, saved);
   int64_t sequences;
   const int32_t* cu = check_offsets(cu_seqlens, saved, &sequences);
@@ -200,9 +207,9 @@ std::vector<Tensor> policy_loss_backward(Tensor grad_loss, Tensor saved,
     gh = out.back().data_ptr();
   }
   check_rc(frwkv_policy_loss_backward(
-      tokens, sequences, cu, m, static_cast<float>(entropy_weight), static_cast<int>(reduction),
-      up, saved.const_data_ptr(), static_cast<size_t>(saved.numel()), io_code(log_probs_dtype),
-      gx, io_code(entropy_dtype), gh, current_stream(saved)));
+      tokens, sequences, cu, m, static_cast<float>(entropy_weight), reduce, up,
+      saved.const_data_ptr(), static_cast<size_t>(saved.numel()), io_code(log_probs_dtype), gx,
+      io_code(entropy_dtype), gh, current_stream(saved)));
   return out;
 }
 
@@ -213,6 +220,7 @@ std::tuple<Tensor, Tensor, Tensor> preference_loss_forward(
     bool normalize, int64_t reduction) {
   const int64_t tokens = log_probs.numel();
   TORCH_CHECK(tokens > 0, "log_probs must hold at least one token");
+  const int reduce = reduction_code(reduction, FRWKV_REDUCE_SUM);
   const TokenColumn x = token_column(log_probs, log_probs, "log_probs");
   const TokenColumn reference =
       token_column(reference_log_probs, log_probs, "reference_log_probs");
@@ -224,13 +232,13 @@ std::tuple<Tensor, Tensor, Tensor> preference_loss_forward(
   c10::DeviceGuard guard(log_probs.device());
   const auto fp32 = log_probs.options().dtype(at::kFloat);
   Tensor loss =
-      reduction == FRWKV_REDUCE_NONE ? at::empty({pairs}, fp32) : at::empty({}, fp32);
+      reduce == FRWKV_REDUCE_NONE ? at::empty({pairs}, fp32) : at::empty({}, fp32);
   Tensor rewards = at::empty({pairs, 2}, fp32);
   const Buffers buffers(log_probs, frwkv_preference_loss_saved_bytes(pairs),
                         frwkv_sequence_loss_workspace_bytes(tokens, sequences));
   check_rc(frwkv_preference_loss_forward(
       tokens, pairs, cu, m, x.dtype, x.data, reference.dtype, reference.data, beta, margin,
-      label_smoothing, static_cast<int>(kind), normalize, static_cast<int>(reduction),
+      label_smoothing, static_cast<int>(kind), normalize, reduce,
       loss.data_ptr<float>(), rewards.data_ptr<float>(), buffers.saved(), buffers.saved_bytes,
       buffers.work(), buffers.work_bytes, current_stream(log_probs)));
   return {loss, rewards, buffers.all};
@@ -241,16 +249,17 @@ Tensor preference_loss_backward(Tensor grad_loss, Tensor saved, Tensor cu_seqlen
                                 at::ScalarType log_probs_dtype, int64_t reduction) {
   check_device_contiguous(saved, "saved");
   refuse_capture(saved, "the preference loss's backward");
+  const int reduce = reduction_code(reduction, FRWKV_REDUCE_SUM);
   const int64_t tokens = c10::multiply_integers(shape);
   int64_t sequences;
   const int32_t* cu = check_offsets(cu_seqlens, saved, &sequences);
   const float* up = check_upstream(
-      grad_loss, reduction == FRWKV_REDUCE_NONE ? sequences / 2 : 1, saved, "grad_loss");
+      grad_loss, reduce == FRWKV_REDUCE_NONE ? sequences / 2 : 1, saved, "grad_loss");
   const uint8_t* m = check_mask(mask, tokens, saved);
   c10::DeviceGuard guard(saved.device());
   Tensor out = at::empty(shape, saved.options().dtype(log_probs_dtype));
   check_rc(frwkv_preference_loss_backward(
-      tokens, sequences / 2, cu, m, static_cast<int>(reduction), up, saved.const_data_ptr(),
+      tokens, sequences / 2, cu, m, reduce, up, saved.const_data_ptr(),
       static_cast<size_t>(saved.numel()), io_code(log_probs_dtype), out.data_ptr(),
       current_stream(saved)));
   return out;

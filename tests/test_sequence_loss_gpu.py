@@ -523,6 +523,29 @@ def test_the_graph_is_kept_or_freed_as_asked():
         loss.backward()
 
 
+@pytest.mark.parametrize("reduction", [-1, 4, 2 ** 32])
+def test_ops_refuse_unknown_reductions(reduction):
+    """Also one whose low 32 bits are a known one."""
+    x, old, _ = _logs(20, seed=27)
+    cu = torch.tensor([0, 11, 20], dtype=torch.int32, device=DEV)
+    ops = torch.ops.flashrwkv2
+    _, saved = ops.policy_loss_forward(x, old, old, None, None, None, None, 0.2, 0.2, 0.0, 0.0,
+                                       0.0, 1, False, True)
+    _, _, pair_saved = ops.preference_loss_forward(x, cu, None, None, 0.1, 0.0, 0.0, 0, False, 1)
+    up = torch.ones((), device=DEV)
+    for call in (
+            lambda: ops.policy_loss_forward(x, old, old, None, None, None, None, 0.2, 0.2, 0.0,
+                                            0.0, 0.0, reduction, False, True),
+            lambda: ops.policy_loss_backward(up, saved, None, None, [20], torch.float32,
+                                             torch.float32, 0.0, reduction, True, False),
+            lambda: ops.preference_loss_forward(x, cu, None, None, 0.1, 0.0, 0.0, 0, False,
+                                                reduction),
+            lambda: ops.preference_loss_backward(up, pair_saved, cu, None, [20], torch.float32,
+                                                 reduction)):
+        with pytest.raises(RuntimeError, match="unknown reduction"):
+            call()
+
+
 def test_forward_mode_is_refused():
     x, old, _ = _logs(20, seed=27)
     with torch.autograd.forward_ad.dual_level():
