@@ -11,7 +11,9 @@ logits. Two ways to train:
 * ``--mode state``: only the initial state, everything else frozen (the weight
   gradients of the head are then never computed).
 
-    python examples/train_head.py [--mode state] [--steps 60]
+``--max-norm`` clips each step's gradients by their norm together.
+
+    python examples/train_head.py [--mode state] [--steps 60] [--max-norm 1]
 """
 
 from __future__ import annotations
@@ -26,6 +28,7 @@ sys.path.insert(0, str(Path(__file__).resolve().parents[1]))
 
 from flashrwkv_amd import (  # noqa: E402
     infer_layer_norm_forward_varlen,
+    pretrain_clip_grad_norm,
     pretrain_layer_norm,
     pretrain_linear_cross_entropy,
     pretrain_linear_topk_distillation,
@@ -113,7 +116,8 @@ def synthetic(vocab: int, tokens: int, top: int, device):
 
 
 def train(mode: str = "full", steps: int = 60, vocab: int = 1000, heads: int = 4,
-          tokens: int = 192, top: int = 16, device: str = "cuda") -> list[float]:
+          tokens: int = 192, top: int = 16, device: str = "cuda",
+          max_norm: float | None = None) -> list[float]:
     """Trains on one synthetic sequence; the loss of every step."""
     torch.manual_seed(0)
     model = Model(vocab, heads).to(device)
@@ -128,6 +132,8 @@ def train(mode: str = "full", steps: int = 60, vocab: int = 1000, heads: int = 4
         optimizer.zero_grad(set_to_none=True)
         loss = step_loss(model, *batch)
         loss.backward()
+        if max_norm is not None:
+            pretrain_clip_grad_norm([p.grad for p in trained], max_norm)
         optimizer.step()
         losses.append(loss.detach())
     return torch.stack(losses).tolist()
@@ -137,8 +143,9 @@ def main() -> None:
     parser = argparse.ArgumentParser(description=__doc__.splitlines()[0])
     parser.add_argument("--mode", choices=("full", "state"), default="full")
     parser.add_argument("--steps", type=int, default=60)
+    parser.add_argument("--max-norm", type=float)
     args = parser.parse_args()
-    losses = train(args.mode, args.steps)
+    losses = train(args.mode, args.steps, max_norm=args.max_norm)
     for i in range(0, len(losses), max(1, len(losses) // 6)):
         print(f"step {i:4d}  loss {losses[i]:.4f}")
     print(f"last       loss {losses[-1]:.4f}")

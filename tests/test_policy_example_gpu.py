@@ -25,11 +25,11 @@ def _require_native():
         pytest.fail("flashrwkv_amd native library is not built (no fallback exists)")
 
 
-def _example():
-    path = Path(__file__).resolve().parents[1] / "examples" / "train_policy.py"
+def _example(name="train_policy"):
+    path = Path(__file__).resolve().parents[1] / "examples" / f"{name}.py"
     sys.path.insert(0, str(path.parent))
     try:
-        spec = importlib.util.spec_from_file_location("train_policy", path)
+        spec = importlib.util.spec_from_file_location(name, path)
         module = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(module)
     finally:
@@ -90,3 +90,29 @@ def test_example_step_matches_logits_written_out(loss):
         allowed = 2.0 ** -7 * (ref[f"abs_{name}"] + ref[name].abs()) + 1e-9
         assert ((got.double() - ref[name]).abs() <= allowed).all(), name
     assert d_head.any() and d_rows.any()
+
+
+@pytest.mark.parametrize("mode", ["full", "state"])
+def test_head_example_clips(mode):
+    losses = _example("train_head").train(mode, steps=3, vocab=300, heads=2, tokens=64, top=4,
+                                          max_norm=0.1)
+    assert len(losses) == 3 and all(math.isfinite(x) for x in losses)
+
+
+def test_head_example_gradients_are_scaled_to_the_norm():
+    """Against the same gradients in 64 bits: the norm is rounded once (2^-24, twice allowed),
+    a gradient by its factor, the product and its type (2 2^-24 and 2^-8)."""
+    example = _example("train_head")
+    torch.manual_seed(2)
+    model = example.Model(300, 2).to(DEV)
+    example.step_loss(model, *example.synthetic(300, 64, 4, DEV)).backward()
+    grads = [p.grad for p in model.parameters()]
+    assert len(grads) == 6 and {g.dtype for g in grads} == {torch.bfloat16, torch.float32}
+    before = [g.clone() for g in grads]
+    most = 0.5 * step.clip(before, 1.0, 0.0)[0]
+    norm = flashrwkv_amd.pretrain_clip_grad_norm(grads, most)
+    want, clipped = step.clip(before, most, 1e-6)
+    assert abs(norm.item() - want) <= 2 ** -23 * want
+    for got, value in zip(grads, clipped):
+        off = 2.0 ** -23 + (2.0 ** -8 if got.dtype == torch.bfloat16 else 0.0)
+        assert ((got.double() - value).abs() <= 1.01 * off * value.abs() + 2.0 ** -134).all()
