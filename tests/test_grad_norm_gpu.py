@@ -226,6 +226,30 @@ def test_calls_repeat_bitwise_on_any_stream_and_in_graphs():
             assert torch.equal(got, first) and all(torch.equal(a, b) for a, b in zip(kept, seen))
 
 
+def test_two_graphs_of_long_lists_in_one_pool():
+    """Lists that stand in the calls' own memory, replayed in turn with eager calls between."""
+    lists = [_tensors(LISTS["long list"], seed=7), _tensors(LISTS["many"], seed=8)]
+    outs = [[torch.zeros_like(t, dtype=torch.float32) for t in tensors] for tensors in lists]
+    graphs, norms, pool = [], [], None
+    for tensors, out in zip(lists, outs):
+        pretrain_clip_grad_norm(tensors, 1.0, out=out)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=pool):
+            norms.append(pretrain_clip_grad_norm(tensors, 1.0, out=out))
+        pool = graph.pool()
+        graphs.append(graph)
+    for k in range(3):
+        for tensors, out, graph, norm in zip(lists, outs, graphs, norms):
+            tensors[k].mul_(1.5 + k)
+            graph.replay()
+            torch.cuda.synchronize()
+            _check(tensors, out, norm, 1.0)
+            eager = [torch.zeros_like(t) for t in out]
+            assert torch.equal(pretrain_clip_grad_norm(tensors, 1.0, out=eager), norm)
+            assert all(torch.equal(x, y) for x, y in zip(eager, out))
+
+
 def test_c_abi_writes_what_the_operators_return():
     tensors = _tensors([(5000,), (0,), (33, 3)], seed=6)
     out = [torch.zeros_like(t) for t in tensors]
