@@ -104,6 +104,10 @@ __device__ __forceinline__ float2 joined(float2 a, float2 b, float scale) {
                               b.y * __builtin_amdgcn_exp2f((b.x - top) * scale));
 }
 
+// 2^d is 0 in fp32 from here on, and d itself, or its product with a sum, may be -inf:
+// products with 2^d are taken with this instead.
+constexpr float kLeastExponent = -200.0f;
+
 // The same with the sum of 2^d d, d = scale (x - maximum), beside the sum of 2^d:
 // moved to another maximum by t, 2^(d + t) (d + t) = 2^t (2^d d + t 2^d).
 struct Moments {
@@ -117,12 +121,9 @@ __device__ __forceinline__ Moments joined(Moments a, Moments b, float scale) {
   const float t = (a.top - top) * scale, u = (b.top - top) * scale;
   const float x = __builtin_amdgcn_exp2f(t), y = __builtin_amdgcn_exp2f(u);
   return {top, a.sum * x + b.sum * y,
-          x * fmaf(t, a.sum, a.moment) + y * fmaf(u, b.sum, b.moment)};
+          x * fmaf(fmaxf(t, kLeastExponent), a.sum, a.moment) +
+              y * fmaf(fmaxf(u, kLeastExponent), b.sum, b.moment)};
 }
-
-// 2^d is 0 in fp32 from here on, and d itself may be -inf: its product with 2^d is
-// taken with this instead.
-constexpr float kLeastExponent = -200.0f;
 
 // Twice: where the two terms of row m of a few stand in dz, 16 rows' first terms
 // and then their second ones, so that a lane of any tile that holds the one holds

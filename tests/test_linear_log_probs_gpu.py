@@ -300,3 +300,33 @@ def test_second_derivatives_and_captures_are_refused():
                 pretrain_linear_log_probs(h, w, targets)
         finally:
             graph.capture_end()
+
+
+@pytest.mark.parametrize("dtype", ROUND)
+@pytest.mark.parametrize("n", [3, 300])
+@pytest.mark.parametrize("temperature", [1.1e-30, 1e-10])
+def test_certain_rows_at_the_least_temperatures(temperature, n, dtype):
+    """A token's distance from the others in units of the temperature, times the tokens of
+    a sum, is beyond fp32: such rows have entropy 0 and no gradient. Rows of equal logits
+    between them have log V. Upstream gradients of the temperature's size cancel 1 / T."""
+    c, v = 64, 65536
+    w = torch.zeros(v, c, device=DEV, dtype=dtype)
+    w[7, 0] = 1.0
+    h = torch.zeros(n, c, device=DEV, dtype=dtype)
+    h[0::3, 0], h[1::3, 0] = 30000.0, 1.0
+    targets = torch.full((n,), 7, device=DEV)
+    up = torch.full((n,), temperature, device=DEV)
+    got = _run(h, w, targets, up, up, temperature=temperature)
+    for first in (0, 1):
+        for name in ("log_probs", "entropy", "dhidden"):
+            assert not got[name][first::3].any(), name
+    # Sums of V equal terms and their logarithm.
+    limit = (math.sqrt(v) + 32) * E * (1 + math.log(v))
+    assert (got["entropy"][2::3] - math.log(v)).abs().max() <= limit
+    assert (got["log_probs"][2::3] + math.log(v)).abs().max() <= limit
+    # dz of the target is 1 - 1 / V, rounded once as an operand and once as an output.
+    dhidden = got["dhidden"][2::3].double()
+    assert (dhidden[:, 0] - (1 - 1 / v)).abs().max() <= 2 * ROUND[dtype] + limit
+    assert not dhidden[:, 1:].any()
+    # The rows with a gradient hold zeros.
+    assert not got["dweight"].any()
