@@ -29,7 +29,7 @@
 // sequence's tiles, so a second pass adds them in order without atomics. The
 // offsets stand on the device and are not trusted: every index that is made from
 // them is bounded, and offsets that do not start at 0, fall or go past the last
-// token make the loss, and with it the gradients, NaN.
+// token make a reduced loss and the gradients of all tokens NaN.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -720,6 +720,7 @@ __global__ __launch_bounds__(kWaves * 64) void policy_grad_kernel(Packed p, Poli
   }
   tile.fetch_part(g.entropy != nullptr ? p.mask : nullptr, part);
   const float share = *s.share;
+  const bool bad = share != share;  // offsets that may not be: NaN for all tokens
 #pragma unroll
   for (int r = 0; r < kRounds; ++r) up[r] *= share;
   const bool by_sequence = g.reduction == FRWKV_REDUCE_SEQUENCE_MEAN;
@@ -741,9 +742,13 @@ __global__ __launch_bounds__(kWaves * 64) void policy_grad_kernel(Packed p, Poli
     if (!tile.has(r)) continue;
     const int64_t i = tile.first + 64 * r + lane_id();
     // A slope of 0, as a token without part has, stays 0 under any upstream.
-    if (g.x != nullptr) store_at(g.x, g.x_dtype, i, slope[r] == 0.0f ? 0.0f : slope[r] * up[r]);
+    if (g.x != nullptr) {
+      const float grad = slope[r] == 0.0f ? 0.0f : slope[r] * up[r];
+      store_at(g.x, g.x_dtype, i, bad ? share : grad);
+    }
     if (g.entropy != nullptr) {
-      store_at(g.entropy, g.entropy_dtype, i, part[r] ? -g.ew * up[r] : 0.0f);
+      const float grad = part[r] ? -g.ew * up[r] : 0.0f;
+      store_at(g.entropy, g.entropy_dtype, i, bad ? share : grad);
     }
   }
 }
@@ -908,6 +913,7 @@ __global__ __launch_bounds__(kWaves * 64) void preference_grad_kernel(
   bool part[kRounds];
   tile.fetch_part(p.mask, part);
   const float share = *s.share;
+  const bool bad = share != share;  // offsets that may not be: NaN for all tokens
   int32_t id[kRounds];
   sequences_of<kRounds>(p, tile.first, id);
 #pragma unroll
@@ -917,7 +923,8 @@ __global__ __launch_bounds__(kWaves * 64) void preference_grad_kernel(
     const bool here = part[r] && id[r] < p.sequences && c != 0.0f;
     const float up = upstream[per_pair ? b / 2 : 0] * share;
     if (tile.has(r)) {
-      store_at(grad_x, x_dtype, tile.first + 64 * r + lane_id(), here ? c * up : 0.0f);
+      const float grad = here ? c * up : 0.0f;
+      store_at(grad_x, x_dtype, tile.first + 64 * r + lane_id(), bad ? share : grad);
     }
   }
 }

@@ -14,7 +14,7 @@ vector is float32, float16 or bfloat16 by itself; ratios and sums are taken in
 64 bits and summed in a fixed order.
 
 Nothing synchronises with the host: offsets that may not be cannot be raised as
-an error, they make a reduced loss and the gradients NaN.
+an error, they make a reduced loss and the gradients of all tokens NaN.
 """
 
 from __future__ import annotations

@@ -758,8 +758,8 @@ int frwkv_linear_log_probs_backward(int io_dtype, int64_t rows, int64_t channels
  * [sequences + 1] on the device (0, not falling, at most tokens; tokens behind the
  * last offset take no part); mask one byte a token (NULL: all take part). What
  * stands in tokens that take no part, NaN included, reaches nothing; their
- * gradients are 0. Offsets that may not be make a reduced loss and the gradients
- * NaN. Sums are in 64 bits and in a fixed order. No counterpart in the reference.
+ * gradients are 0. Offsets that may not be make a reduced loss and the gradients of
+ * all tokens NaN. Sums are in 64 bits and in a fixed order. No counterpart in the reference.
  *
  * frwkv_policy_loss_forward: with d = log_probs - old_log_probs, r = exp(d) and
  * advantage A (one a token or, advantages_per_sequence, one a sequence) a token's

@@ -621,3 +621,40 @@ def test_offsets_that_may_not_be_make_loss_and_gradients_nan(offsets):
         assert torch.isnan(torch.autograd.grad(loss, [leaf])[0]).any()
     loss, _ = pretrain_preference_loss(leaf, cu)
     assert torch.isnan(loss)
+
+
+@pytest.mark.parametrize("log_dtype", ROUND)
+@pytest.mark.parametrize("offsets", ["start", "late fall", "beyond"])
+@pytest.mark.parametrize("n,sequences", [(20, 4), (5000, 10), (5000, 2000), (300_000, 3000)])
+def test_offsets_that_may_not_be_mark_every_gradient(n, sequences, offsets, log_dtype):
+    """In one workgroup's form and in those of two launches, one bad offset among many:
+    gradients of clipped tokens, of satisfied pairs and of masked tokens too."""
+    cu = (torch.arange(sequences + 1) * n // sequences).to(torch.int32)
+    if offsets == "start":
+        cu[0] = 1
+    elif offsets == "late fall":
+        cu[-2] = cu[-3] - 1
+    else:
+        cu[-1] = n + 1
+    cu = cu.to(DEV)
+    x, old, _ = _logs(n, seed=28)
+    # Half of the ratios are clipped, half have an advantage of 0; all pairs are satisfied.
+    x, a = x.to(log_dtype), torch.zeros(n, device=DEV)
+    old[::2], a[::2] = old[::2] - 1000.0, 1.0
+    mask = (torch.rand(n, generator=_gen(29)) >= 0.3).to(DEV)
+    for reduction in ("mean", "sum", "sequence_mean", "none"):
+        print(f"case {n} {sequences} {offsets} {log_dtype} {reduction}", flush=True)
+        leaf = x.clone().requires_grad_()
+        entropy = torch.ones_like(x).requires_grad_()
+        loss = pretrain_policy_loss(leaf, old, a, cu_seqlens=cu, mask=mask, entropy=entropy,
+                                    entropy_weight=0.1, reduction=reduction)
+        assert reduction == "none" or torch.isnan(loss)
+        for grad in torch.autograd.grad(loss.sum(), [leaf, entropy]):
+            assert torch.isnan(grad).all()
+    for reduction in ("mean", "sum", "none"):
+        for kind, margin in (("sigmoid", 0.0), ("hinge", -1e30)):
+            leaf = x.clone().requires_grad_()
+            loss, _ = pretrain_preference_loss(leaf, cu, mask=mask, kind=kind, margin=margin,
+                                               reduction=reduction)
+            assert reduction == "none" or torch.isnan(loss)
+            assert torch.isnan(torch.autograd.grad(loss.sum(), [leaf])[0]).all()
