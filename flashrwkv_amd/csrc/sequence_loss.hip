@@ -19,8 +19,7 @@
 //
 // d decides on which side of a border a token is. Differences of logs are exact up
 // to one rounding; where a rounded one falls on a rounded border, both are taken in
-// 64 bits. A wave adds its up to 256 tokens up in 32 bits, everything beyond is in 64;
-// sums over a sequence, which a mean of answers is made of, are in 64 from the first on.
+// 64 bits. Exponentials and a token's loss are in 32 bits, sums over tokens in 64.
 //
 // A wave takes a tile of 64 x kRounds consecutive tokens with all loads under
 // way at once, and finds the sequence of its first token by itself, 64 offsets a
@@ -416,16 +415,14 @@ struct PolicyOut {
   bool slopes;
 };
 
-// Adds `values` up over the workgroup, in T within a wave; the result is the first
-// wave's.
-template <int kBlockWaves, int kValues, typename T>
-__device__ __forceinline__ void workgroup_sum(const T (&own)[kValues], double (&values)[kValues],
-                                              double* shared) {
+// Adds `values` up over the workgroup; the result is the first wave's.
+template <int kBlockWaves, int kValues>
+__device__ __forceinline__ void workgroup_sum(double (&values)[kValues], double* shared) {
   const int wave = threadIdx.x >> 6;
 #pragma unroll
   for (int v = 0; v < kValues; ++v) {
-    const T x = wave_sum(own[v]);
-    if (lane_id() == 0) shared[v * kBlockWaves + wave] = static_cast<double>(x);
+    const double x = wave_sum(values[v]);
+    if (lane_id() == 0) shared[v * kBlockWaves + wave] = x;
   }
   __syncthreads();
   if (wave == 0) {
@@ -437,15 +434,10 @@ __device__ __forceinline__ void workgroup_sum(const T (&own)[kValues], double (&
   __syncthreads();
 }
 
-template <int kBlockWaves, int kValues>
-__device__ __forceinline__ void workgroup_sum(double (&values)[kValues], double* shared) {
-  workgroup_sum<kBlockWaves, kValues, double>(values, values, shared);
-}
-
 template <int kRounds>
 __device__ __forceinline__ void policy_tile(const Policy& a, const Packed& p, const PolicyOut& o,
                                             const Saved& s, const Scratch& w, int64_t index,
-                                            float (&sums)[kSums]) {
+                                            double (&sums)[kSums]) {
   const Tile<kRounds> tile(index, p.n);
   if (tile.empty()) return;
   uint32_t x[kRounds], old[kRounds], advantage[kRounds], reference[kRounds], entropy[kRounds];
@@ -475,7 +467,7 @@ __device__ __forceinline__ void policy_tile(const Policy& a, const Packed& p, co
   }
   // Vector by vector: what is the same for all tokens is asked once a tile.
   float losses[kRounds], slopes[kRounds];
-  float ratio = 0.0f, old_kl = 0.0f, reference_kl = 0.0f;
+  double ratio = 0.0, old_kl = 0.0, reference_kl = 0.0;
   int32_t count = 0, clipped = 0;
 #pragma unroll
   for (int r = 0; r < kRounds; ++r) {
@@ -521,7 +513,7 @@ __device__ __forceinline__ void policy_tile(const Policy& a, const Packed& p, co
       if (tile.has(r)) to[64 * r + lane_id()] = losses[r];
     }
   }
-  float loss = 0.0f;
+  double loss = 0.0;
   if (by_sequence) {
     Pieces pieces;
     pieces.at = w.pieces + index;
@@ -534,21 +526,20 @@ __device__ __forceinline__ void policy_tile(const Policy& a, const Packed& p, co
 #pragma unroll
     for (int r = 0; r < kRounds; ++r) loss += losses[r];
   }
-  // A wave's counts are small whole numbers.
   sums[kLoss] = loss;
-  sums[kCount] = static_cast<float>(count);
+  sums[kCount] = count;
   sums[kRatio] = ratio;
-  sums[kClipped] = static_cast<float>(clipped);
+  sums[kClipped] = clipped;
   sums[kOld] = old_kl;
   sums[kReference] = reference_kl;
 }
 
 // Offsets that may not be, of a thread's share of the sequences.
-__device__ __forceinline__ float bad_offsets(const Packed& p, int64_t thread, int64_t threads) {
-  if (p.cu == nullptr) return 0.0f;
-  float bad = 0.0f;
+__device__ __forceinline__ double bad_offsets(const Packed& p, int64_t thread, int64_t threads) {
+  if (p.cu == nullptr) return 0.0;
+  double bad = 0.0;
   for (int64_t b = thread; b < p.sequences; b += threads) {
-    if (!in_order(p, static_cast<int32_t>(b))) bad = 1.0f;
+    if (!in_order(p, static_cast<int32_t>(b))) bad = 1.0;
   }
   return bad;
 }
@@ -602,8 +593,9 @@ __device__ __forceinline__ void write_policy(const PolicyOut& o, const Saved& s,
 // joins them, which saves the second launch. kPlain: all vectors are fp32, known to the
 // compiler; a type that is looked at for each value costs as many scalar
 // instructions as there are vector ones.
-// 4M tokens with a reference and a mask in 21 us: 89 MB at 4.1 TB/s, 154 vector
-// instructions for 64 tokens, 16 us of all SIMDs.
+// 4M tokens with a reference and a mask in 24 us: 89 MB at 3.7 TB/s, 185 vector
+// instructions for 64 tokens. With a wave's sums in 32 bits it is 21 and 154, but two
+// ratios of 3e38 have a mean and no such sum, and terms that cancel lose their digits.
 template <int kRounds, int kBlockWaves, bool kAlone, bool kPlain>
 __global__ __launch_bounds__(kBlockWaves * 64) void policy_tokens_kernel(Policy a, Packed p,
                                                                          PolicyOut o, Saved s,
@@ -617,13 +609,12 @@ __global__ __launch_bounds__(kBlockWaves * 64) void policy_tokens_kernel(Policy 
     if (a.reference.given()) a.reference.dtype = FRWKV_DTYPE_F32;
     if (a.entropy.given()) a.entropy.dtype = FRWKV_DTYPE_F32;
   }
-  float own[kSums] = {};
-  policy_tile<kRounds>(a, p, o, s, w,
-                       static_cast<int64_t>(blockIdx.x) * kBlockWaves + wave, own);
-  own[kBad] = bad_offsets(p, static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x,
-                          static_cast<int64_t>(gridDim.x) * kThreads);
   double sums[kSums] = {};
-  workgroup_sum<kBlockWaves>(own, sums, shared);
+  policy_tile<kRounds>(a, p, o, s, w,
+                       static_cast<int64_t>(blockIdx.x) * kBlockWaves + wave, sums);
+  sums[kBad] = bad_offsets(p, static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x,
+                           static_cast<int64_t>(gridDim.x) * kThreads);
+  workgroup_sum<kBlockWaves>(sums, shared);
   if constexpr (kAlone) {
     double found[2] = {};
     join_sequences(p, o, s, w, shift_of(kRounds), tiles, wave, kBlockWaves, found);

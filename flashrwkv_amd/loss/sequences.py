@@ -10,8 +10,10 @@ Both take log probabilities of any shape, read in memory order: what
 do not fall; tokens behind the last one take no part, as a padded batch has
 them); ``mask`` (bool or uint8, one entry a token) leaves tokens out. What stands in tokens that
 take no part, NaN included, reaches nothing, and their gradients are 0. Each
-vector is float32, float16 or bfloat16 by itself; ratios and sums are taken in
-64 bits and summed in a fixed order.
+vector is float32, float16 or bfloat16 by itself. A policy's ratios, and with them a
+token's loss, are in 32 bits from log ratios that are rounded once (on which side of
+a clip border one is, is decided as in 64); sums over tokens, and all of a
+preference pair, are in 64 bits and in a fixed order.
 
 Nothing synchronises with the host: offsets that may not be cannot be raised as
 an error, they make a reduced loss and the gradients of all tokens NaN.

@@ -759,7 +759,9 @@ int frwkv_linear_log_probs_backward(int io_dtype, int64_t rows, int64_t channels
  * last offset take no part); mask one byte a token (NULL: all take part). What
  * stands in tokens that take no part, NaN included, reaches nothing; their
  * gradients are 0. Offsets that may not be make a reduced loss and the gradients of
- * all tokens NaN. Sums are in 64 bits and in a fixed order. No counterpart in the reference.
+ * all tokens NaN. Log ratios of the policy loss are rounded once and its ratios and a
+ * token's loss are in 32 bits; sums over tokens and all of a preference pair are in 64
+ * bits and in a fixed order. No counterpart in the reference.
  *
  * frwkv_policy_loss_forward: with d = log_probs - old_log_probs, r = exp(d) and
  * advantage A (one a token or, advantages_per_sequence, one a sequence) a token's

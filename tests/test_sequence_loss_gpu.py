@@ -658,3 +658,30 @@ def test_offsets_that_may_not_be_mark_every_gradient(n, sequences, offsets, log_
                                                reduction=reduction)
             assert reduction == "none" or torch.isnan(loss)
             assert torch.isnan(torch.autograd.grad(loss.sum(), [leaf])[0]).all()
+
+
+SIZES = [2, 300, 2048, 2049, 4096, 4097, 262144, 262145]
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum", "sequence_mean"])
+@pytest.mark.parametrize("n", SIZES)
+def test_policy_sums_hold_what_32_bits_do_not(n, reduction):
+    """Terms that cancel, each of them exact: 2^25 at the ends and 1 between, whose sum is
+    n - 2, rounded once. And ratios of 3.3e38, of which two have a mean but no sum."""
+    cu, _ = _offsets([n])
+    zeros = torch.zeros(n, device=DEV)
+    a = -torch.ones(n, device=DEV)
+    a[0], a[-1] = -2.0 ** 25, 2.0 ** 25
+    loss = pretrain_policy_loss(zeros, zeros, a, cu_seqlens=cu, reduction=reduction)
+    want = (n - 2) / (1 if reduction == "sum" else n)
+    assert abs(loss.item() - want) <= 2 * E * want
+    if reduction == "sum":
+        return
+    high = torch.full((n,), 88.7, device=DEV)
+    d = high[0].double().item()
+    loss, metrics = pretrain_policy_loss(high, zeros, torch.full_like(high, -1.0), metrics=True,
+                                         cu_seqlens=cu, reduction=reduction)
+    k = (16 + d) * E
+    for value, want in ((loss, math.exp(d)), (metrics[0], math.exp(d)),
+                        (metrics[2], math.expm1(d) - d)):
+        assert abs(value.item() - want) <= k * want
