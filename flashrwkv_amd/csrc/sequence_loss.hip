@@ -795,7 +795,10 @@ __device__ __forceinline__ void preference_term(const Preference& a, double m, d
   if (a.kind == FRWKV_PREFERENCE_SIGMOID) {
     const double e = exp(-fabs(m));  // both log sigmas from it, no overflow
     const double soft = log1p(e), eps = a.smoothing;
-    loss = (1.0 - eps) * (soft + fmax(-m, 0.0)) + eps * (soft + fmax(m, 0.0));
+    loss = (1.0 - eps) * (soft + fmax(-m, 0.0));
+    // Without smoothing the term is not there: m is infinite where the rejected answer
+    // cannot be, and 0 of it would be NaN.
+    if (eps != 0.0) loss += eps * (soft + fmax(m, 0.0));
     // sigma(m) - 1 = -sigma(-m), of which the smaller one keeps its digits.
     const double small = e / (1.0 + e), large = 1.0 / (1.0 + e);
     slope = eps * (m > 0.0 ? large : small) - (1.0 - eps) * (m > 0.0 ? small : large);

@@ -685,3 +685,24 @@ def test_policy_sums_hold_what_32_bits_do_not(n, reduction):
     for value, want in ((loss, math.exp(d)), (metrics[0], math.exp(d)),
                         (metrics[2], math.expm1(d) - d)):
         assert abs(value.item() - want) <= k * want
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_a_rejected_answer_that_cannot_be_has_no_loss(reduction):
+    """m = inf: the term that label_smoothing 0 leaves out is infinite."""
+    cu, n = _offsets([3, 2, 4, 1])
+    x, _, _ = _logs(n, seed=32)
+    x[4] = -math.inf
+    args = {"reference": None, "mask": None, "reduction": reduction}
+    up = torch.ones(2 if reduction == "none" else (), device=DEV)
+    got = _run_preference(x, cu, args, up)
+    clean = x.clone()
+    clean[4] = -1e6
+    want = _run_preference(clean, cu, args, up)
+    assert torch.equal(got["loss"], want["loss"]) and torch.isfinite(got["loss"]).all()
+    assert torch.equal(got["dlog_probs"], want["dlog_probs"])
+    assert not got["dlog_probs"][:5].any() and got["dlog_probs"][5:].all()
+    assert got["rewards"][0, 1].item() == -math.inf
+    # With smoothing the rejected answer's own term is there, and infinite.
+    got = _run_preference(x, cu, args | {"label_smoothing": 0.1}, up)
+    assert math.isinf(got["loss"].flatten()[0].item())
