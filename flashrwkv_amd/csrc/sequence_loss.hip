@@ -486,8 +486,10 @@ __device__ __forceinline__ void policy_tile(const Policy& a, const Packed& p, co
     for (int r = 0; r < kRounds; ++r) {
       const Exponential q =
           exponential(value_of(a.reference, reference[r]) - value_of(a.x, x[r]));
-      losses[r] = fmaf(a.kl, q.k3, losses[r]);
-      slopes[r] = fmaf(-a.kl, q.less_one, slopes[r]);
+      if (a.kl != 0.0f) {  // or only looked at, and 0 of an infinite k3 would be NaN
+        losses[r] = fmaf(a.kl, q.k3, losses[r]);
+        slopes[r] = fmaf(-a.kl, q.less_one, slopes[r]);
+      }
       reference_kl += part[r] ? q.k3 : 0.0f;
     }
   }
@@ -1100,6 +1102,7 @@ int frwkv_policy_loss_forward(int64_t tokens, int64_t sequences, const int32_t* 
   }
   if (rc == FRWKV_OK) rc = check_column(what, "entropy", entropy_dtype, entropy, true, &a.entropy);
   if (rc != FRWKV_OK) return rc;
+  if (entropy_weight == 0.0f) a.entropy = {nullptr, kNone};  // whatever it holds
   if (!(clip_low >= 0.0 && clip_low <= 1.0) || !(clip_high >= 0.0 && clip_high <= 1e30)) {
     return set_error(FRWKV_ERR_INVALID_ARGUMENT,
                      "%s: clip_low must be in [0, 1] and clip_high in [0, 1e30]", what);

@@ -228,7 +228,8 @@ def pretrain_policy_loss(
         + kl_weight k3(reference_log_probs - log_probs) - entropy_weight entropy
 
     with ``k3(x) = exp(x) - 1 - x``; with ``dual_clip`` the first term is at most
-    ``-dual_clip A`` where A < 0. ``reduction``: the mean or sum over the tokens that
+    ``-dual_clip A`` where A < 0. A term whose weight is 0 is not there, whatever it would
+    be. ``reduction``: the mean or sum over the tokens that
     take part, the mean over sequences of each one's mean (``"sequence_mean"``;
     sequences without such tokens do not count), 0 without any, or ``"none"``: a
     loss a token in ``log_probs``' shape.

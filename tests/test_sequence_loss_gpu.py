@@ -706,3 +706,24 @@ def test_a_rejected_answer_that_cannot_be_has_no_loss(reduction):
     # With smoothing the rejected answer's own term is there, and infinite.
     got = _run_preference(x, cu, args | {"label_smoothing": 0.1}, up)
     assert math.isinf(got["loss"].flatten()[0].item())
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum", "sequence_mean", "none"])
+@pytest.mark.parametrize("n", [300, 5000])
+def test_terms_of_weight_zero_are_not_there(n, reduction):
+    """A reference that is only looked at (metrics) and an entropy without a bonus reach
+    neither loss nor gradient, whatever they hold: a reference's k3 is infinite from 89 on."""
+    x, old, a, args, up = _policy([n - 100, 100], reduction=reduction, seed=33)
+    args |= {"reference": None, "entropy": None, "kl_weight": 0.0, "entropy_weight": 0.0}
+    want = _run_policy(x, old, a, args, up)
+    taking = args["mask"].nonzero()[:, 0]
+    reference = x - 0.5
+    reference[taking[3]], reference[taking[7]] = 100.0, 1e30
+    entropy = torch.zeros_like(x)
+    entropy[taking[5]], entropy[taking[9]] = math.inf, math.nan
+    got = _run_policy(x, old, a, args | {"reference": reference, "entropy": entropy}, up)
+    for name in ("loss", "dlog_probs"):
+        assert torch.equal(got[name], want[name]), name
+    assert torch.equal(got["metrics"][:3], want["metrics"][:3])
+    assert got["metrics"][3].item() == math.inf
+    assert not got["dentropy"].any()
