@@ -3,7 +3,8 @@
 //   norm = sqrt(sum over all tensors of x^2),  by = min(1, most / (norm + eps)),
 //   y = x by  (in place, or to other tensors of types of their own).
 // A norm that is not finite leaves by = 1: the gradients stay what they are, and
-// the norm tells the caller.
+// the norm tells the caller. by is rounded to 32 bits, as is its product with an element;
+// below the normal numbers of 32 bits it keeps 64 and the product is made in them.
 //
 // Memory bounds both passes: each tensor is read once for the norm and once more
 // to be scaled. Tensors are cut into units of kUnit elements, so that a list of small
@@ -212,8 +213,8 @@ __device__ __forceinline__ void add_squares(const Entry& e, int64_t first, doubl
 }
 
 // kEach units of a tensor, scaled.
-template <int kEach, bool kStream>
-__device__ __forceinline__ void scale_units(const Entry& e, int64_t first, float by) {
+template <int kEach, bool kStream, typename Factor>
+__device__ __forceinline__ void scale_units(const Entry& e, int64_t first, Factor by) {
   with_dtype(e.dtype, [&](auto type) {
     with_dtype(e.to_dtype, [&](auto to_type) {
       using T = decltype(type);
@@ -227,7 +228,7 @@ __device__ __forceinline__ void scale_units(const Entry& e, int64_t first, float
         const int64_t i = place<kPer>(first, j);
         Pack<To, kPer> y;
 #pragma unroll
-        for (int q = 0; q < kPer; ++q) y.set(q, x[j].at(q) * by);
+        for (int q = 0; q < kPer; ++q) y.set(q, static_cast<float>(x[j].at(q) * by));
         if (whole || (e.to_aligned && e.numel - i >= kPer)) {
           y.template store<kStream>(e.to, i);
         } else {
@@ -377,16 +378,26 @@ __device__ __forceinline__ double total_of(const double* __restrict__ sums, int3
 }
 
 // 1 where the norm as it is returned, in 32 bits, is not finite.
-__device__ __forceinline__ float factor_of(double total, double most, double eps) {
+__device__ __forceinline__ double factor_of(double total, double most, double eps) {
   const double norm = sqrt(total);
-  if (!(static_cast<float>(norm) < __builtin_inff())) return 1.0f;
-  return static_cast<float>(fmin(1.0, most / (norm + eps)));
+  if (!(static_cast<float>(norm) < __builtin_inff())) return 1.0;
+  return fmin(1.0, most / (norm + eps));
+}
+
+// f(factor) in the bits that hold it.
+template <typename F>
+__device__ __forceinline__ void with_factor(double by, F&& f) {
+  if (by >= 0x1p-126) {
+    f(static_cast<float>(by));
+  } else {
+    f(by);
+  }
 }
 
 // factor: null for the norm alone.
 __global__ __launch_bounds__(kThreads) void norm_kernel(const double* __restrict__ sums,
                                                         int32_t groups, double most, double eps,
-                                                        float* norm, float* factor) {
+                                                        float* norm, double* factor) {
   __shared__ double shared[kThreads / 64];
   const double total = total_of<kThreads>(sums, groups, shared);
   if (threadIdx.x != 0) return;
@@ -404,15 +415,17 @@ __global__ __launch_bounds__(kThreads) void run_scale_kernel(Entries entries, Li
   __shared__ double shared[kThreads / 64];
   const double total = total_of<kThreads>(sums, groups, shared);
   if (blockIdx.x == 0 && threadIdx.x == 0) *norm = static_cast<float>(sqrt(total));
-  const float by = factor_of(total, most, eps);
-  if (list.in_place && by == 1.0f) return;
+  const double factor = factor_of(total, most, eps);
+  if (list.in_place && static_cast<float>(factor) == 1.0f) return;
   const Run run = run_of(list.chunks);
-  int at = entry_of(entries.entry, list.count, run.to - 1);
-  for (int32_t c = run.to - 1; c >= run.from; --c) {
-    while (entries.entry[at].first > c) --at;
-    const Entry e = entries.entry[at];
-    scale_units<kEach, false>(e, static_cast<int64_t>(c - e.first) * (kEach * kUnit), by);
-  }
+  with_factor(factor, [&](auto by) {
+    int at = entry_of(entries.entry, list.count, run.to - 1);
+    for (int32_t c = run.to - 1; c >= run.from; --c) {
+      while (entries.entry[at].first > c) --at;
+      const Entry e = entries.entry[at];
+      scale_units<kEach, false>(e, static_cast<int64_t>(c - e.first) * (kEach * kUnit), by);
+    }
+  });
 }
 
 // A unit a workgroup, from the last one (and again, beyond what a launch has). Bound by
@@ -421,14 +434,15 @@ constexpr int kMostScalers = 1 << 22;
 
 template <bool kStream>
 __global__ __launch_bounds__(kThreads) void scale_kernel(Places places, List list,
-                                                         const float* __restrict__ factor) {
-  const float by = *factor;
-  if (list.in_place && by == 1.0f) return;
-  for (int32_t unit = list.chunks - 1 - static_cast<int32_t>(blockIdx.x); unit >= 0;
-       unit -= static_cast<int32_t>(gridDim.x)) {
-    const Entry e = places.entry[places.owner[unit]];
-    scale_units<1, kStream>(e, static_cast<int64_t>(unit - e.first) * kUnit, by);
-  }
+                                                         const double* __restrict__ factor) {
+  if (list.in_place && static_cast<float>(*factor) == 1.0f) return;
+  with_factor(*factor, [&](auto by) {
+    for (int32_t unit = list.chunks - 1 - static_cast<int32_t>(blockIdx.x); unit >= 0;
+         unit -= static_cast<int32_t>(gridDim.x)) {
+      const Entry e = places.entry[places.owner[unit]];
+      scale_units<1, kStream>(e, static_cast<int64_t>(unit - e.first) * kUnit, by);
+    }
+  });
 }
 
 constexpr int64_t kMostElements = int64_t{1} << 40;  // of a tensor
@@ -587,7 +601,7 @@ void with_stream(bool stream, F&& f) {
 // Launches the norm, with the scaling behind it (scale) or without.
 void launch(const Plan& plan, int64_t count, const frwkv_gradient* tensors, bool scale,
             double most, double eps, float* norm, char* workspace, hipStream_t stream) {
-  float* factor = scale ? reinterpret_cast<float*>(workspace) : nullptr;
+  double* factor = scale ? reinterpret_cast<double*>(workspace) : nullptr;
   double* sums = reinterpret_cast<double*>(workspace + 256);
   const int groups = plan.groups();
   List list{static_cast<int32_t>(plan.count), static_cast<int32_t>(plan.chunks), scale};

@@ -115,9 +115,10 @@ def pretrain_clip_grad_norm(
     from before, an fp32 scalar on their device.
 
     In place, or with ``out`` into other tensors of the same shapes and strides
-    and of dtypes of their own, rounded once. Where the norm is not finite nothing is scaled (``out``
-    takes the tensors as they are), so that a caller who looks at the norm can skip the
-    step. A tensor that is written may be its own source but must not overlap
+    and of dtypes of their own. The factor is rounded to 32 bits (below their normal
+    numbers it keeps 64), its product with an element to 32 bits and then to the
+    output's type. Where the norm is not finite nothing is scaled (``out`` takes the
+    tensors as they are), so that a caller who looks at the norm can skip the step. A tensor that is written may be its own source but must not overlap
     any other tensor of the call, so none is scaled twice.
     """
     call = C.whole_call("clip_grad_norm_call")

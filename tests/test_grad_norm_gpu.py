@@ -271,3 +271,19 @@ def test_subclasses_take_the_tables():
     assert pretrain_grad_norm([t]).item() == 10.0
     assert pretrain_clip_grad_norm([t], 5.0, eps=0.0).item() == 10.0
     assert torch.equal(t.as_subclass(torch.Tensor), torch.full((100,), 0.5, device=DEV))
+
+
+@pytest.mark.parametrize("sizes", [[100, 31], [9_000_000], [77] * 200])
+def test_factors_that_32_bits_do_not_hold(sizes):
+    """A norm so far above the maximum that their quotient is not a normal number of 32 bits,
+    or not one at all, while its products with the elements are."""
+    gen = torch.Generator().manual_seed(9)
+    tensors = [(1e34 * torch.randn(n, generator=gen)).to(DEV) for n in sizes]
+    norm = step.clip(tensors, 1.0, 0.0)[0]
+    for by in (3e-41, 2e-47):
+        for dtype in (torch.float32, torch.bfloat16):
+            out = [torch.empty_like(t, dtype=dtype) for t in tensors]
+            _check(tensors, out, pretrain_clip_grad_norm(tensors, norm * by, out=out), norm * by)
+            assert all(t.any() for t in out)
+        copies = [t.clone() for t in tensors]
+        _check(tensors, copies, pretrain_clip_grad_norm(copies, norm * by), norm * by)
