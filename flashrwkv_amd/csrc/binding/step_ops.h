@@ -316,14 +316,20 @@ bool apart(const std::vector<frwkv_gradient>& list) {
   return true;
 }
 
+// out null: nothing is written. A tensor that is written and shares its memory until
+// then gets memory of its own, before any address is taken.
 std::vector<frwkv_gradient> gradient_list(const std::vector<Tensor>& tensors,
                                           const std::vector<Tensor>* out) {
   std::vector<frwkv_gradient> list(tensors.size());
+  for (size_t i = 0; out != nullptr && i < tensors.size(); ++i) {
+    list[i].out = (*out)[i].mutable_data_ptr();
+  }
   for (size_t i = 0; i < tensors.size(); ++i) {
     const Tensor& x = tensors[i];
-    const Tensor& y = out != nullptr ? (*out)[i] : x;
-    list[i] = {x.const_data_ptr(), const_cast<void*>(y.const_data_ptr()), x.numel(),
-               io_code(x.scalar_type()), io_code(y.scalar_type())};
+    list[i].data = x.const_data_ptr();
+    list[i].numel = x.numel();
+    list[i].dtype = io_code(x.scalar_type());
+    list[i].out_dtype = io_code((out != nullptr ? (*out)[i] : x).scalar_type());
   }
   return list;
 }

@@ -287,3 +287,15 @@ def test_factors_that_32_bits_do_not_hold(sizes):
             assert all(t.any() for t in out)
         copies = [t.clone() for t in tensors]
         _check(tensors, copies, pretrain_clip_grad_norm(copies, norm * by), norm * by)
+
+
+def test_tensors_that_share_memory_until_they_are_written():
+    """A lazy copy's own memory is written, not the one that it shares until then."""
+    for out in (False, True):
+        a = torch.ones(100, device=DEV)
+        lazy = torch._lazy_clone(a)
+        norm = pretrain_clip_grad_norm([a.clone() if out else lazy], 1.0, eps=0.0,
+                                       out=[lazy] if out else None)
+        assert norm.item() == 10.0
+        assert torch.equal(a, torch.ones_like(a))
+        assert torch.allclose(lazy, torch.full_like(a, 0.1))
