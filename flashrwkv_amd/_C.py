@@ -216,10 +216,11 @@ def layer_norm_backward(grad_y, normed, grad_stream, weight, mean, rstd):
     return ops.layer_norm_backward(grad_y, normed, grad_stream, weight, mean, rstd)
 
 
-def linear_cross_entropy_forward(hidden, weight, targets, ignore_index, reduction):
+def linear_cross_entropy_forward(hidden, weight, targets, ignore_index, reduction,
+                                 backward_follows=True):
     """(loss, saved); reduction 0 none, 1 mean, 2 sum."""
     return ops.linear_cross_entropy_forward(hidden, weight, targets, int(ignore_index),
-                                            int(reduction))
+                                            int(reduction), bool(backward_follows))
 
 
 def linear_topk_distillation_forward(hidden, weight, teacher_logits, teacher_indices,

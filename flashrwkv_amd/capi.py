@@ -72,6 +72,8 @@ SIGNATURES = {
     "frwkv_linear_loss_backward_plan": [_I64] * 3 + [_VP] * 4,
     "frwkv_linear_cross_entropy_forward": [_INT] + [_I64] * 3 + [_VP, _VP, _INT, _VP, _I64, _INT]
                                           + [_VP, _VP, _SZ, _VP, _SZ, _VP],
+    "frwkv_linear_cross_entropy_score": [_INT] + [_I64] * 3 + [_VP, _VP, _INT, _VP, _I64, _INT]
+                                        + [_VP, _VP, _SZ, _VP, _SZ, _VP],
     "frwkv_linear_topk_distillation_forward": [_INT] + [_I64] * 4 + [_VP, _VP, _INT, _VP, _INT]
                                               + [_VP, _F32, _INT, _VP, _VP, _SZ, _VP, _SZ, _VP],
     "frwkv_linear_loss_backward": [_INT] + [_I64] * 4 + [_VP, _F32, _INT, _VP, _VP, _SZ]
@@ -388,10 +390,12 @@ def _loss_buffers(hidden, vocab, top):
 
 
 def linear_cross_entropy_forward(hidden, weight, targets, *, loss, ignore_index=-100,
-                                 reduction="mean"):
+                                 reduction="mean", backward_follows=True):
     """Writes ``loss`` (fp32) and returns the buffer that the backward reads."""
     rows, c, saved, work = _loss_buffers(hidden, weight.shape[0], 1)
-    _check(library().frwkv_linear_cross_entropy_forward(
+    call = (library().frwkv_linear_cross_entropy_forward if backward_follows
+            else library().frwkv_linear_cross_entropy_score)
+    _check(call(
         DTYPE[hidden.dtype], rows, c, weight.shape[0], _p(hidden), _p(weight),
         targets.element_size(), _p(targets), int(ignore_index), REDUCTIONS[reduction], _p(loss),
         _p(saved), saved.numel(), _p(work), work.numel(), _stream()))

@@ -10,6 +10,7 @@
 
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 
 namespace {
 
@@ -86,12 +87,14 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
 struct LinearLossNode : torch::autograd::Function<LinearLossNode> {
   static Tensor forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight,
                         const Tensor& indices, const std::optional<Tensor>& teacher_logits,
-                        int64_t ignore_index, double temperature, int64_t reduction) {
+                        int64_t ignore_index, double temperature, int64_t reduction,
+                        bool backward_follows) {
     const auto [loss, saved] =
         teacher_logits.has_value()
             ? linear_topk_distillation_forward(hidden, weight, *teacher_logits, indices,
                                                temperature, reduction)
-            : linear_cross_entropy_forward(hidden, weight, indices, ignore_index, reduction);
+            : linear_cross_entropy_forward(hidden, weight, indices, ignore_index, reduction,
+                                           backward_follows);
     ctx->save_for_backward({weight, saved});
     ctx->saved_data["shape"] = hidden.sizes().vec();
     ctx->saved_data["top"] = teacher_logits.has_value() ? indices.size(-1) : int64_t{1};
@@ -110,7 +113,7 @@ struct LinearLossNode : torch::autograd::Function<LinearLossNode> {
         upstream[0].contiguous(), saved[0], saved[1], rows, ctx->saved_data["top"].toInt(),
         ctx->saved_data["temperature"].toDouble(), ctx->saved_data["reduction"].toInt(),
         want_hidden, want_weight);
-    variable_list out(7);
+    variable_list out(8);
     if (want_hidden) out[0] = grads.front().view(shape);
     if (want_weight) out[1] = grads.back();
     return first_order(std::move(out), upstream, "a head loss");
@@ -213,7 +216,8 @@ pybind11::object linear_loss_call(const pybind11::object& hidden_, const pybind1
   {
     pybind11::gil_scoped_release release;
     loss = LinearLossNode::apply(hidden, weight, indices, teacher, ignore_index, temperature,
-                                 reduction);
+                                 reduction,
+                                 torch::autograd::compute_requires_grad(hidden, weight));
   }
   return pybind11::cast(std::move(loss));
 }

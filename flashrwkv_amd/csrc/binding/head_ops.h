@@ -108,7 +108,8 @@ int index_bytes(const Tensor& t, const char* name) {
 
 std::tuple<Tensor, Tensor> linear_cross_entropy_forward(Tensor hidden, Tensor weight,
                                                         Tensor targets, int64_t ignore_index,
-                                                        int64_t reduction) {
+                                                        int64_t reduction,
+                                                        bool backward_follows) {
   const int64_t rows = check_head(hidden, weight, reduction);
   check_device_contiguous(targets, "targets");
   const int bytes = index_bytes(targets, "targets");
@@ -123,7 +124,9 @@ std::tuple<Tensor, Tensor> linear_cross_entropy_forward(Tensor hidden, Tensor we
   const size_t saved_bytes = frwkv_linear_loss_saved_bytes(rows, c, 1);
   const size_t work_bytes = frwkv_linear_loss_forward_workspace_bytes(rows, vocab);
   Tensor saved = workspace_like(hidden, saved_bytes), work = workspace_like(hidden, work_bytes);
-  check_rc(frwkv_linear_cross_entropy_forward(
+  auto* call = backward_follows ? &frwkv_linear_cross_entropy_forward
+                                : &frwkv_linear_cross_entropy_score;
+  check_rc(call(
       io_code(hidden.scalar_type()), rows, c, vocab, hidden.const_data_ptr(),
       weight.const_data_ptr(), bytes, targets.const_data_ptr(), ignore_index,
       static_cast<int>(reduction), loss.data_ptr<float>(), scratch_ptr(saved), saved_bytes,

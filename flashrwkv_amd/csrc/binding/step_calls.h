@@ -4,7 +4,6 @@
 // torch_ops.cpp, behind head_calls.h.
 #pragma once
 
-#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 
 namespace {

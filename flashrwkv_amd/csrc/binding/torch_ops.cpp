@@ -1523,7 +1523,7 @@ TORCH_LIBRARY(flashrwkv2, m) {
       &layer_norm_backward);
   m.def(
       "linear_cross_entropy_forward(Tensor hidden, Tensor weight, Tensor targets, "
-      "int ignore_index, int reduction) -> (Tensor, Tensor)",
+      "int ignore_index, int reduction, bool backward_follows=True) -> (Tensor, Tensor)",
       &linear_cross_entropy_forward);
   m.def(
       "linear_topk_distillation_forward(Tensor hidden, Tensor weight, Tensor teacher_logits, "

@@ -1313,6 +1313,7 @@ struct Plan {
 // slabs weigh more: 9784, 9749, 9715 us). A slab is written in each piece and read
 // once after it.
 constexpr int64_t kCachedBytes = int64_t{192} << 20;
+constexpr int64_t kPartlyCachedBytes = int64_t{320} << 20;
 constexpr int64_t kMostBytes = int64_t{512} << 20;
 constexpr double kGradBytesPerUs = 20.0e6;
 constexpr double kSlabBytesPerUs = 4.0e6;
@@ -1498,9 +1499,11 @@ int run_forward(const Shape& d, const Source& source, const void* hidden, const 
   };
   // Few rows read the weight once: one that no cache holds until the next call goes past
   // them (8 rows, 65536 tokens of 2048 channels: 61.3 -> 53.8 us, of 4096: 107 -> 93;
-  // 8192 tokens of 4096, which stay: 27.2 -> 32.6; with a backward behind it, which
-  // still finds a part of the first: 168 -> 170).
-  const bool past = last_read && static_cast<int64_t>(d.vocab) * d.c * 2 > kCachedBytes;
+  // 8192 tokens of 4096, which stay: 27.2 -> 32.6). A backward behind them still finds a part
+  // of a weight that is not much larger than the last-level cache (8 rows with their gradient:
+  // 268 MB 155 -> 160 us, 336 MB 202 -> 201, 403 MB 311 -> 301, 537 MB 294 -> 287).
+  const int64_t weight_bytes = static_cast<int64_t>(d.vocab) * d.c * 2;
+  const bool past = weight_bytes > (last_read ? kCachedBytes : kPartlyCachedBytes);
   for_sizes<T>(d.vocab, d.n, steps, [&](auto* tile, int grid) {
     using G = std::remove_pointer_t<decltype(tile)>;
     if constexpr (G::kTurns) {
@@ -1714,6 +1717,31 @@ int begin_forward(const char* what, int io_dtype, int64_t n, int64_t c, int64_t 
   return check_memory(what, "workspace", workspace, workspace_bytes, need);
 }
 
+int cross_entropy(const char* what, int io_dtype, int64_t rows, int64_t channels, int64_t vocab,
+                  const void* hidden, const void* weight, int target_bytes, const void* targets,
+                  int64_t ignore_index, int reduction, bool last_read, float* loss, void* saved,
+                  size_t saved_bytes, void* workspace, size_t workspace_bytes, void* stream) {
+  Saved s;
+  const int rc = begin_forward(what, io_dtype, rows, channels, vocab, 1, hidden, weight,
+                               reduction, loss, false, saved, saved_bytes, workspace,
+                               workspace_bytes, &s);
+  if (rc != FRWKV_OK) return rc;
+  if (!targets || (target_bytes != 4 && target_bytes != 8)) {
+    return set_error(FRWKV_ERR_INVALID_ARGUMENT, "%s: targets must be int32 or int64", what);
+  }
+  const hipStream_t q = static_cast<hipStream_t>(stream);
+  const Shape d{static_cast<int32_t>(rows), static_cast<int32_t>(channels),
+                static_cast<int32_t>(vocab), 1};
+  if (target_bytes == 8) {
+    const Labels<int64_t> labels{static_cast<const int64_t*>(targets), ignore_index};
+    return forward<false, false>(io_dtype, d, labels, hidden, weight, 1.0f, reduction, loss,
+                                 nullptr, last_read, s, workspace, q);
+  }
+  const Labels<int32_t> labels{static_cast<const int32_t*>(targets), ignore_index};
+  return forward<false, false>(io_dtype, d, labels, hidden, weight, 1.0f, reduction, loss, nullptr,
+                               last_read, s, workspace, q);
+}
+
 int backward(const char* what, int io_dtype, int64_t rows, int64_t channels, int64_t vocab,
              int64_t top, const void* weight, float temperature, const Upstream& upstream,
              const void* saved, size_t saved_bytes, void* grad_hidden, void* grad_weight,
@@ -1803,28 +1831,20 @@ int frwkv_linear_cross_entropy_forward(int io_dtype, int64_t rows, int64_t chann
                                        int64_t ignore_index, int reduction, float* loss,
                                        void* saved, size_t saved_bytes, void* workspace,
                                        size_t workspace_bytes, void* stream) {
-  using namespace frwkv;
-  const char* what = "frwkv_linear_cross_entropy_forward";
-  Saved s;
-  const int rc = begin_forward(what, io_dtype, rows, channels, vocab, 1, hidden, weight,
-                               reduction, loss, false, saved, saved_bytes, workspace,
-                               workspace_bytes, &s);
-  if (rc != FRWKV_OK) return rc;
-  if (!targets || (target_bytes != 4 && target_bytes != 8)) {
-    return set_error(FRWKV_ERR_INVALID_ARGUMENT, "%s: targets must be int32 or int64", what);
-  }
-  const hipStream_t q = static_cast<hipStream_t>(stream);
-  const int32_t n = static_cast<int32_t>(rows), v = static_cast<int32_t>(vocab);
-  const Shape d{n, static_cast<int32_t>(channels), v, 1};
-  const bool scoring = reduction == FRWKV_REDUCE_NONE;  // most such calls
-  if (target_bytes == 8) {
-    const Labels<int64_t> labels{static_cast<const int64_t*>(targets), ignore_index};
-    return forward<false, false>(io_dtype, d, labels, hidden, weight, 1.0f, reduction, loss,
-                                 nullptr, scoring, s, workspace, q);
-  }
-  const Labels<int32_t> labels{static_cast<const int32_t*>(targets), ignore_index};
-  return forward<false, false>(io_dtype, d, labels, hidden, weight, 1.0f, reduction, loss, nullptr,
-                               scoring, s, workspace, q);
+  return frwkv::cross_entropy("frwkv_linear_cross_entropy_forward", io_dtype, rows, channels,
+                              vocab, hidden, weight, target_bytes, targets, ignore_index,
+                              reduction, false, loss, saved, saved_bytes, workspace,
+                              workspace_bytes, stream);
+}
+
+int frwkv_linear_cross_entropy_score(int io_dtype, int64_t rows, int64_t channels, int64_t vocab,
+                                     const void* hidden, const void* weight, int target_bytes,
+                                     const void* targets, int64_t ignore_index, int reduction,
+                                     float* loss, void* saved, size_t saved_bytes,
+                                     void* workspace, size_t workspace_bytes, void* stream) {
+  return frwkv::cross_entropy("frwkv_linear_cross_entropy_score", io_dtype, rows, channels, vocab,
+                              hidden, weight, target_bytes, targets, ignore_index, reduction,
+                              true, loss, saved, saved_bytes, workspace, workspace_bytes, stream);
 }
 
 size_t frwkv_linear_log_probs_forward_workspace_bytes(int64_t rows, int64_t vocab,

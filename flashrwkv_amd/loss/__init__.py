@@ -126,7 +126,7 @@ class _LinearLoss(torch.autograd.Function):
             shape = hidden.shape[:-1] if reduction == 0 else ()
             ctx.save_for_backward(weight)
             return torch.zeros(shape, device=hidden.device, dtype=torch.float32)
-        loss, saved = launch(hidden, weight)
+        loss, saved = launch(hidden, weight, any(ctx.needs_input_grad))
         ctx.save_for_backward(weight, saved)
         return loss
 
@@ -222,9 +222,9 @@ def pretrain_linear_cross_entropy(
     C.enforce(CROSS_ENTROPY, {"hidden": hidden, "weight": weight, "targets": targets,
                               "ignore_index": ignore_index, "reduction": reduction})
 
-    def launch(h, w):
+    def launch(h, w, backward_follows):
         return C.native().linear_cross_entropy_forward(h, w, targets, ignore_index,
-                                                       REDUCTIONS[reduction])
+                                                       REDUCTIONS[reduction], backward_follows)
 
     return _run("pretrain_linear_cross_entropy", hidden, weight, launch, 1, 1.0, reduction)
 
@@ -263,7 +263,7 @@ def pretrain_linear_topk_distillation(
                              "teacher_indices": teacher_indices, "temperature": temperature,
                              "reduction": reduction})
 
-    def launch(h, w):
+    def launch(h, w, _):
         return C.native().linear_topk_distillation_forward(
             h, w, teacher_logits, teacher_indices, temperature, REDUCTIONS[reduction])
 

@@ -674,7 +674,9 @@ int frwkv_layer_norm_backward(int io_dtype, int64_t rows, int64_t channels, cons
  *
  * Rows without a target have loss 0 and count nowhere; what they hold is not
  * read by the products. A target at or beyond vocab (for cross entropy: any
- * out of range) makes its row's loss NaN. reduction: per row (loss fp32
+ * out of range) makes its row's loss NaN. frwkv_linear_cross_entropy_score is the
+ * cross entropy for calls without a backward behind them: the weight is not read again
+ * soon (a hint; the same bits, saved is written too). reduction: per row (loss fp32
  * [rows]), or the mean over rows with a target (0 without one) or the sum
  * (loss fp32 [1]).
  *
@@ -709,6 +711,11 @@ int frwkv_linear_cross_entropy_forward(int io_dtype, int64_t rows, int64_t chann
                                        int64_t ignore_index, int reduction, float* loss,
                                        void* saved, size_t saved_bytes, void* workspace,
                                        size_t workspace_bytes, void* stream);
+int frwkv_linear_cross_entropy_score(int io_dtype, int64_t rows, int64_t channels, int64_t vocab,
+                                     const void* hidden, const void* weight, int target_bytes,
+                                     const void* targets, int64_t ignore_index, int reduction,
+                                     float* loss, void* saved, size_t saved_bytes,
+                                     void* workspace, size_t workspace_bytes, void* stream);
 int frwkv_linear_topk_distillation_forward(
     int io_dtype, int64_t rows, int64_t channels, int64_t vocab, int64_t top, const void* hidden,
     const void* weight, int teacher_dtype, const void* teacher_logits, int index_bytes,

@@ -330,3 +330,30 @@ def test_certain_rows_at_the_least_temperatures(temperature, n, dtype):
     assert not dhidden[:, 1:].any()
     # The rows with a gradient hold zeros.
     assert not got["dweight"].any()
+
+
+@pytest.mark.parametrize("v", [50000, 90000])
+def test_cross_entropy_with_and_without_a_backward_to_follow(v):
+    """The hint that the weight is not read again soon changes no bits. Weights that are read
+    past the caches without a backward, and with one too."""
+    c = 2048
+    assert 2 * c * v > (192 if v == 50000 else 320) << 20
+    h, w, targets, _, _ = _case(5, c, v, torch.bfloat16, seed=13, masked=0.3)
+    for reduction in ("none", "mean", "sum"):
+        alone = pretrain_linear_cross_entropy(h, w, targets, reduction=reduction)
+        leaf = h.clone().requires_grad_()
+        followed = pretrain_linear_cross_entropy(leaf, w, targets, reduction=reduction)
+        assert torch.equal(alone, followed.detach()) and followed.requires_grad
+        for follows in (True, False):
+            loss = torch.empty(5 if reduction == "none" else 1, device=DEV)
+            capi.linear_cross_entropy_forward(h, w, targets, loss=loss, reduction=reduction,
+                                              backward_follows=follows)
+            assert torch.equal(loss.view(alone.shape), alone)
+        want, = torch.autograd.grad(followed.sum(), [leaf])
+        # What the call without one leaves serves a backward as well.
+        saved = capi.linear_cross_entropy_forward(h, w, targets, loss=loss, reduction=reduction,
+                                                  backward_follows=False)
+        grad = torch.empty_like(h)
+        capi.linear_loss_backward(torch.ones(5 if reduction == "none" else 1, device=DEV), w,
+                                  saved, rows=5, top=1, reduction=reduction, grad_hidden=grad)
+        assert torch.equal(grad, want)
