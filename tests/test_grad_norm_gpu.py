@@ -299,3 +299,71 @@ def test_tensors_that_share_memory_until_they_are_written():
         assert norm.item() == 10.0
         assert torch.equal(a, torch.ones_like(a))
         assert torch.allclose(lazy, torch.full_like(a, 0.1))
+
+
+def _long_list(seed, sizes, offset):
+    """Views of one buffer a type, `offset` elements off 16-byte places, with gaps between."""
+    gen = torch.Generator(device=DEV).manual_seed(seed)
+    room = {dtype: 0 for dtype in TYPES}
+    places = []
+    for i, n in enumerate(sizes):
+        dtype = TYPES[i % len(TYPES)]
+        places.append((dtype, room[dtype] + offset, n))
+        room[dtype] += (n + offset + 63) // 64 * 64
+    flat = {dtype: torch.randn(n, generator=gen, device=DEV).to(dtype)
+            for dtype, n in room.items()}
+    return flat, [flat[dtype][at:at + n] for dtype, at, n in places]
+
+
+def _stands_in_memory(tensors):
+    """Whether the call's memory holds the units' owners, beside at most 17 KB of sums."""
+    units = sum((t.numel() + 2047) // 2048 for t in tensors)
+    need = capi.library().frwkv_grad_norm_workspace_bytes(
+        len(tensors), capi._gradients(tensors, tensors))
+    return len(tensors) > 112 and need >= 4 * units + 32 * len(tensors)
+
+
+@pytest.mark.parametrize("offset", [0, 1])
+@pytest.mark.parametrize("large", [True, False])
+def test_long_lists_of_many_units(large, offset):
+    """Lists that stand in memory, of more units than are summed at a time, beyond the
+    last-level cache and within it; in place and into other types, over the maximum and under."""
+    sizes = [(1_200_000 if large else 150_000) + 1237 * (i % 50) for i in range(120)]
+    sizes[7::10] = [1 + (i * 311) % 5000 for i in range(len(sizes[7::10]))]
+    flat, tensors = _long_list(10, sizes, offset)
+    total = sum(t.numel() for t in tensors)
+    assert total > 4 * 2048 * 2048 * (1 if not large else 4) and _stands_in_memory(tensors)
+    assert (sum(t.numel() * t.element_size() for t in tensors) > 256 << 20) == large
+    norm = step.clip(tensors, 1.0, 0.0)[0]
+    before = {dtype: t.clone() for dtype, t in flat.items()}
+    for by in (0.3, 1.5):
+        out = [torch.full_like(t, math.nan, dtype=TYPES[(i + i // 3) % 3])
+               for i, t in enumerate(tensors)]
+        _check(tensors, out, pretrain_clip_grad_norm(tensors, norm * by, out=out), norm * by)
+        del out
+    assert all(torch.equal(before[dtype], t) for dtype, t in flat.items())
+    assert abs(pretrain_clip_grad_norm(tensors, norm * 1.5).item() - norm) <= 2 * E * norm
+    assert all(torch.equal(before[dtype], t) for dtype, t in flat.items())
+    sources = [before[t.dtype][t.storage_offset():t.storage_offset() + t.numel()]
+               for t in tensors]
+    _check(sources, tensors, pretrain_clip_grad_norm(tensors, norm * 0.3), norm * 0.3)
+    # What stands between the tensors stays.
+    for dtype, t in flat.items():
+        kept = torch.ones(t.numel(), dtype=torch.bool, device=DEV)
+        for x in tensors:
+            if x.dtype == dtype:
+                kept[x.storage_offset():x.storage_offset() + x.numel()] = False
+        assert torch.equal(t[kept], before[dtype][kept])
+
+
+@pytest.mark.parametrize("offset", [0, 3])
+def test_few_tensors_beyond_the_last_level_cache(offset):
+    """A list in the kernels' arguments, read through the caches whatever its size."""
+    flat, tensors = _long_list(11, [45_000_001, 30_000_007, 20_000_000, 2049], offset)
+    assert not _stands_in_memory(tensors)
+    assert sum(t.numel() * t.element_size() for t in tensors) > 256 << 20
+    norm = step.clip(tensors, 1.0, 0.0)[0]
+    out = [torch.empty_like(t, dtype=torch.float32) for t in tensors]
+    _check(tensors, out, pretrain_clip_grad_norm(tensors, norm * 0.1, out=out), norm * 0.1)
+    before = [t.clone() for t in tensors]
+    _check(before, tensors, pretrain_clip_grad_norm(tensors, norm * 0.1), norm * 0.1)

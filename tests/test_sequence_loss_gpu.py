@@ -20,6 +20,7 @@ import math
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 import flashrwkv_amd
 from flashrwkv_amd import capi, pretrain_policy_loss, pretrain_preference_loss
@@ -727,3 +728,163 @@ def test_terms_of_weight_zero_are_not_there(n, reduction):
     assert torch.equal(got["metrics"][:3], want["metrics"][:3])
     assert got["metrics"][3].item() == math.inf
     assert not got["dentropy"].any()
+
+
+# ------------------------------------------------ at the borders of the forms
+# One workgroup with tiles of 128 tokens up to 2048 and of 256 up to 4096; beyond, two launches
+# with tiles of 128 up to 262144 tokens and of 256 from there on; up to 64 pieces (tiles) of a
+# sequence are added by one lane, more by a wave.
+BORDERS = {
+    **{str(n): [n // 3, n - n // 3 - 65, 64, 1] for n in SIZES if n > 300},
+    "tiles of 128": [128, 127, 129, 256, 255, 257, 1, 128, 3900, 5],
+    "64 and 65 pieces": [8192, 8193, 8191, 64],
+    "64 and 65 long pieces": [16384, 16385, 16383, 250000],
+    "one long pair": [200001, 150002],
+    "many": torch.randint(9, (80000,), generator=_gen(34)).tolist(),
+}
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sequence_mean", "none"])
+@pytest.mark.parametrize("layout", BORDERS)
+def test_policy_at_the_borders_of_its_forms(layout, reduction):
+    print(f"case {layout} {reduction}", flush=True)
+    for per_sequence in (False, True):
+        case = _policy(BORDERS[layout], reduction=reduction, per_sequence=per_sequence, seed=35)
+        _check_policy(*case, _run_policy(*case))
+
+
+def _pairs(x, cu, args, upstream):
+    """What oracle/step.py's preference gives, without its loop over sequences, and of each
+    sequence its count, the sum of its terms' sizes and the factor of its sum."""
+    n, offsets = x.numel(), cu.cpu().long()
+    lengths = torch.cat([offsets.diff(), n - offsets[-1:]])
+    owner = torch.arange(lengths.numel()).repeat_interleave(lengths)
+    part = owner < lengths.numel() - 1
+    if args["mask"] is not None:
+        part &= args["mask"].cpu()
+    terms = x.double().cpu()
+    if args["reference"] is not None:
+        terms = terms - args["reference"].double().cpu()
+    zeros = torch.zeros(lengths.numel() - 1, dtype=torch.float64)
+    counts = zeros.index_add(0, owner[part], torch.ones(int(part.sum()), dtype=torch.float64))
+    sums = zeros.index_add(0, owner[part], terms[part])
+    sizes = zeros.index_add(0, owner[part], terms[part].abs())
+    by = 1 / counts.clamp_min(1) if args["normalize"] else torch.ones_like(counts)
+    beta, eps = args["beta"], args["label_smoothing"]
+    rewards = (beta * sums * by).view(-1, 2)
+    m = rewards[:, 0] - rewards[:, 1] - args["margin"]
+    taking = counts.view(-1, 2).amin(1) > 0
+    if args["kind"] == "sigmoid":
+        log_sigmoid = torch.nn.functional.logsigmoid
+        each = -(1 - eps) * log_sigmoid(m) - eps * log_sigmoid(-m)
+        slope = eps * torch.sigmoid(m) - (1 - eps) * torch.sigmoid(-m)
+    elif args["kind"] == "hinge":
+        each, slope = torch.relu(1 - m), -(m < 1).double()
+    else:
+        each, slope = ((m - 0.5) / beta) ** 2, 2 * (m - 0.5) / beta ** 2
+    each, slope = torch.where(taking, each, 0.0), torch.where(taking, slope, 0.0)
+    share = 1 / max(1, int(taking.sum())) if args["reduction"] == "mean" else 1.0
+    up = upstream.double().cpu().expand(m.numel())
+    coefficient = torch.stack([slope, -slope], 1).view(-1) * by * beta * share \
+        * up.repeat_interleave(2)
+    grad = torch.where(part, coefficient[owner.clamp_max(lengths.numel() - 2)], 0.0)
+    return {"m": m, "rewards": rewards, "each": each, "taking": taking, "share": share,
+            "loss": each if args["reduction"] == "none" else each.sum() * share,
+            "dlog_probs": grad, "counts": counts, "sizes": sizes, "by": by, "part": part,
+            "owner": owner.clamp_max(lengths.numel() - 2)}
+
+
+def _check_pairs(x, cu, args, upstream, got):
+    """Within what 64 bits leave of m, and the roundings to 32 bits behind it.
+
+    A sum of L terms is off by at most (L + 8) 2^-53 of the sum of their sizes, here and in
+    the oracle, so m by delta = (L + 8) 2^-52 (beta sum |terms| + |margin|). Loss: |dl/dm|
+    delta (64-bit roundings of the pairs' sum beside it) and two roundings to 32 bits.
+    Gradient: |d2l/dm2| delta through beta, share and 1 / count, and the roundings of
+    coefficient, share and two products to 32 bits."""
+    kind, beta, margin = args["kind"], args["beta"], args["margin"]
+    ref = _pairs(x, cu, args, upstream)
+    if ref["m"].numel() < 100:
+        plain = step.preference(x, cu, upstream=upstream, **args)
+        for name in ("m", "loss", "rewards", "dlog_probs"):
+            torch.testing.assert_close(ref[name], plain[name], rtol=1e-9, atol=1e-12)
+    m, by, share, taking = ref["m"], ref["by"], ref["share"], ref["taking"]
+    off = 2.0 ** -52 * (ref["counts"].max() + 8)
+    reward_off = off * beta * ref["sizes"] * by
+    delta = reward_off.view(-1, 2).sum(1) + off * abs(margin)
+    want = ref["rewards"].flatten()
+    value = got["rewards"].double().cpu().flatten()
+    assert ((value - want).abs() <= reward_off + E * want.abs()).all()
+    if kind == "sigmoid":
+        steep, curved = torch.ones_like(m), torch.full_like(m, 0.25)
+    elif kind == "hinge":
+        steep, curved = torch.ones_like(m), torch.zeros_like(m)
+        assert ((1 - m).abs() > delta)[taking].all()  # none is on the kink
+    else:
+        curved = torch.full_like(m, 2 / beta ** 2)
+        steep = curved * ((m - 0.5).abs() + delta)
+    each_off = torch.where(taking, steep * delta + 2.0 ** -49 * ref["each"].abs(), 0.0)
+    value = got["loss"].double().cpu()
+    if args["reduction"] == "none":
+        allowed = each_off + 2 * E * ref["each"].abs()
+    else:
+        allowed = share * (each_off.sum() + m.numel() * 2.0 ** -52 * ref["each"].abs().sum()) \
+            + 2 * E * ref["loss"].abs()
+    assert ((value - ref["loss"]).abs() <= allowed).all(), (value, ref["loss"])
+    up = upstream.double().cpu().abs().expand(m.numel())
+    slack = (curved * delta * beta * share * up).repeat_interleave(2) * by
+    want, value = ref["dlog_probs"], got["dlog_probs"].double().cpu()
+    allowed = 4 * E * (1 + 4 * E) * want.abs() + STEP[x.dtype] + torch.where(
+        ref["part"], slack[ref["owner"]], 0.0)
+    assert ((value - want).abs() <= allowed).all(), ((value - want).abs() - allowed).max()
+    # What is compared is far above what is allowed.
+    largest = want.abs().argmax()
+    assert want[largest].abs() >= 1e4 * allowed[largest] > 0.0
+
+
+@pytest.mark.parametrize("kind", ["sigmoid", "hinge", "squared"])
+@pytest.mark.parametrize("layout", BORDERS)
+def test_preference_at_the_borders_of_its_forms(layout, kind):
+    lengths = BORDERS[layout]
+    print(f"case {layout} {kind} {sum(lengths)} tokens, {len(lengths)} sequences", flush=True)
+    for normalize, masked, reduction in ((False, 0.0, "mean"), (True, 0.3, "mean"),
+                                         (False, 0.3, "sum"), (True, 0.0, "none")):
+        cu, n = _offsets(lengths, tail=9 if masked else 0)
+        x, _, reference = _logs(n, seed=len(lengths) + 36)
+        mask = (torch.rand(n, generator=_gen(37)) >= masked).to(DEV) if masked else None
+        args = {"reference": None if normalize else reference, "mask": mask, "beta": 1.0,
+                "margin": 0.1, "kind": kind, "normalize": normalize, "reduction": reduction,
+                "label_smoothing": 0.1 if kind == "sigmoid" else 0.0}
+        # m within 0.9, where no kind is flat or saturated.
+        up = torch.randn(len(lengths) // 2, generator=_gen(38)).to(DEV) if reduction == "none" \
+            else torch.tensor(0.6, device=DEV)
+        args["beta"] = 0.8 / _pairs(x, cu, args, up)["rewards"].diff(dim=1).abs().max().item()
+        _check_pairs(x, cu, args, up, _run_preference(x, cu, args, up))
+
+
+def test_the_borders_are_those_of_the_forms():
+    assert sum(BORDERS["many"]) > 262145 and len(BORDERS["many"]) > 64 * 1024
+    assert sum(BORDERS["64 and 65 pieces"]) in range(4097, 262145)
+    assert sum(BORDERS["64 and 65 long pieces"]) > 262144
+
+
+def test_what_is_kept_may_be_moved_or_made_again():
+    """Hooks on saved tensors: kept on the host between forward and backward, or made again by
+    a checkpoint."""
+    case = x, old, a, args, up = _policy([3000, 2100], reduction="sequence_mean", seed=39)
+    cu = args["cu_seqlens"]
+    pairs = {"reference": old, "mask": args["mask"]}
+    for run in (lambda: _run_policy(*case), lambda: _run_preference(x, cu, pairs, up)):
+        want = run()
+        with torch.autograd.graph.save_on_cpu():
+            got = run()
+        assert all(torch.equal(got[name], want[name]) for name in want)
+    leaf = x.clone().requires_grad_()
+
+    def both(leaf):
+        return (pretrain_policy_loss(leaf, old, a, cu_seqlens=cu, mask=args["mask"])
+                + pretrain_preference_loss(leaf, cu, mask=args["mask"])[0])
+
+    want, = torch.autograd.grad(both(leaf), [leaf])
+    again = torch.utils.checkpoint.checkpoint(both, leaf, use_reentrant=False)
+    assert torch.equal(torch.autograd.grad(again, [leaf])[0], want)
