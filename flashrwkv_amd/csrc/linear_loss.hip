@@ -1313,7 +1313,9 @@ struct Plan {
 // slabs weigh more: 9784, 9749, 9715 us). A slab is written in each piece and read
 // once after it.
 constexpr int64_t kCachedBytes = int64_t{192} << 20;
-constexpr int64_t kPartlyCachedBytes = int64_t{320} << 20;
+// Weights that the last-level cache keeps from one read to the next, wholly or in part.
+constexpr int64_t kKeptBytes = int64_t{248} << 20;
+constexpr int64_t kPartlyKeptBytes = int64_t{320} << 20;
 constexpr int64_t kMostBytes = int64_t{512} << 20;
 constexpr double kGradBytesPerUs = 20.0e6;
 constexpr double kSlabBytesPerUs = 4.0e6;
@@ -1498,12 +1500,13 @@ int run_forward(const Shape& d, const Source& source, const void* hidden, const 
                        stream, a, b, d.c, scale, d.k == 1, w.part, w.moments, pad, s);
   };
   // Few rows read the weight once: one that no cache holds until the next call goes past
-  // them (8 rows, 65536 tokens of 2048 channels: 61.3 -> 53.8 us, of 4096: 107 -> 93;
-  // 8192 tokens of 4096, which stay: 27.2 -> 32.6). A backward behind them still finds a part
-  // of a weight that is not much larger than the last-level cache (8 rows with their gradient:
-  // 268 MB 155 -> 160 us, 336 MB 202 -> 201, 403 MB 311 -> 301, 537 MB 294 -> 287).
+  // them (8 rows, 65536 tokens of 2048 channels: 61.3 -> 53.8 us, of 4096: 107 -> 93; weights
+  // that stay are slower so: 64 MB 27.2 -> 32.6, 201 MB 40.9 -> 42.5, 252 MB 47.2 -> 49.2). A
+  // backward behind them still finds a part of a weight that is not much larger than the
+  // last-level cache (8 rows with their gradient: 268 MB 155 -> 160 us, 336 MB 202 -> 201, 403
+  // MB 311 -> 301, 537 MB 294 -> 287).
   const int64_t weight_bytes = static_cast<int64_t>(d.vocab) * d.c * 2;
-  const bool past = weight_bytes > (last_read ? kCachedBytes : kPartlyCachedBytes);
+  const bool past = weight_bytes > (last_read ? kKeptBytes : kPartlyKeptBytes);
   for_sizes<T>(d.vocab, d.n, steps, [&](auto* tile, int grid) {
     using G = std::remove_pointer_t<decltype(tile)>;
     if constexpr (G::kTurns) {

@@ -332,12 +332,12 @@ def test_certain_rows_at_the_least_temperatures(temperature, n, dtype):
     assert not got["dweight"].any()
 
 
-@pytest.mark.parametrize("v", [50000, 90000])
+@pytest.mark.parametrize("v", [65536, 90000])
 def test_cross_entropy_with_and_without_a_backward_to_follow(v):
     """The hint that the weight is not read again soon changes no bits. Weights that are read
     past the caches without a backward, and with one too."""
     c = 2048
-    assert 2 * c * v > (192 if v == 50000 else 320) << 20
+    assert 2 * c * v > (248 if v == 65536 else 320) << 20
     h, w, targets, _, _ = _case(5, c, v, torch.bfloat16, seed=13, masked=0.3)
     for reduction in ("none", "mean", "sum"):
         alone = pretrain_linear_cross_entropy(h, w, targets, reduction=reduction)
@@ -357,3 +357,16 @@ def test_cross_entropy_with_and_without_a_backward_to_follow(v):
         capi.linear_loss_backward(torch.ones(5 if reduction == "none" else 1, device=DEV), w,
                                   saved, rows=5, top=1, reduction=reduction, grad_hidden=grad)
         assert torch.equal(grad, want)
+
+
+@pytest.mark.parametrize("n", [1, 40])
+@pytest.mark.parametrize("v", [65536, 90000])
+def test_scores_from_weights_that_no_cache_keeps(n, v):
+    """Read past the caches without a backward to follow, and the larger one with one too."""
+    c = 2048
+    assert 2 * c * v > (248 if v == 65536 else 320) << 20
+    h, w, targets, _, _ = _case(n, c, v, torch.bfloat16, seed=14, masked=0.0)
+    alone = pretrain_linear_log_probs(h, w, targets, entropy=True)
+    followed = pretrain_linear_log_probs(h.clone().requires_grad_(), w, targets, entropy=True)
+    assert all(torch.equal(a, b) for a, b in zip(alone, followed))
+    _check(h, w, targets, dict(zip(("log_probs", "entropy"), alone)), temperature=1.0)
