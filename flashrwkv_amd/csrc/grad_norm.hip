@@ -13,7 +13,8 @@
 // of many of them loses nothing. Workgroups leave one sum each, added in a fixed order:
 // two calls give the same bits. Two forms, by plan_of's rule:
 //
-// Short lists of few elements stand in the kernels' arguments. A workgroup takes a
+// Short lists of few elements stand in the kernels' arguments, and are read through the
+// caches. A workgroup takes a
 // run of consecutive chunks and searches the list for the first of them. All workgroups
 // that scale add up the sums by themselves, which saves the launch that would.
 //
@@ -429,7 +430,8 @@ __global__ __launch_bounds__(kThreads) void run_scale_kernel(Entries entries, Li
 }
 
 // A unit a workgroup, from the last one (and again, beyond what a launch has). Bound by
-// HBM: 449M bf16 elements into fp32 in 445 us, 6.0 TB/s.
+// HBM: 449M bf16 elements into fp32 in 445 us, 6.0 TB/s; in place 316 us, 5.7 TB/s, and 47 us
+// where nothing is to be scaled.
 constexpr int kMostScalers = 1 << 22;
 
 template <bool kStream>
@@ -483,7 +485,7 @@ int64_t chunks_of(int64_t numel, int64_t each) {
 // Most chunks of a list in the arguments: runs of eight, beyond which the order of
 // memory makes up for the launches that the other form has more.
 constexpr int64_t kMostRuns = 8 * kMostGroups;
-// The last-level cache's size: what is read twice and is larger passes by it.
+// The last-level cache's size: what the list's form reads twice and is larger passes by it.
 constexpr int64_t kCacheBytes = int64_t{256} << 20;
 
 Plan plan_of(int64_t count, const frwkv_gradient* tensors) {
