@@ -14,9 +14,9 @@
 // two calls give the same bits. Two forms, by plan_of's rule:
 //
 // Short lists of few elements stand in the kernels' arguments, and are read through the
-// caches. A workgroup takes a
-// run of consecutive chunks and searches the list for the first of them. All workgroups
-// that scale add up the sums by themselves, which saves the launch that would.
+// caches. A workgroup takes a run of consecutive chunks and searches the list for the first
+// of them. All workgroups that scale add up the sums by themselves, which saves the launch
+// that would.
 //
 // Others are written to the workspace by small kernels that take the list in their
 // arguments (nothing is copied from the host, and a captured call keeps its

@@ -775,9 +775,10 @@ int frwkv_linear_log_probs_backward(int io_dtype, int64_t rows, int64_t channels
  * loss is -min(r A, clamp(r, 1 - clip_low, 1 + clip_high) A), for A < 0 and
  * dual_clip > 1 (0: none) at most -dual_clip A, plus kl_weight k3(reference -
  * log_probs), k3(x) = exp(x) - 1 - x, minus entropy_weight entropy (reference and
- * entropy NULL: none; a term of weight 0 is left out, whatever it would be). loss: fp32 [tokens] (FRWKV_REDUCE_NONE), or [1] with their
- * mean or sum over tokens that take part, or FRWKV_REDUCE_SEQUENCE_MEAN, the mean of
- * each sequence's mean over sequences with such tokens; 0 without any. metrics fp32
+ * entropy NULL: none; a term of weight 0 is left out, whatever it would be). loss:
+ * fp32 [tokens] (FRWKV_REDUCE_NONE), or [1] with their mean or sum over tokens that
+ * take part, or FRWKV_REDUCE_SEQUENCE_MEAN, the mean of each sequence's mean over
+ * sequences with such tokens; 0 without any. metrics fp32
  * [4] (NULL: none): means over those tokens of r, of whether the gradient is clipped,
  * of k3(d) and of the reference's k3. cu_seqlens may be NULL with 0 sequences.
  * saved (256-byte aligned) is what the backward reads; want_slopes 0 leaves it

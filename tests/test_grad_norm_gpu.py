@@ -367,3 +367,17 @@ def test_few_tensors_beyond_the_last_level_cache(offset):
     _check(tensors, out, pretrain_clip_grad_norm(tensors, norm * 0.1, out=out), norm * 0.1)
     before = [t.clone() for t in tensors]
     _check(before, tensors, pretrain_clip_grad_norm(tensors, norm * 0.1), norm * 0.1)
+
+
+def test_offsets_of_elements_beyond_32_bits():
+    """One tensor of 2^31 elements and some, whose last units stand behind 2^32 bytes."""
+    n = 2 ** 31 + 4099
+    t = torch.full((n,), 0.5, device=DEV, dtype=torch.bfloat16)
+    t[-1], t[2 ** 31] = 1000.0, -2000.0
+    norm = math.sqrt(0.25 * (n - 2) + 1000.0 ** 2 + 2000.0 ** 2)
+    assert abs(pretrain_grad_norm([t]).item() - norm) <= 2 * E * norm
+    assert abs(pretrain_clip_grad_norm([t], norm / 4, eps=0.0).item() - norm) <= 2 * E * norm
+    # A quarter of each, within a rounding of the norm and one of the factor and the product.
+    assert t[-1].item() == 250.0 and t[2 ** 31].item() == -500.0
+    t[-1], t[2 ** 31] = 0.125, 0.125
+    assert t.min().item() == t.max().item() == 0.125

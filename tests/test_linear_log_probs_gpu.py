@@ -370,3 +370,42 @@ def test_scores_from_weights_that_no_cache_keeps(n, v):
     followed = pretrain_linear_log_probs(h.clone().requires_grad_(), w, targets, entropy=True)
     assert all(torch.equal(a, b) for a, b in zip(alone, followed))
     _check(h, w, targets, dict(zip(("log_probs", "entropy"), alone)), temperature=1.0)
+
+
+@pytest.mark.parametrize("n", [3, 300])
+def test_a_weight_beyond_32_bits_of_bytes(n):
+    """300000 tokens of 8192 channels, 4.9 GB, all of logit 0 but the first and the last two:
+    what is read or written at the end is found behind 2^32 bytes."""
+    c, v = 8192, 300_000
+    w = torch.zeros(v, c, device=DEV, dtype=torch.bfloat16)
+    w[0], w[v - 2], w[v - 1] = 2.0 ** -11, 2.0 ** -12, 2.0 ** -10
+    h = torch.ones(n, c, device=DEV, dtype=torch.bfloat16)
+    targets = (v - 1 - torch.arange(n) % 2).to(DEV)
+    z = torch.zeros(v, dtype=torch.float64)
+    z[0], z[v - 2], z[v - 1] = 4.0, 2.0, 8.0
+    log_q = torch.log_softmax(z, 0)
+    q, entropy = log_q.exp(), -(log_q.exp() * log_q).sum()
+    # Sums of V terms and the logarithms of them; logits are exact.
+    delta = (math.sqrt(v) + 32) * E * (1 + math.log(v))
+    got = pretrain_linear_log_probs(h, w, targets, entropy=True)
+    assert (got[0].double().cpu() - log_q[targets.cpu()]).abs().max() <= delta
+    assert (got[1].double().cpu() - entropy).abs().max() <= 2 * delta * (1 + entropy)
+    up, ue = torch.ones(n, device=DEV), torch.full((n,), 0.5, device=DEV)
+    out = _run(h, w, targets, up, ue)
+    assert torch.equal(out["log_probs"], got[0]) and torch.equal(out["entropy"], got[1])
+    b = torch.zeros(n, v, dtype=torch.float64)
+    b[torch.arange(n), targets.cpu()] = 1.0
+    dz = b - q - 0.5 * q * (log_q + entropy)
+    # One or two roundings of dz to 16 bits and one of the gradient; what the scores are off by.
+    u = ROUND[torch.bfloat16]
+    off = dz.abs() * 2 * u + delta * (b + 2 * q * (1 + log_q.abs() + entropy))
+    weights = w[[0, v - 2, v - 1], 0].double().cpu()
+    rows = [0, v - 2, v - 1]
+    value, want = out["dhidden"].double().cpu(), dz[:, rows] @ weights
+    allowed = off[:, rows] @ weights + 2 * u * want.abs()
+    assert ((value - want[:, None]).abs() <= allowed[:, None]).all()
+    want, allowed = dz.sum(0), off.sum(0) + 2 * u * dz.sum(0).abs()
+    for first in (0, v // 2, 262144 - 64, v - 128):
+        value = out["dweight"][first:first + 128].double().cpu()
+        there = slice(first, first + 128)
+        assert ((value - want[there, None]).abs() <= allowed[there, None]).all(), first

@@ -888,3 +888,42 @@ def test_what_is_kept_may_be_moved_or_made_again():
     want, = torch.autograd.grad(both(leaf), [leaf])
     again = torch.utils.checkpoint.checkpoint(both, leaf, use_reentrant=False)
     assert torch.equal(torch.autograd.grad(again, [leaf])[0], want)
+
+
+def test_as_many_tokens_as_offsets_can_name():
+    """2^31 - 1 tokens in three sequences and an empty one: ratios of 1, a ratio of 2 at the
+    ends of the sequences, whose tokens are found behind 2^32 bytes."""
+    n = 2 ** 31 - 1
+    cu = torch.tensor([0, 5, n - 1000, n - 1000, n - 1], dtype=torch.int32, device=DEV)
+    x = torch.zeros(n, device=DEV)
+    x[4] = x[n - 1001] = x[n - 2] = math.log(2.0)
+    x[n - 1] = math.nan  # behind the last sequence
+    old = torch.zeros(n, device=DEV, dtype=torch.bfloat16)
+    a = torch.tensor([-1.0, -2.0, 7.0, -4.0], device=DEV)
+    leaf = x.requires_grad_()
+    means = [(6.0, 5), (2.0 * (n - 1005) + 2.0, n - 1005), (4.0 * 999 + 4.0, 999)]
+    for reduction, want in (("sequence_mean", sum(s / k for s, k in means) / 3),
+                            ("mean", sum(s for s, _ in means) / (n - 1))):
+        loss, metrics = pretrain_policy_loss(leaf, old, a, cu_seqlens=cu, reduction=reduction,
+                                             metrics=True)
+        assert abs(loss.item() - want) <= 24 * E * want
+        assert abs(metrics[0].item() - 1.0) <= 24 * E
+        grad, = torch.autograd.grad(loss, [leaf])
+        for i, slope, k in ((4, 2.0, 5), (0, 1.0, 5), (5, 2.0, n - 1005), (n - 1001, 4.0, n - 1005),
+                            (n - 1000, 4.0, 999), (n - 2, 8.0, 999), (n - 1, 0.0, 1)):
+            share = 1 / (3 * k) if reduction == "sequence_mean" else 1 / (n - 1)
+            assert abs(grad[i].item() - slope * share) <= 24 * E * slope * share
+        del grad, loss
+    # Pairs: the second has an empty side and takes no part.
+    cu = torch.tensor([0, 5, n - 1000, n - 1000, n - 1], dtype=torch.int32, device=DEV)
+    loss, rewards = pretrain_preference_loss(leaf, cu, beta=1.0)
+    two = math.log(2.0)
+    want = [two, two, 0.0, two]
+    assert all(abs(r - w) <= 4 * E for r, w in zip(rewards.flatten().tolist(), want))
+    assert abs(loss.item() - two) <= 4 * E
+    grad, = torch.autograd.grad(loss, [leaf])
+    for i, value in ((0, -0.5), (4, -0.5), (5, 0.5), (n - 1001, 0.5), (n - 1000, 0.0),
+                     (n - 2, 0.0), (n - 1, 0.0)):
+        assert abs(grad[i].item() - value) <= 4 * E
+    assert grad[5:n - 1000].min().item() == grad[5:n - 1000].max().item()
+    assert not grad[n - 1000:].any()
